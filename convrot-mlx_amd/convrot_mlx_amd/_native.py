@@ -22,9 +22,10 @@ PREP_PACKED, PREP_INT8, PREP_ROTATE, PREP_FP6, PREP_INT8_BLOCKED, PREP_NO_ROTATE
 PRODUCER_PLAIN, PRODUCER_MODULATE, PRODUCER_GELU = 0, 1, 2
 LAYOUT_NK, LAYOUT_KN, LAYOUT_CDNA4 = 0, 1, 2
 ACT_PACKED, ACT_INT8, ACT_INT8_BLOCKED = 0, 1, 2
+POS_F32, POS_F64, POS_I32, POS_I64 = 0, 1, 2, 3
 
 # Every symbol the header declares, with its ctypes signature.
-_vp, _i64, _i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+_vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 SIGNATURES = {
     "convrot_prepare": (_i32, [_vp, _i32, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
     "convrot_prepare_modulated": (_i32, [_vp, _i32, _i64, _i64, _i32, _i32, _vp, _vp, _i64, ctypes.c_float, _vp,
@@ -62,6 +63,21 @@ SIGNATURES = {
     "convrot_weight_fp6_compact": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "convrot_w4a4_gemm_fp6_compact": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
                                              _i32, _vp]),
+    "convrot_quantize_int8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "convrot_w8a8_gemm": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
+                                 _i32, _vp]),
+    "convrot_layer_norm": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _i64, _f32, _vp, _vp, _vp, _vp]),
+    "convrot_layer_norm_int8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _i64, _f32, _vp, _i64, _vp,
+                                       _vp]),
+    "convrot_layer_norm_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "convrot_layer_norm_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i64, _vp, _i32, _i32, _i64,
+                                           _vp, _vp, _vp, _vp, _i64, _vp]),
+    "convrot_axes_table": (_i32, [_vp, _i32, _i64, _i32, _vp, ctypes.c_double, _vp, _vp]),
+    "convrot_qk_rotary": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i32, _vp, _i32, _i64, _vp,
+                                 _vp, _i32, _f32, _i32, _vp]),
+    "convrot_qk_rotary_workspace_bytes": (_i64, [_i32]),
+    "convrot_qk_rotary_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64,
+                                          _i32, _vp, _i32, _i64, _vp, _vp, _i32, _f32, _i32, _vp, _i64, _vp]),
     "convrot_last_error": (ctypes.c_char_p, []),
     "convrot_set_tuning": (_i32, [ctypes.c_char_p, ctypes.c_char_p]),
     "convrot_version": (ctypes.c_char_p, []),
@@ -149,7 +165,8 @@ def set_tuning(name: str, value: str | None) -> None:
     (A/B/C/D/E/F, S: split K, T), w4a16_tile ("BMxBN"), prep_ni (1/3/4), sk_spin_limit, gemm_persist (0: never;
     G: always, on G workgroups), gemm_mfma32 (0/1), fp6_tile ("BMxBN": 256x256, 256x224, 128x256, 128x192, 128x128),
     linear_rows_cfg (1/2/3/5/16), w4a4_midm_cfg (10 * row tiles + weight tiles),
-    fp6_split (1/2/4: parts of each 256x256 FP6 tile past the whole rounds)."""
+    fp6_split (1/2/4: parts of each 256x256 FP6 tile past the whole rounds),
+    w8a8_tile ("BMxBN": 256x256 or 128x128; "0x0": the few-row kernel)."""
     check(load().convrot_set_tuning(name.encode(), None if value is None else str(value).encode()))
 
 

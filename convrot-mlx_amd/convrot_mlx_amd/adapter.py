@@ -18,6 +18,7 @@ import torch
 from torch import nn
 
 from .core import CONVROT_GROUP_SIZE, ConvRotLinear, eligible_linear, quantize_convrot_weight
+from .int8 import Int8Linear
 
 
 def _set_submodule(root: nn.Module, name: str, module: nn.Module) -> None:
@@ -57,3 +58,20 @@ def replace_convrot_linears(
         _set_submodule(model, name, layer)
         names.append(name)
     return names
+
+
+def replace_int8_linears(model: nn.Module, *, select=None, convert: bool = True) -> list[str]:
+    """Replace Linears of `model` with Int8Linear layers in place; return the replaced names in
+    `named_modules` order.  `select(name, linear)` says which (all by default): used before
+    replace_convrot_linears it keeps the layers that 4 bits hurt at 8, the rest follow at 4.
+    convert=False installs zero weights and unit scales, ready for load_state_dict."""
+    selected = [(name, module) for name, module in model.named_modules()
+                if name and isinstance(module, nn.Linear) and (select is None or select(name, module))]
+    for name, dense in selected:
+        out_features, in_features = dense.weight.shape
+        layer = Int8Linear(in_features, out_features, bias=dense.bias is not None, device=dense.weight.device)
+        if convert:
+            with torch.no_grad():
+                layer.load_weight(dense.weight.detach(), None if dense.bias is None else dense.bias.detach())
+        _set_submodule(model, name, layer)
+    return [name for name, _ in selected]

@@ -1,0 +1,222 @@
+"""Linears of 8-bit integers (W8A8): one scale a token, one an output channel.
+
+For the layers that 4 bits hurt, or whose features no rotation group divides: rows are
+quantized symmetrically to [-127, 127] (codes = round(x * (127 / absmax)), scale = absmax / 127),
+the integer product is exact and the epilogue is that of the 4-bit linears,
+((dot * xscale) * wscale) + bias in float32, then the optional gated residual.  Weights stay
+row-major int8 [N, K], as 8-bit checkpoints hold them.  No counterpart in the reference, which
+quantizes to 4 bits only.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import _native as nat
+from .core import GatedResidual, _f32, _gated_residual
+from .norm import norm_operands, rows_of
+
+INT8_MAX = 127
+MAX_FEATURES = 65536
+
+
+def _round16(k: int) -> int:
+    return (k + 15) // 16 * 16
+
+
+def quantize_int8_rowwise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of x [M, K] (any strides) as (int8 codes [M, K], float32 scales [M]).
+
+    A row that holds a NaN or an infinity gets the scale NaN (its products are NaN); a row whose
+    largest magnitude is below 2^-100 counts as zero.  Where K is no multiple of 16 the codes are a
+    view of rows padded to one, as the matrix product reads them."""
+    if x.ndim != 2:
+        raise ValueError(f"rowwise int8 quantization expects 2D input, got {tuple(x.shape)}")
+    nat.require_device(x)
+    x = rows_of(x)
+    m, k = x.shape
+    codes = torch.empty((m, _round16(k)), dtype=torch.int8, device=x.device)
+    scales = torch.empty((m,), dtype=torch.float32, device=x.device)
+    nat.check(nat.load().convrot_quantize_int8(nat.ptr(x), nat.dtype_code(x.dtype), m, k, x.stride(0), nat.ptr(codes),
+                                               codes.shape[1], nat.ptr(scales), nat.stream_of(x.device)))
+    if k == 0:
+        scales.zero_()
+    return codes if codes.shape[1] == k else codes[:, :k], scales
+
+
+def _operand(t: torch.Tensor, what: str, zero_tail: bool) -> torch.Tensor:
+    """An int8 matrix as rows the product can read: adjacent features, 16-byte aligned rows that
+    cover the features rounded up to 16 (past them zeros, with `zero_tail`); else a padded copy."""
+    if t.ndim != 2 or t.dtype != torch.int8:
+        raise ValueError(f"W8A8 {what} must be 2D int8, got {tuple(t.shape)} {t.dtype}")
+    k = t.shape[1]
+    if (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= _round16(k) and t.data_ptr() % 16 == 0
+            and (k % 16 == 0 or (not zero_tail and t.shape[0] * t.stride(0) + t.storage_offset()
+                                 <= t.untyped_storage().nbytes()))):
+        return t
+    return torch.nn.functional.pad(t, (0, -k % 16)) if k % 16 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_scales(name: str, t: torch.Tensor, n: int) -> None:
+    if tuple(t.shape) != (n,):
+        raise ValueError(f"W8A8 {name} must have shape {(n,)}, got {tuple(t.shape)}")
+
+
+def _w8a8(act, weight, xscales, wscales, bias, k: int, dtype: torch.dtype, gr: GatedResidual | None) -> torch.Tensor:
+    """The product of operands as the kernel reads them (see _operand)."""
+    m, n = act.shape[0], weight.shape[0]
+    if gr is not None and gr.inplace:
+        out = gr.residual.view(m, n)
+    else:
+        out = torch.empty((m, n), dtype=dtype, device=act.device)
+    nat.check(nat.load().convrot_w8a8_gemm(
+        nat.ptr(act), act.stride(0), nat.ptr(xscales), nat.ptr(weight), weight.stride(0), nat.ptr(wscales),
+        nat.ptr(bias), m, n, k, nat.ptr(gr.residual if gr is not None else None),
+        nat.ptr(gr.gate if gr is not None else None), gr.stride if gr is not None else 0,
+        gr.rows_per_gate if gr is not None else 1, nat.ptr(out), nat.dtype_code(dtype), nat.stream_of(act.device)))
+    return out
+
+
+def _check_product(k: int, weight: torch.Tensor, wscales, bias) -> int:
+    if weight.ndim != 2 or weight.dtype != torch.int8:
+        raise ValueError(f"W8A8 weight must be 2D int8, got {tuple(weight.shape)} {weight.dtype}")
+    n = weight.shape[0]
+    if weight.shape[1] != k:
+        raise ValueError(f"W8A8 weight must be N x K with K={k}, got {tuple(weight.shape)}")
+    if not 0 < k <= MAX_FEATURES:
+        raise ValueError(f"W8A8 product needs 1 to {MAX_FEATURES} features, got {k}")
+    _check_scales("weight scales", wscales, n)
+    if bias is not None:
+        _check_scales("bias", bias, n)
+    return n
+
+
+def _residual(residual, gate, inplace: bool, m: int, n: int, dtype: torch.dtype) -> GatedResidual | None:
+    if residual is None:
+        if gate is not None or inplace:
+            raise ValueError("gate and inplace need a residual")
+        return None
+    if residual.ndim < 1 or residual.shape[-1] != n or residual.numel() != m * n:
+        raise ValueError(f"residual {tuple(residual.shape)} must hold the [{m}, {n}] output as [..., {n}]")
+    return _gated_residual(residual, gate, tuple(residual.shape), dtype, inplace)
+
+
+def hip_w8a8_matmul(qact: torch.Tensor, qweight: torch.Tensor, xscales: torch.Tensor, wscales: torch.Tensor,
+                    bias: torch.Tensor | None = None, *, output_dtype: torch.dtype, residual=None, gate=None,
+                    inplace: bool = False) -> torch.Tensor:
+    """int8 activations [M, K] x int8 weight [N, K] -> output_dtype [M, N]:
+    ((dot * xscales[m]) * wscales[n]) + bias[n]; residual, gate and inplace as in hip_w4a4_matmul."""
+    if qact.ndim != 2 or qact.dtype != torch.int8:
+        raise ValueError(f"W8A8 activation must be 2D int8, got {tuple(qact.shape)} {qact.dtype}")
+    m, k = qact.shape
+    n = _check_product(k, qweight, wscales, bias)
+    _check_scales("activation scales", xscales, m)
+    nat.dtype_code(output_dtype)
+    nat.require_device(qact, qweight, xscales, wscales, bias)
+    gr = _residual(residual, gate, inplace, m, n, output_dtype)
+    return _w8a8(_operand(qact, "activation", False), _operand(qweight, "weight", True), _f32(xscales), _f32(wscales),
+                 _f32(bias), k, output_dtype, gr)
+
+
+def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, bias: torch.Tensor | None = None,
+                    *, residual=None, gate=None, inplace: bool = False) -> torch.Tensor:
+    """x [..., K] (float32, float16 or bfloat16), quantized row by row, times the int8 weight
+    [N, K] -> [..., N] of x's type; residual, gate and inplace as in ConvRotLinear.forward."""
+    k = x.shape[-1]
+    n = _check_product(k, qweight, wscales, bias)
+    device = nat.require_device(x, qweight, wscales, bias)
+    x2d = rows_of(x.reshape(-1, k))
+    m = x2d.shape[0]
+    gr = _residual(residual, gate, inplace, m, n, x.dtype)
+    weight = _operand(qweight, "weight", True)
+    lib, dtype, k16 = nat.load(), nat.dtype_code(x.dtype), _round16(k)
+    codes = torch.empty((m, k16), dtype=torch.int8, device=device)
+    scales = torch.empty((m,), dtype=torch.float32, device=device)
+    nat.check(lib.convrot_quantize_int8(nat.ptr(x2d), dtype, m, k, x2d.stride(0), nat.ptr(codes), k16,
+                                        nat.ptr(scales), nat.stream_of(device)))
+    out = _w8a8(codes, weight, scales, _f32(wscales), _f32(bias), k, x.dtype, gr)
+    return residual if inplace else out.reshape(*x.shape[:-1], n)
+
+
+class Int8Linear(nn.Module):
+    """A linear layer stored and executed in 8 bits: `qweight` int8 [N, K], `scales` float32 [N]
+    (ones), `bias` float32 [N] (zeros); the output type is the input type.  The calls of
+    ConvRotLinear: forward and forward_modulated, each with residual=, gate= and inplace=."""
+
+    def __init__(self, in_features: int, out_features: int, *, bias: bool = True, device=None):
+        super().__init__()
+        if not 0 < in_features <= MAX_FEATURES:
+            raise ValueError(f"W8A8 product needs 1 to {MAX_FEATURES} features, got {in_features}")
+        self.in_features, self.out_features = in_features, out_features
+        self.register_buffer("qweight", torch.zeros((out_features, in_features), dtype=torch.int8, device=device))
+        self.register_buffer("scales", torch.ones((out_features,), dtype=torch.float32, device=device))
+        self.register_buffer("bias", torch.zeros((out_features,), dtype=torch.float32, device=device))
+        self.source_has_bias = bias
+        self._padded: tuple | None = None
+
+    def load_weight(self, weight: torch.Tensor, bias: torch.Tensor | None = None) -> Int8Linear:
+        """Quantize a dense (out, in) weight into this layer."""
+        if tuple(weight.shape) != (self.out_features, self.in_features):
+            raise ValueError(f"weight must have shape {(self.out_features, self.in_features)}, got "
+                             f"{tuple(weight.shape)}")
+        codes, self.scales = quantize_int8_rowwise(weight)
+        self.qweight = codes.contiguous()
+        if bias is not None:
+            self.bias = bias.to(torch.float32)
+        return self
+
+    def _weight(self) -> torch.Tensor:
+        """The weight as the kernels read it: itself, or where in_features is no multiple of 16 a
+        copy with padded rows, made once per tensor version."""
+        q = self.qweight
+        if self.in_features % 16 == 0:
+            return q
+        key = (q.data_ptr(), q._version, tuple(q.shape), q.device)
+        if self._padded is None or self._padded[0] != key:
+            self._padded = (key, torch.nn.functional.pad(q, (0, -self.in_features % 16)))
+        return self._padded[1]
+
+    def forward(self, x: torch.Tensor, *, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                inplace: bool = False) -> torch.Tensor:
+        """linear(x); with `residual`, residual + gate * linear(x), as ConvRotLinear.forward."""
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"Int8Linear expected K={self.in_features}, got {x.shape[-1]}")
+        if residual is not None and tuple(residual.shape) != (*x.shape[:-1], self.out_features):
+            raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
+                             f"{(*x.shape[:-1], self.out_features)}")
+        weight = self._weight()
+        if self.in_features % 16 == 0:
+            return hip_w8a8_linear(x, weight, self.scales, self.bias, residual=residual, gate=gate, inplace=inplace)
+        codes, scales = quantize_int8_rowwise(x.reshape(-1, self.in_features))
+        gr = _residual(residual, gate, inplace, codes.shape[0], self.out_features, x.dtype)
+        out = _w8a8(codes, weight, scales, _f32(self.scales), _f32(self.bias), self.in_features, x.dtype, gr)
+        return residual if inplace else out.reshape(*x.shape[:-1], self.out_features)
+
+    def forward_modulated(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, eps: float = 1e-6, *,
+                          residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                          inplace: bool = False) -> torch.Tensor:
+        """self((1 + scale) * layer_norm(x) + shift), the norm and the quantization in one kernel (the
+        normalized row goes to codes unrounded); residual, gate and inplace as in forward."""
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"Int8Linear expected K={self.in_features}, got {x.shape[-1]}")
+        if residual is not None and tuple(residual.shape) != (*x.shape[:-1], self.out_features):
+            raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
+                             f"{(*x.shape[:-1], self.out_features)}")
+        k = self.in_features
+        x2d = rows_of(x.reshape(-1, k))
+        m = x2d.shape[0]
+        gr = _residual(residual, gate, inplace, m, self.out_features, x.dtype)
+        gain, sh, each, _ = norm_operands(x2d, None, None, scale, shift)
+        device = nat.require_device(x2d, gain, sh, self.qweight)
+        codes = torch.empty((m, _round16(k)), dtype=torch.int8, device=device)
+        scales = torch.empty((m,), dtype=torch.float32, device=device)
+        nat.check(nat.load().convrot_layer_norm_int8(
+            nat.ptr(x2d), nat.dtype_code(x.dtype), m, k, x2d.stride(0), nat.ptr(gain), nat.ptr(sh),
+            nat.dtype_code(gain.dtype), 1, each, float(eps), nat.ptr(codes), codes.shape[1], nat.ptr(scales),
+            nat.stream_of(device)))
+        out = _w8a8(codes, self._weight(), scales, _f32(self.scales), _f32(self.bias), k, x.dtype, gr)
+        return residual if inplace else out.reshape(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}"

@@ -1,0 +1,162 @@
+"""Layer norm with a weight and bias, or with the shift and scale of adaptive layer norm (adaLN),
+and its gradient.
+
+    y = u * g + b,  u = (x - mean) / sqrt(var + eps),  g = weight or 1 + scale, b = bias or shift
+
+in float32, rounded once.  hip_layer_norm and hip_layer_norm_backward are the two kernels;
+layer_norm is the operator that torch differentiates through.  No counterpart in the reference,
+whose example model runs the norm as array operations (examples/flux1_dev/adapter.py:45-70).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+
+MAX_BACKWARD_FEATURES = 32768
+
+
+def rows_of(x: torch.Tensor) -> torch.Tensor:
+    """A 2-D tensor with adjacent features and rows at one stride (else a contiguous copy)."""
+    if (x.shape[1] > 1 and x.stride(1) != 1) or x.stride(0) < 0:
+        return x.contiguous()
+    return x
+
+
+def norm_operands(x2d, weight, bias, scale, shift):
+    """(gain [V, K] or None, shift [V, K] or None, rows a vector, plus one?) of a norm's
+    parameters, both of one type that the kernels take beside x's."""
+    rows, k = x2d.shape
+    if (weight is not None or bias is not None) and (scale is not None or shift is not None):
+        raise ValueError("layer norm takes weight and bias, or scale and shift")
+    plus_one = scale is not None or shift is not None
+    gain, add = (scale, shift) if plus_one else (weight, bias)
+    given = [t for t in (gain, add) if t is not None]
+    if not given:
+        return None, None, max(1, rows), plus_one
+    for t in given:
+        if t.ndim < 1 or t.shape[-1] != k or t.numel() == 0 or (not plus_one and t.ndim != 1):
+            what = "scale and shift must end in" if plus_one else "weight and bias must have"
+            raise ValueError(f"layer norm {what} {k} features, got {tuple(t.shape)}")
+    vectors = given[0].numel() // k
+    if given[-1].numel() // k != vectors:
+        raise ValueError(f"shift has {given[-1].numel() // k} rows but scale has {vectors}")
+    if rows % vectors:
+        raise ValueError(f"{rows} activation rows do not split evenly over {vectors} modulation vectors")
+    kind = x2d.dtype if all(t.dtype == x2d.dtype for t in given) else torch.float32
+    gain, add = (None if t is None else t.reshape(vectors, k).to(kind).contiguous() for t in (gain, add))
+    return gain, add, max(1, rows // vectors), plus_one
+
+
+def hip_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+                   scale: torch.Tensor | None = None, shift: torch.Tensor | None = None, eps: float = 1e-6,
+                   return_stats: bool = False):
+    """Layer norm over the last axis of x [..., K] (rows at any one stride), of x's type.
+
+    weight, bias: [K].  Or scale, shift: [V, K] or [V, 1, K], the rows split evenly over the V
+    vectors in order, as x [B, L, K] beside scale [B, 1, K] does: (1 + scale) * u + shift.  Either
+    of a pair may be None.  With return_stats also the rows' float32 mean and 1 / sqrt(var + eps)."""
+    nat.require_device(x, weight, bias, scale, shift)
+    k = x.shape[-1]
+    x2d = rows_of(x.reshape(-1, k))
+    rows = x2d.shape[0]
+    gain, add, each, plus_one = norm_operands(x2d, weight, bias, scale, shift)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if return_stats else None
+    mean, rstd = (None, None) if stats is None else stats.unbind(0)
+    kind = gain if gain is not None else add
+    nat.check(nat.load().convrot_layer_norm(
+        nat.ptr(x2d), nat.dtype_code(x.dtype), rows, k, x2d.stride(0), nat.ptr(gain), nat.ptr(add),
+        nat.dtype_code(x.dtype if kind is None else kind.dtype), int(plus_one), each, float(eps), nat.ptr(out),
+        nat.ptr(mean), nat.ptr(rstd), nat.stream_of(x.device)))
+    return out if stats is None else (out, mean, rstd)
+
+
+def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, *,
+                            weight: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                            vectors: int | None = None, param_grads: bool = True):
+    """Gradients of hip_layer_norm from dy, its input and its stats: (dx, dgain, dshift).
+
+    dgain is the gradient of weight (or scale), dshift that of bias (or shift), [K] beside a
+    weight, else of scale's shape ([vectors, K] where the norm had a shift alone: pass `vectors`);
+    both are of the parameter's type (x's without one), None without param_grads.  Sums over rows
+    are float32 in a fixed order: results repeat bit for bit."""
+    nat.require_device(dy, x, mean, rstd, weight, scale)
+    k = x.shape[-1]
+    if dy.shape != x.shape:
+        raise ValueError(f"dy {tuple(dy.shape)} must have the shape of x {tuple(x.shape)}")
+    if dy.dtype != x.dtype:
+        raise ValueError(f"dy dtype {dy.dtype} differs from x dtype {x.dtype}")
+    if k > MAX_BACKWARD_FEATURES:
+        raise ValueError(f"the layer norm's gradient supports at most {MAX_BACKWARD_FEATURES} features, got {k}")
+    x2d, dy2d = rows_of(x.reshape(-1, k)), rows_of(dy.reshape(-1, k))
+    rows = x2d.shape[0]
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if tuple(t.shape) != (rows,) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 {(rows,)}, got {t.dtype} {tuple(t.shape)}")
+    gain, _, each, plus_one = norm_operands(x2d, weight, None, scale, None)
+    if gain is None and vectors is not None:
+        if vectors < 1 or rows % vectors:
+            raise ValueError(f"{rows} activation rows do not split evenly over {vectors} modulation vectors")
+        each = max(1, rows // vectors)
+    if gain is not None:
+        vectors = gain.shape[0]
+    given = scale if scale is not None else weight
+    kind = x.dtype if gain is None else gain.dtype
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    grads = work = None
+    lib = nat.load()
+    if param_grads:
+        grads = torch.empty((2, vectors or 1, k), dtype=kind, device=x.device)
+        work = torch.empty((lib.convrot_layer_norm_workspace_bytes(rows, k, each),), dtype=torch.uint8,
+                           device=x.device)
+    nat.check(lib.convrot_layer_norm_backward(
+        nat.ptr(dy2d), dy2d.stride(0), nat.ptr(x2d), x2d.stride(0), nat.ptr(mean), nat.ptr(rstd),
+        nat.dtype_code(x.dtype), rows, k, nat.ptr(gain), nat.dtype_code(kind), int(plus_one), each, nat.ptr(dx),
+        nat.ptr(None if grads is None else grads[0]), nat.ptr(None if grads is None else grads[1]), nat.ptr(work),
+        0 if work is None else work.numel(), nat.stream_of(x.device)))
+    if grads is None:
+        return dx, None, None
+    if rows == 0:
+        grads.zero_()
+    if given is not None:
+        grads = grads.to(given.dtype).reshape(2, *given.shape)
+    elif vectors is None:
+        grads = grads.reshape(2, k)
+    return dx, grads[0], grads[1]
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, scale, shift, eps):
+        y, mean, rstd = hip_layer_norm(x, weight, bias, scale=scale, shift=shift, eps=eps, return_stats=True)
+        ctx.save_for_backward(x, mean, rstd, weight, scale)
+        add = bias if bias is not None else shift
+        ctx.adaptive = scale is not None or shift is not None
+        ctx.add = None if add is None else (add.shape, add.dtype)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, mean, rstd, weight, scale = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        vectors = None
+        if ctx.adaptive and scale is None:
+            vectors = ctx.add[0].numel() // max(1, x.shape[-1])
+        dx, dgain, dadd = hip_layer_norm_backward(dy, x, mean, rstd, weight=weight, scale=scale, vectors=vectors,
+                                                  param_grads=any(needs[1:5]))
+        if dadd is not None and ctx.add is not None:
+            dadd = dadd.reshape(ctx.add[0]).to(ctx.add[1])
+        a = ctx.adaptive
+        return (dx if needs[0] else None, dgain if needs[1] and not a else None, dadd if needs[2] and not a else None,
+                dgain if needs[3] and a else None, dadd if needs[4] and a else None, None)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+               scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
+               eps: float = 1e-6) -> torch.Tensor:
+    """hip_layer_norm, with gradients for x and for the parameters that need them."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, scale, shift)):
+        return _LayerNorm.apply(x, weight, bias, scale, shift, eps)
+    return hip_layer_norm(x, weight, bias, scale=scale, shift=shift, eps=eps)

@@ -98,7 +98,8 @@ int convrot_set_tuning(const char* name, const char* value) {
                 {"prep_ni", kTunePrepNi},             {"sk_spin_limit", kTuneSkSpinLimit},
                 {"gemm_persist", kTuneGemmPersist},   {"gemm_mfma32", kTuneGemmMfma32},
                 {"fp6_tile", kTuneFp6Tile},           {"linear_rows_cfg", kTuneRowsCfg},
-                {"w4a4_midm_cfg", kTuneMidmCfg},      {"fp6_split", kTuneFp6Split}};
+                {"w4a4_midm_cfg", kTuneMidmCfg},      {"fp6_split", kTuneFp6Split},
+                {"w8a8_tile", kTuneW8a8Tile}};
   int key = -1;
   for (const auto& n : kNames)
     if (strcmp(n.name, name) == 0) key = n.key;
@@ -116,11 +117,14 @@ int convrot_set_tuning(const char* name, const char* value) {
         break;
       }
       case kTuneFp6Tile:
+      case kTuneW8a8Tile:
       case kTuneW4a16Tile: {
         int bm = 0, bn = 0;
         char tail = 0;
         good = sscanf(value, "%dx%d%c", &bm, &bn, &tail) == 2 &&
-               (key == kTuneFp6Tile ? fp6_tile_known(bm, bn) : w4a16_tile_known(bm, bn));
+               (key == kTuneFp6Tile    ? fp6_tile_known(bm, bn)
+                : key == kTuneW8a8Tile ? w8a8_tile_known(bm, bn)
+                                       : w4a16_tile_known(bm, bn));
         v = bm | bn << 10;
         break;
       }
@@ -698,6 +702,243 @@ int convrot_weight_fp6(const uint8_t* cdna4, uint8_t* fp6, int64_t N, int64_t K,
   if (!aligned(cdna4, 16) || !aligned(fp6, 16)) return fail(CONVROT_ERR_INVALID, "cdna4 and fp6 must be 16-byte aligned");
   return launch_status(convrot::launch_weight_fp6(cdna4, fp6, N, K, (hipStream_t)stream),
                        "convrot_weight_fp6");
+}
+
+namespace {
+
+constexpr int64_t kMaxInt8Stride = int64_t(1) << 22;  // of a W8A8 operand's rows: a tile's offsets stay below 2^31
+constexpr int64_t kMaxRows = 0x7fffffff;
+
+// Checks shared by the row operators; `features` may not exceed `most`.
+int check_rows(const char* what, const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride,
+               int64_t most) {
+  if (!valid_dtype(dtype)) return fail(CONVROT_ERR_INVALID, "unsupported activation dtype code %d", dtype);
+  if (rows < 0 || features < 0)
+    return fail(CONVROT_ERR_INVALID, "invalid shape rows=%lld features=%lld", (long long)rows, (long long)features);
+  if (features > most)
+    return fail(CONVROT_ERR_UNSUPPORTED, "%s supports at most %lld features, got %lld", what, (long long)most,
+                (long long)features);
+  if (rows > kMaxRows) return fail(CONVROT_ERR_UNSUPPORTED, "%s supports at most 2^31-1 rows", what);
+  if (rows == 0 || features == 0) return ok();
+  if (!x) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (rows > 1 && x_stride < 0) return fail(CONVROT_ERR_INVALID, "negative row stride %lld", (long long)x_stride);
+  if (!aligned(x, dtype == CONVROT_DTYPE_F32 ? 4 : 2)) return fail(CONVROT_ERR_INVALID, "x is not aligned to its type");
+  return ok();
+}
+
+int check_codes(const int8_t* codes, int64_t stride, int64_t features, const float* scales) {
+  if (!codes || !scales) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (stride < features || stride % 16 || !aligned(codes, 16))
+    return fail(CONVROT_ERR_INVALID, "codes need 16-byte aligned rows of at least %lld bytes, got a stride of %lld",
+                (long long)features, (long long)stride);
+  if (stride > (features + 15) / 16 * 16 + 1024 || stride > 65536)
+    return fail(CONVROT_ERR_UNSUPPORTED, "codes stride %lld too long for %lld features", (long long)stride,
+                (long long)features);
+  return ok();
+}
+
+int check_params(const void* gain, const void* shift, int dtype, int param_dtype, int64_t rows,
+                 int64_t rows_per_vector) {
+  if (!gain && !shift && rows_per_vector <= 0) return ok();
+  if (param_dtype != dtype && param_dtype != CONVROT_DTYPE_F32)
+    return fail(CONVROT_ERR_INVALID, "norm parameters must have the activations' type or float32, got %s",
+                dtype_name(param_dtype));
+  if (rows_per_vector <= 0 || rows % rows_per_vector)
+    return fail(CONVROT_ERR_INVALID, "%lld rows do not split into vectors of %lld rows", (long long)rows,
+                (long long)rows_per_vector);
+  const uintptr_t a = param_dtype == CONVROT_DTYPE_F32 ? 4 : 2;
+  if (!aligned(gain, a) || !aligned(shift, a))
+    return fail(CONVROT_ERR_INVALID, "norm parameters are not aligned to their type");
+  return ok();
+}
+
+int check_rotary(int dtype, int batch, int q_heads, int k_heads, int64_t length, int dim, const float* table,
+                 int pairs, int64_t table_batch_stride, const void* q_weight, const void* k_weight, int weight_dtype,
+                 const int64_t* strides) {
+  if (!valid_dtype(dtype)) return fail(CONVROT_ERR_INVALID, "unsupported activation dtype code %d", dtype);
+  if (batch < 0 || q_heads < 0 || k_heads < 0 || length < 0 || dim < 0 || pairs < 0)
+    return fail(CONVROT_ERR_INVALID, "invalid rotary shape batch=%d heads=%d/%d length=%lld dim=%d pairs=%d", batch,
+                q_heads, k_heads, (long long)length, dim, pairs);
+  if (2 * (int64_t)pairs > dim)
+    return fail(CONVROT_ERR_INVALID, "%d pairs do not fit a head of %d features", pairs, dim);
+  if (dim > 512) return fail(CONVROT_ERR_UNSUPPORTED, "rotary positions support heads of up to 512 features, got %d", dim);
+  if (q_heads > 65536 || k_heads > 65536 || (int64_t)batch * length > kMaxRows || length > kMaxRows)
+    return fail(CONVROT_ERR_UNSUPPORTED, "rotary positions support at most 2^31-1 tokens and 65536 heads");
+  if ((q_weight || k_weight) && weight_dtype != dtype && weight_dtype != CONVROT_DTYPE_F32)
+    return fail(CONVROT_ERR_INVALID, "norm weights must have the activations' type or float32, got %s",
+                dtype_name(weight_dtype));
+  if (batch == 0 || length == 0 || dim == 0 || q_heads + k_heads == 0) return ok();
+  if (!strides || (pairs > 0 && !table)) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(table, 4) || table_batch_stride < 0) return fail(CONVROT_ERR_INVALID, "invalid rotary table");
+  return ok();
+}
+
+}  // namespace
+
+int convrot_quantize_int8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride, int8_t* codes,
+                          int64_t codes_stride, float* scales, void* stream) {
+  if (int rc = check_rows("8-bit quantization", x, dtype, rows, features, x_stride, kMaxFeatures)) return rc;
+  if (rows == 0 || features == 0) return ok();
+  if (int rc = check_codes(codes, codes_stride, features, scales)) return rc;
+  return launch_status(convrot::launch_quantize_int8(x, dtype, rows, features, x_stride, codes, codes_stride, scales,
+                                                     (hipStream_t)stream),
+                       "convrot_quantize_int8");
+}
+
+int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscales, const int8_t* weight,
+                      int64_t weight_stride, const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K,
+                      const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate, void* out,
+                      int out_dtype, void* stream) {
+  if (!valid_dtype(out_dtype)) return fail(CONVROT_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
+  if (M < 0 || N < 0 || K <= 0)
+    return fail(CONVROT_ERR_INVALID, "invalid GEMM shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  if (K > kMaxFeatures)
+    return fail(CONVROT_ERR_UNSUPPORTED, "W8A8 GEMM supports K up to %lld, got %lld", (long long)kMaxFeatures, (long long)K);
+  // 2^31 - 1 less what rounding a dimension up to whole tiles adds
+  if (M > 0x7ffffe00 || N > 0x7ffffe00) return fail(CONVROT_ERR_UNSUPPORTED, "GEMM dimension too large");
+  if (gate && !residual) return fail(CONVROT_ERR_INVALID, "a gate needs a residual");
+  if (gate && rows_per_gate <= 0)
+    return fail(CONVROT_ERR_INVALID, "rows_per_gate must be positive, got %lld", (long long)rows_per_gate);
+  if (M == 0 || N == 0) return ok();
+  if (!act || !weight || !xscales || !wscales || !out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  const int64_t k16 = (K + 15) / 16 * 16;
+  if (act_stride < k16 || weight_stride < k16 || act_stride % 16 || weight_stride % 16 || !aligned(act, 16) ||
+      !aligned(weight, 16) || !aligned(out, 16))
+    return fail(CONVROT_ERR_INVALID,
+                "W8A8 operands need 16-byte aligned rows that cover K rounded up to 16 (K=%lld, strides %lld and %lld)",
+                (long long)K, (long long)act_stride, (long long)weight_stride);
+  if (act_stride > kMaxInt8Stride || weight_stride > kMaxInt8Stride)
+    return fail(CONVROT_ERR_UNSUPPORTED, "W8A8 row strides are limited to %lld bytes", (long long)kMaxInt8Stride);
+  convrot::GatedResidual gr{};
+  if (residual)
+    if (int rc = check_residual(residual, gate, gate_stride, rows_per_gate, M, N, &gr)) return rc;
+  return launch_status(convrot::launch_w8a8_gemm(act, act_stride, xscales, weight, weight_stride, wscales, bias, M, N,
+                                                 K, out, out_dtype, (hipStream_t)stream, gr),
+                       "convrot_w8a8_gemm");
+}
+
+int convrot_layer_norm(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride, const void* gain,
+                       const void* shift, int param_dtype, int plus_one, int64_t rows_per_vector, float eps,
+                       void* out, float* mean, float* rstd, void* stream) {
+  if (int rc = check_rows("layer norm", x, dtype, rows, features, x_stride, kMaxFeatures)) return rc;
+  if (int rc = check_params(gain, shift, dtype, param_dtype, rows, rows_per_vector)) return rc;
+  if (!mean != !rstd) return fail(CONVROT_ERR_INVALID, "mean and rstd come together");
+  if (rows == 0 || features == 0) return ok();
+  if (!out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(out, dtype == CONVROT_DTYPE_F32 ? 4 : 2)) return fail(CONVROT_ERR_INVALID, "out is not aligned to its type");
+  return launch_status(convrot::launch_layer_norm(x, dtype, rows, features, x_stride, gain, shift, param_dtype,
+                                                  plus_one != 0, rows_per_vector, eps, out, mean, rstd,
+                                                  (hipStream_t)stream),
+                       "convrot_layer_norm");
+}
+
+int convrot_layer_norm_int8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride,
+                            const void* gain, const void* shift, int param_dtype, int plus_one,
+                            int64_t rows_per_vector, float eps, int8_t* codes, int64_t codes_stride, float* scales,
+                            void* stream) {
+  if (int rc = check_rows("layer norm", x, dtype, rows, features, x_stride, kMaxFeatures)) return rc;
+  if (int rc = check_params(gain, shift, dtype, param_dtype, rows, rows_per_vector)) return rc;
+  if (rows == 0 || features == 0) return ok();
+  if (int rc = check_codes(codes, codes_stride, features, scales)) return rc;
+  return launch_status(convrot::launch_layer_norm_int8(x, dtype, rows, features, x_stride, gain, shift, param_dtype,
+                                                       plus_one != 0, rows_per_vector, eps, codes, codes_stride,
+                                                       scales, (hipStream_t)stream),
+                       "convrot_layer_norm_int8");
+}
+
+int64_t convrot_layer_norm_workspace_bytes(int64_t rows, int64_t features, int64_t rows_per_vector) {
+  if (rows <= 0 || features <= 0 || rows_per_vector <= 0 || rows % rows_per_vector) return 0;
+  return (rows / rows_per_vector) * convrot::layer_norm_parts(rows, features, rows_per_vector) * 2 * features * 4;
+}
+
+int convrot_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* mean,
+                                const float* rstd, int dtype, int64_t rows, int64_t features, const void* gain,
+                                int param_dtype, int plus_one, int64_t rows_per_vector, void* dx, void* dgain,
+                                void* dshift, void* workspace, int64_t workspace_bytes, void* stream) {
+  constexpr int64_t most = 32768;  // a thread keeps the gradient sums of 32 features
+  if (int rc = check_rows("the layer norm's gradient", x, dtype, rows, features, x_stride, most)) return rc;
+  if (int rc = check_rows("the layer norm's gradient", dy, dtype, rows, features, dy_stride, most)) return rc;
+  if (rows_per_vector <= 0) return fail(CONVROT_ERR_INVALID, "rows_per_vector must be positive, got %lld", (long long)rows_per_vector);
+  if (int rc = check_params(gain, nullptr, dtype, param_dtype, rows, rows_per_vector)) return rc;
+  if (rows == 0 || features == 0) return ok();
+  if (!mean || !rstd || !dx) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(dx, dtype == CONVROT_DTYPE_F32 ? 4 : 2)) return fail(CONVROT_ERR_INVALID, "dx is not aligned to its type");
+  if ((dgain || dshift) &&
+      (!workspace || !aligned(workspace, 16) ||
+       workspace_bytes < convrot_layer_norm_workspace_bytes(rows, features, rows_per_vector)))
+    return fail(CONVROT_ERR_INVALID, "the layer norm's gradient needs a 16-byte aligned workspace of %lld bytes, got %lld",
+                (long long)convrot_layer_norm_workspace_bytes(rows, features, rows_per_vector),
+                (long long)workspace_bytes);
+  return launch_status(convrot::launch_layer_norm_backward(dy, dy_stride, x, x_stride, mean, rstd, dtype, rows,
+                                                           features, gain, param_dtype, plus_one != 0,
+                                                           rows_per_vector, dx, dgain, dshift, (float*)workspace,
+                                                           (hipStream_t)stream),
+                       "convrot_layer_norm_backward");
+}
+
+int convrot_axes_table(const void* positions, int kind, int64_t rows, int axes, const int* dims, double theta,
+                       float* out, void* stream) {
+  if (kind < CONVROT_POS_F32 || kind > CONVROT_POS_I64) return fail(CONVROT_ERR_INVALID, "unknown position type %d", kind);
+  if (axes < 1 || axes > 8 || !dims) return fail(CONVROT_ERR_INVALID, "positions need 1 to 8 axes, got %d", axes);
+  int64_t pairs = 0;
+  for (int a = 0; a < axes; ++a) {
+    if (dims[a] < 0 || dims[a] % 2 || dims[a] > 65536)
+      return fail(CONVROT_ERR_INVALID, "an axis turns an even number of features, got %d", dims[a]);
+    pairs += dims[a] / 2;
+  }
+  if (!(theta > 0.0)) return fail(CONVROT_ERR_INVALID, "theta must be positive");
+  if (rows < 0) return fail(CONVROT_ERR_INVALID, "invalid shape rows=%lld", (long long)rows);
+  if (rows == 0 || pairs == 0) return ok();
+  if (rows > kMaxRows || rows * pairs > (int64_t(1) << 38)) return fail(CONVROT_ERR_UNSUPPORTED, "too many positions");
+  if (!positions || !out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  return launch_status(convrot::launch_axes_table(positions, kind, rows, axes, dims, theta, out, (hipStream_t)stream),
+                       "convrot_axes_table");
+}
+
+int convrot_qk_rotary(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, int dtype,
+                      int batch, int q_heads, int k_heads, int64_t length, int dim, const float* table, int pairs,
+                      int64_t table_batch_stride, const void* q_weight, const void* k_weight, int weight_dtype,
+                      float eps, int interleaved, void* stream) {
+  if (int rc = check_rotary(dtype, batch, q_heads, k_heads, length, dim, table, pairs, table_batch_stride, q_weight,
+                            k_weight, weight_dtype, strides))
+    return rc;
+  if (batch == 0 || length == 0 || dim == 0 || q_heads + k_heads == 0) return ok();
+  if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)))
+    return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  const convrot::RotaryShape sh{dtype,    batch,    q_heads,      k_heads, length,          dim, pairs, table, table_batch_stride,
+                                q_weight, k_weight, weight_dtype, eps,     interleaved != 0};
+  return launch_status(convrot::launch_qk_rotary(sh, q, k, q_out, k_out, strides, (hipStream_t)stream),
+                       "convrot_qk_rotary");
+}
+
+int64_t convrot_qk_rotary_workspace_bytes(int dim) {
+  return dim > 0 && dim <= 512 ? convrot::qk_rotary_workspace_bytes(dim) : 0;
+}
+
+int convrot_qk_rotary_backward(const void* dq, const void* dk, const void* q, const void* k, void* q_grad,
+                               void* k_grad, void* q_weight_grad, void* k_weight_grad, const int64_t* strides,
+                               int dtype, int batch, int q_heads, int k_heads, int64_t length, int dim,
+                               const float* table, int pairs, int64_t table_batch_stride, const void* q_weight,
+                               const void* k_weight, int weight_dtype, float eps, int interleaved, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  if (int rc = check_rotary(dtype, batch, q_heads, k_heads, length, dim, table, pairs, table_batch_stride, q_weight,
+                            k_weight, weight_dtype, strides))
+    return rc;
+  if ((q_weight_grad && !q_weight) || (k_weight_grad && !k_weight))
+    return fail(CONVROT_ERR_INVALID, "a weight's gradient needs the weight");
+  if (batch == 0 || length == 0 || dim == 0 || q_heads + k_heads == 0) return ok();
+  if ((q_heads && (!dq || !q_grad || (q_weight && !q))) || (k_heads && (!dk || !k_grad || (k_weight && !k))))
+    return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if ((q_weight_grad || k_weight_grad) &&
+      (!workspace || !aligned(workspace, 16) || workspace_bytes < convrot_qk_rotary_workspace_bytes(dim)))
+    return fail(CONVROT_ERR_INVALID, "the rotary gradient needs a 16-byte aligned workspace of %lld bytes, got %lld",
+                (long long)convrot_qk_rotary_workspace_bytes(dim), (long long)workspace_bytes);
+  const convrot::RotaryShape sh{dtype,    batch,    q_heads,      k_heads, length,          dim, pairs, table, table_batch_stride,
+                                q_weight, k_weight, weight_dtype, eps,     interleaved != 0};
+  return launch_status(convrot::launch_qk_rotary_backward(sh, dq, dk, q, k, q_grad, k_grad, q_weight_grad,
+                                                          k_weight_grad, strides, (float*)workspace,
+                                                          (hipStream_t)stream),
+                       "convrot_qk_rotary_backward");
 }
 
 }  // extern "C"

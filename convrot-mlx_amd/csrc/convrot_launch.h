@@ -31,6 +31,7 @@ enum TuneKey : int {
   kTuneRowsCfg,          // few-row linear: weight tiles a workgroup (1, 2, 3, 5), or 16: one tile on 16 waves
   kTuneMidmCfg,          // W4A4 kernel of blocked codes: 10 * row tiles + weight tiles of a workgroup
   kTuneFp6Split,         // FP6 256x256 tiles past the whole rounds: as 1, 2 or 4 workgroups
+  kTuneW8a8Tile,         // W8A8 tile: bm | bn << 10, 0 the few-row kernel
   kTuneCount
 };
 int tuning(TuneKey key);
@@ -41,6 +42,7 @@ int tuning(TuneKey key);
 bool w4a4_tile_known(int bm, int bn, int wm, int wn, int stages);
 bool fp6_tile_known(int bm, int bn);
 bool w4a16_tile_known(int bm, int bn);
+bool w8a8_tile_known(int bm, int bn);  // 0 x 0: the few-row kernel
 
 // The FP6 W4A4 tile the plan (and the fp6_tile override) picks for M x N on operand
 // blocks, and on compact weights, where each 256 x 256 tile past the whole rounds
@@ -181,5 +183,54 @@ hipError_t launch_weight_fp6(const uint8_t* cdna4, uint8_t* fp6, int64_t N, int6
 // zeroed, then set to 1 if a code is -8 (no compact field: those blocks are void).
 hipError_t launch_weight_fp6c(const uint8_t* cdna4, uint8_t* fp6c, int* minus8, int64_t N, int64_t K,
                               hipStream_t stream);
+
+// ---- 8-bit linears (gemm_w8a8.hip), layer norm and the 8-bit quantizer
+// (norm.hip), rotary positions (rotary.hip)
+
+hipError_t launch_w8a8_gemm(const int8_t* act, int64_t lda, const float* xscales, const int8_t* weight, int64_t ldw,
+                            const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K, void* out,
+                            int out_dtype, hipStream_t stream, const GatedResidual& gr);
+
+hipError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride, int8_t* codes,
+                                int64_t codes_stride, float* scales, hipStream_t stream);
+
+hipError_t launch_layer_norm(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride, const void* gain,
+                             const void* shift, int param_dtype, int plus_one, int64_t rows_per_vector, float eps,
+                             void* out, float* mean, float* rstd, hipStream_t stream);
+
+hipError_t launch_layer_norm_int8(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride,
+                                  const void* gain, const void* shift, int param_dtype, int plus_one,
+                                  int64_t rows_per_vector, float eps, int8_t* codes, int64_t codes_stride,
+                                  float* scales, hipStream_t stream);
+
+// Workgroups that share the rows of one vector in the backward kernel: the
+// workspace holds vectors * parts * 2 * K floats.
+int layer_norm_parts(int64_t rows, int64_t K, int64_t rows_per_vector);
+hipError_t launch_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                      const float* mean, const float* rstd, int dtype, int64_t rows, int64_t K,
+                                      const void* gain, int param_dtype, int plus_one, int64_t rows_per_vector,
+                                      void* dx, void* dgain, void* dshift, float* workspace, hipStream_t stream);
+
+struct RotaryShape {
+  int dtype, batch, q_heads, k_heads;
+  int64_t length;
+  int dim, pairs;
+  const float* table;
+  int64_t table_batch_stride;
+  const void *q_weight, *k_weight;
+  int weight_dtype;
+  float eps;
+  bool interleaved;
+};
+// strides: batch, head and token of q, k, q_out, k_out (backward: dq, dk, q, k, q_grad, k_grad)
+hipError_t launch_qk_rotary(const RotaryShape& shape, const void* q, const void* k, void* q_out, void* k_out,
+                            const int64_t* strides, hipStream_t stream);
+int64_t qk_rotary_workspace_bytes(int dim);
+hipError_t launch_qk_rotary_backward(const RotaryShape& shape, const void* dq, const void* dk, const void* q,
+                                     const void* k, void* q_grad, void* k_grad, void* q_weight_grad,
+                                     void* k_weight_grad, const int64_t* strides, float* workspace,
+                                     hipStream_t stream);
+hipError_t launch_axes_table(const void* positions, int kind, int64_t rows, int axes, const int* dims, double theta,
+                             float* out, hipStream_t stream);
 
 }  // namespace convrot

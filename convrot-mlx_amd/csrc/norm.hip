@@ -1,0 +1,472 @@
+// Layer norm, its gradient, and the quantizer of activation rows to 8 bits.
+//
+// Forward, row by row, in float32:
+//   mean = sum(x) / K,  rstd = 1 / sqrt(sum((x - mean)^2) / K + eps),
+//   y = (x - mean) rstd g + b,
+// with g, b a weight and bias of all rows, or g = 1 + scale[v], b = shift[v] of
+// the row's group v (the adaptive norm of a diffusion transformer); y is
+// rounded once.  The row stays in registers between the sums, so it is read
+// once; the second sum takes differences from the mean (no cancellation).
+//
+// Backward, with u = (x - mean) rstd and h = dy g:
+//   dx = rstd (h - sum(h) / K - u sum(h u) / K),  dg = sum_rows dy u,  db = sum_rows dy.
+//
+// Quantizer: a = max |x|, codes = round(x (127 / a)) to nearest even,
+// scale = a (1 / 127).  With the norm in front, the normalized row goes to
+// codes from registers.  A row that holds a NaN or an infinity gets the scale
+// NaN and codes 0, so every product of it is NaN; a row below 2^-100 counts as
+// zero (codes 0, scale 0), where 127 / a would overflow.
+#include "convrot_launch.h"
+#include "row_device.h"
+
+namespace convrot {
+namespace {
+
+enum RowOp : int { kNormOut = 0, kNormCodes = 1, kCodes = 2 };
+
+constexpr float kTiny = 0x1p-100f;
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+// Sum over a team of T threads (T / 64 waves, `red` its own floats), in every
+// thread.  Every thread of the workgroup calls it.
+template <int T, int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float (*red)[T / 64], int team_wave) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[i][team_wave] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = red[i][0];
+#pragma unroll
+      for (int w = 1; w < T / 64; ++w) v[i] += red[i][w];
+    }
+  }
+}
+
+// One row a team; a workgroup is one team, or four one-wave teams.
+template <int DT, int T, int C, bool VEC, int OP>
+__global__ __launch_bounds__(T == 64 ? 256 : T) void row_kernel(
+    const void* __restrict__ x, int64_t rows, int K, int64_t x_stride, const void* __restrict__ gain,
+    const void* __restrict__ shift, int param_dtype, int plus_one, int64_t rows_per_vector, float eps,
+    void* __restrict__ out, int64_t out_stride, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+    float* __restrict__ scales) {
+  typedef typename Elem<DT>::T E;
+  constexpr int TEAMS = T == 64 ? 4 : 1, W = T / 64;
+  __shared__ float red[3][1][W];
+  __shared__ uint32_t redmax[W];
+  const int t = threadIdx.x % T, wave = t >> 6;
+  const int64_t row = (int64_t)blockIdx.x * TEAMS + (TEAMS > 1 ? threadIdx.x / T : 0);
+  if (TEAMS > 1 && row >= rows) return;  // one-wave teams: no barrier below
+
+  float v[C][8];
+  const E* xr = (const E*)x + row * x_stride;
+#pragma unroll
+  for (int c = 0; c < C; ++c) load_chunk<DT, T, C, VEC>(xr, K, t, c, v[c]);
+
+  if constexpr (OP != kCodes) {
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[0] += v[c][j];
+    team_sum<T>(s, red[0], wave);
+    const float mean = s[0] / (float)K;
+    float q[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[c][j] -= mean;
+        const float sq = v[c][j] * v[c][j];
+        q[0] += feature_of<T, C, VEC>(t, c, j) < K ? sq : 0.0f;
+      }
+    team_sum<T>(q, red[1], wave);
+    const float rstd = 1.0f / sqrtf(q[0] / (float)K + eps);
+    if (t == 0 && mean_out) mean_out[row] = mean, rstd_out[row] = rstd;
+    const uint32_t param_row = rows_per_vector > 0 ? (uint32_t)row / (uint32_t)rows_per_vector : 0;
+    const size_t psize = param_dtype == kF32 ? 4 : 2;
+    const char* gr = gain ? (const char*)gain + (size_t)param_row * K * psize : nullptr;
+    const char* br = shift ? (const char*)shift + (size_t)param_row * K * psize : nullptr;
+    const float one = plus_one ? 1.0f : 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float g[8], b[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = 1.0f, b[j] = 0.0f;
+      if (gr) {
+        load_param<DT, T, C, VEC>(gr, param_dtype, K, t, c, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] += one;
+      }
+      if (br) load_param<DT, T, C, VEC>(br, param_dtype, K, t, c, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[c][j] = v[c][j] * rstd * g[j] + b[j];
+    }
+  }
+
+  if constexpr (OP == kNormOut) {
+    E* o = (E*)out + row * out_stride;
+#pragma unroll
+    for (int c = 0; c < C; ++c) store_chunk<DT, T, C, VEC>(o, K, t, c, v[c]);
+  } else {
+    // As unsigned words, |x| orders infinity above every number and NaN above infinity.
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t a = __builtin_bit_cast(uint32_t, v[c][j]) & 0x7fffffffu;
+        most = max(most, feature_of<T, C, VEC>(t, c, j) < K ? a : 0u);
+      }
+    most = wave_max(most);
+    if constexpr (T > 64) {
+      if ((t & 63) == 0) redmax[wave] = most;
+      __syncthreads();
+      most = redmax[0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) most = max(most, redmax[w]);
+    }
+    const float a = __builtin_bit_cast(float, most);
+    const bool finite = most < kInfBits, zero = a < kTiny;
+    const float inv = finite && !zero ? 127.0f / a : 0.0f;
+    if (t == 0) scales[row] = !finite ? __builtin_nanf("") : zero ? 0.0f : a * (1.0f / 127.0f);
+    int8_t* o = (int8_t*)out + row * out_stride;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      int q[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // |x inv| <= 127 up to its last bit, which the rounding drops; a row that is not finite gets zeros
+        const bool in = feature_of<T, C, VEC>(t, c, j) < K;
+        q[j] = in && finite ? (int)rintf(v[c][j] * inv) : 0;
+      }
+      // columns K .. stride - 1 are zero
+      if constexpr (VEC) {
+        const int f = feature_of<T, C, VEC>(t, c, 0);
+        if (f < out_stride) {
+          uint32_t w[2] = {0, 0};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j / 4] |= (uint32_t)(q[j] & 0xff) << (8 * (j & 3));
+          *(uint2*)(o + f) = make_uint2(w[0], w[1]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int f = feature_of<T, C, VEC>(t, c, j);
+          if (f < out_stride) o[f] = (int8_t)q[j];
+        }
+      }
+    }
+  }
+}
+
+struct RowArgs {
+  const void* x;
+  int64_t rows, K, x_stride;
+  const void *gain, *shift;
+  int param_dtype, plus_one;
+  int64_t rows_per_vector;
+  float eps;
+  void* out;
+  int64_t out_stride;
+  float *mean, *rstd, *scales;
+};
+
+template <int DT, int OP, int T, int C, bool VEC>
+void run_rows(const RowArgs& a, hipStream_t stream) {
+  constexpr int TEAMS = T == 64 ? 4 : 1;
+  row_kernel<DT, T, C, VEC, OP><<<dim3((unsigned)((a.rows + TEAMS - 1) / TEAMS)), dim3(T * TEAMS), 0, stream>>>(
+      a.x, a.rows, (int)a.K, a.x_stride, a.gain, a.shift, a.param_dtype, a.plus_one, a.rows_per_vector, a.eps, a.out,
+      a.out_stride, a.mean, a.rstd, a.scales);
+}
+
+template <int DT, int OP>
+hipError_t pick_rows(const RowArgs& a, bool vec, hipStream_t stream) {
+  const int64_t k = OP == kNormOut ? a.K : a.out_stride;  // codes are written up to their stride
+  if (vec) {
+    if (k <= 512) run_rows<DT, OP, 64, 1, true>(a, stream);
+    else if (k <= 1024) run_rows<DT, OP, 64, 2, true>(a, stream);
+    else if (k <= 2048) run_rows<DT, OP, 256, 1, true>(a, stream);
+    else if (k <= 4096) run_rows<DT, OP, 256, 2, true>(a, stream);
+    else if (k <= 6144) run_rows<DT, OP, 256, 3, true>(a, stream);
+    else if (k <= 8192) run_rows<DT, OP, 256, 4, true>(a, stream);
+    else if (k <= 16384) run_rows<DT, OP, 1024, 2, true>(a, stream);
+    else if (k <= 32768) run_rows<DT, OP, 1024, 4, true>(a, stream);
+    else run_rows<DT, OP, 1024, 8, true>(a, stream);
+  } else {
+    if (k <= 2048) run_rows<DT, OP, 256, 1, false>(a, stream);
+    else if (k <= 8192) run_rows<DT, OP, 256, 4, false>(a, stream);
+    else if (k <= 32768) run_rows<DT, OP, 1024, 4, false>(a, stream);
+    else run_rows<DT, OP, 1024, 8, false>(a, stream);
+  }
+  return hipGetLastError();
+}
+
+template <int OP>
+hipError_t launch_rows(const RowArgs& a, int dtype, hipStream_t stream) {
+  const size_t es = dtype == kF32 ? 4 : 2;
+  auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+  bool vec = a.K % 8 == 0 && al(a.x) && (a.x_stride * es) % 16 == 0 && al(a.out) && al(a.gain) && al(a.shift);
+  if (OP == kNormOut) vec = vec && (a.out_stride * es) % 16 == 0;
+  else vec = vec && a.out_stride % 8 == 0;
+  switch (dtype) {
+    case kF32: return pick_rows<kF32, OP>(a, vec, stream);
+    case kF16: return pick_rows<kF16, OP>(a, vec, stream);
+    default: return pick_rows<kBF16, OP>(a, vec, stream);
+  }
+}
+
+// ---- backward
+//
+// A workgroup of 1024 threads is TEAMS teams that walk the rows of one group
+// (vector) of the norm's parameters; each thread keeps the sums of dg and db of
+// its features in registers, the teams' sums are added through LDS at the end
+// and stored as one partial of the workgroup.  A second kernel adds the
+// partials in order, so gradients repeat bit for bit.
+
+template <int DT, int T, int C, bool VEC>
+__global__ __launch_bounds__(1024) void norm_backward_kernel(
+    const void* __restrict__ dy, int64_t dy_stride, const void* __restrict__ x, int64_t x_stride,
+    const float* __restrict__ mean, const float* __restrict__ rstd, int64_t rows, int K,
+    const void* __restrict__ gain, int param_dtype, int plus_one, int64_t rows_per_vector, int parts,
+    void* __restrict__ dx, float* __restrict__ partial) {
+  typedef typename Elem<DT>::T E;
+  constexpr int TEAMS = 1024 / T, W = T / 64;
+  __shared__ float red[2][TEAMS][2][W];
+  extern __shared__ float sums[];  // [2][K] of the teams' sums, where TEAMS > 1
+  const int team = threadIdx.x / T, t = threadIdx.x % T, wave = t >> 6;
+  const int64_t vector = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int64_t r0 = vector * rows_per_vector, r1 = r0 + rows_per_vector;
+  const size_t psize = param_dtype == kF32 ? 4 : 2;
+  const char* gr = gain ? (const char*)gain + (size_t)vector * K * psize : nullptr;
+
+  float dg[C][8], db[C][8], g[C][8];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dg[c][j] = db[c][j] = 0.0f, g[c][j] = 1.0f;
+    if (gr) {
+      load_param<DT, T, C, VEC>(gr, param_dtype, K, t, c, g[c]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[c][j] += plus_one ? 1.0f : 0.0f;
+    }
+  }
+
+  // every team makes as many steps (the barriers below): rows past the end count as zeros
+  int flip = 0;
+  for (int64_t base = r0 + part * TEAMS; base < r1; base += (int64_t)parts * TEAMS) {
+    const int64_t row = base + team;
+    const bool live = row < r1;
+    float u[C][8], d[C][8];
+    float s[2] = {0.0f, 0.0f};
+    float rs = 0.0f;
+    if (live) {
+      const E* xr = (const E*)x + row * x_stride;
+      const E* dr = (const E*)dy + row * dy_stride;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        load_chunk<DT, T, C, VEC>(xr, K, t, c, u[c]);
+        load_chunk<DT, T, C, VEC>(dr, K, t, c, d[c]);
+      }
+      const float mu = mean[row];
+      rs = rstd[row];
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = feature_of<T, C, VEC>(t, c, j) < K;
+          u[c][j] = in ? (u[c][j] - mu) * rs : 0.0f;  // d is zero past the row
+          db[c][j] += d[c][j];
+          dg[c][j] += d[c][j] * u[c][j];
+          d[c][j] *= g[c][j];
+          s[0] += d[c][j];
+          s[1] += d[c][j] * u[c][j];
+        }
+    }
+    team_sum<T>(s, red[flip][team], wave);
+    flip ^= 1;  // the next step's sums go elsewhere: one barrier a step is enough
+    if (live) {
+      const float m0 = s[0] / (float)K, m1 = s[1] / (float)K;
+      E* o = (E*)dx + row * (int64_t)K;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[c][j] = rs * (d[c][j] - m0 - u[c][j] * m1);
+        store_chunk<DT, T, C, VEC>(o, K, t, c, d[c]);
+      }
+    }
+  }
+
+  if (!partial) return;
+  if constexpr (TEAMS > 1) {
+    // team by team, in order
+    for (int i = TEAMS - 1; i > 0; --i) {
+      __syncthreads();
+      if (team == i) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int f = feature_of<T, C, VEC>(t, c, j);
+            if (f < K) {
+              sums[f] = i == TEAMS - 1 ? dg[c][j] : sums[f] + dg[c][j];
+              sums[K + f] = i == TEAMS - 1 ? db[c][j] : sums[K + f] + db[c][j];
+            }
+          }
+      }
+    }
+    __syncthreads();
+    if (team != 0) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int f = feature_of<T, C, VEC>(t, c, j);
+        if (f < K) dg[c][j] += sums[f], db[c][j] += sums[K + f];
+      }
+  }
+  float* p = partial + (size_t)blockIdx.x * 2 * K;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    store_chunk<kF32, T, C, VEC>(p, K, t, c, dg[c]);
+    store_chunk<kF32, T, C, VEC>(p + K, K, t, c, db[c]);
+  }
+}
+
+// out[v][f] = sum over the parts of partial[v][part][which][f], f < K: 16
+// threads a feature each add every 16th part, then their sums in order.
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float* __restrict__ partial, int parts, int K,
+                                                         void* __restrict__ dgain, void* __restrict__ dshift,
+                                                         int dtype) {
+  __shared__ float red[16][64];
+  const int col = threadIdx.x & 63, lot = threadIdx.x >> 6;
+  const int blocks = (2 * K + 63) / 64;  // of one vector
+  const int64_t vector = blockIdx.x / blocks;
+  const int f = (blockIdx.x % blocks) * 64 + col;  // of 2 K: dg then db
+  float s = 0.0f;
+  if (f < 2 * K) {
+    const float* p = partial + (size_t)vector * parts * 2 * K + f;
+#pragma unroll 4
+    for (int i = lot; i < parts; i += 16) s += p[(size_t)i * 2 * K];
+  }
+  red[lot][col] = s;
+  __syncthreads();
+  if (lot != 0 || f >= 2 * K) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[i][col];
+  void* o = f < K ? dgain : dshift;
+  if (!o) return;
+  const int64_t at = vector * K + (f < K ? f : f - K);
+  if (dtype == kF32) store_out<kF32>(o, at, s);
+  else if (dtype == kF16) store_out<kF16>(o, at, s);
+  else store_out<kBF16>(o, at, s);
+}
+
+struct BackwardArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const float *mean, *rstd;
+  int64_t rows, K;
+  const void* gain;
+  int param_dtype, plus_one;
+  int64_t rows_per_vector;
+  int parts;
+  void* dx;
+  float* partial;
+};
+
+// Threads a row takes in the backward kernel.
+int backward_team(int64_t K) { return K <= 512 ? 64 : K <= 1024 ? 128 : K <= 6144 ? 256 : K <= 12288 ? 512 : 1024; }
+
+template <int DT, int T, int C, bool VEC>
+hipError_t run_backward(const BackwardArgs& a, hipStream_t stream) {
+  const size_t lds = T < 1024 && a.partial ? (size_t)a.K * 8 : 0;
+  auto kernel = norm_backward_kernel<DT, T, C, VEC>;
+  if (lds > 48 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  const int64_t vectors = a.rows / a.rows_per_vector;
+  kernel<<<dim3((unsigned)(vectors * a.parts)), dim3(1024), lds, stream>>>(
+      a.dy, a.dy_stride, a.x, a.x_stride, a.mean, a.rstd, a.rows, (int)a.K, a.gain, a.param_dtype, a.plus_one,
+      a.rows_per_vector, a.parts, a.dx, a.partial);
+  return hipGetLastError();
+}
+
+template <int DT, bool VEC>
+hipError_t pick_backward(const BackwardArgs& a, hipStream_t s) {
+  const int64_t k = a.K;
+  if (k <= 512) return run_backward<DT, 64, 1, VEC>(a, s);
+  if (k <= 1024) return run_backward<DT, 128, 1, VEC>(a, s);
+  if (k <= 2048) return run_backward<DT, 256, 1, VEC>(a, s);
+  if (k <= 4096) return run_backward<DT, 256, 2, VEC>(a, s);
+  if (k <= 6144) return run_backward<DT, 256, 3, VEC>(a, s);
+  if (k <= 8192) return run_backward<DT, 512, 2, VEC>(a, s);
+  if (k <= 12288) return run_backward<DT, 512, 3, VEC>(a, s);
+  if (k <= 16384) return run_backward<DT, 1024, 2, VEC>(a, s);
+  return run_backward<DT, 1024, 4, VEC>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride, int8_t* codes,
+                                int64_t codes_stride, float* scales, hipStream_t stream) {
+  RowArgs a{x, rows, K, x_stride, nullptr, nullptr, kF32, 0, 0, 0.0f, codes, codes_stride, nullptr, nullptr, scales};
+  return launch_rows<kCodes>(a, dtype, stream);
+}
+
+hipError_t launch_layer_norm(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride, const void* gain,
+                             const void* shift, int param_dtype, int plus_one, int64_t rows_per_vector, float eps,
+                             void* out, float* mean, float* rstd, hipStream_t stream) {
+  RowArgs a{x, rows, K, x_stride, gain, shift, param_dtype, plus_one, rows_per_vector, eps, out, K, mean, rstd, nullptr};
+  return launch_rows<kNormOut>(a, dtype, stream);
+}
+
+hipError_t launch_layer_norm_int8(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride,
+                                  const void* gain, const void* shift, int param_dtype, int plus_one,
+                                  int64_t rows_per_vector, float eps, int8_t* codes, int64_t codes_stride,
+                                  float* scales, hipStream_t stream) {
+  RowArgs a{x,   rows,  K,            x_stride, gain,    shift,  param_dtype, plus_one, rows_per_vector,
+            eps, codes, codes_stride, nullptr,  nullptr, scales};
+  return launch_rows<kNormCodes>(a, dtype, stream);
+}
+
+// Workgroups that share the rows of one vector: a workgroup a CU in all, and
+// no more than the rows feed.
+int layer_norm_parts(int64_t rows, int64_t K, int64_t rows_per_vector) {
+  const int64_t teams = 1024 / backward_team(K), vectors = rows / rows_per_vector;
+  const int64_t steps = (rows_per_vector + teams - 1) / teams;
+  int64_t parts = (256 + vectors - 1) / vectors;
+  if (parts > steps) parts = steps;
+  return (int)(parts < 1 ? 1 : parts);
+}
+
+hipError_t launch_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                      const float* mean, const float* rstd, int dtype, int64_t rows, int64_t K,
+                                      const void* gain, int param_dtype, int plus_one, int64_t rows_per_vector,
+                                      void* dx, void* dgain, void* dshift, float* workspace, hipStream_t stream) {
+  BackwardArgs a{dy, dy_stride, x, x_stride, mean, rstd, rows, K, gain, param_dtype, plus_one, rows_per_vector,
+                 layer_norm_parts(rows, K, rows_per_vector), dx, (dgain || dshift) ? workspace : nullptr};
+  const size_t es = dtype == kF32 ? 4 : 2;
+  auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+  const bool vec = K % 8 == 0 && al(dy) && al(x) && al(dx) && al(gain) && (dy_stride * es) % 16 == 0 &&
+                   (x_stride * es) % 16 == 0;
+  hipError_t e;
+  if (dtype == kF32) e = vec ? pick_backward<kF32, true>(a, stream) : pick_backward<kF32, false>(a, stream);
+  else if (dtype == kF16) e = vec ? pick_backward<kF16, true>(a, stream) : pick_backward<kF16, false>(a, stream);
+  else e = vec ? pick_backward<kBF16, true>(a, stream) : pick_backward<kBF16, false>(a, stream);
+  if (e != hipSuccess || !a.partial) return e;
+  const int64_t vectors = rows / rows_per_vector;
+  sum_parts_kernel<<<dim3((unsigned)(vectors * ((2 * K + 63) / 64))), dim3(1024), 0, stream>>>(
+      a.partial, a.parts, (int)K, dgain, dshift, param_dtype);
+  return hipGetLastError();
+}
+
+}  // namespace convrot

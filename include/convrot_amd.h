@@ -424,6 +424,119 @@ int convrot_w4a4_gemm_fp6_compact(const uint8_t* act6, const float* xscales, con
                                   const void* residual, const void* gate, int64_t gate_stride,
                                   int64_t rows_per_gate, void* out, int out_dtype, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Operators around the quantized linears.  No counterpart in the reference,
+ * whose example model runs them as separate array operations.
+ * Rows, features and lengths of zero are no error: nothing is launched.
+ */
+
+/*
+ * 8-bit codes of activation rows, one scale a row:
+ *   a = max |x|, codes = round_to_even(x * (127 / a)), scale = a * (1 / 127), in float32.
+ * A row holding a NaN or an infinity gets codes 0 and the scale NaN (its
+ * products are NaN); a row whose a is below 2^-100 gets codes 0 and scale 0.
+ * x [rows, features] with rows x_stride elements apart (any alignment of the
+ * element type); codes int8 with rows codes_stride bytes apart, a multiple of
+ * 16 of at least features, the columns past features are written as zeros;
+ * codes 16-byte aligned.  features <= 65536.
+ */
+int convrot_quantize_int8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride,
+                          int8_t* codes, int64_t codes_stride, float* scales, void* stream);
+
+/*
+ * W8A8 GEMM: out[m][n] = dt(((float(sum_k act[m][k] * weight[n][k]) * xscales[m]) * wscales[n]) + bias[n]),
+ * the integer sum exact, optionally followed by the gated residual of
+ * convrot_w4a4_gemm_residual (residual NULL: none; gate NULL: residual + linear).
+ * act int8 [M, K] and weight int8 [N, K], row-major with row strides in bytes
+ * (multiples of 16, at most 2^22), 16-byte aligned.  Where K is no multiple of
+ * 16, a stride covers the next one, and the weight's bytes from K to there are
+ * zero (the activations' may be anything).  K <= 65536.  out [M, N] contiguous.
+ */
+int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscales, const int8_t* weight,
+                      int64_t weight_stride, const float* wscales, const float* bias, int64_t M, int64_t N,
+                      int64_t K, const void* residual, const void* gate, int64_t gate_stride,
+                      int64_t rows_per_gate, void* out, int out_dtype, void* stream);
+
+/*
+ * Layer norm: out = dt((x - mean) * rstd * g + b), in float32, rounded once,
+ * rstd = 1 / sqrt(mean((x - mean)^2) + eps).  gain and shift (either may be
+ * NULL) are [V, features] of param_dtype (the activations' or float32); row r
+ * takes vector r / rows_per_vector; g = gain, or 1 + gain with plus_one (the
+ * adaptive norm's scale).  x rows x_stride elements apart, out [rows, features]
+ * contiguous.  mean and rstd (float32 [rows], both or neither) are what the
+ * backward pass reads.  features <= 65536.
+ */
+int convrot_layer_norm(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride, const void* gain,
+                       const void* shift, int param_dtype, int plus_one, int64_t rows_per_vector, float eps,
+                       void* out, float* mean, float* rstd, void* stream);
+
+/* The same norm with its result, unrounded, as convrot_quantize_int8's codes and scales. */
+int convrot_layer_norm_int8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride,
+                            const void* gain, const void* shift, int param_dtype, int plus_one,
+                            int64_t rows_per_vector, float eps, int8_t* codes, int64_t codes_stride, float* scales,
+                            void* stream);
+
+/*
+ * Gradients of convrot_layer_norm: with u = (x - mean) rstd and h = dy g,
+ *   dx = rstd (h - mean(h) - u mean(h u)),  dgain = sum over a vector's rows of dy u,  dshift = sum of dy.
+ * dx [rows, features] contiguous, of the activations' dtype; dgain and dshift
+ * [V, features] of param_dtype, V = rows / rows_per_vector (exact; either may be
+ * NULL).  workspace: convrot_layer_norm_workspace_bytes bytes, 16-byte aligned, of any content
+ * (not needed when both are NULL).  Sums are float32 in a fixed order.  features <= 32768.
+ */
+int64_t convrot_layer_norm_workspace_bytes(int64_t rows, int64_t features, int64_t rows_per_vector);
+int convrot_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                const float* mean, const float* rstd, int dtype, int64_t rows, int64_t features,
+                                const void* gain, int param_dtype, int plus_one, int64_t rows_per_vector, void* dx,
+                                void* dgain, void* dshift, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Cosines and sines of positions with several axes (time, height, width):
+ * positions [rows, axes] of a CONVROT_POS_* type; axis a turns dims[a] features
+ * (even, 0 for none) in dims[a] / 2 pairs, the i-th by the angle
+ * position * theta^(-2 i / dims[a]).  out float32 [rows, P, 2] (cosine, sine), P = sum(dims) / 2,
+ * the axes' pairs behind each other.  Angles in float64.  dims is a host array; axes <= 8.
+ */
+#define CONVROT_POS_F32 0
+#define CONVROT_POS_F64 1
+#define CONVROT_POS_I32 2
+#define CONVROT_POS_I64 3
+int convrot_axes_table(const void* positions, int kind, int64_t rows, int axes, const int* dims, double theta,
+                       float* out, void* stream);
+
+/*
+ * Per-head RMS norm and rotary positions of queries and keys, in float32,
+ * rounded once:  n = x / sqrt(mean(x^2) + eps) * weight over a head's dim
+ * features (weight NULL: n = x), then the first 2 * pairs features in pairs
+ * (a, b) -> (a cos - b sin, a sin + b cos): features (2 p, 2 p + 1) when
+ * interleaved, else (p, pairs + p); the rest stay as n has them.
+ * q, k and their outputs are [batch, heads, length, dim] with any strides of
+ * batch, head and token: `strides` (host) holds them, in elements, of q, k,
+ * q_out, k_out; features are adjacent.  q_heads and k_heads may differ, either may be 0.
+ * An output may be its input.  table float32 [batch][length][pairs][2],
+ * table_batch_stride floats between batch entries (0: one table for all).
+ * weights [dim] of weight_dtype (the activations' or float32).  dim <= 512.
+ */
+int convrot_qk_rotary(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, int dtype,
+                      int batch, int q_heads, int k_heads, int64_t length, int dim, const float* table, int pairs,
+                      int64_t table_batch_stride, const void* q_weight, const void* k_weight, int weight_dtype,
+                      float eps, int interleaved, void* stream);
+
+/*
+ * Gradients of convrot_qk_rotary: from dq, dk (of the outputs) and the inputs q,
+ * k to q_grad, k_grad and, with weights, q_weight_grad, k_weight_grad [dim] of
+ * weight_dtype (may be NULL).  strides: dq, dk, q, k, q_grad, k_grad.  workspace:
+ * convrot_qk_rotary_workspace_bytes(dim) bytes, 16-byte aligned, of any content (not needed
+ * without weight gradients).  Sums are float32 in a fixed order.
+ */
+int64_t convrot_qk_rotary_workspace_bytes(int dim);
+int convrot_qk_rotary_backward(const void* dq, const void* dk, const void* q, const void* k, void* q_grad,
+                               void* k_grad, void* q_weight_grad, void* k_weight_grad, const int64_t* strides,
+                               int dtype, int batch, int q_heads, int k_heads, int64_t length, int dim,
+                               const float* table, int pairs, int64_t table_batch_stride, const void* q_weight,
+                               const void* k_weight, int weight_dtype, float eps, int interleaved, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 /* Thread-local message of the last failed call on this thread ("" if none). */
 const char* convrot_last_error(void);
 
@@ -449,6 +562,7 @@ const char* convrot_last_error(void);
  *   gemm_mfma32      "0" | "1"            4-wave 256x256 W4A4 tile on 32x32x32 MFMAs: never,
  *                                         or always (plain 16-bit outputs)
  *   fp6_tile         "BMxBN"              FP6 W4A4 tile: 256x256, 256x224, 128x256, 128x192 or 128x128
+ *   w8a8_tile        "BMxBN"              W8A8 tile: 256x256 or 128x128; "0x0": the few-row kernel
  * Returns CONVROT_ERR_INVALID for an unknown name, a malformed value or a
  * tile the library does not build.
  */
