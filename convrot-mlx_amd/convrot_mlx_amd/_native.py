@@ -166,7 +166,7 @@ def set_tuning(name: str, value: str | None) -> None:
     G: always, on G workgroups), gemm_mfma32 (0/1), fp6_tile ("BMxBN": 256x256, 256x224, 128x256, 128x192, 128x128),
     linear_rows_cfg (1/2/3/5/16), w4a4_midm_cfg (10 * row tiles + weight tiles),
     fp6_split (1/2/4: parts of each 256x256 FP6 tile past the whole rounds),
-    w8a8_tile ("BMxBN": 256x256 or 128x128; "0x0": the few-row kernel)."""
+    w8a8_tile ("BMxBN", 256x256 to 64x64; "0x0": the few-row kernel)."""
     check(load().convrot_set_tuning(name.encode(), None if value is None else str(value).encode()))
 
 

@@ -3,7 +3,8 @@
 For the layers that 4 bits hurt, or whose features no rotation group divides: rows are
 quantized symmetrically to [-127, 127] (codes = round(x * (127 / absmax)), scale = absmax / 127),
 the integer product is exact and the epilogue is that of the 4-bit linears,
-((dot * xscale) * wscale) + bias in float32, then the optional gated residual.  Weights stay
+((dot * xscale) * wscale) + bias in float32.  A gated residual, residual + gate * linear, is taken
+in float32 too and rounded once (the 4-bit linears round each operation).  Weights stay
 row-major int8 [N, K], as 8-bit checkpoints hold them.  No counterpart in the reference, which
 quantizes to 4 bits only.
 """
@@ -106,7 +107,7 @@ def hip_w8a8_matmul(qact: torch.Tensor, qweight: torch.Tensor, xscales: torch.Te
                     bias: torch.Tensor | None = None, *, output_dtype: torch.dtype, residual=None, gate=None,
                     inplace: bool = False) -> torch.Tensor:
     """int8 activations [M, K] x int8 weight [N, K] -> output_dtype [M, N]:
-    ((dot * xscales[m]) * wscales[n]) + bias[n]; residual, gate and inplace as in hip_w4a4_matmul."""
+    ((dot * xscales[m]) * wscales[n]) + bias[n]; residual, gate and inplace as in hip_w4a4_matmul, with one rounding at the end."""
     if qact.ndim != 2 or qact.dtype != torch.int8:
         raise ValueError(f"W8A8 activation must be 2D int8, got {tuple(qact.shape)} {qact.dtype}")
     m, k = qact.shape
@@ -122,7 +123,8 @@ def hip_w8a8_matmul(qact: torch.Tensor, qweight: torch.Tensor, xscales: torch.Te
 def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, bias: torch.Tensor | None = None,
                     *, residual=None, gate=None, inplace: bool = False) -> torch.Tensor:
     """x [..., K] (float32, float16 or bfloat16), quantized row by row, times the int8 weight
-    [N, K] -> [..., N] of x's type; residual, gate and inplace as in ConvRotLinear.forward."""
+    [N, K] -> [..., N] of x's type; residual, gate and inplace as in ConvRotLinear.forward, with one
+    rounding at the end."""
     k = x.shape[-1]
     n = _check_product(k, qweight, wscales, bias)
     device = nat.require_device(x, qweight, wscales, bias)

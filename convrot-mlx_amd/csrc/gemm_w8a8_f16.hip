@@ -1,0 +1,6 @@
+// The tiled W8A8 kernels with float16 outputs.
+#include "gemm_w8a8_tile.h"
+
+namespace convrot {
+template hipError_t launch_w8a8_tile<kF16>(int tile, const W8a8Operands& p, hipStream_t stream);
+}

@@ -445,8 +445,8 @@ int convrot_quantize_int8(const void* x, int dtype, int64_t rows, int64_t featur
 
 /*
  * W8A8 GEMM: out[m][n] = dt(((float(sum_k act[m][k] * weight[n][k]) * xscales[m]) * wscales[n]) + bias[n]),
- * the integer sum exact, optionally followed by the gated residual of
- * convrot_w4a4_gemm_residual (residual NULL: none; gate NULL: residual + linear).
+ * the integer sum exact; with a residual, dt(residual[m][n] + gate[m / rows_per_gate][n] * that float)
+ * (gate NULL: 1), operands as in convrot_w4a4_gemm_residual but one rounding at the end.
  * act int8 [M, K] and weight int8 [N, K], row-major with row strides in bytes
  * (multiples of 16, at most 2^22), 16-byte aligned.  Where K is no multiple of
  * 16, a stride covers the next one, and the weight's bytes from K to there are
@@ -562,7 +562,7 @@ const char* convrot_last_error(void);
  *   gemm_mfma32      "0" | "1"            4-wave 256x256 W4A4 tile on 32x32x32 MFMAs: never,
  *                                         or always (plain 16-bit outputs)
  *   fp6_tile         "BMxBN"              FP6 W4A4 tile: 256x256, 256x224, 128x256, 128x192 or 128x128
- *   w8a8_tile        "BMxBN"              W8A8 tile: 256x256 or 128x128; "0x0": the few-row kernel
+ *   w8a8_tile        "BMxBN"              W8A8 tile (256x256 .. 64x64); "0x0": the few-row kernel
  * Returns CONVROT_ERR_INVALID for an unknown name, a malformed value or a
  * tile the library does not build.
  */

@@ -57,7 +57,11 @@ def test_product(dev, m, n, k, dtype):
     assert torch.equal(got.cpu(), product_plain(*host[:4], None, dtype))
 
 
-@pytest.mark.parametrize("tile", ["256x256", "128x128", "0x0"])
+TILES = ["256x256", "256x224", "224x256", "256x192", "192x256", "256x128", "128x256", "192x192", "192x128", "128x192",
+         "160x128", "128x160", "128x128", "128x64", "64x128", "64x64", "0x0"]
+
+
+@pytest.mark.parametrize("tile", TILES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (31, 70, 256), (130, 300, 1168), (520, 513, 384), (300, 264, 4000)])
 def test_every_kernel(dev, tuning, tile, m, n, k):
     from convrot_mlx_amd import hip_w8a8_matmul
@@ -127,15 +131,15 @@ def test_quantizer_of_views_and_odd_rows(dev):
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("m,n", [(1, 64), (6, 50), (40, 136), (300, 264), (520, 515), (528, 1024)])
 def test_gated_residual(dev, m, n, dtype):
-    """residual + gate * linear, each operation rounded as torch rounds it, out of place and in place."""
+    """residual + gate * linear in float32, rounded once, out of place and in place."""
     from convrot_mlx_amd import hip_w8a8_matmul
 
     host, (qa, qw, xs, ws, bias) = operands(m + n, m, n, 192, dev)
-    lin = product_plain(*host, dtype)
+    lin = product_plain(*host, F32)
     g = torch.Generator().manual_seed(n)
     res = torch.randn((m, n), generator=g).to(dtype)
     for gate in (None, torch.randn((1, n), generator=g).to(dtype), torch.randn((m, n), generator=g).to(dtype)):
-        want = res + lin if gate is None else res + gate * lin
+        want = (res.float() + lin if gate is None else res.float() + gate.float() * lin).to(dtype)
         r, gd = res.to(dev), None if gate is None else gate.to(dev)
         got = hip_w8a8_matmul(qa, qw, xs, ws, bias, output_dtype=dtype, residual=r, gate=gd)
         assert torch.equal(got.cpu(), want)
@@ -143,7 +147,7 @@ def test_gated_residual(dev, m, n, dtype):
         assert got.data_ptr() == r.data_ptr() and torch.equal(r.cpu(), want)
     if m % 2 == 0:
         gate = torch.randn((2, 1, n), generator=g).to(dtype)
-        want = res.reshape(2, m // 2, n) + gate * lin.reshape(2, m // 2, n)
+        want = (res.float().reshape(2, m // 2, n) + gate.float() * lin.reshape(2, m // 2, n)).to(dtype)
         got = hip_w8a8_matmul(qa, qw, xs, ws, bias, output_dtype=dtype, residual=res.reshape(2, m // 2, n).to(dev),
                               gate=gate.to(dev))
         assert torch.equal(got.cpu(), want.reshape(m, n))
@@ -177,21 +181,23 @@ def test_layer(dev):
     assert np.array_equal(layer.qweight.cpu().numpy(), qw)
     x = torch.randn((2, 7, 256), generator=g).to(BF16)
     codes, xs = quantize_plain(x.reshape(14, 256))
-    want = product_plain(codes, qw, xs, ws, b.numpy(), BF16).reshape(2, 7, 150)
+    lin = product_plain(codes, qw, xs, ws, b.numpy(), F32).reshape(2, 7, 150)
+    want = lin.to(BF16)
     y = layer(x.to(dev))
     assert torch.equal(y.cpu(), want)
     res, gate = torch.randn((2, 7, 150), generator=g).to(BF16), torch.randn((2, 1, 150), generator=g).to(BF16)
-    assert torch.equal(layer(x.to(dev), residual=res.to(dev), gate=gate.to(dev)).cpu(), res + gate * want)
+    gated = (res.float() + gate.float() * lin).to(BF16)
+    assert torch.equal(layer(x.to(dev), residual=res.to(dev), gate=gate.to(dev)).cpu(), gated)
     assert layer(x[:0].to(dev)).shape == (0, 7, 150)
     # the norm's result goes to codes from float32: the product of those codes, which are the
     # quantizer's of the same norm in float32
     shift, scale = (torch.randn((2, 1, 256), generator=g).to(BF16).to(dev) * 0.3 for _ in range(2))
     n32 = hip_layer_norm(x.float().to(dev), scale=scale.float(), shift=shift.float(), eps=1e-6)
     c32, s32 = quantize_int8_rowwise(n32.reshape(14, 256))
-    want = product_plain(c32.cpu().numpy(), qw, s32.cpu().numpy(), ws, b.numpy(), BF16).reshape(2, 7, 150)
-    assert torch.equal(layer.forward_modulated(x.to(dev), shift, scale, eps=1e-6).cpu(), want)
+    lin = product_plain(c32.cpu().numpy(), qw, s32.cpu().numpy(), ws, b.numpy(), F32).reshape(2, 7, 150)
+    assert torch.equal(layer.forward_modulated(x.to(dev), shift, scale, eps=1e-6).cpu(), lin.to(BF16))
     got = layer.forward_modulated(x.to(dev), shift, scale, residual=res.to(dev), gate=gate.to(dev))
-    assert torch.equal(got.cpu(), res + gate * want)
+    assert torch.equal(got.cpu(), (res.float() + gate.float() * lin).to(BF16))
 
 
 def test_replace_int8_linears(dev):
