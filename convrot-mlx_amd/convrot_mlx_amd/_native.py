@@ -65,7 +65,11 @@ SIGNATURES = {
                                              _i32, _vp]),
     "convrot_quantize_int8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "convrot_w8a8_gemm": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
-                                 _i32, _vp]),
+                                 _i64, _vp, _i32, _vp]),
+    "convrot_w8a8_scratch_bytes": (_i64, [_i64, _i64]),
+    "convrot_w8a8_fused": (_i32, [_vp, _i32, _i64, _i64, _i64]),
+    "convrot_w8a8_linear": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
+                                   _i64, _vp, _i64, _vp, _vp]),
     "convrot_layer_norm": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _i64, _f32, _vp, _vp, _vp, _vp]),
     "convrot_layer_norm_int8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _i64, _f32, _vp, _i64, _vp,
                                        _vp]),
@@ -166,7 +170,8 @@ def set_tuning(name: str, value: str | None) -> None:
     G: always, on G workgroups), gemm_mfma32 (0/1), fp6_tile ("BMxBN": 256x256, 256x224, 128x256, 128x192, 128x128),
     linear_rows_cfg (1/2/3/5/16), w4a4_midm_cfg (10 * row tiles + weight tiles),
     fp6_split (1/2/4: parts of each 256x256 FP6 tile past the whole rounds),
-    w8a8_tile ("BMxBN", 256x256 to 64x64; "0x0": the few-row kernel)."""
+    w8a8_tile ("BMxBN", 256x256 to 64x64),
+    w8a8_split (workgroups that share a W8A8 tile's K)."""
     check(load().convrot_set_tuning(name.encode(), None if value is None else str(value).encode()))
 
 

@@ -15,7 +15,7 @@ import torch
 from torch import nn
 
 from . import _native as nat
-from .core import GatedResidual, _f32, _gated_residual
+from .core import GatedResidual, _f32, _gated_residual, _workspace
 from .norm import norm_operands, rows_of
 
 INT8_MAX = 127
@@ -64,19 +64,54 @@ def _check_scales(name: str, t: torch.Tensor, n: int) -> None:
         raise ValueError(f"W8A8 {name} must have shape {(n,)}, got {tuple(t.shape)}")
 
 
+def _residual_args(gr: GatedResidual | None) -> tuple:
+    """(residual, gate, gate stride, rows per gate) of a library call."""
+    if gr is None:
+        return None, None, 0, 1
+    return gr.residual.data_ptr(), None if gr.gate is None else gr.gate.data_ptr(), gr.stride, gr.rows_per_gate
+
+
+def _output(gr: GatedResidual | None, m: int, n: int, dtype: torch.dtype, device) -> torch.Tensor:
+    if gr is not None and gr.inplace:
+        return gr.residual.view(m, n)
+    return torch.empty((m, n), dtype=dtype, device=device)
+
+
 def _w8a8(act, weight, xscales, wscales, bias, k: int, dtype: torch.dtype, gr: GatedResidual | None) -> torch.Tensor:
     """The product of operands as the kernel reads them (see _operand)."""
     m, n = act.shape[0], weight.shape[0]
-    if gr is not None and gr.inplace:
-        out = gr.residual.view(m, n)
-    else:
-        out = torch.empty((m, n), dtype=dtype, device=act.device)
+    out = _output(gr, m, n, dtype, act.device)
+    stream = torch.cuda.current_stream(act.device).cuda_stream
+    work = _workspace(act.device, stream)
     nat.check(nat.load().convrot_w8a8_gemm(
-        nat.ptr(act), act.stride(0), nat.ptr(xscales), nat.ptr(weight), weight.stride(0), nat.ptr(wscales),
-        nat.ptr(bias), m, n, k, nat.ptr(gr.residual if gr is not None else None),
-        nat.ptr(gr.gate if gr is not None else None), gr.stride if gr is not None else 0,
-        gr.rows_per_gate if gr is not None else 1, nat.ptr(out), nat.dtype_code(dtype), nat.stream_of(act.device)))
+        act.data_ptr(), act.stride(0), xscales.data_ptr(), weight.data_ptr(), weight.stride(0), wscales.data_ptr(),
+        None if bias is None else bias.data_ptr(), m, n, k, *_residual_args(gr),
+        None if work is None else work.data_ptr(), 0 if work is None else work.numel(), out.data_ptr(),
+        nat.dtype_code(dtype), stream))
     return out
+
+
+def _linear(x: torch.Tensor, weight: torch.Tensor, wscales, bias, k: int, residual, gate, inplace: bool) -> torch.Tensor:
+    """x [..., k] times a weight as the kernel reads it, one library call."""
+    n, device = weight.shape[0], x.device
+    x2d = rows_of(x if x.ndim == 2 else x.reshape(-1, k))
+    m = x2d.shape[0]
+    gr = _residual(residual, gate, inplace, m, n, x.dtype)
+    out = _output(gr, m, n, x.dtype, device)
+    lib, dtype, stride = nat.load(), nat.dtype_code(x.dtype), x2d.stride(0)
+    scratch = None
+    if gr is not None or m > 16 or not lib.convrot_w8a8_fused(x2d.data_ptr(), dtype, m, k, stride):
+        scratch = torch.empty((m * (_round16(k) + 4),), dtype=torch.uint8, device=device)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    work = _workspace(device, stream)
+    nat.check(lib.convrot_w8a8_linear(
+        x2d.data_ptr(), dtype, stride, weight.data_ptr(), weight.stride(0), wscales.data_ptr(),
+        None if bias is None else bias.data_ptr(), m, n, k, *_residual_args(gr),
+        None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
+        None if work is None else work.data_ptr(), 0 if work is None else work.numel(), out.data_ptr(), stream))
+    if inplace:
+        return residual
+    return out if x.ndim == 2 else out.reshape(*x.shape[:-1], n)
 
 
 def _check_product(k: int, weight: torch.Tensor, wscales, bias) -> int:
@@ -126,19 +161,9 @@ def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tenso
     [N, K] -> [..., N] of x's type; residual, gate and inplace as in ConvRotLinear.forward, with one
     rounding at the end."""
     k = x.shape[-1]
-    n = _check_product(k, qweight, wscales, bias)
-    device = nat.require_device(x, qweight, wscales, bias)
-    x2d = rows_of(x.reshape(-1, k))
-    m = x2d.shape[0]
-    gr = _residual(residual, gate, inplace, m, n, x.dtype)
-    weight = _operand(qweight, "weight", True)
-    lib, dtype, k16 = nat.load(), nat.dtype_code(x.dtype), _round16(k)
-    codes = torch.empty((m, k16), dtype=torch.int8, device=device)
-    scales = torch.empty((m,), dtype=torch.float32, device=device)
-    nat.check(lib.convrot_quantize_int8(nat.ptr(x2d), dtype, m, k, x2d.stride(0), nat.ptr(codes), k16,
-                                        nat.ptr(scales), nat.stream_of(device)))
-    out = _w8a8(codes, weight, scales, _f32(wscales), _f32(bias), k, x.dtype, gr)
-    return residual if inplace else out.reshape(*x.shape[:-1], n)
+    _check_product(k, qweight, wscales, bias)
+    nat.require_device(x, qweight, wscales, bias)
+    return _linear(x, _operand(qweight, "weight", True), _f32(wscales), _f32(bias), k, residual, gate, inplace)
 
 
 class Int8Linear(nn.Module):
@@ -187,13 +212,8 @@ class Int8Linear(nn.Module):
         if residual is not None and tuple(residual.shape) != (*x.shape[:-1], self.out_features):
             raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
                              f"{(*x.shape[:-1], self.out_features)}")
-        weight = self._weight()
-        if self.in_features % 16 == 0:
-            return hip_w8a8_linear(x, weight, self.scales, self.bias, residual=residual, gate=gate, inplace=inplace)
-        codes, scales = quantize_int8_rowwise(x.reshape(-1, self.in_features))
-        gr = _residual(residual, gate, inplace, codes.shape[0], self.out_features, x.dtype)
-        out = _w8a8(codes, weight, scales, _f32(self.scales), _f32(self.bias), self.in_features, x.dtype, gr)
-        return residual if inplace else out.reshape(*x.shape[:-1], self.out_features)
+        nat.require_device(x, self.qweight)
+        return _linear(x, self._weight(), _f32(self.scales), _f32(self.bias), self.in_features, residual, gate, inplace)
 
     def forward_modulated(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, eps: float = 1e-6, *,
                           residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,

@@ -99,7 +99,7 @@ int convrot_set_tuning(const char* name, const char* value) {
                 {"gemm_persist", kTuneGemmPersist},   {"gemm_mfma32", kTuneGemmMfma32},
                 {"fp6_tile", kTuneFp6Tile},           {"linear_rows_cfg", kTuneRowsCfg},
                 {"w4a4_midm_cfg", kTuneMidmCfg},      {"fp6_split", kTuneFp6Split},
-                {"w8a8_tile", kTuneW8a8Tile}};
+                {"w8a8_tile", kTuneW8a8Tile},         {"w8a8_split", kTuneW8a8Split}};
   int key = -1;
   for (const auto& n : kNames)
     if (strcmp(n.name, name) == 0) key = n.key;
@@ -143,6 +143,10 @@ int convrot_set_tuning(const char* name, const char* value) {
       case kTuneFp6Split:
         v = atoi(value);
         good = v == 1 || v == 2 || v == 4;
+        break;
+      case kTuneW8a8Split:
+        v = atoi(value);
+        good = v >= 1 && v <= 64;
         break;
       case kTuneMidmCfg:
         v = atoi(value);
@@ -785,10 +789,13 @@ int convrot_quantize_int8(const void* x, int dtype, int64_t rows, int64_t featur
                        "convrot_quantize_int8");
 }
 
-int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscales, const int8_t* weight,
-                      int64_t weight_stride, const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K,
-                      const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate, void* out,
-                      int out_dtype, void* stream) {
+namespace {
+
+// Checks of a W8A8 product but for its activations; CONVROT_OK when the launch
+// may proceed (M == 0 or N == 0 included).
+int check_w8a8(int64_t M, int64_t N, int64_t K, const int8_t* weight, int64_t weight_stride, const float* wscales,
+               const void* gate, const void* residual, int64_t rows_per_gate, const void* workspace,
+               int64_t workspace_bytes, const void* out, int out_dtype) {
   if (!valid_dtype(out_dtype)) return fail(CONVROT_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
   if (M < 0 || N < 0 || K <= 0)
     return fail(CONVROT_ERR_INVALID, "invalid GEMM shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
@@ -799,22 +806,88 @@ int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscale
   if (gate && !residual) return fail(CONVROT_ERR_INVALID, "a gate needs a residual");
   if (gate && rows_per_gate <= 0)
     return fail(CONVROT_ERR_INVALID, "rows_per_gate must be positive, got %lld", (long long)rows_per_gate);
+  if (workspace_bytes < 0 || (workspace_bytes > 0 && !workspace))
+    return fail(CONVROT_ERR_INVALID, "invalid workspace (%lld bytes)", (long long)workspace_bytes);
+  if (workspace && !aligned(workspace, 256)) return fail(CONVROT_ERR_INVALID, "workspace must be 256-byte aligned");
   if (M == 0 || N == 0) return ok();
-  if (!act || !weight || !xscales || !wscales || !out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
-  const int64_t k16 = (K + 15) / 16 * 16;
-  if (act_stride < k16 || weight_stride < k16 || act_stride % 16 || weight_stride % 16 || !aligned(act, 16) ||
-      !aligned(weight, 16) || !aligned(out, 16))
+  if (!weight || !wscales || !out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (weight_stride < (K + 15) / 16 * 16 || weight_stride % 16 || !aligned(weight, 16) || !aligned(out, 16))
     return fail(CONVROT_ERR_INVALID,
-                "W8A8 operands need 16-byte aligned rows that cover K rounded up to 16 (K=%lld, strides %lld and %lld)",
-                (long long)K, (long long)act_stride, (long long)weight_stride);
-  if (act_stride > kMaxInt8Stride || weight_stride > kMaxInt8Stride)
+                "W8A8 operands need 16-byte aligned rows that cover K rounded up to 16 (K=%lld, weight stride %lld)",
+                (long long)K, (long long)weight_stride);
+  if (weight_stride > kMaxInt8Stride)
+    return fail(CONVROT_ERR_UNSUPPORTED, "W8A8 row strides are limited to %lld bytes", (long long)kMaxInt8Stride);
+  return ok();
+}
+
+}  // namespace
+
+int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscales, const int8_t* weight,
+                      int64_t weight_stride, const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K,
+                      const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate,
+                      void* workspace, int64_t workspace_bytes, void* out, int out_dtype, void* stream) {
+  if (int rc = check_w8a8(M, N, K, weight, weight_stride, wscales, gate, residual, rows_per_gate, workspace,
+                          workspace_bytes, out, out_dtype))
+    return rc;
+  if (M == 0 || N == 0) return ok();
+  if (!act || !xscales) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (act_stride < (K + 15) / 16 * 16 || act_stride % 16 || !aligned(act, 16))
+    return fail(CONVROT_ERR_INVALID,
+                "W8A8 operands need 16-byte aligned rows that cover K rounded up to 16 (K=%lld, activation stride %lld)",
+                (long long)K, (long long)act_stride);
+  if (act_stride > kMaxInt8Stride)
     return fail(CONVROT_ERR_UNSUPPORTED, "W8A8 row strides are limited to %lld bytes", (long long)kMaxInt8Stride);
   convrot::GatedResidual gr{};
   if (residual)
     if (int rc = check_residual(residual, gate, gate_stride, rows_per_gate, M, N, &gr)) return rc;
+  const convrot::Workspace work{(uint8_t*)workspace, workspace ? (size_t)workspace_bytes : 0};
   return launch_status(convrot::launch_w8a8_gemm(act, act_stride, xscales, weight, weight_stride, wscales, bias, M, N,
-                                                 K, out, out_dtype, (hipStream_t)stream, gr),
+                                                 K, out, out_dtype, (hipStream_t)stream, gr, work),
                        "convrot_w8a8_gemm");
+}
+
+int64_t convrot_w8a8_scratch_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  return M * ((K + 15) / 16 * 16) + M * 4;
+}
+
+int convrot_w8a8_linear(const void* x, int dtype, int64_t x_stride, const int8_t* weight, int64_t weight_stride,
+                        const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K,
+                        const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate,
+                        void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* out,
+                        void* stream) {
+  if (int rc = check_rows("8-bit quantization", x, dtype, M, K, x_stride, kMaxFeatures)) return rc;
+  if (int rc = check_w8a8(M, N, K, weight, weight_stride, wscales, gate, residual, rows_per_gate, workspace,
+                          workspace_bytes, out, dtype))
+    return rc;
+  if (M == 0 || N == 0) return ok();
+  convrot::GatedResidual gr{};
+  if (residual)
+    if (int rc = check_residual(residual, gate, gate_stride, rows_per_gate, M, N, &gr)) return rc;
+  const convrot::Workspace work{(uint8_t*)workspace, workspace ? (size_t)workspace_bytes : 0};
+  // a fused launch's workgroups all read x: none may write into it
+  const int64_t es = dtype == CONVROT_DTYPE_F32 ? 4 : 2;
+  const uintptr_t xa = (uintptr_t)x, oa = (uintptr_t)out;
+  const bool apart = oa + (uintptr_t)(M * N * es) <= xa || xa + (uintptr_t)(((M - 1) * x_stride + K) * es) <= oa;
+  if (apart && convrot::w8a8_fused(x, dtype, M, K, x_stride))
+    return launch_status(convrot::launch_w8a8_fused(x, x_stride, dtype, weight, weight_stride, wscales, bias, M, N, K,
+                                                    out, (hipStream_t)stream, gr, work),
+                         "convrot_w8a8_linear");
+  if (!scratch || !aligned(scratch, 16) || scratch_bytes < convrot_w8a8_scratch_bytes(M, K))
+    return fail(CONVROT_ERR_INVALID, "the W8A8 linear needs a 16-byte aligned scratch buffer of %lld bytes, got %lld",
+                (long long)convrot_w8a8_scratch_bytes(M, K), (long long)scratch_bytes);
+  const int64_t stride = (K + 15) / 16 * 16;
+  int8_t* codes = (int8_t*)scratch;
+  float* scales = (float*)(codes + M * stride);
+  hipError_t e = convrot::launch_quantize_int8(x, dtype, M, K, x_stride, codes, stride, scales, (hipStream_t)stream);
+  if (e == hipSuccess)
+    e = convrot::launch_w8a8_gemm(codes, stride, scales, weight, weight_stride, wscales, bias, M, N, K, out, dtype,
+                                  (hipStream_t)stream, gr, work);
+  return launch_status(e, "convrot_w8a8_linear");
+}
+
+int convrot_w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
+  return M > 0 && K > 0 && valid_dtype(dtype) && convrot::w8a8_fused(x, dtype, M, K, x_stride) ? 1 : 0;
 }
 
 int convrot_layer_norm(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride, const void* gain,

@@ -31,7 +31,8 @@ enum TuneKey : int {
   kTuneRowsCfg,          // few-row linear: weight tiles a workgroup (1, 2, 3, 5), or 16: one tile on 16 waves
   kTuneMidmCfg,          // W4A4 kernel of blocked codes: 10 * row tiles + weight tiles of a workgroup
   kTuneFp6Split,         // FP6 256x256 tiles past the whole rounds: as 1, 2 or 4 workgroups
-  kTuneW8a8Tile,         // W8A8 tile: bm | bn << 10, 0 the few-row kernel
+  kTuneW8a8Tile,         // W8A8 tile: bm | bn << 10
+  kTuneW8a8Split,        // workgroups that share a W8A8 tile's K
   kTuneCount
 };
 int tuning(TuneKey key);
@@ -42,7 +43,7 @@ int tuning(TuneKey key);
 bool w4a4_tile_known(int bm, int bn, int wm, int wn, int stages);
 bool fp6_tile_known(int bm, int bn);
 bool w4a16_tile_known(int bm, int bn);
-bool w8a8_tile_known(int bm, int bn);  // 0 x 0: the few-row kernel
+bool w8a8_tile_known(int bm, int bn);
 
 // The FP6 W4A4 tile the plan (and the fp6_tile override) picks for M x N on operand
 // blocks, and on compact weights, where each 256 x 256 tile past the whole rounds
@@ -189,7 +190,21 @@ hipError_t launch_weight_fp6c(const uint8_t* cdna4, uint8_t* fp6c, int* minus8, 
 
 hipError_t launch_w8a8_gemm(const int8_t* act, int64_t lda, const float* xscales, const int8_t* weight, int64_t ldw,
                             const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K, void* out,
-                            int out_dtype, hipStream_t stream, const GatedResidual& gr);
+                            int out_dtype, hipStream_t stream, const GatedResidual& gr, const Workspace& work);
+
+// Whether a few rows are quantized inside their product's launch, and that launch.
+bool w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride);
+hipError_t launch_w8a8_fused(const void* x, int64_t x_stride, int dtype, const int8_t* weight, int64_t ldw,
+                             const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K, void* out,
+                             hipStream_t stream, const GatedResidual& gr, const Workspace& work);
+
+// Workgroups that share a W8A8 tile's K use the workspace of the other linears
+// on their stream: one arrival counter a tile in the words of the W4A16 split's
+// counters (zero between launches, both), partial sums from the same offset on.
+constexpr size_t kW8a8CounterOffset = kW4a16CounterOffset;
+constexpr int kW8a8Counters = 3072;
+constexpr size_t kW8a8PartialOffset = kW4a16PartialOffset;
+static_assert(kW8a8CounterOffset + kW8a8Counters * 4 <= kW8a8PartialOffset, "counters");
 
 hipError_t launch_quantize_int8(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride, int8_t* codes,
                                 int64_t codes_stride, float* scales, hipStream_t stream);

@@ -1,11 +1,10 @@
 // W8A8 GEMM for gfx950 (8-bit integer activations and weights; the product and its
 // numerics are stated in gemm_w8a8_tile.h): the kernel for a few token rows, and
 // the choice of kernel.
-#include <stdlib.h>
-
 #include <algorithm>
 
 #include "convrot_launch.h"
+#include "row_device.h"
 #include "w8a8_device.h"
 
 namespace convrot {
@@ -13,110 +12,270 @@ namespace {
 
 // ---- few rows
 //
-// The weights' bytes bound it: each is read once, straight into registers.  A
-// workgroup owns NB tiles of 16 output channels and 16 FM tokens; its SPLIT
-// waves share K, a block of 128 in turn, and add their integer sums through LDS.
-template <int FM, int NB, int SPLIT, int UNROLL, int ODT>
-__global__ __launch_bounds__(SPLIT * 64) void w8a8_rows_kernel(W8a8Operands p) {
-  __shared__ __attribute__((aligned(16))) i32x4 red[SPLIT][NB * FM][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r = lane & 15;
-  const int n0 = blockIdx.x * (16 * NB), m0 = blockIdx.y * (16 * FM);
-  const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u;
-  const int mrows = min(16 * FM, p.M - m0), nrows = min(16 * NB, p.N - n0);
-  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-  const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(p.act + (int64_t)m0 * p.lda), (short)0, (int)((uint32_t)(mrows - 1) * (uint32_t)p.lda + k16), 0x00020000);
-  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(p.weight + (int64_t)n0 * p.ldw), (short)0, (int)((uint32_t)(nrows - 1) * (uint32_t)p.ldw + k16),
-      0x00020000);
-  i32x4 acc[NB][FM];
-#pragma unroll
-  for (int a = 0; a < NB; ++a)
-#pragma unroll
-    for (int b = 0; b < FM; ++b) acc[a][b] = (i32x4){0, 0, 0, 0};
+// Up to 16 token rows: the weights' bytes bound it, each read once.  A workgroup
+// owns 64 output channels, each of its 4 waves 16 of them and, for itself (no
+// barrier in the loop), a ring of STAGES blocks of 128 features in LDS that it
+// keeps full by direct-to-LDS loads; the rows' codes lie in LDS from the start.
+// Where the channels make too few workgroups for the chip, several share K and
+// the last to arrive adds their integer sums.  With FUSED the rows come as they
+// are and each workgroup quantizes them itself (as convrot_quantize_int8 does)
+// while the first weights are on their way: one launch instead of two.
+constexpr int kRowsMax = 16, kRowsN = 64;
+constexpr int kFusedChunks = 12;  // of 8 values a thread: the rows of a fused call hold up to 24576
+constexpr int64_t kFusedMax = 256 * 8 * kFusedChunks;
 
-  const uint32_t steps = (k16 + 63) / 64;  // of 64 features
-  for (uint32_t s0 = wave * UNROLL; s0 < steps; s0 += SPLIT * UNROLL) {
-    u32x4 w[UNROLL][NB], a[UNROLL][FM];
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i) {
-      const uint32_t k = (s0 + i) * 64u + (uint32_t)q * 16u;  // the lane's 16 features
-      const uint32_t wo = k < k16 ? (uint32_t)r * (uint32_t)p.ldw + k : kOutOfRange;
-#pragma unroll
-      for (int t = 0; t < NB; ++t)
-        w[i][t] = __builtin_amdgcn_raw_buffer_load_b128(rw, (int)(wo + (uint32_t)t * 16u * (uint32_t)p.ldw), 0, 0);
-#pragma unroll
-      for (int f = 0; f < FM; ++f)
-        a[i][f] = __builtin_amdgcn_raw_buffer_load_b128(ra, (int)((uint32_t)(16 * f + r) * (uint32_t)p.lda + k), 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i)
-#pragma unroll
-      for (int t = 0; t < NB; ++t)
-#pragma unroll
-        for (int f = 0; f < FM; ++f)
-          acc[t][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w[i][t]),
-                                                            __builtin_bit_cast(i32x4, a[i][f]), acc[t][f], 0, 0, 0);
-  }
-#pragma unroll
-  for (int t = 0; t < NB; ++t)
-#pragma unroll
-    for (int f = 0; f < FM; ++f) red[wave][t * FM + f][lane] = acc[t][f];
-  __syncthreads();
-  // wave w finishes the output tiles w, w + SPLIT, ..
-  const bool vec = (p.N & 3) == 0;
-  for (int i = wave; i < NB * FM; i += SPLIT) {
-    const int t = i / FM, f = i % FM;
-    i32x4 s = red[0][i][lane];
-#pragma unroll
-    for (int w2 = 1; w2 < SPLIT; ++w2) s += red[w2][i][lane];
-    const int m = m0 + f * 16 + r, n = n0 + t * 16 + 4 * q;
-    if (m >= p.M || n >= p.N) continue;
-    const float xs = p.xscales[m];
-    float o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int nn = min(n + j, p.N - 1);
-      o[j] = (((float)s[j] * xs) * p.wscales[nn]) + (p.bias ? p.bias[nn] : 0.0f);
-    }
-    store4<ODT>(p, m, n, vec, o);
-  }
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppHalfMirror, 0xf, 0xf, true));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppMirror, 0xf, 0xf, true));
 }
 
-template <int FM, int NB, int SPLIT, int UNROLL, int ODT>
-hipError_t launch_rows(const W8a8Operands& p, hipStream_t s) {
-  const dim3 grid((unsigned)((p.N + 16 * NB - 1) / (16 * NB)), (unsigned)((p.M + 16 * FM - 1) / (16 * FM)));
-  w8a8_rows_kernel<FM, NB, SPLIT, UNROLL, ODT><<<grid, dim3(SPLIT * 64), 0, s>>>(p);
+template <int DT, bool FUSED, int STAGES>
+__global__ __launch_bounds__(256) void w8a8_rows_kernel(W8a8Operands p, const void* __restrict__ x, int64_t x_stride,
+                                                        W8a8Split split, int tiles) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  __shared__ uint32_t row_max[kRowsMax];
+  __shared__ float row_scale[kRowsMax];
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
+  const int kblocks = (p.K + 127) / 128, kb0 = part * split.kblocks, n = min(split.kblocks, kblocks - kb0);
+  const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u, k0 = (uint32_t)kb0 * 128u, kn = (uint32_t)n * 128u;
+  uint8_t* ring = smem + wave * (STAGES * 2048);
+  uint8_t* codes = smem + 4 * STAGES * 2048;  // [M][kn], chunks swizzled
+  const uint32_t ring_addr = (uint32_t)(uintptr_t)ring;
+
+  // the wave's 16 weight rows (none past N)
+  const int nw = tile * kRowsN + wave * 16, nrows = min(16, p.N - nw);
+  const i32x4_sgpr rw =
+      buffer_rsrc(p.weight + (int64_t)(nrows > 0 ? nw : 0) * p.ldw, nrows > 0 ? (uint32_t)(nrows - 1) * (uint32_t)p.ldw + k16 : 0u);
+  const int rl = lane >> 3, c = lane & 7;
+  const uint32_t rest = k16 & 127u, tail_kb = rest ? k16 >> 7 : ~0u, lastkb = (uint32_t)(kb0 + n - 1);
+  uint32_t vw[2];
+  bool past[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t cw = 16u * (uint32_t)(c ^ rl ^ j);
+    vw[j] = (uint32_t)(8 * j + rl) * (uint32_t)p.ldw + cw;
+    past[j] = cw >= rest;
+  }
+  auto issue = [&](uint32_t kb, int stage) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t off = vw[j] + kb * 128u;
+      if (kb == tail_kb) off = past[j] ? kOutOfRange : off;
+      dma16(rw, off, ring_addr + (uint32_t)(stage * 2048 + j * 1024));
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) issue(min((uint32_t)(kb0 + s), lastkb), s);
+
+  // place of the 8 or 16 codes at feature k of row r
+  auto code_at = [&](int r, uint32_t k) {
+    const uint32_t b = (k - k0) >> 7, ch = (k >> 4) & 7;
+    return codes + (uint32_t)r * kn + b * 128u + ((ch ^ (uint32_t)chunk_swizzle(r)) << 4) + (k & 15u);
+  };
+  if constexpr (FUSED) {
+    typedef typename Elem<DT>::T E;
+    constexpr int W = DT == kF32 ? 2 : 1;
+    if (tid < kRowsMax) row_max[tid] = 0;
+    __syncthreads();
+    const uint32_t total = (uint32_t)p.M * (uint32_t)p.K;
+    uint4 raw[kFusedChunks][W];
+    uint32_t row[kFusedChunks], col[kFusedChunks];
+#pragma unroll
+    for (int i = 0; i < kFusedChunks; ++i) {
+      const uint32_t at = (uint32_t)(i * 256 + tid) * 8u;
+      row[i] = at / (uint32_t)p.K;
+      col[i] = at - row[i] * (uint32_t)p.K;
+#pragma unroll
+      for (int w = 0; w < W; ++w) raw[i][w] = make_uint4(0, 0, 0, 0);
+      if (at < total) {
+        const uint4* src = (const uint4*)((const E*)x + (int64_t)row[i] * x_stride + col[i]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) raw[i][w] = src[w];
+      }
+    }
+    auto values = [&](int i, float (&v)[8]) { load8<DT>((const E*)&raw[i][0], v); };
+#pragma unroll
+    for (int i = 0; i < kFusedChunks; ++i) {
+      if ((uint32_t)i * 2048u >= total) break;
+      float v[8];
+      values(i, v);
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+      const bool live = (uint32_t)(i * 256 + tid) * 8u < total;
+      if ((p.K & 127) == 0) {  // 16 lanes of one row (or past the end, zeros)
+        most = max16(most);
+        if ((lane & 15) == 0 && live) atomicMax(&row_max[row[i]], most);
+      } else if (live) {
+        atomicMax(&row_max[row[i]], most);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kFusedChunks; ++i) {
+      if ((uint32_t)i * 2048u >= total) break;
+      if ((uint32_t)(i * 256 + tid) * 8u >= total || col[i] < k0 || col[i] >= k0 + kn) continue;
+      const Int8Row q = int8_row(row_max[row[i]]);
+      float v[8];
+      values(i, v);
+      *(uint2*)code_at((int)row[i], col[i]) = int8_codes(v, q);
+    }
+    if (tid < p.M) row_scale[tid] = int8_row(row_max[tid]).scale;
+  } else {
+    const uint32_t per_row = kn / 16u;
+    for (uint32_t i = tid; i < (uint32_t)p.M * per_row; i += 256) {
+      const uint32_t r = i / per_row, k = k0 + (i - r * per_row) * 16u;
+      if (k < k16) *(uint4*)code_at((int)r, k) = *(const uint4*)(p.act + (int64_t)r * p.lda + k);
+    }
+    if (tid < p.M) row_scale[tid] = p.xscales[tid];
+  }
+  __syncthreads();
+
+  const int q = lane >> 4, r = lane & 15, ra = min(r, p.M - 1);  // columns past M: some row's, never stored
+  i32x4 acc = {0, 0, 0, 0};
+  int st = 0;
+  for (int i = 0; i < n; ++i) {
+    wait_vmcnt<2 * (STAGES - 1)>();
+    i32x4 w[2], a[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      w[ks] = *(const i32x4*)(ring + st * 2048 + r * 128 + (((2 * q + ks) ^ chunk_swizzle(r)) << 4));
+      a[ks] = *(const i32x4*)(codes + (uint32_t)ra * kn + (uint32_t)i * 128u +
+                              (((2 * q + ks) ^ chunk_swizzle(ra)) << 4));
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[ks], a[ks], acc, 0, 0, 0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the stage has been read
+    asm volatile("" ::: "memory");
+    issue(min((uint32_t)(kb0 + i + STAGES), lastkb), st);
+    st = st + 1 == STAGES ? 0 : st + 1;
+  }
+  wait_vmcnt<0>();
+
+  if (split.splits > 1) {
+    const __amdgpu_buffer_rsrc_t rp =
+        partial_rsrc(split.partials + (size_t)tile * split.splits * 4096, (uint32_t)split.splits * 4096u);
+    store_partial(rp, (uint32_t)(part * 4096 + tid * 16), acc);
+    if (!last_to_arrive(split.counters + tile, split.splits, &last)) return;
+    acc = (i32x4){0, 0, 0, 0};
+    for (int s = 0; s < split.splits; ++s) acc += load_partial(rp, (uint32_t)(s * 4096 + tid * 16));
+  }
+  const int nn = nw + 4 * q;
+  if (r >= p.M || nn >= p.N) return;
+  const float xs = row_scale[r];
+  float o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int at = min(nn + j, p.N - 1);
+    o[j] = (((float)acc[j] * xs) * p.wscales[at]) + (p.bias ? p.bias[at] : 0.0f);
+  }
+  store4<DT>(p, r, nn, (p.N & 3) == 0, o);
+}
+
+// ---- choice of kernel
+
+// Seconds of a tile's k-block (alone on its CU, and with every CU busy, where the
+// clock drops) and what its prologue, epilogue and stores add, in microseconds.
+struct Cost {
+  int bm, bn, per_cu;
+  float lone, full, fixed;
+};
+constexpr Cost kCosts[] = {
+    {256, 256, 1, 1.07f, 1.24f, 16.0f}, {256, 224, 1, 0.95f, 1.10f, 14.5f}, {224, 256, 1, 0.95f, 1.10f, 14.5f},
+    {256, 192, 1, 0.84f, 1.00f, 13.0f}, {192, 256, 1, 0.84f, 1.05f, 13.0f}, {256, 128, 1, 0.63f, 0.77f, 9.0f},
+    {128, 256, 1, 0.63f, 0.77f, 9.0f},  {192, 192, 1, 0.67f, 0.80f, 10.0f}, {192, 128, 1, 0.49f, 0.58f, 7.5f},
+    {128, 192, 1, 0.49f, 0.58f, 7.5f},  {160, 128, 1, 0.42f, 0.52f, 7.0f},  {128, 160, 1, 0.42f, 0.52f, 7.0f},
+    {128, 128, 2, 0.62f, 0.85f, 7.0f},  {128, 64, 2, 0.265f, 0.50f, 6.0f},  {64, 128, 2, 0.265f, 0.50f, 6.0f},
+    {64, 64, 2, 0.18f, 0.32f, 4.5f}};
+
+// Splits of K for a grid of `tiles` workgroups that walk `kblocks` each.
+int choose_splits(int64_t tiles, int kblocks, int64_t tile_bytes, const Workspace& work) {
+  const int forced = tuning(kTuneW8a8Split);
+  const int64_t most_bytes = work.ptr ? (int64_t)work.bytes - (int64_t)kW8a8PartialOffset : 0;
+  if (most_bytes <= 0 || tiles > kW8a8Counters) return 1;
+  int64_t s = forced > 0 ? forced : std::min<int64_t>(256 / tiles, kblocks / 8);
+  s = std::min({s, (int64_t)kblocks, most_bytes / (tiles * tile_bytes), (int64_t)64});
+  return (int)std::max<int64_t>(1, s);
+}
+
+W8a8Split make_split(int splits, int kblocks, const Workspace& work) {
+  W8a8Split s;
+  s.kblocks = (kblocks + splits - 1) / splits;
+  s.splits = (kblocks + s.kblocks - 1) / s.kblocks;  // no workgroup without a block
+  if (s.splits > 1) {
+    s.counters = (int*)(work.ptr + kW8a8CounterOffset);
+    s.partials = work.ptr + kW8a8PartialOffset;
+  }
+  return s;
+}
+
+int choose_tile(int64_t M, int64_t N, int64_t K) {
+  const int forced = tuning(kTuneW8a8Tile);
+  if (forced > 0) return forced;
+  const float kblocks = (float)((K + 127) / 128);
+  float best = 0.0f;
+  int tile = 0;
+  for (const Cost& c : kCosts) {
+    const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), slots = 256 * c.per_cu;
+    const int64_t rounds = tiles / slots;
+    const float part = (float)(tiles - rounds * slots) / (float)slots;
+    const float per = kblocks * c.full + c.fixed;
+    float t = (float)rounds * per;
+    if (part > 0.0f)  // few workgroups run at a higher clock, and alone on their CUs
+      t += kblocks * (c.lone + (c.full - c.lone) * part) + c.fixed * (0.65f + 0.35f * part);
+    if (tile == 0 || t < best) best = t, tile = tile_code(c.bm, c.bn);
+  }
+  return tile;
+}
+
+bool rows_kernel(int64_t M) {
+  const int forced = tuning(kTuneW8a8Tile);
+  return forced > 0 ? false : M <= kRowsMax;
+}
+
+// LDS of the few-row kernel: ring and codes.
+size_t rows_lds(int64_t M, int stages, int kblocks) { return (size_t)stages * 8192 + (size_t)M * kblocks * 128; }
+
+template <int DT, bool FUSED, int STAGES>
+hipError_t launch_rows_s(const W8a8Operands& p, const void* x, int64_t x_stride, const W8a8Split& split, int tiles,
+                         hipStream_t s) {
+  const size_t lds = rows_lds(p.M, STAGES, split.kblocks);
+  w8a8_rows_kernel<DT, FUSED, STAGES><<<dim3((unsigned)(tiles * split.splits)), dim3(256), lds, s>>>(p, x, x_stride,
+                                                                                                    split, tiles);
   return hipGetLastError();
 }
 
-// Kernel of a product: 0 few rows, else tile_code of a tile.
-int plan(int64_t M, int64_t N, int64_t K) {
-  const int forced = tuning(kTuneW8a8Tile);
-  if (forced >= 0) return forced;
-  if (M <= 64) return 0;
-  return N >= 512 && M >= 512 ? tile_code(256, 256) : tile_code(128, 128);
+template <int DT, bool FUSED>
+hipError_t launch_rows(const W8a8Operands& p, const void* x, int64_t x_stride, const Workspace& work, hipStream_t s) {
+  const int64_t tiles = (p.N + kRowsN - 1) / kRowsN;
+  const int kblocks = (p.K + 127) / 128;
+  W8a8Split split = make_split(choose_splits(tiles, kblocks, 4096, work), kblocks, work);
+  // two workgroups a CU where the codes leave room beside the deep ring, else beside the short one
+  const bool deep = rows_lds(p.M, 8, split.kblocks) <= 80 * 1024 || rows_lds(p.M, 4, split.kblocks) > 80 * 1024;
+  if (deep) return launch_rows_s<DT, FUSED, 8>(p, x, x_stride, split, (int)tiles, s);
+  return launch_rows_s<DT, FUSED, 4>(p, x, x_stride, split, (int)tiles, s);
 }
 
-template <int ODT>
-hipError_t launch_t(const W8a8Operands& p, hipStream_t s) {
-  const int tile = plan(p.M, p.N, p.K);
-  switch (tile) {
-    case 0:
-      if (p.M <= 16) {
-        if (p.N <= 8192) return launch_rows<1, 1, 16, 4, ODT>(p, s);
-        return launch_rows<1, 1, 4, 6, ODT>(p, s);
-      }
-      if (p.M <= 32) return launch_rows<2, 1, 8, 4, ODT>(p, s);
-      return launch_rows<4, 1, 8, 2, ODT>(p, s);
-    default: return launch_w8a8_tile<ODT>(tile, p, s);
-  }
+// Whether the few-row kernel has room for the codes of a product's rows, whatever the split.
+bool rows_fit(int64_t M, int64_t K) { return rows_lds(M, 8, (int)((K + 127) / 128)) + 256 <= 160 * 1024; }
+
+template <int DT>
+hipError_t launch_t(const W8a8Operands& p, const Workspace& work, hipStream_t s) {
+  if (rows_kernel(p.M) && rows_fit(p.M, p.K)) return launch_rows<DT, false>(p, nullptr, 0, work, s);
+  const int tile = choose_tile(p.M, p.N, p.K), bm = tile & 1023, bn = tile >> 10;
+  const int kblocks = (p.K + 127) / 128;
+  const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);
+  const int splits = bm * bn <= kMaxSplitTile ? choose_splits(tiles, kblocks, (int64_t)bm * bn * 4, work) : 1;
+  return launch_w8a8_tile<DT>(tile, p, make_split(splits, kblocks, work), s);
 }
 
 }  // namespace
 
 bool w8a8_tile_known(int bm, int bn) {
-  if (bm == 0 && bn == 0) return true;
 #define W8A8_KNOWN(BM, BN, STAGES, PER_CU) \
   if (bm == BM && bn == BN) return true;
   W8A8_TILES(W8A8_KNOWN)
@@ -126,12 +285,29 @@ bool w8a8_tile_known(int bm, int bn) {
 
 hipError_t launch_w8a8_gemm(const int8_t* act, int64_t lda, const float* xscales, const int8_t* weight, int64_t ldw,
                             const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K, void* out,
-                            int out_dtype, hipStream_t stream, const GatedResidual& gr) {
+                            int out_dtype, hipStream_t stream, const GatedResidual& gr, const Workspace& work) {
   const W8a8Operands p{act, weight, lda, ldw, xscales, wscales, bias, out, (int)M, (int)N, (int)K, gr};
   switch (out_dtype) {
-    case kF32: return launch_t<kF32>(p, stream);
-    case kF16: return launch_t<kF16>(p, stream);
-    default: return launch_t<kBF16>(p, stream);
+    case kF32: return launch_t<kF32>(p, work, stream);
+    case kF16: return launch_t<kF16>(p, work, stream);
+    default: return launch_t<kBF16>(p, work, stream);
+  }
+}
+
+bool w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
+  const size_t es = dtype == kF32 ? 4 : 2;
+  return rows_kernel(M) && M * K <= kFusedMax && K % 16 == 0 && ((uintptr_t)x & 15) == 0 &&
+         (M == 1 || (x_stride * es) % 16 == 0) && rows_fit(M, K);
+}
+
+hipError_t launch_w8a8_fused(const void* x, int64_t x_stride, int dtype, const int8_t* weight, int64_t ldw,
+                             const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K, void* out,
+                             hipStream_t stream, const GatedResidual& gr, const Workspace& work) {
+  const W8a8Operands p{nullptr, weight, 0, ldw, nullptr, wscales, bias, out, (int)M, (int)N, (int)K, gr};
+  switch (dtype) {
+    case kF32: return launch_rows<kF32, true>(p, x, x_stride, work, stream);
+    case kF16: return launch_rows<kF16, true>(p, x, x_stride, work, stream);
+    default: return launch_rows<kBF16, true>(p, x, x_stride, work, stream);
   }
 }
 

@@ -2,5 +2,5 @@
 #include "gemm_w8a8_tile.h"
 
 namespace convrot {
-template hipError_t launch_w8a8_tile<kF32>(int tile, const W8a8Operands& p, hipStream_t stream);
+template hipError_t launch_w8a8_tile<kF32>(int tile, const W8a8Operands& p, const W8a8Split& split, hipStream_t stream);
 }

@@ -68,7 +68,6 @@ __device__ __forceinline__ void mfma_drain(i32x4 (&acc)[FN][FM]) {
 // Both operands take a byte a value in LDS, so a wave's corner has to be large:
 // of the LDS port's 128 bytes a clock, 128 x 128 corners (256 x 256 tile) take
 // 64 for reads and 32 for the DMA's writes, 64 x 64 corners 128 and 64.
-__device__ __forceinline__ int chunk_swizzle(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 template <int BM, int BN, int STAGES>
 struct Engine {
@@ -174,13 +173,14 @@ struct Engine {
   // n fillers spread over the first `span` MFMA slots: those after slot t are
   // filler(t) .. filler(t + 1) - 1.
   static constexpr int filler(int t, int n, int span) { return t >= span ? n : (t * n + span - 1) / span; }
-  __device__ __forceinline__ void run(int kblocks, i32x4 (&acc)[FN][FM]) {
+  // acc += the products of k-blocks kb0 .. kb0 + n - 1, n >= 1.
+  __device__ __forceinline__ void run(uint32_t kb0, int n, i32x4 (&acc)[FN][FM]) {
     i32x4 w0[FN], a0[FM], w1[FN], a1[FM];
-    const uint32_t last = (uint32_t)kblocks - 1;
+    const uint32_t last = kb0 + (uint32_t)n - 1;
 #pragma unroll
     for (int s = 0; s < STAGES; ++s)
 #pragma unroll
-      for (int i = 0; i < LPW; ++i) issue_piece(min((uint32_t)s, last), s, i);
+      for (int i = 0; i < LPW; ++i) issue_piece(min(kb0 + s, last), s, i);
     wait_vmcnt<(STAGES - 1) * LPW>();  // block 0 and the epilogue's operands
     __builtin_amdgcn_s_barrier();
     {
@@ -188,7 +188,7 @@ struct Engine {
       static_for<READS>([&](auto i) __attribute__((always_inline)) { read<i.value>(sw, sa, w0, a0); });
     }
     int st = 0;
-    for (uint32_t kb = 0; kb <= last; ++kb) {
+    for (uint32_t kb = kb0; kb <= last; ++kb) {
       const int nst = st + 1 == STAGES ? 0 : st + 1;
       {
         const uint8_t *sw = w_frag(st, 1), *sa = a_frag(st, 1);
@@ -361,13 +361,14 @@ __device__ __forceinline__ void epilogue(const E& e, const i32x4 (&acc)[E::FN][E
 
 template <int BM, int BN, int STAGES, int PER_CU, int ODT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER_CU))) void w8a8_tile_kernel(
-    W8a8Operands p, int tiles_m, int tiles_n) {
+    W8a8Operands p, int tiles_m, int tiles_n, W8a8Split split) {
   using E = Engine<BM, BN, STAGES>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES];
   E e(smem);
   // tiles that one XCD (one L2) runs are neighbours, in groups of kGroupM tile rows
   const int tiles = tiles_m * tiles_n, per_xcd = tiles / kXcds;
-  int t = blockIdx.x;
+  const int part = BM * BN <= kMaxSplitTile && split.splits > 1 ? blockIdx.x / tiles : 0;
+  int t = blockIdx.x - part * tiles;
   if (t < per_xcd * kXcds) t = (t % kXcds) * per_xcd + t / kXcds;
   const int group = t / (kGroupM * tiles_n), first_m = group * kGroupM;
   const int group_rows = min(kGroupM, tiles_m - first_m), in_group = t - group * kGroupM * tiles_n;
@@ -380,26 +381,54 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER
   for (int a = 0; a < E::FN; ++a)
 #pragma unroll
     for (int b = 0; b < E::FM; ++b) acc[a][b] = (i32x4){0, 0, 0, 0};
-  e.run((p.K + 127) / 128, acc);
+  const int kblocks = (p.K + 127) / 128;
+  if (BM * BN > kMaxSplitTile || split.splits == 1) {
+    e.run(0, kblocks, acc);
+  } else if constexpr (BM * BN <= kMaxSplitTile) {
+    e.run((uint32_t)(part * split.kblocks), min(split.kblocks, kblocks - part * split.kblocks), acc);
+    // partials [tile][part][fragment][thread], added by the last workgroup of the tile to arrive
+    __shared__ int last;
+    constexpr uint32_t BYTES = BM * BN * 4;
+    const __amdgpu_buffer_rsrc_t r =
+        partial_rsrc(split.partials + (size_t)t * split.splits * BYTES, (uint32_t)split.splits * BYTES);
+    const uint32_t at = threadIdx.x * 16u;
+    static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+      for (int fm = 0; fm < E::FM; ++fm)
+        store_partial(r, (uint32_t)part * BYTES + (uint32_t)(fn.value * E::FM + fm) * 4096u + at, acc[fn.value][fm]);
+    });
+    if (!last_to_arrive(split.counters + t, split.splits, &last)) return;
+    static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+      for (int fm = 0; fm < E::FM; ++fm) acc[fn.value][fm] = (i32x4){0, 0, 0, 0};
+    });
+    for (int q = 0; q < split.splits; ++q)  // sums of integers: any order gives the same
+      static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+        for (int fm = 0; fm < E::FM; ++fm)
+          acc[fn.value][fm] += load_partial(r, (uint32_t)q * BYTES + (uint32_t)(fn.value * E::FM + fm) * 4096u + at);
+      });
+  }
   __syncthreads();  // every wave is done with the ring before it stages outputs
   epilogue<E, ODT>(e, acc, p, m0, n0);
 }
 
 template <int BM, int BN, int STAGES, int PER_CU, int ODT>
-hipError_t launch_tile(const W8a8Operands& p, hipStream_t s) {
+hipError_t launch_tile(const W8a8Operands& p, const W8a8Split& split, hipStream_t s) {
   const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-  if (tm * tn > 0x7fffffff) return hipErrorInvalidValue;
-  w8a8_tile_kernel<BM, BN, STAGES, PER_CU, ODT><<<dim3((unsigned)(tm * tn)), dim3(256), 0, s>>>(p, (int)tm, (int)tn);
+  if (tm * tn * split.splits > 0x7fffffff) return hipErrorInvalidValue;
+  w8a8_tile_kernel<BM, BN, STAGES, PER_CU, ODT><<<dim3((unsigned)(tm * tn * split.splits)), dim3(256), 0, s>>>(
+      p, (int)tm, (int)tn, split);
   return hipGetLastError();
 }
 
 }  // namespace
 
 template <int ODT>
-hipError_t launch_w8a8_tile(int tile, const W8a8Operands& p, hipStream_t stream) {
+hipError_t launch_w8a8_tile(int tile, const W8a8Operands& p, const W8a8Split& split, hipStream_t stream) {
   switch (tile) {
 #define W8A8_CASE(BM, BN, STAGES, PER_CU) \
-  case tile_code(BM, BN): return launch_tile<BM, BN, STAGES, PER_CU, ODT>(p, stream);
+  case tile_code(BM, BN): return launch_tile<BM, BN, STAGES, PER_CU, ODT>(p, split, stream);
     W8A8_TILES(W8A8_CASE)
 #undef W8A8_CASE
     default: return hipErrorInvalidValue;

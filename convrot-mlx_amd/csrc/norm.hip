@@ -16,6 +16,8 @@
 // codes from registers.  A row that holds a NaN or an infinity gets the scale
 // NaN and codes 0, so every product of it is NaN; a row below 2^-100 counts as
 // zero (codes 0, scale 0), where 127 / a would overflow.
+#include <algorithm>
+
 #include "convrot_launch.h"
 #include "row_device.h"
 
@@ -23,9 +25,6 @@ namespace convrot {
 namespace {
 
 enum RowOp : int { kNormOut = 0, kNormCodes = 1, kCodes = 2 };
-
-constexpr float kTiny = 0x1p-100f;
-constexpr uint32_t kInfBits = 0x7f800000u;
 
 // Sum over a team of T threads (T / 64 waves, `red` its own floats), in every
 // thread.  Every thread of the workgroup calls it.
@@ -131,34 +130,22 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_kernel(
 #pragma unroll
       for (int w = 1; w < W; ++w) most = max(most, redmax[w]);
     }
-    const float a = __builtin_bit_cast(float, most);
-    const bool finite = most < kInfBits, zero = a < kTiny;
-    const float inv = finite && !zero ? 127.0f / a : 0.0f;
-    if (t == 0) scales[row] = !finite ? __builtin_nanf("") : zero ? 0.0f : a * (1.0f / 127.0f);
+    const Int8Row q = int8_row(most);
+    if (t == 0) scales[row] = q.scale;
     int8_t* o = (int8_t*)out + row * out_stride;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      int q[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // |x inv| <= 127 up to its last bit, which the rounding drops; a row that is not finite gets zeros
-        const bool in = feature_of<T, C, VEC>(t, c, j) < K;
-        q[j] = in && finite ? (int)rintf(v[c][j] * inv) : 0;
-      }
-      // columns K .. stride - 1 are zero
+      for (int j = 0; j < 8; ++j)  // columns K .. stride - 1 are zero
+        v[c][j] = feature_of<T, C, VEC>(t, c, j) < K ? v[c][j] : 0.0f;
       if constexpr (VEC) {
         const int f = feature_of<T, C, VEC>(t, c, 0);
-        if (f < out_stride) {
-          uint32_t w[2] = {0, 0};
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j / 4] |= (uint32_t)(q[j] & 0xff) << (8 * (j & 3));
-          *(uint2*)(o + f) = make_uint2(w[0], w[1]);
-        }
+        if (f < out_stride) *(uint2*)(o + f) = int8_codes(v[c], q);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int f = feature_of<T, C, VEC>(t, c, j);
-          if (f < out_stride) o[f] = (int8_t)q[j];
+          if (f < out_stride) o[f] = (int8_t)int8_code(v[c][j], q);
         }
       }
     }
@@ -223,83 +210,119 @@ hipError_t launch_rows(const RowArgs& a, int dtype, hipStream_t stream) {
 
 // ---- backward
 //
-// A workgroup of 1024 threads is TEAMS teams that walk the rows of one group
-// (vector) of the norm's parameters; each thread keeps the sums of dg and db of
+// A workgroup is TEAMS teams that walk the rows of one group (vector) of the
+// norm's parameters, R rows a step; each thread keeps the sums of dg and db of
 // its features in registers, the teams' sums are added through LDS at the end
 // and stored as one partial of the workgroup.  A second kernel adds the
-// partials in order, so gradients repeat bit for bit.
+// partials in order, so gradients repeat bit for bit.  The next step's rows are
+// loaded before this step's sums meet (PREFETCH), and rows are kept as they were
+// loaded: what the second half of a step needs is computed again from them.
 
-template <int DT, int T, int C, bool VEC>
-__global__ __launch_bounds__(1024) void norm_backward_kernel(
+template <int DT, int T, int C, bool VEC, int TEAMS>
+__global__ __launch_bounds__(T* TEAMS) void norm_backward_kernel(
     const void* __restrict__ dy, int64_t dy_stride, const void* __restrict__ x, int64_t x_stride,
-    const float* __restrict__ mean, const float* __restrict__ rstd, int64_t rows, int K,
-    const void* __restrict__ gain, int param_dtype, int plus_one, int64_t rows_per_vector, int parts,
-    void* __restrict__ dx, float* __restrict__ partial) {
+    const float* __restrict__ mean, const float* __restrict__ rstd, int K, const void* __restrict__ gain,
+    int param_dtype, int plus_one, int64_t rows_per_vector, int parts, void* __restrict__ dx,
+    float* __restrict__ partial) {
   typedef typename Elem<DT>::T E;
-  constexpr int TEAMS = 1024 / T, W = T / 64;
-  __shared__ float red[2][TEAMS][2][W];
+  constexpr int W = T / 64, R = C == 1 ? 2 : 1;
+  constexpr bool PREFETCH = C == 1;
+  __shared__ float red[2][TEAMS][2 * R][W];
   extern __shared__ float sums[];  // [2][K] of the teams' sums, where TEAMS > 1
-  const int team = threadIdx.x / T, t = threadIdx.x % T, wave = t >> 6;
+  const int team = TEAMS > 1 ? threadIdx.x / T : 0, t = TEAMS > 1 ? threadIdx.x % T : threadIdx.x, wave = t >> 6;
   const int64_t vector = blockIdx.x / parts, part = blockIdx.x % parts;
-  const int64_t r0 = vector * rows_per_vector, r1 = r0 + rows_per_vector;
+  const int64_t r0 = vector * rows_per_vector, r1 = r0 + rows_per_vector, step = (int64_t)parts * TEAMS * R;
   const size_t psize = param_dtype == kF32 ? 4 : 2;
   const char* gr = gain ? (const char*)gain + (size_t)vector * K * psize : nullptr;
-
-  float dg[C][8], db[C][8], g[C][8];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) dg[c][j] = db[c][j] = 0.0f, g[c][j] = 1.0f;
+  const float one = plus_one ? 1.0f : 0.0f, inv_k = 1.0f / (float)K;
+  auto gains = [&](int c, float (&g)[8]) {
     if (gr) {
-      load_param<DT, T, C, VEC>(gr, param_dtype, K, t, c, g[c]);
+      load_param<DT, T, C, VEC>(gr, param_dtype, K, t, c, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[c][j] += plus_one ? 1.0f : 0.0f;
+      for (int j = 0; j < 8; ++j) g[j] += one;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = 1.0f;
     }
-  }
+  };
 
-  // every team makes as many steps (the barriers below): rows past the end count as zeros
+  struct Rows {
+    RawChunk<DT, T, C, VEC> x[R][C], d[R][C];
+    float mu[R], rs[R];
+  };
+  // rows past the end count as zeros (every team makes as many steps: the barriers below)
+  auto load = [&](Rows& q, int64_t base) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t row = base + team * R + i;
+      const bool live = row < r1;
+      q.mu[i] = live ? mean[row] : 0.0f;
+      q.rs[i] = live ? rstd[row] : 0.0f;
+      const int k = live ? K : 0;
+      const E* xr = (const E*)x + (live ? row : r0) * x_stride;
+      const E* dr = (const E*)dy + (live ? row : r0) * dy_stride;
+#pragma unroll
+      for (int c = 0; c < C; ++c) q.x[i][c].load(xr, k, t, c), q.d[i][c].load(dr, k, t, c);
+    }
+  };
+
+  float dg[C][8], db[C][8], g1[8];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dg[c][j] = db[c][j] = 0.0f;
+  if constexpr (C == 1) gains(0, g1);
+  Rows cur, next;
+  load(cur, r0 + part * TEAMS * R);
   int flip = 0;
-  for (int64_t base = r0 + part * TEAMS; base < r1; base += (int64_t)parts * TEAMS) {
-    const int64_t row = base + team;
-    const bool live = row < r1;
-    float u[C][8], d[C][8];
-    float s[2] = {0.0f, 0.0f};
-    float rs = 0.0f;
-    if (live) {
-      const E* xr = (const E*)x + row * x_stride;
-      const E* dr = (const E*)dy + row * dy_stride;
+  for (int64_t base = r0 + part * TEAMS * R; base < r1; base += step) {
+    if constexpr (PREFETCH) load(next, base + step);
+    float s[2 * R];
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        load_chunk<DT, T, C, VEC>(xr, K, t, c, u[c]);
-        load_chunk<DT, T, C, VEC>(dr, K, t, c, d[c]);
-      }
-      const float mu = mean[row];
-      rs = rstd[row];
+    for (int i = 0; i < 2 * R; ++i) s[i] = 0.0f;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
+      float g[8];
+      if constexpr (C > 1) gains(c, g);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        float u[8], d[8];
+        cur.x[i][c].get(u), cur.d[i][c].get(d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const bool in = feature_of<T, C, VEC>(t, c, j) < K;
-          u[c][j] = in ? (u[c][j] - mu) * rs : 0.0f;  // d is zero past the row
-          db[c][j] += d[c][j];
-          dg[c][j] += d[c][j] * u[c][j];
-          d[c][j] *= g[c][j];
-          s[0] += d[c][j];
-          s[1] += d[c][j] * u[c][j];
+          // features past the row: d is zero
+          u[j] = (u[j] - cur.mu[i]) * cur.rs[i];
+          db[c][j] += d[j];
+          dg[c][j] += d[j] * u[j];
+          const float h = d[j] * (C == 1 ? g1[j] : g[j]);
+          s[2 * i] += h;
+          s[2 * i + 1] += h * u[j];
         }
+      }
     }
     team_sum<T>(s, red[flip][team], wave);
     flip ^= 1;  // the next step's sums go elsewhere: one barrier a step is enough
-    if (live) {
-      const float m0 = s[0] / (float)K, m1 = s[1] / (float)K;
-      E* o = (E*)dx + row * (int64_t)K;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
+    for (int c = 0; c < C; ++c) {
+      float g[8];
+      if constexpr (C > 1) gains(c, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[c][j] = rs * (d[c][j] - m0 - u[c][j] * m1);
-        store_chunk<DT, T, C, VEC>(o, K, t, c, d[c]);
+      for (int i = 0; i < R; ++i) {
+        const int64_t row = base + team * R + i;
+        if (row >= r1) continue;
+        const float m0 = s[2 * i] * inv_k, m1 = s[2 * i + 1] * inv_k;
+        float u[8], d[8];
+        cur.x[i][c].get(u), cur.d[i][c].get(d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u[j] = (u[j] - cur.mu[i]) * cur.rs[i];
+          d[j] = cur.rs[i] * (d[j] * (C == 1 ? g1[j] : g[j]) - m0 - u[j] * m1);
+        }
+        store_chunk<DT, T, C, VEC>((E*)dx + row * (int64_t)K, K, t, c, d);
       }
     }
+    if constexpr (PREFETCH) cur = next;
+    else load(cur, base + step);
   }
 
   if (!partial) return;
@@ -382,36 +405,41 @@ struct BackwardArgs {
   float* partial;
 };
 
-// Threads a row takes in the backward kernel.
-int backward_team(int64_t K) { return K <= 512 ? 64 : K <= 1024 ? 128 : K <= 6144 ? 256 : K <= 12288 ? 512 : 1024; }
+// Threads a row takes in the backward kernel, 8 features each (16 or 32 past
+// 8192 features), and the teams of a workgroup.
+constexpr int kTeamThreads[] = {64, 128, 256, 384, 512, 640, 768, 1024};
+int backward_team(int64_t K) {
+  for (int t : kTeamThreads)
+    if (K <= 8 * t) return t;
+  return 1024;
+}
+constexpr int backward_teams(int T) { return T <= 256 ? 512 / T : 1; }
 
 template <int DT, int T, int C, bool VEC>
 hipError_t run_backward(const BackwardArgs& a, hipStream_t stream) {
-  const size_t lds = T < 1024 && a.partial ? (size_t)a.K * 8 : 0;
-  auto kernel = norm_backward_kernel<DT, T, C, VEC>;
-  if (lds > 48 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
+  constexpr int TEAMS = backward_teams(T);
+  const size_t lds = TEAMS > 1 && a.partial ? (size_t)a.K * 8 : 0;  // at most 16 KB
   const int64_t vectors = a.rows / a.rows_per_vector;
-  kernel<<<dim3((unsigned)(vectors * a.parts)), dim3(1024), lds, stream>>>(
-      a.dy, a.dy_stride, a.x, a.x_stride, a.mean, a.rstd, a.rows, (int)a.K, a.gain, a.param_dtype, a.plus_one,
+  norm_backward_kernel<DT, T, C, VEC, TEAMS><<<dim3((unsigned)(vectors * a.parts)), dim3(T * TEAMS), lds, stream>>>(
+      a.dy, a.dy_stride, a.x, a.x_stride, a.mean, a.rstd, (int)a.K, a.gain, a.param_dtype, a.plus_one,
       a.rows_per_vector, a.parts, a.dx, a.partial);
   return hipGetLastError();
 }
 
 template <int DT, bool VEC>
 hipError_t pick_backward(const BackwardArgs& a, hipStream_t s) {
-  const int64_t k = a.K;
-  if (k <= 512) return run_backward<DT, 64, 1, VEC>(a, s);
-  if (k <= 1024) return run_backward<DT, 128, 1, VEC>(a, s);
-  if (k <= 2048) return run_backward<DT, 256, 1, VEC>(a, s);
-  if (k <= 4096) return run_backward<DT, 256, 2, VEC>(a, s);
-  if (k <= 6144) return run_backward<DT, 256, 3, VEC>(a, s);
-  if (k <= 8192) return run_backward<DT, 512, 2, VEC>(a, s);
-  if (k <= 12288) return run_backward<DT, 512, 3, VEC>(a, s);
-  if (k <= 16384) return run_backward<DT, 1024, 2, VEC>(a, s);
-  return run_backward<DT, 1024, 4, VEC>(a, s);
+  if (a.K > 16384) return run_backward<DT, 1024, 4, VEC>(a, s);
+  if (a.K > 8192) return run_backward<DT, 1024, 2, VEC>(a, s);
+  switch (backward_team(a.K)) {
+    case 64: return run_backward<DT, 64, 1, VEC>(a, s);
+    case 128: return run_backward<DT, 128, 1, VEC>(a, s);
+    case 256: return run_backward<DT, 256, 1, VEC>(a, s);
+    case 384: return run_backward<DT, 384, 1, VEC>(a, s);
+    case 512: return run_backward<DT, 512, 1, VEC>(a, s);
+    case 640: return run_backward<DT, 640, 1, VEC>(a, s);
+    case 768: return run_backward<DT, 768, 1, VEC>(a, s);
+    default: return run_backward<DT, 1024, 1, VEC>(a, s);
+  }
 }
 
 }  // namespace
@@ -438,14 +466,14 @@ hipError_t launch_layer_norm_int8(const void* x, int dtype, int64_t rows, int64_
   return launch_rows<kNormCodes>(a, dtype, stream);
 }
 
-// Workgroups that share the rows of one vector: a workgroup a CU in all, and
-// no more than the rows feed.
+// Workgroups that share the rows of one vector: up to 16 waves a CU in all (each
+// workgroup costs a partial of 2 K floats), and no more than the rows feed.
 int layer_norm_parts(int64_t rows, int64_t K, int64_t rows_per_vector) {
-  const int64_t teams = 1024 / backward_team(K), vectors = rows / rows_per_vector;
-  const int64_t steps = (rows_per_vector + teams - 1) / teams;
-  int64_t parts = (256 + vectors - 1) / vectors;
-  if (parts > steps) parts = steps;
-  return (int)(parts < 1 ? 1 : parts);
+  const int64_t team = backward_team(K), teams = backward_teams((int)team), vectors = rows / rows_per_vector;
+  const int64_t step = teams * (K <= 8192 ? 2 : 1), steps = (rows_per_vector + step - 1) / step;
+  const int64_t groups = 256 * std::max<int64_t>(1, 1024 / (team * teams));
+  const int64_t parts = std::min((groups + vectors - 1) / vectors, steps);
+  return (int)std::max<int64_t>(1, parts);
 }
 
 hipError_t launch_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,

@@ -45,14 +45,6 @@ struct RotaryArgs {
   float* partial;              // backward: [workgroups][2][D]
 };
 
-// Sum over aligned groups of G lanes.
-template <int G>
-__device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < G; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
-
 // Where lane c of a head's group finds its two chunks of 8 features: those of
 // pairs 8 c .. 8 c + 7, or behind them 16 features that are not turned.
 template <bool PAIRS>

@@ -59,10 +59,56 @@ __device__ __forceinline__ void store4(const W8a8Operands& p, int m, int n, bool
   }
 }
 
+// LDS position of a 16-byte chunk of a 128-byte row: 16 rows of one fragment read meet no bank twice.
+__device__ __forceinline__ int chunk_swizzle(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+// Partial sums of workgroups that share a tile's K travel through the caller's
+// workspace with device scope (sc1): coherent across the XCDs' L2s without
+// writing one back.  Both are ordinary buffer accesses to the compiler, which
+// waits for them.
+constexpr int kDeviceScope = 16;  // sc1
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t partial_rsrc(void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(base, (short)0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ void store_partial(__amdgpu_buffer_rsrc_t r, uint32_t off, const i32x4& v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, (int)off, 0, kDeviceScope);
+}
+__device__ __forceinline__ i32x4 load_partial(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, kDeviceScope));
+}
+
+// Called by every thread of a workgroup after its store_partials: whether it is
+// the last of the `splits` workgroups of its tile to arrive, whose partials are
+// then all in memory.  The counter is back at zero when the launch ends.
+__device__ __forceinline__ bool last_to_arrive(int* counter, int splits, int* shared) {
+  __builtin_amdgcn_s_waitcnt(0);  // this wave's partials are at the coherence point
+  asm volatile("" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int n = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool last = n == splits - 1;
+    if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *shared = last;
+  }
+  __syncthreads();
+  return *shared != 0;
+}
+
+constexpr int kMaxSplitTile = 128 * 128;  // tiles up to this size may share their K between workgroups
+
+// How a launch shares K: `splits` workgroups a tile, each `kblocks` blocks of 128.
+struct W8a8Split {
+  int splits = 1, kblocks = 0;
+  int* counters = nullptr;
+  uint8_t* partials = nullptr;
+};
+
 // The tiled product of one output type (gemm_w8a8_tile.h, one source a type);
 // `tile` is one of W8A8_TILES.
 template <int ODT>
-hipError_t launch_w8a8_tile(int tile, const W8a8Operands& p, hipStream_t stream);
+hipError_t launch_w8a8_tile(int tile, const W8a8Operands& p, const W8a8Split& split, hipStream_t stream);
 
 constexpr int tile_code(int bm, int bn) { return bm | bn << 10; }
 

@@ -451,11 +451,30 @@ int convrot_quantize_int8(const void* x, int dtype, int64_t rows, int64_t featur
  * (multiples of 16, at most 2^22), 16-byte aligned.  Where K is no multiple of
  * 16, a stride covers the next one, and the weight's bytes from K to there are
  * zero (the activations' may be anything).  K <= 65536.  out [M, N] contiguous.
+ * workspace (may be NULL): the W4A4 / W4A16 GEMMs' (convrot_w4a4_workspace_bytes,
+ * zero-filled once), which lets workgroups share the K of few tiles; the same
+ * bits with and without it.
  */
 int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscales, const int8_t* weight,
                       int64_t weight_stride, const float* wscales, const float* bias, int64_t M, int64_t N,
                       int64_t K, const void* residual, const void* gate, int64_t gate_stride,
-                      int64_t rows_per_gate, void* out, int out_dtype, void* stream);
+                      int64_t rows_per_gate, void* workspace, int64_t workspace_bytes, void* out, int out_dtype,
+                      void* stream);
+
+/*
+ * The whole 8-bit linear: convrot_quantize_int8 of x, then convrot_w8a8_gemm to
+ * the type of x, the same bits as the two calls.  scratch holds the codes and
+ * scales between them: convrot_w8a8_scratch_bytes(M, K) bytes, 16-byte aligned,
+ * of any content.  It may be NULL where convrot_w8a8_fused says that the rows
+ * are quantized inside the product's launch (few rows) and out does not overlap x.
+ */
+int64_t convrot_w8a8_scratch_bytes(int64_t M, int64_t K);
+int convrot_w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride);
+int convrot_w8a8_linear(const void* x, int dtype, int64_t x_stride, const int8_t* weight, int64_t weight_stride,
+                        const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K,
+                        const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate,
+                        void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* out,
+                        void* stream);
 
 /*
  * Layer norm: out = dt((x - mean) * rstd * g + b), in float32, rounded once,
@@ -562,7 +581,8 @@ const char* convrot_last_error(void);
  *   gemm_mfma32      "0" | "1"            4-wave 256x256 W4A4 tile on 32x32x32 MFMAs: never,
  *                                         or always (plain 16-bit outputs)
  *   fp6_tile         "BMxBN"              FP6 W4A4 tile: 256x256, 256x224, 128x256, 128x192 or 128x128
- *   w8a8_tile        "BMxBN"              W8A8 tile (256x256 .. 64x64); "0x0": the few-row kernel
+ *   w8a8_tile        "BMxBN"              W8A8 tile (256x256 .. 64x64), for few rows too
+ *   w8a8_split       "1" .. "64"          workgroups that share a W8A8 tile's K (with a workspace)
  * Returns CONVROT_ERR_INVALID for an unknown name, a malformed value or a
  * tile the library does not build.
  */

@@ -58,7 +58,7 @@ def test_product(dev, m, n, k, dtype):
 
 
 TILES = ["256x256", "256x224", "224x256", "256x192", "192x256", "256x128", "128x256", "192x192", "192x128", "128x192",
-         "160x128", "128x160", "128x128", "128x64", "64x128", "64x64", "0x0"]
+         "160x128", "128x160", "128x128", "128x64", "64x128", "64x64"]
 
 
 @pytest.mark.parametrize("tile", TILES)
@@ -70,6 +70,56 @@ def test_every_kernel(dev, tuning, tile, m, n, k):
     for dtype in (BF16, F32):
         host, (qa, qw, xs, ws, bias) = operands(m + k, m, n, k, dev)
         assert torch.equal(hip_w8a8_matmul(qa, qw, xs, ws, bias, output_dtype=dtype).cpu(), product_plain(*host, dtype))
+
+
+@pytest.mark.parametrize("split", [2, 3, 7, 64])
+@pytest.mark.parametrize("tile,m", [(None, 1), (None, 16), ("64x64", 70), ("128x64", 200), ("64x128", 65), ("128x128", 300)])
+def test_shared_k(dev, tuning, tile, m, split):
+    """Workgroups that share a tile's K add integer sums: the same bits, launch after launch."""
+    from convrot_mlx_amd import hip_w8a8_matmul
+
+    tuning.set("w8a8_tile", tile)
+    tuning.set("w8a8_split", split)
+    for n, k in ((70, 1000), (200, 4112)):
+        k16 = k - k % 16
+        host, (qa, qw, xs, ws, bias) = operands(m + k, m, n, k16, dev)
+        want = product_plain(*host, BF16)
+        for _ in range(3):
+            assert torch.equal(hip_w8a8_matmul(qa, qw, xs, ws, bias, output_dtype=BF16).cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,k", [(1, 16), (1, 3072), (1, 12288), (1, 24576), (2, 4112), (3, 128), (7, 1040), (8, 3072),
+                                 (16, 1536), (16, 1600), (5, 6144)])
+def test_few_rows_quantized_in_the_launch(dev, m, k, dtype):
+    from convrot_mlx_amd import hip_w8a8_linear, hip_w8a8_matmul, quantize_int8_rowwise
+
+    n = 150
+    host, (_, qw, _, ws, bias) = operands(m + k, m, n, k, dev)
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(k)) * 2
+    if m > 2:
+        x[1], x[2, k // 2] = 0.0, float("nan")
+    x = x.to(dtype).to(dev)
+    got = hip_w8a8_linear(x, qw, ws, bias)
+    codes, scales = quantize_int8_rowwise(x)
+    want = hip_w8a8_matmul(codes, qw, scales, ws, bias, output_dtype=dtype)
+    assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0))
+    clean = [r for r in range(m) if not (m > 2 and r == 2)]
+    plain = product_plain(codes.cpu().numpy(), host[1], scales.cpu().numpy(), *host[3:], dtype)
+    assert torch.equal(got.cpu()[clean], plain[clean])
+    if m > 2:
+        assert got[2].isnan().all()
+
+
+def test_few_rows_in_place_over_their_input(dev):
+    """x as its own residual: every workgroup reads all of x, so the rows are quantized first."""
+    from convrot_mlx_amd import hip_w8a8_linear
+
+    _, (_, qw, _, ws, bias) = operands(3, 4, 256, 256, dev)
+    x = torch.randn((4, 256), generator=torch.Generator().manual_seed(3)).to(BF16).to(dev)
+    want = hip_w8a8_linear(x, qw, ws, bias, residual=x.clone())
+    got = hip_w8a8_linear(x, qw, ws, bias, residual=x, inplace=True)
+    assert got.data_ptr() == x.data_ptr() and torch.equal(x, want)
 
 
 @pytest.mark.parametrize("k", [1, 5, 15, 17, 100, 127, 129, 1001])
