@@ -46,12 +46,12 @@ def quantize_int8_rowwise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return codes if codes.shape[1] == k else codes[:, :k], scales
 
 
-def _operand(t: torch.Tensor, what: str, zero_tail: bool) -> torch.Tensor:
+def _operand(t: torch.Tensor, zero_tail: bool) -> torch.Tensor:
     """An int8 matrix as rows the product can read: adjacent features, 16-byte aligned rows that
     cover the features rounded up to 16 (past them zeros, with `zero_tail`); else a padded copy."""
-    if t.ndim != 2 or t.dtype != torch.int8:
-        raise ValueError(f"W8A8 {what} must be 2D int8, got {tuple(t.shape)} {t.dtype}")
     k = t.shape[1]
+    if k % 16 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     if (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= _round16(k) and t.data_ptr() % 16 == 0
             and (k % 16 == 0 or (not zero_tail and t.shape[0] * t.stride(0) + t.storage_offset()
                                  <= t.untyped_storage().nbytes()))):
@@ -59,8 +59,12 @@ def _operand(t: torch.Tensor, what: str, zero_tail: bool) -> torch.Tensor:
     return torch.nn.functional.pad(t, (0, -k % 16)) if k % 16 else t.clone(memory_format=torch.contiguous_format)
 
 
+def _scales(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else _f32(t)
+
+
 def _check_scales(name: str, t: torch.Tensor, n: int) -> None:
-    if tuple(t.shape) != (n,):
+    if t.ndim != 1 or t.shape[0] != n:
         raise ValueError(f"W8A8 {name} must have shape {(n,)}, got {tuple(t.shape)}")
 
 
@@ -81,7 +85,7 @@ def _w8a8(act, weight, xscales, wscales, bias, k: int, dtype: torch.dtype, gr: G
     """The product of operands as the kernel reads them (see _operand)."""
     m, n = act.shape[0], weight.shape[0]
     out = _output(gr, m, n, dtype, act.device)
-    stream = torch.cuda.current_stream(act.device).cuda_stream
+    stream = nat.stream_handle(act.device)
     work = _workspace(act.device, stream)
     nat.check(nat.load().convrot_w8a8_gemm(
         act.data_ptr(), act.stride(0), xscales.data_ptr(), weight.data_ptr(), weight.stride(0), wscales.data_ptr(),
@@ -102,7 +106,7 @@ def _linear(x: torch.Tensor, weight: torch.Tensor, wscales, bias, k: int, residu
     scratch = None
     if gr is not None or m > 16 or not lib.convrot_w8a8_fused(x2d.data_ptr(), dtype, m, k, stride):
         scratch = torch.empty((m * (_round16(k) + 4),), dtype=torch.uint8, device=device)
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = nat.stream_handle(device)
     work = _workspace(device, stream)
     nat.check(lib.convrot_w8a8_linear(
         x2d.data_ptr(), dtype, stride, weight.data_ptr(), weight.stride(0), wscales.data_ptr(),
@@ -149,10 +153,10 @@ def hip_w8a8_matmul(qact: torch.Tensor, qweight: torch.Tensor, xscales: torch.Te
     n = _check_product(k, qweight, wscales, bias)
     _check_scales("activation scales", xscales, m)
     nat.dtype_code(output_dtype)
-    nat.require_device(qact, qweight, xscales, wscales, bias)
+    nat.on_device(qact, qweight, xscales, wscales, bias)
     gr = _residual(residual, gate, inplace, m, n, output_dtype)
-    return _w8a8(_operand(qact, "activation", False), _operand(qweight, "weight", True), _f32(xscales), _f32(wscales),
-                 _f32(bias), k, output_dtype, gr)
+    return _w8a8(_operand(qact, False), _operand(qweight, True), _scales(xscales), _scales(wscales),
+                 _scales(bias), k, output_dtype, gr)
 
 
 def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, bias: torch.Tensor | None = None,
@@ -162,8 +166,8 @@ def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tenso
     rounding at the end."""
     k = x.shape[-1]
     _check_product(k, qweight, wscales, bias)
-    nat.require_device(x, qweight, wscales, bias)
-    return _linear(x, _operand(qweight, "weight", True), _f32(wscales), _f32(bias), k, residual, gate, inplace)
+    nat.on_device(x, qweight, wscales, bias)
+    return _linear(x, _operand(qweight, True), _scales(wscales), _scales(bias), k, residual, gate, inplace)
 
 
 class Int8Linear(nn.Module):
@@ -212,8 +216,8 @@ class Int8Linear(nn.Module):
         if residual is not None and tuple(residual.shape) != (*x.shape[:-1], self.out_features):
             raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
                              f"{(*x.shape[:-1], self.out_features)}")
-        nat.require_device(x, self.qweight)
-        return _linear(x, self._weight(), _f32(self.scales), _f32(self.bias), self.in_features, residual, gate, inplace)
+        nat.on_device(x, self.qweight, self.scales, self.bias)
+        return _linear(x, self._weight(), _scales(self.scales), _scales(self.bias), self.in_features, residual, gate, inplace)
 
     def forward_modulated(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, eps: float = 1e-6, *,
                           residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
@@ -237,7 +241,7 @@ class Int8Linear(nn.Module):
             nat.ptr(x2d), nat.dtype_code(x.dtype), m, k, x2d.stride(0), nat.ptr(gain), nat.ptr(sh),
             nat.dtype_code(gain.dtype), 1, each, float(eps), nat.ptr(codes), codes.shape[1], nat.ptr(scales),
             nat.stream_of(device)))
-        out = _w8a8(codes, self._weight(), scales, _f32(self.scales), _f32(self.bias), k, x.dtype, gr)
+        out = _w8a8(codes, self._weight(), scales, _scales(self.scales), _scales(self.bias), k, x.dtype, gr)
         return residual if inplace else out.reshape(*x.shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:

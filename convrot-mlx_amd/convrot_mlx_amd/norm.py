@@ -25,8 +25,8 @@ def rows_of(x: torch.Tensor) -> torch.Tensor:
 
 
 def norm_operands(x2d, weight, bias, scale, shift):
-    """(gain [V, K] or None, shift [V, K] or None, rows a vector, plus one?) of a norm's
-    parameters, both of one type that the kernels take beside x's."""
+    """(gain or None, shift or None, rows a vector, plus one?) of a norm's parameters: contiguous
+    rows of K, both of one type that the kernels take beside x's."""
     rows, k = x2d.shape
     if (weight is not None or bias is not None) and (scale is not None or shift is not None):
         raise ValueError("layer norm takes weight and bias, or scale and shift")
@@ -44,8 +44,14 @@ def norm_operands(x2d, weight, bias, scale, shift):
         raise ValueError(f"shift has {given[-1].numel() // k} rows but scale has {vectors}")
     if rows % vectors:
         raise ValueError(f"{rows} activation rows do not split evenly over {vectors} modulation vectors")
-    kind = x2d.dtype if all(t.dtype == x2d.dtype for t in given) else torch.float32
-    gain, add = (None if t is None else t.reshape(vectors, k).to(kind).contiguous() for t in (gain, add))
+    kind = x2d.dtype
+    for t in given:
+        if t.dtype != kind:
+            kind = torch.float32
+    if gain is not None and not (gain.dtype == kind and gain.is_contiguous()):
+        gain = gain.to(kind).contiguous()
+    if add is not None and not (add.dtype == kind and add.is_contiguous()):
+        add = add.to(kind).contiguous()
     return gain, add, max(1, rows // vectors), plus_one
 
 
@@ -57,19 +63,19 @@ def hip_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     weight, bias: [K].  Or scale, shift: [V, K] or [V, 1, K], the rows split evenly over the V
     vectors in order, as x [B, L, K] beside scale [B, 1, K] does: (1 + scale) * u + shift.  Either
     of a pair may be None.  With return_stats also the rows' float32 mean and 1 / sqrt(var + eps)."""
-    nat.require_device(x, weight, bias, scale, shift)
+    device = nat.on_device(x, weight, bias, scale, shift)
     k = x.shape[-1]
-    x2d = rows_of(x.reshape(-1, k))
+    x2d = rows_of(x if x.ndim == 2 else x.reshape(-1, k))
     rows = x2d.shape[0]
     gain, add, each, plus_one = norm_operands(x2d, weight, bias, scale, shift)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty(x.shape, dtype=x.dtype, device=device)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if return_stats else None
     mean, rstd = (None, None) if stats is None else stats.unbind(0)
     kind = gain if gain is not None else add
     nat.check(nat.load().convrot_layer_norm(
-        nat.ptr(x2d), nat.dtype_code(x.dtype), rows, k, x2d.stride(0), nat.ptr(gain), nat.ptr(add),
-        nat.dtype_code(x.dtype if kind is None else kind.dtype), int(plus_one), each, float(eps), nat.ptr(out),
-        nat.ptr(mean), nat.ptr(rstd), nat.stream_of(x.device)))
+        x2d.data_ptr(), nat.dtype_code(x.dtype), rows, k, x2d.stride(0), nat.address(gain), nat.address(add),
+        nat.dtype_code(x.dtype if kind is None else kind.dtype), plus_one, each, eps, out.data_ptr(),
+        nat.address(mean), nat.address(rstd), nat.stream_handle(device)))
     return out if stats is None else (out, mean, rstd)
 
 
@@ -101,7 +107,7 @@ def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
             raise ValueError(f"{rows} activation rows do not split evenly over {vectors} modulation vectors")
         each = max(1, rows // vectors)
     if gain is not None:
-        vectors = gain.shape[0]
+        vectors = gain.numel() // k
     given = scale if scale is not None else weight
     kind = x.dtype if gain is None else gain.dtype
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -112,10 +118,10 @@ def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
         work = torch.empty((lib.convrot_layer_norm_workspace_bytes(rows, k, each),), dtype=torch.uint8,
                            device=x.device)
     nat.check(lib.convrot_layer_norm_backward(
-        nat.ptr(dy2d), dy2d.stride(0), nat.ptr(x2d), x2d.stride(0), nat.ptr(mean), nat.ptr(rstd),
-        nat.dtype_code(x.dtype), rows, k, nat.ptr(gain), nat.dtype_code(kind), int(plus_one), each, nat.ptr(dx),
-        nat.ptr(None if grads is None else grads[0]), nat.ptr(None if grads is None else grads[1]), nat.ptr(work),
-        0 if work is None else work.numel(), nat.stream_of(x.device)))
+        dy2d.data_ptr(), dy2d.stride(0), x2d.data_ptr(), x2d.stride(0), mean.data_ptr(), rstd.data_ptr(),
+        nat.dtype_code(x.dtype), rows, k, nat.address(gain), nat.dtype_code(kind), plus_one, each, dx.data_ptr(),
+        None if grads is None else grads[0].data_ptr(), None if grads is None else grads[1].data_ptr(),
+        nat.address(work), 0 if work is None else work.numel(), nat.stream_handle(x.device)))
     if grads is None:
         return dx, None, None
     if rows == 0:

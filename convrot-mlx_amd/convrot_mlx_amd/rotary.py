@@ -51,27 +51,31 @@ def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
 
 def _check(q, k, table, q_weight, k_weight):
     b, _, length, d = q.shape
-    if k.shape[0] != b or k.shape[2] != length or k.shape[3] != d:
+    kb, _, klength, kd = k.shape
+    if kb != b or klength != length or kd != d:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch, length and dim")
     if k.dtype != q.dtype:
         raise ValueError(f"k dtype {k.dtype} differs from q dtype {q.dtype}")
     if d > MAX_HEAD_DIM:
         raise ValueError(f"rotary positions support heads of up to {MAX_HEAD_DIM} features, got {d}")
-    if table.ndim not in (3, 4) or table.shape[-1] != 2 or table.shape[-3] != length or table.dtype != torch.float32:
+    size = table.shape
+    if len(size) not in (3, 4) or size[-1] != 2 or size[-3] != length or table.dtype != torch.float32:
         raise ValueError(f"table must be float32 [batch or 1, {length}, pairs, 2], got {table.dtype} "
                          f"{tuple(table.shape)}")
-    if table.ndim == 4 and table.shape[0] not in (1, b):
-        raise ValueError(f"table has {table.shape[0]} batch entries for a batch of {b}")
-    if 2 * table.shape[-2] > d:
-        raise ValueError(f"{table.shape[-2]} pairs do not fit a head of {d} features")
+    if len(size) == 4 and size[0] not in (1, b):
+        raise ValueError(f"table has {size[0]} batch entries for a batch of {b}")
+    if 2 * size[-2] > d:
+        raise ValueError(f"{size[-2]} pairs do not fit a head of {d} features")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and tuple(w.shape) != (d,):
             raise ValueError(f"{name} must have shape {(d,)}, got {tuple(w.shape)}")
-    nat.require_device(q, k, table, q_weight, k_weight)
+    nat.on_device(q, k, table, q_weight, k_weight)
 
 
 def _weights(q_weight, k_weight, dtype):
     """The norm weights in one type that the kernel takes (x's or float32)."""
+    if q_weight is None and k_weight is None:
+        return None, None, dtype
     given = [w for w in (q_weight, k_weight) if w is not None]
     kind = dtype if all(w.dtype == dtype for w in given) else torch.float32
     qw, kw = (None if w is None else w.to(kind).contiguous() for w in (q_weight, k_weight))
@@ -80,8 +84,9 @@ def _weights(q_weight, k_weight, dtype):
 
 def _table_args(table: torch.Tensor):
     """(table, floats between batch entries): its last three axes dense."""
-    pairs = table.shape[-2]
-    dense = (2 * pairs, 2, 1)
+    if table.is_contiguous():
+        return table, table.stride(0) if table.ndim == 4 and table.shape[0] > 1 else 0
+    dense = (2 * table.shape[-2], 2, 1)
     if any(n > 1 and s != want for n, s, want in zip(table.shape[-3:], table.stride()[-3:], dense)):
         table = table.contiguous()
     stride = table.stride(0) if table.ndim == 4 and table.shape[0] > 1 else 0
@@ -116,13 +121,14 @@ def hip_qk_rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, *, q_we
     _check(q, k, table, q_weight, k_weight)
     qw, kw, kind = _weights(q_weight, k_weight, q.dtype)
     table, table_stride = _table_args(table)
+    if q_out is not None or k_out is not None:
+        nat.on_device(q, q_out, k_out)
     q_out, k_out = _out("q_out", q_out, q), _out("k_out", k_out, k)
-    nat.require_device(q, q_out, k_out)
     b, hq, length, d = q.shape
     nat.check(nat.load().convrot_qk_rotary(
-        nat.ptr(q), nat.ptr(k), nat.ptr(q_out), nat.ptr(k_out), _strides(q, k, q_out, k_out),
-        nat.dtype_code(q.dtype), b, hq, k.shape[1], length, d, nat.ptr(table), table.shape[-2], table_stride,
-        nat.ptr(qw), nat.ptr(kw), nat.dtype_code(kind), float(eps), int(interleaved), nat.stream_of(q.device)))
+        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), _strides(q, k, q_out, k_out),
+        nat.dtype_code(q.dtype), b, hq, k.shape[1], length, d, table.data_ptr(), table.shape[-2], table_stride,
+        nat.address(qw), nat.address(kw), nat.dtype_code(kind), eps, interleaved, nat.stream_handle(q.device)))
     return q_out, k_out
 
 
@@ -138,7 +144,7 @@ def hip_qk_rotary_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, 
     if dq.shape != q.shape or dk.shape != k.shape or dq.dtype != q.dtype or dk.dtype != q.dtype:
         raise ValueError(f"dq {dq.dtype} {tuple(dq.shape)} and dk {dk.dtype} {tuple(dk.shape)} must match q "
                          f"{q.dtype} {tuple(q.shape)} and k {tuple(k.shape)}")
-    nat.require_device(q, dq, dk)
+    nat.on_device(q, dq, dk)
     qw, kw, kind = _weights(q_weight, k_weight, q.dtype)
     table, table_stride = _table_args(table)
     b, hq, length, d = q.shape
@@ -154,11 +160,11 @@ def hip_qk_rotary_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, 
         gw = torch.empty((2, d), dtype=kind, device=q.device)
         work = torch.empty((lib.convrot_qk_rotary_workspace_bytes(d),), dtype=torch.uint8, device=q.device)
     nat.check(lib.convrot_qk_rotary_backward(
-        nat.ptr(dq), nat.ptr(dk), nat.ptr(q), nat.ptr(k), nat.ptr(gq), nat.ptr(gk),
-        nat.ptr(gw[0] if qw is not None else None), nat.ptr(gw[1] if kw is not None else None),
-        _strides(dq, dk, q, k, gq, gk), nat.dtype_code(q.dtype), b, hq, k.shape[1], length, d, nat.ptr(table),
-        table.shape[-2], table_stride, nat.ptr(qw), nat.ptr(kw), nat.dtype_code(kind), float(eps), int(interleaved),
-        nat.ptr(work), 0 if work is None else work.numel(), nat.stream_of(q.device)))
+        dq.data_ptr(), dk.data_ptr(), q.data_ptr(), k.data_ptr(), gq.data_ptr(), gk.data_ptr(),
+        None if qw is None else gw[0].data_ptr(), None if kw is None else gw[1].data_ptr(),
+        _strides(dq, dk, q, k, gq, gk), nat.dtype_code(q.dtype), b, hq, k.shape[1], length, d, table.data_ptr(),
+        table.shape[-2], table_stride, nat.address(qw), nat.address(kw), nat.dtype_code(kind), eps, interleaved,
+        nat.address(work), 0 if work is None else work.numel(), nat.stream_handle(q.device)))
     if gw is not None and b * length * (hq + k.shape[1]) == 0:
         gw.zero_()
     return (gq, gk, None if qw is None else gw[0].to(q_weight.dtype), None if kw is None else gw[1].to(k_weight.dtype))

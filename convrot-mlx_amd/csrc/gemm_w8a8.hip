@@ -18,11 +18,11 @@ namespace {
 // keeps full by direct-to-LDS loads; the rows' codes lie in LDS from the start.
 // Where the channels make too few workgroups for the chip, several share K and
 // the last to arrive adds their integer sums.  With FUSED the rows come as they
-// are and each workgroup quantizes them itself (as convrot_quantize_int8 does)
-// while the first weights are on their way: one launch instead of two.
+// are and each workgroup quantizes them itself (as convrot_quantize_int8 does):
+// one launch instead of two.  Rows or codes are the first loads, the ring's fill
+// the next: the quantization runs while the first weights are on their way.
 constexpr int kRowsMax = 16, kRowsN = 64;
-constexpr int kFusedChunks = 12;  // of 8 values a thread: the rows of a fused call hold up to 24576
-constexpr int64_t kFusedMax = 256 * 8 * kFusedChunks;
+constexpr int kFusedBytes = 16384;  // of a fused call's rows, which lie in LDS beside their codes
 
 __device__ __forceinline__ uint32_t max16(uint32_t v) {
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xf, 0xf, true));
@@ -43,8 +43,29 @@ __global__ __launch_bounds__(256) void w8a8_rows_kernel(W8a8Operands p, const vo
   const int kblocks = (p.K + 127) / 128, kb0 = part * split.kblocks, n = min(split.kblocks, kblocks - kb0);
   const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u, k0 = (uint32_t)kb0 * 128u, kn = (uint32_t)n * 128u;
   uint8_t* ring = smem + wave * (STAGES * 2048);
-  uint8_t* codes = smem + 4 * STAGES * 2048;  // [M][kn], chunks swizzled
+  uint8_t* codes = smem + 4 * STAGES * 2048;      // [M][kn], chunks swizzled
+  uint8_t* raw = codes + (uint32_t)p.M * kn;      // FUSED: the rows as they are
   const uint32_t ring_addr = (uint32_t)(uintptr_t)ring;
+
+  if constexpr (FUSED) {
+    // 16-byte chunk i of the rows behind each other, a wave 64 of them at a time
+    constexpr uint32_t ES = DT == kF32 ? 4 : 2;
+    const uint32_t per_row = (uint32_t)p.K * ES / 16u, chunks = (uint32_t)p.M * per_row;
+    const i32x4_sgpr rx = buffer_rsrc(x, (uint32_t)(((int64_t)(p.M - 1) * x_stride + p.K) * ES));
+    for (uint32_t i0 = wave * 64u; i0 < chunks; i0 += 256u) {
+      const uint32_t i = i0 + (uint32_t)lane, r = p.M == 1 ? 0u : i / per_row;
+      const uint32_t off = i < chunks ? (uint32_t)(r * (uint32_t)x_stride * ES) + (i - r * per_row) * 16u : kOutOfRange;
+      dma16(rx, off, (uint32_t)(uintptr_t)raw + i0 * 16u);
+    }
+  } else {
+    const uint32_t per_row = kn / 16u, chunks = (uint32_t)p.M * per_row;
+    const i32x4_sgpr ra = buffer_rsrc(p.act, (uint32_t)(p.M - 1) * (uint32_t)p.lda + k16);
+    for (uint32_t i0 = wave * 64u; i0 < chunks; i0 += 256u) {
+      const uint32_t i = i0 + (uint32_t)lane, r = p.M == 1 ? 0u : i / per_row, at = i - r * per_row;
+      const uint32_t k = k0 + (at >> 3) * 128u + (((at & 7u) ^ (uint32_t)chunk_swizzle((int)r)) << 4);
+      dma16(ra, i < chunks && k < k16 ? r * (uint32_t)p.lda + k : kOutOfRange, (uint32_t)(uintptr_t)codes + i0 * 16u);
+    }
+  }
 
   // the wave's 16 weight rows (none past N)
   const int nw = tile * kRowsN + wave * 16, nrows = min(16, p.N - nw);
@@ -71,69 +92,45 @@ __global__ __launch_bounds__(256) void w8a8_rows_kernel(W8a8Operands p, const vo
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) issue(min((uint32_t)(kb0 + s), lastkb), s);
 
-  // place of the 8 or 16 codes at feature k of row r
+  if (FUSED && tid < kRowsMax) row_max[tid] = 0;
+  wait_vmcnt<2 * STAGES>();  // the rows, but not the ring
+  __syncthreads();
+  // place of the codes at feature k of row r
   auto code_at = [&](int r, uint32_t k) {
     const uint32_t b = (k - k0) >> 7, ch = (k >> 4) & 7;
     return codes + (uint32_t)r * kn + b * 128u + ((ch ^ (uint32_t)chunk_swizzle(r)) << 4) + (k & 15u);
   };
   if constexpr (FUSED) {
     typedef typename Elem<DT>::T E;
-    constexpr int W = DT == kF32 ? 2 : 1;
-    if (tid < kRowsMax) row_max[tid] = 0;
-    __syncthreads();
     const uint32_t total = (uint32_t)p.M * (uint32_t)p.K;
-    uint4 raw[kFusedChunks][W];
-    uint32_t row[kFusedChunks], col[kFusedChunks];
-#pragma unroll
-    for (int i = 0; i < kFusedChunks; ++i) {
-      const uint32_t at = (uint32_t)(i * 256 + tid) * 8u;
-      row[i] = at / (uint32_t)p.K;
-      col[i] = at - row[i] * (uint32_t)p.K;
-#pragma unroll
-      for (int w = 0; w < W; ++w) raw[i][w] = make_uint4(0, 0, 0, 0);
-      if (at < total) {
-        const uint4* src = (const uint4*)((const E*)x + (int64_t)row[i] * x_stride + col[i]);
-#pragma unroll
-        for (int w = 0; w < W; ++w) raw[i][w] = src[w];
-      }
-    }
-    auto values = [&](int i, float (&v)[8]) { load8<DT>((const E*)&raw[i][0], v); };
-#pragma unroll
-    for (int i = 0; i < kFusedChunks; ++i) {
-      if ((uint32_t)i * 2048u >= total) break;
-      float v[8];
-      values(i, v);
+    // 8 values a thread, 16 lanes' 128 in one row where K % 128 == 0 (past the end: zeros)
+    for (uint32_t i0 = 0; i0 < total; i0 += 2048u) {
+      const uint32_t at = i0 + (uint32_t)tid * 8u, r = p.M == 1 ? 0u : at / (uint32_t)p.K;
       uint32_t most = 0;
+      if (at < total) {
+        float v[8];
+        load8<DT>((const E*)raw + at, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
-      const bool live = (uint32_t)(i * 256 + tid) * 8u < total;
-      if ((p.K & 127) == 0) {  // 16 lanes of one row (or past the end, zeros)
+        for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+      }
+      if ((p.K & 127) == 0) {
         most = max16(most);
-        if ((lane & 15) == 0 && live) atomicMax(&row_max[row[i]], most);
-      } else if (live) {
-        atomicMax(&row_max[row[i]], most);
+        if ((lane & 15) == 0 && at < total) atomicMax(&row_max[r], most);
+      } else if (at < total) {
+        atomicMax(&row_max[r], most);
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kFusedChunks; ++i) {
-      if ((uint32_t)i * 2048u >= total) break;
-      if ((uint32_t)(i * 256 + tid) * 8u >= total || col[i] < k0 || col[i] >= k0 + kn) continue;
-      const Int8Row q = int8_row(row_max[row[i]]);
+    for (uint32_t at = (uint32_t)tid * 8u; at < total; at += 2048u) {
+      const uint32_t r = p.M == 1 ? 0u : at / (uint32_t)p.K, k = at - r * (uint32_t)p.K;
+      if (k < k0 || k >= k0 + kn) continue;
       float v[8];
-      values(i, v);
-      *(uint2*)code_at((int)row[i], col[i]) = int8_codes(v, q);
+      load8<DT>((const E*)raw + at, v);
+      *(uint2*)code_at((int)r, k) = int8_codes(v, int8_row(row_max[r]));
     }
     if (tid < p.M) row_scale[tid] = int8_row(row_max[tid]).scale;
-  } else {
-    const uint32_t per_row = kn / 16u;
-    for (uint32_t i = tid; i < (uint32_t)p.M * per_row; i += 256) {
-      const uint32_t r = i / per_row, k = k0 + (i - r * per_row) * 16u;
-      if (k < k16) *(uint4*)code_at((int)r, k) = *(const uint4*)(p.act + (int64_t)r * p.lda + k);
-    }
-    if (tid < p.M) row_scale[tid] = p.xscales[tid];
+    __syncthreads();
   }
-  __syncthreads();
 
   const int q = lane >> 4, r = lane & 15, ra = min(r, p.M - 1);  // columns past M: some row's, never stored
   i32x4 acc = {0, 0, 0, 0};
@@ -166,7 +163,7 @@ __global__ __launch_bounds__(256) void w8a8_rows_kernel(W8a8Operands p, const vo
   }
   const int nn = nw + 4 * q;
   if (r >= p.M || nn >= p.N) return;
-  const float xs = row_scale[r];
+  const float xs = FUSED ? row_scale[r] : p.xscales[r];
   float o[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -237,13 +234,15 @@ bool rows_kernel(int64_t M) {
   return forced > 0 ? false : M <= kRowsMax;
 }
 
-// LDS of the few-row kernel: ring and codes.
-size_t rows_lds(int64_t M, int stages, int kblocks) { return (size_t)stages * 8192 + (size_t)M * kblocks * 128; }
+// LDS of the few-row kernel: ring, codes and (fused) the rows as they are, in whole DMAs of 1 KB.
+size_t rows_lds(int64_t M, int stages, int kblocks, int64_t raw_bytes) {
+  return (size_t)stages * 8192 + ((size_t)M * kblocks * 128 + 1023) / 1024 * 1024 + (size_t)(raw_bytes + 1023) / 1024 * 1024;
+}
 
 template <int DT, bool FUSED, int STAGES>
 hipError_t launch_rows_s(const W8a8Operands& p, const void* x, int64_t x_stride, const W8a8Split& split, int tiles,
                          hipStream_t s) {
-  const size_t lds = rows_lds(p.M, STAGES, split.kblocks);
+  const size_t lds = rows_lds(p.M, STAGES, split.kblocks, FUSED ? (int64_t)p.M * p.K * (DT == kF32 ? 4 : 2) : 0);
   w8a8_rows_kernel<DT, FUSED, STAGES><<<dim3((unsigned)(tiles * split.splits)), dim3(256), lds, s>>>(p, x, x_stride,
                                                                                                     split, tiles);
   return hipGetLastError();
@@ -255,13 +254,15 @@ hipError_t launch_rows(const W8a8Operands& p, const void* x, int64_t x_stride, c
   const int kblocks = (p.K + 127) / 128;
   W8a8Split split = make_split(choose_splits(tiles, kblocks, 4096, work), kblocks, work);
   // two workgroups a CU where the codes leave room beside the deep ring, else beside the short one
-  const bool deep = rows_lds(p.M, 8, split.kblocks) <= 80 * 1024 || rows_lds(p.M, 4, split.kblocks) > 80 * 1024;
+  const int64_t raw = FUSED ? (int64_t)p.M * p.K * (DT == kF32 ? 4 : 2) : 0;
+  const bool deep =
+      rows_lds(p.M, 8, split.kblocks, raw) <= 80 * 1024 || rows_lds(p.M, 4, split.kblocks, raw) > 80 * 1024;
   if (deep) return launch_rows_s<DT, FUSED, 8>(p, x, x_stride, split, (int)tiles, s);
   return launch_rows_s<DT, FUSED, 4>(p, x, x_stride, split, (int)tiles, s);
 }
 
 // Whether the few-row kernel has room for the codes of a product's rows, whatever the split.
-bool rows_fit(int64_t M, int64_t K) { return rows_lds(M, 8, (int)((K + 127) / 128)) + 256 <= 160 * 1024; }
+bool rows_fit(int64_t M, int64_t K) { return rows_lds(M, 8, (int)((K + 127) / 128), 0) + 1024 <= 160 * 1024; }
 
 template <int DT>
 hipError_t launch_t(const W8a8Operands& p, const Workspace& work, hipStream_t s) {
@@ -296,8 +297,8 @@ hipError_t launch_w8a8_gemm(const int8_t* act, int64_t lda, const float* xscales
 
 bool w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
   const size_t es = dtype == kF32 ? 4 : 2;
-  return rows_kernel(M) && M * K <= kFusedMax && K % 16 == 0 && ((uintptr_t)x & 15) == 0 &&
-         (M == 1 || (x_stride * es) % 16 == 0) && rows_fit(M, K);
+  return rows_kernel(M) && M * K * (int64_t)es <= kFusedBytes && K % 16 == 0 && ((uintptr_t)x & 15) == 0 &&
+         (M == 1 || ((x_stride * es) % 16 == 0 && x_stride < (int64_t(1) << 24)));
 }
 
 hipError_t launch_w8a8_fused(const void* x, int64_t x_stride, int dtype, const int8_t* weight, int64_t ldw,
