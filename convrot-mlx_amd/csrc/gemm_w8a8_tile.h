@@ -69,17 +69,20 @@ __device__ __forceinline__ void mfma_drain(i32x4 (&acc)[FN][FM]) {
 // of the LDS port's 128 bytes a clock, 128 x 128 corners (256 x 256 tile) take
 // 64 for reads and 32 for the DMA's writes, 64 x 64 corners 128 and 64.
 
-template <int BM, int BN, int STAGES>
+template <int BM, int BN, int STAGES, bool LATE_EPI>
 struct Engine {
   static constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 16, FN = TN / 16;
   static constexpr int APW = BM / 32, BPW = BN / 32, LPW = APW + BPW;  // 1 KB pieces a wave moves
   static constexpr int STAGE_BYTES = (BM + BN) * 128;
   static constexpr int STAGING = 4 * TM * (TN * 2 + 16);  // 16-bit epilogue
-  static constexpr int RING = STAGES * STAGE_BYTES > STAGING ? STAGES * STAGE_BYTES : STAGING;
+  // The epilogue's operands come with the first k-blocks, or (LATE_EPI, where two workgroups
+  // fill the CU's LDS) after the last, behind the staged outputs in the ring.
+  static constexpr int BASE = LATE_EPI ? STAGING : STAGES * STAGE_BYTES > STAGING ? STAGES * STAGE_BYTES : STAGING;
   // xs, ws, bias of the tile, in 256-byte DMAs
   static constexpr int XS_DMAS = (BM * 4 + 255) / 256, WS_DMAS = (BN * 4 + 255) / 256;
-  static constexpr int XS_OFF = RING, WS_OFF = XS_OFF + XS_DMAS * 256, BIAS_OFF = WS_OFF + WS_DMAS * 256;
-  static constexpr int SMEM_BYTES = BIAS_OFF + WS_DMAS * 256;
+  static constexpr int XS_OFF = BASE, WS_OFF = XS_OFF + XS_DMAS * 256, BIAS_OFF = WS_OFF + WS_DMAS * 256;
+  static constexpr int EPI_END = BIAS_OFF + WS_DMAS * 256;
+  static constexpr int SMEM_BYTES = EPI_END > STAGES * STAGE_BYTES ? EPI_END : STAGES * STAGE_BYTES;
   static constexpr int SLOTS = FM * FN, READS = FM + FN;
   static_assert(SMEM_BYTES <= 160 * 1024, "LDS of one CU");
   static_assert(STAGES >= 2 && (STAGES - 1) * LPW <= 63, "vmcnt counts at most 63 DMAs");
@@ -233,25 +236,30 @@ __device__ __forceinline__ void wave_lds_fence() {
 template <int TM, int TN, bool ALIGNED, bool STORE>
 __device__ __forceinline__ void move_corner(uint8_t* region, uint16_t* base, int lane, int mw, int nw, int M, int N) {
   constexpr int RS = TN * 2 + 16, CPR = ALIGNED ? TN / 8 : TN / 8 + 1, NIT = (TM * CPR + 63) / 64;
-  const int cols = min(TN, N - nw);
+  const int cols = min(TN, N - nw), rows = min(TM, M - mw);
 #pragma unroll 4
   for (int it = 0; it < NIT; ++it) {
-    const int c = it * 64 + lane, row = c / CPR, ch = c % CPR, m = mw + row;
-    if (row >= TM || m >= M) continue;
-    const int64_t start = (int64_t)m * N + nw;
+    const int c = it * 64 + lane, row = c / CPR, ch = c % CPR;
+    const int64_t start = (int64_t)(mw + row) * N + nw;
     const int first = ALIGNED ? ch * 8 : ch * 8 - (int)(start & 7);  // the chunk's first column
+    if (row >= rows || first < 0 || first + 8 > cols) continue;
     uint8_t* at = region + row * RS + ch * 16;
     uint16_t* g = base + start + first;
-    if (first >= 0 && first + 8 <= cols) {
-      if constexpr (STORE) *(uint4*)g = *(const uint4*)at;
-      else *(uint4*)at = *(const uint4*)g;
-    } else if (!ALIGNED || first < cols) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (first + j >= 0 && first + j < cols) {
-          if constexpr (STORE) g[j] = ((const uint16_t*)at)[j];
-          else ((uint16_t*)at)[j] = g[j];
-        }
+    if constexpr (STORE) *(uint4*)g = *(const uint4*)at;
+    else *(uint4*)at = *(const uint4*)g;
+  }
+  if constexpr (!ALIGNED) {
+    // the part chunks: up to 7 elements at either end of a row, 16 lanes a row
+#pragma unroll 4
+    for (int it = 0; it < TM / 4; ++it) {
+      const int row = it * 4 + (lane >> 4), e = lane & 7;
+      const int64_t start = (int64_t)(mw + row) * N + nw;
+      const int s = (int)(start & 7), head = min((8 - s) & 7, cols), body = (cols - head) / 8 * 8;
+      const int col = lane & 8 ? head + body + e : e;  // the tail's or the head's e-th
+      if (row >= rows || col >= (lane & 8 ? cols : head)) continue;
+      uint16_t* at = (uint16_t*)(region + row * RS) + s + col;
+      if constexpr (STORE) base[start + col] = *at;
+      else *at = base[start + col];
     }
   }
 }
@@ -362,7 +370,8 @@ __device__ __forceinline__ void epilogue(const E& e, const i32x4 (&acc)[E::FN][E
 template <int BM, int BN, int STAGES, int PER_CU, int ODT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER_CU))) void w8a8_tile_kernel(
     W8a8Operands p, int tiles_m, int tiles_n, W8a8Split split) {
-  using E = Engine<BM, BN, STAGES>;
+  constexpr bool LATE_EPI = PER_CU == 2 && BM * BN > 128 * 128;
+  using E = Engine<BM, BN, STAGES, LATE_EPI>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES];
   E e(smem);
   // tiles that one XCD (one L2) runs are neighbours, in groups of kGroupM tile rows
@@ -375,7 +384,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER
   const int m0 = (first_m + in_group % group_rows) * BM, n0 = (in_group / group_rows) * BN;
 
   e.set_tile(p, m0, n0);
-  e.issue_epi(p, m0, n0);
+  if constexpr (!LATE_EPI) e.issue_epi(p, m0, n0);
   i32x4 acc[E::FN][E::FM];
 #pragma unroll
   for (int a = 0; a < E::FN; ++a)
@@ -410,6 +419,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER
       });
   }
   __syncthreads();  // every wave is done with the ring before it stages outputs
+  if constexpr (LATE_EPI) {
+    e.issue_epi(p, m0, n0);
+    wait_vmcnt<0>();
+    __syncthreads();
+  }
   epilogue<E, ODT>(e, acc, p, m0, n0);
 }
 

@@ -115,7 +115,7 @@ constexpr int tile_code(int bm, int bn) { return bm | bn << 10; }
 // The tiles built: BM, BN, ring stages, workgroups a CU.
 #define W8A8_TILES(X) \
   X(256, 256, 2, 1) X(256, 224, 2, 1) X(224, 256, 2, 1) X(256, 192, 2, 1) X(192, 256, 2, 1) X(256, 128, 3, 1) \
-  X(128, 256, 3, 1) X(192, 192, 3, 1) X(192, 128, 3, 1) X(128, 192, 3, 1) X(160, 128, 4, 1) X(128, 160, 4, 1) \
+  X(128, 256, 3, 1) X(192, 192, 3, 1) X(192, 128, 2, 2) X(128, 192, 2, 2) X(160, 128, 4, 1) X(128, 160, 4, 1) \
   X(128, 128, 2, 2) X(128, 64, 3, 2) X(64, 128, 3, 2) X(64, 64, 4, 2)
 
 }  // namespace convrot
