@@ -237,16 +237,36 @@ template <int TM, int TN, bool ALIGNED, bool STORE>
 __device__ __forceinline__ void move_corner(uint8_t* region, uint16_t* base, int lane, int mw, int nw, int M, int N) {
   constexpr int RS = TN * 2 + 16, CPR = ALIGNED ? TN / 8 : TN / 8 + 1, NIT = (TM * CPR + 63) / 64;
   const int cols = min(TN, N - nw), rows = min(TM, M - mw);
+  if constexpr (!STORE) {
+    // 16 loads in flight at a time
+    constexpr int BATCH = 16;
+    for (int b0 = 0; b0 < NIT; b0 += BATCH) {
+      u32x4 v[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int c = (b0 + i) * 64 + lane, row = c / CPR, ch = c % CPR;
+        const int64_t start = (int64_t)(mw + row) * N + nw;
+        const int first = ALIGNED ? ch * 8 : ch * 8 - (int)(start & 7);
+        v[i] = (u32x4){0, 0, 0, 0};
+        if (row < rows && first >= 0 && first + 8 <= cols) v[i] = *(const u32x4*)(base + start + first);
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int c = (b0 + i) * 64 + lane;
+        if (c < TM * CPR) *(u32x4*)(region + c / CPR * RS + c % CPR * 16) = v[i];
+      }
+    }
+  } else {
 #pragma unroll 4
-  for (int it = 0; it < NIT; ++it) {
-    const int c = it * 64 + lane, row = c / CPR, ch = c % CPR;
-    const int64_t start = (int64_t)(mw + row) * N + nw;
-    const int first = ALIGNED ? ch * 8 : ch * 8 - (int)(start & 7);  // the chunk's first column
-    if (row >= rows || first < 0 || first + 8 > cols) continue;
-    uint8_t* at = region + row * RS + ch * 16;
-    uint16_t* g = base + start + first;
-    if constexpr (STORE) *(uint4*)g = *(const uint4*)at;
-    else *(uint4*)at = *(const uint4*)g;
+    for (int it = 0; it < NIT; ++it) {
+      const int c = it * 64 + lane, row = c / CPR, ch = c % CPR;
+      const int64_t start = (int64_t)(mw + row) * N + nw;
+      const int first = ALIGNED ? ch * 8 : ch * 8 - (int)(start & 7);  // the chunk's first column
+      if (row >= rows || first < 0 || first + 8 > cols) continue;
+      uint8_t* at = region + row * RS + ch * 16;
+      uint16_t* g = base + start + first;
+      *(uint4*)g = *(const uint4*)at;
+    }
   }
   if constexpr (!ALIGNED) {
     // the part chunks: up to 7 elements at either end of a row, 16 lanes a row
@@ -279,12 +299,17 @@ __device__ __forceinline__ void epilogue16(const E& e, const i32x4 (&acc)[E::FN]
   const float* bias_lds = (const float*)(e.smem + E::BIAS_OFF) + e.wn * TN;
   uint8_t* region = e.smem + e.wave * (TM * RS);
   const bool residual = p.gr.residual != nullptr;
+  // rows of the corner under one gate row: its values are loaded once, ahead of the residual
+  const bool one_gate = residual && mw / p.gr.rows_per_gate == (min(mw + TM, p.M) - 1) / p.gr.rows_per_gate;
+  float gates[FN][4];
+  if (one_gate) {
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn) load_gate4<ODT>(p.gr, mw, nw + fn * 16 + 4 * (lane >> 4), p.N, gates[fn]);
+  }
   if (residual) {
     move_corner<TM, TN, ALIGNED, false>(region, (uint16_t*)p.gr.residual, lane, mw, nw, p.M, p.N);
     wave_lds_fence();
   }
-  // rows of the corner under one gate row: its values are loaded once a column fragment
-  const bool one_gate = residual && mw / p.gr.rows_per_gate == (min(mw + TM, p.M) - 1) / p.gr.rows_per_gate;
   float xs[FM];
   uint8_t* at[FM];  // the lane's row of each fragment, at the corner's first column
 #pragma unroll
@@ -299,7 +324,8 @@ __device__ __forceinline__ void epilogue16(const E& e, const i32x4 (&acc)[E::FN]
     const float4 w4 = *(const float4*)(ws_lds + nl), b4 = *(const float4*)(bias_lds + nl);
     const float wsv[4] = {w4.x, w4.y, w4.z, w4.w}, bv[4] = {b4.x, b4.y, b4.z, b4.w};
     float g[4];
-    if (one_gate) load_gate4<ODT>(p.gr, mw, nw + nl, p.N, g);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) g[r] = gates[fn][r];
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
       float o[4];
