@@ -391,7 +391,9 @@ __global__ __launch_bounds__(256) void axes_table_kernel(const PT* __restrict__ 
   out[2 * i + 1] = (float)sin(angle);
 }
 
-constexpr int kBackwardGroups = 1024;
+// Workgroups of the backward kernels: each leaves a partial of dw (512 against 1024: 41.0 -> 37.8 us
+// at 4608 tokens of 24 heads, 24.4 -> 19.6 at 4000 of 16 heads of 64).
+constexpr int kBackwardGroups = 512;
 
 int64_t backward_groups(int64_t units) {
   const int64_t g = (units + 3) / 4;

@@ -78,12 +78,16 @@ def apply_rope(x: torch.Tensor, freqs: torch.Tensor) -> torch.Tensor:
 
 
 def attention(q, k, v, pe):
-    """Joint attention over [B, H, L, D] heads, RoPE applied in float32, heads merged.
+    """Joint attention over [B, H, L, D] heads, RoPE applied in float32, heads merged."""
+    return merged_attention(apply_rope(q, pe).to(v.dtype), apply_rope(k, pe).to(v.dtype), v)
+
+
+def merged_attention(q, k, v):
+    """Attention over [B, H, L, D] heads that carry their positions, heads merged.
 
     On the GPU this is torch's fused scaled-dot-product attention restricted to its flash /
     memory-efficient kernels (the unfused math backend is excluded, so an unsupported case
     raises instead of falling back).  Elsewhere it is written out in float32."""
-    q, k = apply_rope(q, pe).to(v.dtype), apply_rope(k, pe).to(v.dtype)
     if q.is_cuda:
         with sdpa_kernel([SDPBackend.FLASH_ATTENTION, SDPBackend.EFFICIENT_ATTENTION]):
             out = F.scaled_dot_product_attention(q, k, v)
@@ -132,6 +136,15 @@ class QKNorm(nn.Module):
     def forward(self, q, k):
         return self.query_norm(q), self.key_norm(k)
 
+    def rotated(self, q, k, table, q_out=None, k_out=None):
+        """The norms and the rotary positions of `table` in one kernel, into q_out and k_out if given."""
+        from convrot_mlx_amd import hip_qk_rotary, qk_rotary
+
+        kw = dict(q_weight=self.query_norm.scale, k_weight=self.key_norm.scale, eps=1e-6)
+        if q_out is None:
+            return qk_rotary(q, k, table, **kw)
+        return hip_qk_rotary(q, k, table, q_out=q_out, k_out=k_out, **kw)
+
 
 class Modulation(nn.Module):
     def __init__(self, dim: int, double: bool):
@@ -146,12 +159,18 @@ class Modulation(nn.Module):
         return first, second  # (shift, scale, gate)
 
 
-def modulated(linear: nn.Module, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, fused: bool):
-    """linear((1 + scale) * layer_norm(x) + shift).  With `fused` and a ConvRotLinear the
-    normalization and modulation run inside its activation preparation (one kernel);
-    otherwise as torch ops."""
+def modulated(linear: nn.Module, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, fused: bool,
+              fused_norm: bool = False):
+    """linear((1 + scale) * layer_norm(x) + shift).  With `fused` and a ConvRotLinear or Int8Linear the
+    normalization and modulation run inside its activation preparation (one kernel); with
+    `fused_norm` in front of any other Linear as one operator, which has gradients; otherwise as
+    torch ops."""
     if fused and hasattr(linear, "forward_modulated"):
         return linear.forward_modulated(x, shift, scale, eps=1e-6)
+    if fused_norm:
+        from convrot_mlx_amd import layer_norm
+
+        return linear(layer_norm(x, scale=scale, shift=shift, eps=1e-6))
     return linear((1 + scale) * F.layer_norm(x, (x.shape[-1],), eps=1e-6) + shift)
 
 
@@ -179,6 +198,23 @@ def set_fused_residual(model: nn.Module, on: bool) -> None:
             m.fused_residual = on
 
 
+def set_fused_rotary(model: nn.Module, on: bool) -> None:
+    """With `on`, the head norms and rotary positions of queries and keys run as one operator
+    (qk_rotary, which has gradients) that reads the fused projections' outputs in place and, in the
+    double blocks, writes each stream into its part of the joint sequence."""
+    for m in model.modules():
+        if hasattr(m, "fused_rotary"):
+            m.fused_rotary = on
+
+
+def set_fused_norm(model: nn.Module, on: bool) -> None:
+    """With `on`, the adaptive norms in front of Linears that do not take them in run as one
+    operator (layer_norm, which has gradients)."""
+    for m in model.modules():
+        if hasattr(m, "fused_norm"):
+            m.fused_norm = on
+
+
 def project(linear: nn.Module, x: torch.Tensor, *, gelu: bool = False, head: torch.Tensor | None = None,
             residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
             fused_gelu: bool = False, fused_residual: bool = False) -> torch.Tensor:
@@ -187,7 +223,8 @@ def project(linear: nn.Module, x: torch.Tensor, *, gelu: bool = False, head: tor
     gated residual move into a ConvRotLinear's preparation and epilogue when their flags are
     set; otherwise they are the torch ops FLUX uses."""
     convrot = hasattr(linear, "forward_gelu")
-    kw = dict(residual=residual, gate=gate) if fused_residual and convrot and residual is not None else {}
+    quantized = hasattr(linear, "forward_modulated")  # a ConvRotLinear or Int8Linear
+    kw = dict(residual=residual, gate=gate) if fused_residual and quantized and residual is not None else {}
     if gelu and fused_gelu and convrot:
         out = linear.forward_gelu(x, head=head, **kw)
     else:
@@ -212,7 +249,7 @@ class DoubleStreamBlock(nn.Module):
         super().__init__()
         mlp_hidden = int(hidden * mlp_ratio)
         self.heads = heads
-        self.fused_modulation = self.fused_gelu = self.fused_residual = False
+        self.fused_modulation = self.fused_gelu = self.fused_residual = self.fused_rotary = self.fused_norm = False
         for side in ("img", "txt"):
             setattr(self, f"{side}_mod", Modulation(hidden, double=True))
             setattr(self, f"{side}_qkv", nn.Linear(hidden, 3 * hidden, bias=qkv_bias))
@@ -224,20 +261,31 @@ class DoubleStreamBlock(nn.Module):
     def forward(self, img, txt, vec, pe):
         (i_shift1, i_scale1, i_gate1), (i_shift2, i_scale2, i_gate2) = self.img_mod(vec)
         (t_shift1, t_scale1, t_gate1), (t_shift2, t_scale2, t_gate2) = self.txt_mod(vec)
-        fu = self.fused_modulation
-        iq, ik, iv = _split_heads(modulated(self.img_qkv, img, i_shift1, i_scale1, fu), self.heads)
-        tq, tk, tv = _split_heads(modulated(self.txt_qkv, txt, t_shift1, t_scale1, fu), self.heads)
-        iq, ik = self.img_qknorm(iq, ik)
-        tq, tk = self.txt_qknorm(tq, tk)
-        attn = attention(torch.cat([tq, iq], 2), torch.cat([tk, ik], 2), torch.cat([tv, iv], 2), pe)
+        fu = dict(fused=self.fused_modulation, fused_norm=self.fused_norm)
+        iq, ik, iv = _split_heads(modulated(self.img_qkv, img, i_shift1, i_scale1, **fu), self.heads)
+        tq, tk, tv = _split_heads(modulated(self.txt_qkv, txt, t_shift1, t_scale1, **fu), self.heads)
+        if not self.fused_rotary:
+            iq, ik = self.img_qknorm(iq, ik)
+            tq, tk = self.txt_qknorm(tq, tk)
+            attn = attention(torch.cat([tq, iq], 2), torch.cat([tk, ik], 2), torch.cat([tv, iv], 2), pe)
+        else:
+            b, h, lt, d = tq.shape
+            if torch.is_grad_enabled() and (iq.requires_grad or tq.requires_grad):
+                parts = self.txt_qknorm.rotated(tq, tk, pe[:, :lt]), self.img_qknorm.rotated(iq, ik, pe[:, lt:])
+                q, k = torch.cat([parts[0][0], parts[1][0]], 2), torch.cat([parts[0][1], parts[1][1]], 2)
+            else:
+                q, k = (torch.empty((b, h, lt + iq.shape[2], d), dtype=tq.dtype, device=tq.device) for _ in range(2))
+                self.txt_qknorm.rotated(tq, tk, pe[:, :lt], q[:, :, :lt], k[:, :, :lt])
+                self.img_qknorm.rotated(iq, ik, pe[:, lt:], q[:, :, lt:], k[:, :, lt:])
+            attn = merged_attention(q, k, torch.cat([tv, iv], 2))
         t_attn, i_attn = attn[:, : txt.shape[1]], attn[:, txt.shape[1]:]
         flags = dict(fused_gelu=self.fused_gelu, fused_residual=self.fused_residual)
         # img_mlp[1] / txt_mlp[1] are nn.GELU(approximate="tanh"): project applies it (gelu=True)
         img = project(self.img_proj, i_attn, residual=img, gate=i_gate1, **flags)
-        img = project(self.img_mlp[2], modulated(self.img_mlp[0], img, i_shift2, i_scale2, fu), gelu=True,
+        img = project(self.img_mlp[2], modulated(self.img_mlp[0], img, i_shift2, i_scale2, **fu), gelu=True,
                       residual=img, gate=i_gate2, **flags)
         txt = project(self.txt_proj, t_attn, residual=txt, gate=t_gate1, **flags)
-        txt = project(self.txt_mlp[2], modulated(self.txt_mlp[0], txt, t_shift2, t_scale2, fu), gelu=True,
+        txt = project(self.txt_mlp[2], modulated(self.txt_mlp[0], txt, t_shift2, t_scale2, **fu), gelu=True,
                       residual=txt, gate=t_gate2, **flags)
         return img, txt
 
@@ -251,15 +299,18 @@ class SingleStreamBlock(nn.Module):
         self.linear2 = nn.Linear(hidden + self.mlp_hidden, hidden)
         self.norm = QKNorm(hidden // heads)
         self.modulation = Modulation(hidden, double=False)
-        self.fused_modulation = self.fused_gelu = self.fused_residual = False
+        self.fused_modulation = self.fused_gelu = self.fused_residual = self.fused_rotary = self.fused_norm = False
 
     def forward(self, x, vec, pe):
         (shift, scale, gate), _ = self.modulation(vec)
-        h = modulated(self.linear1, x, shift, scale, self.fused_modulation)
+        h = modulated(self.linear1, x, shift, scale, self.fused_modulation, self.fused_norm)
         qkv, mlp = torch.split(h, [3 * self.hidden, self.mlp_hidden], dim=-1)
         q, k, v = _split_heads(qkv, self.heads)
-        q, k = self.norm(q, k)
-        attn = attention(q, k, v, pe)
+        if self.fused_rotary:
+            attn = merged_attention(*self.norm.rotated(q, k, pe), v)
+        else:
+            q, k = self.norm(q, k)
+            attn = attention(q, k, v, pe)
         return project(self.linear2, mlp, gelu=True, head=attn, residual=x, gate=gate,
                        fused_gelu=self.fused_gelu, fused_residual=self.fused_residual)
 
@@ -281,7 +332,7 @@ class Flux(nn.Module):
             [SingleStreamBlock(h, p.num_heads, p.mlp_ratio) for _ in range(p.depth_single_blocks)])
         self.final_adaln = nn.Linear(h, 2 * h)
         self.final_linear = nn.Linear(h, p.in_channels)
-        self.fused_modulation = False
+        self.fused_modulation = self.fused_rotary = self.fused_norm = False
 
     def forward(self, img, img_ids, txt, txt_ids, timesteps, y, guidance=None):
         img = self.img_in(img)
@@ -290,7 +341,13 @@ class Flux(nn.Module):
             vec = vec + self.guidance_in(timestep_embedding(guidance, 256).to(img.dtype))
         vec = vec + self.vector_in(y)
         txt = self.txt_in(txt)
-        pe = self.pe_embedder(torch.cat([txt_ids, img_ids], dim=1))
+        ids = torch.cat([txt_ids, img_ids], dim=1)
+        if self.fused_rotary:
+            from convrot_mlx_amd import rotary_axes_table
+
+            pe = rotary_axes_table(ids, self.p.axes_dim, self.p.theta)  # [B, L, D / 2, 2], for every block
+        else:
+            pe = self.pe_embedder(ids)
         for block in self.double_blocks:
             img, txt = block(img, txt, vec, pe)
         x = torch.cat([txt, img], dim=1)
@@ -298,7 +355,7 @@ class Flux(nn.Module):
             x = block(x, vec, pe)
         img = x[:, txt.shape[1]:]
         shift, scale = self.final_adaln(F.silu(vec))[:, None, :].chunk(2, dim=-1)
-        return modulated(self.final_linear, img, shift, scale, self.fused_modulation)
+        return modulated(self.final_linear, img, shift, scale, self.fused_modulation, self.fused_norm)
 
 
 def make_inputs(p: FluxParams, img_tokens: int, txt_tokens: int, device, seed: int = 5):
@@ -545,6 +602,83 @@ def config5_figure(p: FluxParams | None = None, img_tokens: int = 1024, txt_toke
     }
 
 
+def keep_at_8_bits(name: str, linear: nn.Module) -> bool:
+    """The layers that a mixed model keeps at 8 bits: the single-row modulation layers, the
+    embedders and the first and last projections, whose errors reach every token."""
+    return "mod" in name or "adaln" in name or "_in" in name or name == "final_linear"
+
+
+def int8_figure(p: FluxParams | None = None, img_tokens: int = 1024, txt_tokens: int = 512, group_size: int = 64,
+                steps: int = 5) -> dict:
+    """One denoising step: dense bf16 against every Linear at 8 bits (Int8Linear), and against a
+    mixed model (keep_at_8_bits, the rest W4A4), both with the norms inside the linears'
+    preparations, gated residuals in their epilogues, and head norms and rotary positions in one
+    kernel."""
+    from convrot_mlx_amd import replace_convrot_linears, replace_int8_linears
+
+    p = p or FluxParams()
+    dev = torch.device("cuda:0")
+    inputs = make_inputs(p, img_tokens, txt_tokens, dev)
+
+    def run(convert, rotary=True):
+        model = build(p, dev)
+        counts = convert(model)
+        for setter in (set_fused_modulation, set_fused_gelu, set_fused_residual):
+            setter(model, bool(counts))
+        set_fused_rotary(model, rotary)
+        out, eager_ms, graph_ms = time_step(model, inputs, steps)
+        del model
+        torch.cuda.empty_cache()
+        return out.float(), {"eager_ms": round(eager_ms, 2), "graph_ms": round(graph_ms, 2), "linears": counts}
+
+    def mixed(model):
+        return [len(replace_int8_linears(model, select=keep_at_8_bits)),
+                len(replace_convrot_linears(model, backend="hip-w4a4", group_size=group_size))]
+
+    dense, dense_t = run(lambda model: [], rotary=False)
+    figure = {"what": f"random-init FLUX.1-dev DiT, one denoising step, batch 1, {img_tokens} image + {txt_tokens} "
+                      "text tokens, bf16", "dense_bf16": dense_t}
+    for name, convert, rotary in (
+            ("dense_bf16_fused_rotary", lambda model: [], True),
+            ("w8a8", lambda model: [len(replace_int8_linears(model))], True),
+            ("w8a8_torch_rotary", lambda model: [len(replace_int8_linears(model))], False),
+            ("w8a8_and_w4a4", mixed, True)):
+        out, t = run(convert, rotary)
+        figure[name] = {**t, "graph_speedup_vs_dense": round(dense_t["graph_ms"] / t["graph_ms"], 3),
+                        "rel_l2_vs_dense": round(((out - dense).norm() / dense.norm()).item(), 4)}
+    return figure
+
+
+def train_figure(tokens: int = 1536, steps: int = 5) -> dict:
+    """One training step (forward and backward) of a single-stream block in bf16: torch's norms and
+    positions against the layer_norm and qk_rotary operators."""
+    p = FluxParams()
+    dev = torch.device("cuda:0")
+    torch.manual_seed(0)
+    with torch.device(dev):
+        block = SingleStreamBlock(p.hidden_size, p.num_heads, p.mlp_ratio).to(torch.bfloat16)
+    x = torch.randn((1, tokens, p.hidden_size), device=dev).bfloat16().requires_grad_()
+    vec, dy = torch.randn((1, p.hidden_size), device=dev).bfloat16(), torch.randn_like(x)
+    ids = torch.zeros((1, tokens, 3), device=dev)
+    ids[..., 1], ids[..., 2] = torch.arange(tokens, device=dev) // 32, torch.arange(tokens, device=dev) % 32
+    from convrot_mlx_amd import rotary_axes_table
+
+    pes = {False: EmbedND(p.theta, p.axes_dim)(ids), True: rotary_axes_table(ids, p.axes_dim, p.theta)}
+    leaves = [x, *block.parameters()]
+
+    def step(on):
+        set_fused_rotary(block, on)
+        set_fused_norm(block, on)
+        return torch.autograd.grad(block(x, vec, pes[on]), leaves, dy)
+
+    plain, fused = step(False), step(True)
+    far = max(((a.float() - b.float()).norm() / a.float().norm().clamp_min(1e-20)).item()
+              for a, b in zip(plain, fused))
+    return {"what": f"single-stream block of FLUX.1-dev, forward and backward, {tokens} tokens, bf16",
+            "torch_ms": round(_median_ms(lambda: step(False), steps), 3),
+            "operators_ms": round(_median_ms(lambda: step(True), steps), 3), "largest_rel_l2_of_gradients": round(far, 5)}
+
+
 def profile_variant(variant: str, steps: int, group_size: int = 64) -> dict:
     """Eager steps of one variant only (for a kernel trace whose statistics cover one model)."""
     from convrot_mlx_amd import replace_convrot_linears
@@ -570,14 +704,19 @@ def main() -> int:
     ap = argparse.ArgumentParser()
     ap.add_argument("--steps", type=int, default=5)
     ap.add_argument("--group-size", type=int, default=64)
-    ap.add_argument("--variant", choices=["both", "dense", "convrot", "fused", "fused_gelu", "fused_all"],
+    ap.add_argument("--variant", choices=["both", "dense", "convrot", "fused", "fused_gelu", "fused_all", "int8", "train"],
                     default="both",
                     help="'dense', 'convrot', 'fused' (convrot with fused modulation), 'fused_gelu' (and the "
                          "MLP GELUs fused too) or 'fused_all' (and the gated residuals in the GEMM epilogue) "
-                         "runs eager steps of that model only, for profiling")
+                         "runs eager steps of that model only, for profiling; 'int8' measures the 8-bit and mixed "
+                         "models, 'train' a block's training step")
     args = ap.parse_args()
     if args.variant == "both":
         print(json.dumps(config5_figure(group_size=args.group_size, steps=args.steps)), flush=True)
+    elif args.variant == "int8":
+        print(json.dumps(int8_figure(group_size=args.group_size, steps=args.steps)), flush=True)
+    elif args.variant == "train":
+        print(json.dumps(train_figure(steps=args.steps)), flush=True)
     else:
         print(json.dumps(profile_variant(args.variant, args.steps, args.group_size)), flush=True)
     return 0
