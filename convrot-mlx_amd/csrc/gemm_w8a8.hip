@@ -20,9 +20,17 @@ namespace {
 // the last to arrive adds their integer sums.  With FUSED the rows come as they
 // are and each workgroup quantizes them itself (as convrot_quantize_int8 does):
 // one launch instead of two.  Rows or codes are the first loads, the ring's fill
-// the next: the quantization runs while the first weights are on their way.
+// the next: the quantization runs while the first weights are on their way (with
+// the rows behind the ring, 1 row of 3072 -> 18432 took 18.2 us, so 12.9).
+// Measured: 1 row 3072 -> 18432 12.3 us without the quantization, 56.6 MB of
+// weights at 4.6 TB/s; 8 rows 8192 -> 8192 14.3 us, 4.7 TB/s.  Against the 64 x 64
+// tile: 12.3 and 13.4 us, 7.5 and 8.8 (16 rows, 4096 -> 4096).
 constexpr int kRowsMax = 16, kRowsN = 64;
-constexpr int kFusedBytes = 16384;  // of a fused call's rows, which lie in LDS beside their codes
+// Rows of a fused call, which lie in LDS beside their codes.  One launch and two, in a graph:
+// 1 row 3072 -> 18432 12.9 and 15.0 us, 2 rows of 4096 -> 4096 9.0 and 9.2, 8 rows of 1024 -> 4096 6.5
+// and 6.4; an eager call saves 4 us of host time besides.
+constexpr int kFusedBytes = 16384;
+constexpr size_t kTwoPerCu = 79 * 1024;  // dynamic LDS of two workgroups a CU
 
 __device__ __forceinline__ uint32_t max16(uint32_t v) {
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xf, 0xf, true));
@@ -175,8 +183,11 @@ __global__ __launch_bounds__(256) void w8a8_rows_kernel(W8a8Operands p, const vo
 
 // ---- choice of kernel
 
-// Seconds of a tile's k-block (alone on its CU, and with every CU busy, where the
-// clock drops) and what its prologue, epilogue and stores add, in microseconds.
+// Time of a tile's k-block (alone on its CU, and with every CU busy, where the
+// clock drops) and what its prologue, epilogue and stores add, in microseconds,
+// fitted to 13 shapes x 16 tiles.  The tile the model picks is within 7 % of the
+// fastest measured on all of them (4608 x 3072 -> 12288: 256 x 224 165 us, the
+// others 165 to 286; 1536 x 15360 -> 3072: 160 x 128 71 us, 256 x 256 153).
 struct Cost {
   int bm, bn, per_cu;
   float lone, full, fixed;
@@ -189,12 +200,15 @@ constexpr Cost kCosts[] = {
     {128, 128, 2, 0.62f, 0.85f, 7.0f},  {128, 64, 2, 0.265f, 0.50f, 6.0f},  {64, 128, 2, 0.265f, 0.50f, 6.0f},
     {64, 64, 2, 0.18f, 0.32f, 4.5f}};
 
-// Splits of K for a grid of `tiles` workgroups that walk `kblocks` each.
+// Splits of K for a grid of `tiles` workgroups that walk `kblocks` each: while the
+// chip is not full and a part keeps 8 blocks.  The exchange of partial sums costs
+// 2 to 4 us: 24 rows 12288 -> 3072 (48 tiles) 21.2 us with one, 14.6 with two, 12.7
+// with four, 14.7 with six; 77 rows 3072 -> 9216 (288 tiles) 10.3 with one, 15.9 with two.
 int choose_splits(int64_t tiles, int kblocks, int64_t tile_bytes, const Workspace& work) {
   const int forced = tuning(kTuneW8a8Split);
   const int64_t most_bytes = work.ptr ? (int64_t)work.bytes - (int64_t)kW8a8PartialOffset : 0;
   if (most_bytes <= 0 || tiles > kW8a8Counters) return 1;
-  int64_t s = forced > 0 ? forced : std::min<int64_t>(256 / tiles, kblocks / 8);
+  int64_t s = forced > 0 ? forced : std::min<int64_t>(192 / tiles, kblocks / 8);
   s = std::min({s, (int64_t)kblocks, most_bytes / (tiles * tile_bytes), (int64_t)64});
   return (int)std::max<int64_t>(1, s);
 }
@@ -256,17 +270,23 @@ hipError_t launch_rows(const W8a8Operands& p, const void* x, int64_t x_stride, c
   // two workgroups a CU where the codes leave room beside the deep ring, else beside the short one
   const int64_t raw = FUSED ? (int64_t)p.M * p.K * (DT == kF32 ? 4 : 2) : 0;
   const bool deep =
-      rows_lds(p.M, 8, split.kblocks, raw) <= 80 * 1024 || rows_lds(p.M, 4, split.kblocks, raw) > 80 * 1024;
+      rows_lds(p.M, 8, split.kblocks, raw) <= kTwoPerCu || rows_lds(p.M, 4, split.kblocks, raw) > kTwoPerCu;
   if (deep) return launch_rows_s<DT, FUSED, 8>(p, x, x_stride, split, (int)tiles, s);
   return launch_rows_s<DT, FUSED, 4>(p, x, x_stride, split, (int)tiles, s);
 }
 
-// Whether the few-row kernel has room for the codes of a product's rows, whatever the split.
-bool rows_fit(int64_t M, int64_t K) { return rows_lds(M, 8, (int)((K + 127) / 128), 0) + 1024 <= 160 * 1024; }
+// Whether the few-row kernel has room for the codes of a product's rows, whatever the split, and
+// room for two workgroups a CU where there are more of them than CUs (16 rows 3072 -> 18432, one a
+// CU: 15.8 us, on tiles 14.0).
+bool rows_fit(int64_t M, int64_t N, int64_t K) {
+  const int kblocks = (int)((K + 127) / 128);
+  return rows_lds(M, 8, kblocks, 0) + 1024 <= 160 * 1024 &&
+         ((N + kRowsN - 1) / kRowsN <= 256 || rows_lds(M, 4, kblocks, 0) <= kTwoPerCu);
+}
 
 template <int DT>
 hipError_t launch_t(const W8a8Operands& p, const Workspace& work, hipStream_t s) {
-  if (rows_kernel(p.M) && rows_fit(p.M, p.K)) return launch_rows<DT, false>(p, nullptr, 0, work, s);
+  if (rows_kernel(p.M) && rows_fit(p.M, p.N, p.K)) return launch_rows<DT, false>(p, nullptr, 0, work, s);
   const int tile = choose_tile(p.M, p.N, p.K), bm = tile & 1023, bn = tile >> 10;
   const int kblocks = (p.K + 127) / 128;
   const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);

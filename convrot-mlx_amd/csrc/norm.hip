@@ -6,13 +6,14 @@
 // with g, b a weight and bias of all rows, or g = 1 + scale[v], b = shift[v] of
 // the row's group v (the adaptive norm of a diffusion transformer); y is
 // rounded once.  The row stays in registers between the sums, so it is read
-// once; the second sum takes differences from the mean (no cancellation).
+// once; the second sum takes differences from the mean (no cancellation).  Memory
+// bounds it: 8800 x 5120 bf16 38 us, 180 MB at 4.7 TB/s (a large copy: 5.0).
 //
 // Backward, with u = (x - mean) rstd and h = dy g:
 //   dx = rstd (h - sum(h) / K - u sum(h u) / K),  dg = sum_rows dy u,  db = sum_rows dy.
 //
 // Quantizer: a = max |x|, codes = round(x (127 / a)) to nearest even,
-// scale = a (1 / 127).  With the norm in front, the normalized row goes to
+// scale = a (1 / 127) (10017 x 2688 f16 16.6 us, 81 MB at 4.9 TB/s).  With the norm in front, the normalized row goes to
 // codes from registers.  A row that holds a NaN or an infinity gets the scale
 // NaN and codes 0, so every product of it is NaN; a row below 2^-100 counts as
 // zero (codes 0, scale 0), where 127 / a would overflow.
@@ -216,7 +217,9 @@ hipError_t launch_rows(const RowArgs& a, int dtype, hipStream_t stream) {
 // and stored as one partial of the workgroup.  A second kernel adds the
 // partials in order, so gradients repeat bit for bit.  The next step's rows are
 // loaded before this step's sums meet (PREFETCH), and rows are kept as they were
-// loaded: what the second half of a step needs is computed again from them.
+// loaded: what the second half of a step needs is computed again from them (held
+// as floats in teams of 256 it spilled: 8800 x 5120 bf16 141 us, so 59, 270 MB at
+// 4.6 TB/s, the partials' 21 MB not counted).
 
 template <int DT, int T, int C, bool VEC, int TEAMS>
 __global__ __launch_bounds__(T* TEAMS) void norm_backward_kernel(
