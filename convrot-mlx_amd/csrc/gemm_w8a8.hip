@@ -200,17 +200,20 @@ constexpr Cost kCosts[] = {
     {128, 128, 2, 0.62f, 0.85f, 7.0f},  {128, 64, 2, 0.265f, 0.50f, 6.0f},  {64, 128, 2, 0.265f, 0.50f, 6.0f},
     {64, 64, 2, 0.18f, 0.32f, 4.5f}};
 
-// Splits of K for a grid of `tiles` workgroups that walk `kblocks` each: while the
-// chip is not full and a part keeps 8 blocks.  The exchange of partial sums costs
-// 2 to 4 us: 24 rows 12288 -> 3072 (48 tiles) 21.2 us with one, 14.6 with two, 12.7
-// with four, 14.7 with six; 77 rows 3072 -> 9216 (288 tiles) 10.3 with one, 15.9 with two.
-int choose_splits(int64_t tiles, int kblocks, int64_t tile_bytes, const Workspace& work) {
+// The most workgroups that may share the K of one of `tiles` tiles.
+int most_splits(int64_t tiles, int kblocks, int64_t tile_bytes, const Workspace& work) {
+  const int64_t bytes = work.ptr ? (int64_t)work.bytes - (int64_t)kW8a8PartialOffset : 0;
+  if (bytes <= 0 || tiles > kW8a8Counters) return 1;
+  return (int)std::max<int64_t>(1, std::min({(int64_t)kblocks, bytes / (tiles * tile_bytes), (int64_t)64}));
+}
+
+// Splits of K of the few-row kernel: while the chip is not full and a part keeps 8
+// blocks.  The exchange of partial sums costs 2 to 4 us: 16 rows 12288 -> 3072 (48
+// tiles) 21.0 us with one, 14.4 with two, 12.5 with four, 14.3 with six.
+int rows_splits(int64_t tiles, int kblocks, const Workspace& work) {
   const int forced = tuning(kTuneW8a8Split);
-  const int64_t most_bytes = work.ptr ? (int64_t)work.bytes - (int64_t)kW8a8PartialOffset : 0;
-  if (most_bytes <= 0 || tiles > kW8a8Counters) return 1;
-  int64_t s = forced > 0 ? forced : std::min<int64_t>(192 / tiles, kblocks / 8);
-  s = std::min({s, (int64_t)kblocks, most_bytes / (tiles * tile_bytes), (int64_t)64});
-  return (int)std::max<int64_t>(1, s);
+  const int64_t s = forced > 0 ? forced : std::min<int64_t>(192 / tiles, kblocks / 8);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(s, most_splits(tiles, kblocks, 4096, work)));
 }
 
 W8a8Split make_split(int splits, int kblocks, const Workspace& work) {
@@ -224,23 +227,37 @@ W8a8Split make_split(int splits, int kblocks, const Workspace& work) {
   return s;
 }
 
-int choose_tile(int64_t M, int64_t N, int64_t K) {
-  const int forced = tuning(kTuneW8a8Tile);
-  if (forced > 0) return forced;
-  const float kblocks = (float)((K + 127) / 128);
-  float best = 0.0f;
-  int tile = 0;
+struct Choice {
+  int tile, splits;
+};
+
+// The tile, and the workgroups that share its K, that the costs make fastest.  What
+// sharing adds is the exchange of partial sums, written once and read once; more than
+// a workgroup a CU loses: 24 rows
+// 12288 -> 3072 (48 tiles of 64 x 64) 21.2 us with one, 14.6 with two, 12.7 with
+// four, 14.7 with six; 77 rows 3072 -> 9216 (288 tiles) 10.3 with one, 15.9 with two.
+Choice choose(int64_t M, int64_t N, int64_t K, const Workspace& work) {
+  const int forced_tile = tuning(kTuneW8a8Tile), forced_splits = tuning(kTuneW8a8Split);
+  const int kblocks = (int)((K + 127) / 128);
+  Choice best{0, 1};
+  float best_time = 0.0f;
   for (const Cost& c : kCosts) {
+    if (forced_tile > 0 && forced_tile != tile_code(c.bm, c.bn)) continue;
     const int64_t tiles = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn), slots = 256 * c.per_cu;
-    const int64_t rounds = tiles / slots;
-    const float part = (float)(tiles - rounds * slots) / (float)slots;
-    const float per = kblocks * c.full + c.fixed;
-    float t = (float)rounds * per;
-    if (part > 0.0f)  // few workgroups run at a higher clock, and alone on their CUs
-      t += kblocks * (c.lone + (c.full - c.lone) * part) + c.fixed * (0.65f + 0.35f * part);
-    if (tile == 0 || t < best) best = t, tile = tile_code(c.bm, c.bn);
+    const int64_t bytes = (int64_t)c.bm * c.bn * 4;
+    const int most = c.bm * c.bn <= kMaxSplitTile ? most_splits(tiles, kblocks, bytes, work) : 1;
+    for (int s = 1; s <= most; ++s) {
+      if (forced_splits > 0 ? s != std::min(forced_splits, most) : s > 1 && (kblocks < 8 * s || tiles * s > 256)) continue;
+      const int64_t groups = tiles * s, rounds = groups / slots;
+      const float part = (float)(groups - rounds * slots) / (float)slots, blocks = (float)((kblocks + s - 1) / s);
+      float t = (float)rounds * (blocks * c.full + c.fixed);
+      if (part > 0.0f)  // few workgroups run at a higher clock, and alone on their CUs
+        t += blocks * (c.lone + (c.full - c.lone) * part) + c.fixed * (0.65f + 0.35f * part);
+      if (s > 1) t += 2.0f + (float)(groups * bytes) * 2.0f / 3.0e6f;
+      if (best.tile == 0 || t < best_time) best_time = t, best = {tile_code(c.bm, c.bn), s};
+    }
   }
-  return tile;
+  return best;
 }
 
 bool rows_kernel(int64_t M) {
@@ -266,7 +283,7 @@ template <int DT, bool FUSED>
 hipError_t launch_rows(const W8a8Operands& p, const void* x, int64_t x_stride, const Workspace& work, hipStream_t s) {
   const int64_t tiles = (p.N + kRowsN - 1) / kRowsN;
   const int kblocks = (p.K + 127) / 128;
-  W8a8Split split = make_split(choose_splits(tiles, kblocks, 4096, work), kblocks, work);
+  W8a8Split split = make_split(rows_splits(tiles, kblocks, work), kblocks, work);
   // two workgroups a CU where the codes leave room beside the deep ring, else beside the short one
   const int64_t raw = FUSED ? (int64_t)p.M * p.K * (DT == kF32 ? 4 : 2) : 0;
   const bool deep =
@@ -287,11 +304,8 @@ bool rows_fit(int64_t M, int64_t N, int64_t K) {
 template <int DT>
 hipError_t launch_t(const W8a8Operands& p, const Workspace& work, hipStream_t s) {
   if (rows_kernel(p.M) && rows_fit(p.M, p.N, p.K)) return launch_rows<DT, false>(p, nullptr, 0, work, s);
-  const int tile = choose_tile(p.M, p.N, p.K), bm = tile & 1023, bn = tile >> 10;
-  const int kblocks = (p.K + 127) / 128;
-  const int64_t tiles = (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn);
-  const int splits = bm * bn <= kMaxSplitTile ? choose_splits(tiles, kblocks, (int64_t)bm * bn * 4, work) : 1;
-  return launch_w8a8_tile<DT>(tile, p, make_split(splits, kblocks, work), s);
+  const Choice c = choose(p.M, p.N, p.K, work);
+  return launch_w8a8_tile<DT>(c.tile, p, make_split(c.splits, (p.K + 127) / 128, work), s);
 }
 
 }  // namespace

@@ -96,7 +96,7 @@ __device__ __forceinline__ bool last_to_arrive(int* counter, int splits, int* sh
   return *shared != 0;
 }
 
-constexpr int kMaxSplitTile = 128 * 128;  // tiles up to this size may share their K between workgroups
+constexpr int kMaxSplitTile = 160 * 128;  // tiles up to this size may share their K between workgroups
 
 // How a launch shares K: `splits` workgroups a tile, each `kblocks` blocks of 128.
 struct W8a8Split {
