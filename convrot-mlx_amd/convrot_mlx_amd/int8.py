@@ -203,10 +203,10 @@ class Int8Linear(nn.Module):
         q = self.qweight
         if self.in_features % 16 == 0:
             return q
-        key = (q.data_ptr(), q._version, tuple(q.shape), q.device)
-        if self._padded is None or self._padded[0] != key:
-            self._padded = (key, torch.nn.functional.pad(q, (0, -self.in_features % 16)))
-        return self._padded[1]
+        # the source is held beside its copy, so no other tensor can take its place unseen
+        if self._padded is None or self._padded[0] is not q or self._padded[1] != q._version:
+            self._padded = (q, q._version, torch.nn.functional.pad(q, (0, -self.in_features % 16)))
+        return self._padded[2]
 
     def forward(self, x: torch.Tensor, *, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                 inplace: bool = False) -> torch.Tensor:

@@ -11,6 +11,7 @@ whose example model runs the norm as array operations (examples/flux1_dev/adapte
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -144,6 +145,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, mean, rstd, weight, scale = ctx.saved_tensors
         needs = ctx.needs_input_grad

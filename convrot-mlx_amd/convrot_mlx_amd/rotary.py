@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -178,6 +179,7 @@ class _QkRotary(torch.autograd.Function):
         return hip_qk_rotary(q, k, table, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, table, q_weight, k_weight = ctx.saved_tensors
         gq, gk, gqw, gkw = hip_qk_rotary_backward(dq, dk, q, k, table, q_weight=q_weight, k_weight=k_weight,

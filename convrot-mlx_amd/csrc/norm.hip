@@ -199,7 +199,9 @@ template <int OP>
 hipError_t launch_rows(const RowArgs& a, int dtype, hipStream_t stream) {
   const size_t es = dtype == kF32 ? 4 : 2;
   auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
-  bool vec = a.K % 8 == 0 && al(a.x) && (a.x_stride * es) % 16 == 0 && al(a.out) && al(a.gain) && al(a.shift);
+  // the stride of a single row says nothing
+  bool vec = a.K % 8 == 0 && al(a.x) && (a.rows == 1 || (a.x_stride * es) % 16 == 0) && al(a.out) && al(a.gain) &&
+             al(a.shift);
   if (OP == kNormOut) vec = vec && (a.out_stride * es) % 16 == 0;
   else vec = vec && a.out_stride % 8 == 0;
   switch (dtype) {
@@ -487,8 +489,8 @@ hipError_t launch_layer_norm_backward(const void* dy, int64_t dy_stride, const v
                  layer_norm_parts(rows, K, rows_per_vector), dx, (dgain || dshift) ? workspace : nullptr};
   const size_t es = dtype == kF32 ? 4 : 2;
   auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
-  const bool vec = K % 8 == 0 && al(dy) && al(x) && al(dx) && al(gain) && (dy_stride * es) % 16 == 0 &&
-                   (x_stride * es) % 16 == 0;
+  const bool vec = K % 8 == 0 && al(dy) && al(x) && al(dx) && al(gain) &&
+                   (rows == 1 || ((dy_stride * es) % 16 == 0 && (x_stride * es) % 16 == 0));
   hipError_t e;
   if (dtype == kF32) e = vec ? pick_backward<kF32, true>(a, stream) : pick_backward<kF32, false>(a, stream);
   else if (dtype == kF16) e = vec ? pick_backward<kF16, true>(a, stream) : pick_backward<kF16, false>(a, stream);

@@ -488,7 +488,10 @@ RotaryArgs rotary_args(const RotaryShape& sh) {
   return r;
 }
 
-HeadTensor head_tensor(const void* p, const int64_t* st) { return HeadTensor{p, st[0], st[1], st[2]}; }
+// The stride of an axis of one entry says nothing (and need not be aligned).
+HeadTensor head_tensor(const RotaryArgs& r, int which, const void* p, const int64_t* st) {
+  return HeadTensor{p, r.batch > 1 ? st[0] : 0, r.heads[which] > 1 ? st[1] : 0, r.length > 1 ? st[2] : 0};
+}
 
 hipError_t dispatch(const RotaryArgs& r, int dtype, bool interleaved, bool backward, hipStream_t s) {
   switch (dtype) {
@@ -503,8 +506,8 @@ hipError_t dispatch(const RotaryArgs& r, int dtype, bool interleaved, bool backw
 hipError_t launch_qk_rotary(const RotaryShape& sh, const void* q, const void* k, void* q_out, void* k_out,
                             const int64_t* strides, hipStream_t stream) {
   RotaryArgs r = rotary_args(sh);
-  r.in[0] = head_tensor(q, strides), r.in[1] = head_tensor(k, strides + 3);
-  r.out[0] = head_tensor(q_out, strides + 6), r.out[1] = head_tensor(k_out, strides + 9);
+  r.in[0] = head_tensor(r, 0, q, strides), r.in[1] = head_tensor(r, 1, k, strides + 3);
+  r.out[0] = head_tensor(r, 0, q_out, strides + 6), r.out[1] = head_tensor(r, 1, k_out, strides + 9);
   return dispatch(r, sh.dtype, sh.interleaved, false, stream);
 }
 
@@ -515,9 +518,9 @@ hipError_t launch_qk_rotary_backward(const RotaryShape& sh, const void* dq, cons
                                      void* k_weight_grad, const int64_t* strides, float* workspace,
                                      hipStream_t stream) {
   RotaryArgs r = rotary_args(sh);
-  r.grad[0] = head_tensor(dq, strides), r.grad[1] = head_tensor(dk, strides + 3);
-  r.in[0] = head_tensor(q, strides + 6), r.in[1] = head_tensor(k, strides + 9);
-  r.out[0] = head_tensor(q_grad, strides + 12), r.out[1] = head_tensor(k_grad, strides + 15);
+  r.grad[0] = head_tensor(r, 0, dq, strides), r.grad[1] = head_tensor(r, 1, dk, strides + 3);
+  r.in[0] = head_tensor(r, 0, q, strides + 6), r.in[1] = head_tensor(r, 1, k, strides + 9);
+  r.out[0] = head_tensor(r, 0, q_grad, strides + 12), r.out[1] = head_tensor(r, 1, k_grad, strides + 15);
   r.partial = q_weight_grad || k_weight_grad ? workspace : nullptr;
   const hipError_t e = dispatch(r, sh.dtype, sh.interleaved, true, stream);
   if (e != hipSuccess || !r.partial) return e;

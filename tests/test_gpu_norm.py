@@ -175,6 +175,20 @@ def test_only_some_gradients_and_expanded_dy(dev):
     assert torch.equal(s.grad, torch.full((2, 64), 4.0, device=dev))
 
 
+def test_second_gradient_is_refused(dev):
+    from convrot_mlx_amd import layer_norm, qk_rotary
+
+    x = torch.randn((4, 64), device=dev, requires_grad=True)
+    first = torch.autograd.grad(layer_norm(x).square().sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first.sum().backward()
+    q = torch.randn((1, 2, 3, 16), device=dev, requires_grad=True)
+    table = torch.randn((3, 8, 2), device=dev)
+    first = torch.autograd.grad(qk_rotary(q, q, table)[0].square().sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first.sum().backward()
+
+
 def test_side_stream_and_graph_replays(dev):
     from convrot_mlx_amd import hip_layer_norm, hip_layer_norm_backward
 

@@ -250,6 +250,22 @@ def test_layer(dev):
     assert torch.equal(got.cpu(), (res.float() + gate.float() * lin).to(BF16))
 
 
+def test_layer_follows_its_weight(dev):
+    """A layer whose rows need padding reads the weight it has now: assigned anew (its memory may be
+    the old one's), or changed in place."""
+    from convrot_mlx_amd import Int8Linear, hip_w8a8_linear
+
+    g = torch.Generator().manual_seed(5)
+    layer = Int8Linear(50, 40, device=dev)
+    x = torch.randn((3, 50), generator=g).to(BF16).to(dev)
+    for seed in range(4):
+        layer.qweight = None
+        layer.qweight = torch.randint(-127, 128, (40, 50), generator=g, dtype=torch.int8).to(dev)
+        assert torch.equal(layer(x), hip_w8a8_linear(x, layer.qweight, layer.scales, layer.bias))
+        layer.qweight.neg_()
+        assert torch.equal(layer(x), hip_w8a8_linear(x, layer.qweight, layer.scales, layer.bias))
+
+
 def test_replace_int8_linears(dev):
     from torch import nn
 
