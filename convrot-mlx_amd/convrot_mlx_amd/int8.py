@@ -103,16 +103,19 @@ def _linear(x: torch.Tensor, weight: torch.Tensor, wscales, bias, k: int, residu
     gr = _residual(residual, gate, inplace, m, n, x.dtype)
     out = _output(gr, m, n, x.dtype, device)
     lib, dtype, stride = nat.load(), nat.dtype_code(x.dtype), x2d.stride(0)
-    scratch = None
-    if gr is not None or m > 16 or not lib.convrot_w8a8_fused(x2d.data_ptr(), dtype, m, k, stride):
-        scratch = torch.empty((m * (_round16(k) + 4),), dtype=torch.uint8, device=device)
     stream = nat.stream_handle(device)
     work = _workspace(device, stream)
+    work_bytes = 0 if work is None else work.numel()
+    # codes and scales between the two launches: the end of the stream's workspace holds up to a
+    # quarter of it; a graph, which may be replayed beside this stream, holds its own
+    need, scratch = m * ((k + 127) // 128 * 128 + 4), None
+    if need * 4 > work_bytes or torch.cuda.is_current_stream_capturing():
+        scratch = torch.empty((need,), dtype=torch.uint8, device=device)
     nat.check(lib.convrot_w8a8_linear(
         x2d.data_ptr(), dtype, stride, weight.data_ptr(), weight.stride(0), wscales.data_ptr(),
         None if bias is None else bias.data_ptr(), m, n, k, *_residual_args(gr),
-        None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
-        None if work is None else work.data_ptr(), 0 if work is None else work.numel(), out.data_ptr(), stream))
+        None if scratch is None else scratch.data_ptr(), need, None if work is None else work.data_ptr(), work_bytes,
+        out.data_ptr(), stream))
     if inplace:
         return residual
     return out if x.ndim == 2 else out.reshape(*x.shape[:-1], n)

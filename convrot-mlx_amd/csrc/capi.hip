@@ -846,9 +846,12 @@ int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscale
                        "convrot_w8a8_gemm");
 }
 
+// Rows of codes in whole cache lines (rows of 2112 bytes: the product 10 % slower).
+static int64_t codes_stride_of(int64_t K) { return (K + 127) / 128 * 128; }
+
 int64_t convrot_w8a8_scratch_bytes(int64_t M, int64_t K) {
   if (M <= 0 || K <= 0) return 0;
-  return M * ((K + 15) / 16 * 16) + M * 4;
+  return M * codes_stride_of(K) + M * 4;
 }
 
 int convrot_w8a8_linear(const void* x, int dtype, int64_t x_stride, const int8_t* weight, int64_t weight_stride,
@@ -873,16 +876,24 @@ int convrot_w8a8_linear(const void* x, int dtype, int64_t x_stride, const int8_t
     return launch_status(convrot::launch_w8a8_fused(x, x_stride, dtype, weight, weight_stride, wscales, bias, M, N, K,
                                                     out, (hipStream_t)stream, gr, work),
                          "convrot_w8a8_linear");
-  if (!scratch || !aligned(scratch, 16) || scratch_bytes < convrot_w8a8_scratch_bytes(M, K))
+  const int64_t need = convrot_w8a8_scratch_bytes(M, K);
+  convrot::Workspace rest = work;
+  if (!scratch && need <= workspace_bytes / 4) {
+    // the end of the workspace, away from the partial sums that share K
+    rest.bytes = (size_t)(workspace_bytes - need) & ~(size_t)255;
+    scratch = rest.ptr + rest.bytes;
+    scratch_bytes = need;
+  }
+  if (!scratch || !aligned(scratch, 16) || scratch_bytes < need)
     return fail(CONVROT_ERR_INVALID, "the W8A8 linear needs a 16-byte aligned scratch buffer of %lld bytes, got %lld",
-                (long long)convrot_w8a8_scratch_bytes(M, K), (long long)scratch_bytes);
-  const int64_t stride = (K + 15) / 16 * 16;
+                (long long)need, (long long)scratch_bytes);
+  const int64_t stride = codes_stride_of(K);
   int8_t* codes = (int8_t*)scratch;
   float* scales = (float*)(codes + M * stride);
   hipError_t e = convrot::launch_quantize_int8(x, dtype, M, K, x_stride, codes, stride, scales, (hipStream_t)stream);
   if (e == hipSuccess)
     e = convrot::launch_w8a8_gemm(codes, stride, scales, weight, weight_stride, wscales, bias, M, N, K, out, dtype,
-                                  (hipStream_t)stream, gr, work);
+                                  (hipStream_t)stream, gr, rest);
   return launch_status(e, "convrot_w8a8_linear");
 }
 

@@ -111,6 +111,25 @@ def test_few_rows_quantized_in_the_launch(dev, m, k, dtype):
         assert got[2].isnan().all()
 
 
+@pytest.mark.parametrize("m,k", [(20, 64), (70, 2000), (300, 528), (40, 12288), (5000, 4096)])
+def test_codes_in_the_workspace_or_apart(dev, m, k):
+    """The codes between the two launches lie at the end of the stream's workspace where they are at
+    most a quarter of it, beside partial sums (40 rows of 12288) or not, else in memory of their own."""
+    from convrot_mlx_amd import core, hip_w8a8_linear
+
+    host, (_, qw, _, ws, bias) = operands(m, m, 96, k, dev)
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(k)).to(BF16)
+    codes, scales = quantize_plain(x)
+    want = product_plain(codes, host[1], scales, *host[3:], BF16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for stream in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(stream):
+            for _ in range(2):
+                assert torch.equal(hip_w8a8_linear(x.to(dev), qw, ws, bias).cpu(), want)
+    assert (dev.index or 0, side.cuda_stream) in core._WORKSPACES
+
+
 def test_few_rows_in_place_over_their_input(dev):
     """x as its own residual: every workgroup reads all of x, so the rows are quantized first."""
     from convrot_mlx_amd import hip_w8a8_linear

@@ -68,7 +68,7 @@ def test_product(lib, kw, code, text):
 
 
 def test_linear_scratch(lib):
-    assert lib.convrot_w8a8_scratch_bytes(5, 100) == 5 * 112 + 20
+    assert lib.convrot_w8a8_scratch_bytes(5, 100) == 5 * 128 + 20
     assert lib.convrot_w8a8_scratch_bytes(0, 100) == 0
     assert lib.convrot_w8a8_fused(P, BF16, 1, 4096, 4096) == 1
     assert lib.convrot_w8a8_fused(P, BF16, 17, 64, 64) == 0  # more rows than the kernel holds
@@ -77,9 +77,9 @@ def test_linear_scratch(lib):
     far = 1 << 30
     args = lambda m, scratch, nbytes, out: (P, BF16, 64, P, 64, P, None, m, 8, 64, None, None, 0, 1, scratch,  # noqa: E731
                                             nbytes, None, 0, out, None)
-    refused(lib, lib.convrot_w8a8_linear(*args(40, None, 0, far)), 1, "scratch buffer of 2720 bytes")
-    refused(lib, lib.convrot_w8a8_linear(*args(40, P, 2719, far)), 1, "scratch buffer")
-    refused(lib, lib.convrot_w8a8_linear(*args(40, P + 4, 4000, far)), 1, "scratch buffer")
+    refused(lib, lib.convrot_w8a8_linear(*args(40, None, 0, far)), 1, "scratch buffer of 5280 bytes")
+    refused(lib, lib.convrot_w8a8_linear(*args(40, P, 5279, far)), 1, "scratch buffer")
+    refused(lib, lib.convrot_w8a8_linear(*args(40, P + 4, 6000, far)), 1, "scratch buffer")
     refused(lib, lib.convrot_w8a8_linear(*args(2, None, 0, P)), 1, "scratch buffer")  # out over x: not in one launch
 
 
