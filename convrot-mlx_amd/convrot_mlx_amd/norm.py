@@ -69,7 +69,7 @@ def hip_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     x2d = rows_of(x if x.ndim == 2 else x.reshape(-1, k))
     rows = x2d.shape[0]
     gain, add, each, plus_one = norm_operands(x2d, weight, bias, scale, shift)
-    out = torch.empty(x.shape, dtype=x.dtype, device=device)
+    out = x.new_empty(x.shape)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if return_stats else None
     mean, rstd = (None, None) if stats is None else stats.unbind(0)
     kind = gain if gain is not None else add

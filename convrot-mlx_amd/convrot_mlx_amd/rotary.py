@@ -94,13 +94,19 @@ def _table_args(table: torch.Tensor):
     return table, stride
 
 
+_Int64x12, _Int64x18 = ctypes.c_int64 * 12, ctypes.c_int64 * 18
+
+
 def _strides(*tensors):
-    return (ctypes.c_int64 * (3 * len(tensors)))(*(s for t in tensors for s in t.stride()[:3]))
+    flat = []
+    for t in tensors:
+        flat += t.stride()[:3]
+    return (_Int64x12 if len(flat) == 12 else _Int64x18)(*flat)
 
 
 def _out(name: str, out, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(like.shape)
     if out.shape != like.shape or out.dtype != like.dtype or (out.shape[3] > 1 and out.stride(3) != 1):
         raise ValueError(f"{name} must be {like.dtype} {tuple(like.shape)} with adjacent features, got {out.dtype} "
                          f"{tuple(out.shape)}")
