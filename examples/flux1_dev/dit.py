@@ -430,13 +430,17 @@ def time_step(model, inputs, steps: int) -> tuple[torch.Tensor, float, float]:
 
 
 def linear_weight_bytes(model: nn.Module) -> dict:
-    """Device bytes the model's Linears hold: dense weights and biases, or a ConvRotLinear's
-    qweight, scales and bias plus the derived forms it caches (the FP6 operand weight, and the
+    """Device bytes the model's Linears hold: dense weights and biases, an Int8Linear's qweight,
+    scales and bias, or a ConvRotLinear's qweight, scales and bias plus the derived forms it caches (the FP6 operand weight, and the
     CDNA4 repack of a K x packed-N qweight), and the weight count they serve."""
-    from convrot_mlx_amd import ConvRotLinear
+    from convrot_mlx_amd import ConvRotLinear, Int8Linear
 
     stored = derived = weights = 0
     for m in model.modules():
+        if isinstance(m, Int8Linear):
+            weights += m.qweight.numel()
+            stored += sum(t.numel() * t.element_size() for t in (m.qweight, m.scales, m.bias))
+            continue
         if isinstance(m, ConvRotLinear):
             weights += m.in_features * m.out_features
             stored += sum(t.numel() * t.element_size() for t in (m.qweight, m.scales, m.bias))
@@ -627,9 +631,11 @@ def int8_figure(p: FluxParams | None = None, img_tokens: int = 1024, txt_tokens:
             setter(model, bool(counts))
         set_fused_rotary(model, rotary)
         out, eager_ms, graph_ms = time_step(model, inputs, steps)
+        weight_bytes = linear_weight_bytes(model)["bytes_per_weight"]
         del model
         torch.cuda.empty_cache()
-        return out.float(), {"eager_ms": round(eager_ms, 2), "graph_ms": round(graph_ms, 2), "linears": counts}
+        return out.float(), {"eager_ms": round(eager_ms, 2), "graph_ms": round(graph_ms, 2), "linears": counts,
+                             "bytes_per_weight": weight_bytes}
 
     def mixed(model):
         return [len(replace_int8_linears(model, select=keep_at_8_bits)),
