@@ -16,7 +16,7 @@ from torch import nn
 
 from . import _native as nat
 from .core import GatedResidual, _f32, _gated_residual, _workspace
-from .norm import norm_operands, rows_of
+from .norm import flat_rows, norm_operands, rows_of
 
 INT8_MAX = 127
 MAX_FEATURES = 65536
@@ -98,7 +98,7 @@ def _w8a8(act, weight, xscales, wscales, bias, k: int, dtype: torch.dtype, gr: G
 def _linear(x: torch.Tensor, weight: torch.Tensor, wscales, bias, k: int, residual, gate, inplace: bool) -> torch.Tensor:
     """x [..., k] times a weight as the kernel reads it, one library call."""
     n, device = weight.shape[0], x.device
-    x2d = rows_of(x if x.ndim == 2 else x.reshape(-1, k))
+    x2d = flat_rows(x)
     m = x2d.shape[0]
     gr = _residual(residual, gate, inplace, m, n, x.dtype)
     out = _output(gr, m, n, x.dtype, device)
@@ -233,7 +233,7 @@ class Int8Linear(nn.Module):
             raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
                              f"{(*x.shape[:-1], self.out_features)}")
         k = self.in_features
-        x2d = rows_of(x.reshape(-1, k))
+        x2d = flat_rows(x)
         m = x2d.shape[0]
         gr = _residual(residual, gate, inplace, m, self.out_features, x.dtype)
         gain, sh, each, _ = norm_operands(x2d, None, None, scale, shift)

@@ -25,6 +25,15 @@ def rows_of(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
+def flat_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [..., K] as rows_of's two dimensions."""
+    if x.ndim < 1:
+        raise ValueError("rows of features need at least one dimension")
+    if x.ndim != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.new_empty((0, 0))
+    return rows_of(x)
+
+
 def norm_operands(x2d, weight, bias, scale, shift):
     """(gain or None, shift or None, rows a vector, plus one?) of a norm's parameters: contiguous
     rows of K, both of one type that the kernels take beside x's."""
@@ -65,9 +74,8 @@ def hip_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     vectors in order, as x [B, L, K] beside scale [B, 1, K] does: (1 + scale) * u + shift.  Either
     of a pair may be None.  With return_stats also the rows' float32 mean and 1 / sqrt(var + eps)."""
     device = nat.on_device(x, weight, bias, scale, shift)
-    k = x.shape[-1]
-    x2d = rows_of(x if x.ndim == 2 else x.reshape(-1, k))
-    rows = x2d.shape[0]
+    x2d = flat_rows(x)
+    rows, k = x2d.shape
     gain, add, each, plus_one = norm_operands(x2d, weight, bias, scale, shift)
     out = x.new_empty(x.shape)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if return_stats else None
@@ -90,15 +98,14 @@ def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
     both are of the parameter's type (x's without one), None without param_grads.  Sums over rows
     are float32 in a fixed order: results repeat bit for bit."""
     nat.require_device(dy, x, mean, rstd, weight, scale)
-    k = x.shape[-1]
     if dy.shape != x.shape:
         raise ValueError(f"dy {tuple(dy.shape)} must have the shape of x {tuple(x.shape)}")
     if dy.dtype != x.dtype:
         raise ValueError(f"dy dtype {dy.dtype} differs from x dtype {x.dtype}")
+    x2d, dy2d = flat_rows(x), flat_rows(dy)
+    rows, k = x2d.shape
     if k > MAX_BACKWARD_FEATURES:
         raise ValueError(f"the layer norm's gradient supports at most {MAX_BACKWARD_FEATURES} features, got {k}")
-    x2d, dy2d = rows_of(x.reshape(-1, k)), rows_of(dy.reshape(-1, k))
-    rows = x2d.shape[0]
     for name, t in (("mean", mean), ("rstd", rstd)):
         if tuple(t.shape) != (rows,) or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous float32 {(rows,)}, got {t.dtype} {tuple(t.shape)}")

@@ -132,6 +132,17 @@ def test_non_finite_constant_and_empty_rows(dev):
             assert not dw.any() and not db.any()
 
 
+def test_no_features_and_one_dimension(dev):
+    from convrot_mlx_amd import hip_layer_norm
+
+    assert hip_layer_norm(torch.zeros((3, 0), device=dev)).shape == (3, 0)
+    assert hip_layer_norm(torch.zeros((2, 3, 0), device=dev)).shape == (2, 3, 0)
+    x = torch.randn(96, generator=torch.Generator().manual_seed(1)).to(dev)
+    assert torch.equal(hip_layer_norm(x), hip_layer_norm(x[None])[0])
+    with pytest.raises(ValueError, match="at least one dimension"):
+        hip_layer_norm(torch.zeros((), device=dev))
+
+
 @pytest.mark.parametrize("adaptive", [False, True])
 def test_autograd_and_differences(dev, adaptive):
     """The operator's gradients in float32 against the formula, and along one direction against
