@@ -188,7 +188,7 @@ hipError_t pick_rows(const RowArgs& a, bool vec, hipStream_t stream) {
     else run_rows<DT, OP, 1024, 8, true>(a, stream);
   } else {
     if (k <= 2048) run_rows<DT, OP, 256, 1, false>(a, stream);
-    else if (k <= 8192) run_rows<DT, OP, 256, 4, false>(a, stream);
+    else if (k <= 8192) run_rows<DT, OP, 1024, 1, false>(a, stream);
     else if (k <= 32768) run_rows<DT, OP, 1024, 4, false>(a, stream);
     else run_rows<DT, OP, 1024, 8, false>(a, stream);
   }
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(T* TEAMS) void norm_backward_kernel(
     int param_dtype, int plus_one, int64_t rows_per_vector, int parts, void* __restrict__ dx,
     float* __restrict__ partial) {
   typedef typename Elem<DT>::T E;
-  constexpr int W = T / 64, R = C == 1 ? 2 : 1;
+  constexpr int W = T / 64, R = C == 1 && T < 1024 ? 2 : 1;  // teams of 1024 have 128 registers a thread
   constexpr bool PREFETCH = C == 1;
   __shared__ float red[2][TEAMS][2 * R][W];
   extern __shared__ float sums[];  // [2][K] of the teams' sums, where TEAMS > 1
@@ -475,7 +475,7 @@ hipError_t launch_layer_norm_int8(const void* x, int dtype, int64_t rows, int64_
 // workgroup costs a partial of 2 K floats), and no more than the rows feed.
 int layer_norm_parts(int64_t rows, int64_t K, int64_t rows_per_vector) {
   const int64_t team = backward_team(K), teams = backward_teams((int)team), vectors = rows / rows_per_vector;
-  const int64_t step = teams * (K <= 8192 ? 2 : 1), steps = (rows_per_vector + step - 1) / step;
+  const int64_t step = teams * (team < 1024 ? 2 : 1), steps = (rows_per_vector + step - 1) / step;
   const int64_t groups = 256 * std::max<int64_t>(1, 1024 / (team * teams));
   const int64_t parts = std::min((groups + vectors - 1) / vectors, steps);
   return (int)std::max<int64_t>(1, parts);

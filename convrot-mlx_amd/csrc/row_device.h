@@ -91,7 +91,7 @@ __device__ __forceinline__ void store_chunk(typename Elem<DT>::T* row, int K, in
 // Eight values of a row as they were loaded (widened to floats only when used).
 template <int DT, int T, int C, bool VEC>
 struct RawChunk {
-  static constexpr int W = DT == kF32 ? 8 : VEC ? 4 : 8;  // 32-bit words
+  static constexpr int W = DT == kF32 ? 8 : 4;  // 32-bit words
   uint32_t w[W];
   __device__ __forceinline__ void load(const typename Elem<DT>::T* row, int K, int t, int c) {
     if constexpr (VEC) {
@@ -102,11 +102,19 @@ struct RawChunk {
         if (f < K) v = ((const uint4*)(row + f))[i];
         w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
       }
-    } else {
-      float v[8];
-      load_chunk<DT, T, C, VEC>(row, K, t, c, v);
+    } else if constexpr (DT == kF32) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = __builtin_bit_cast(uint32_t, v[j]);
+      for (int j = 0; j < 8; ++j) {
+        const int f = feature_of<T, C, VEC>(t, c, j);
+        w[j] = f < K ? ((const uint32_t*)row)[f] : 0;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const int f = feature_of<T, C, VEC>(t, c, j), g = feature_of<T, C, VEC>(t, c, j + 1);
+        const uint32_t lo = f < K ? ((const uint16_t*)row)[f] : 0, hi = g < K ? ((const uint16_t*)row)[g] : 0;
+        w[j / 2] = lo | hi << 16;
+      }
     }
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
