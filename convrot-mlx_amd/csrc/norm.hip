@@ -189,6 +189,7 @@ hipError_t pick_rows(const RowArgs& a, bool vec, hipStream_t stream) {
   } else {
     if (k <= 2048) run_rows<DT, OP, 256, 1, false>(a, stream);
     else if (k <= 8192) run_rows<DT, OP, 1024, 1, false>(a, stream);
+    else if (k <= 16384) run_rows<DT, OP, 1024, 2, false>(a, stream);
     else if (k <= 32768) run_rows<DT, OP, 1024, 4, false>(a, stream);
     else run_rows<DT, OP, 1024, 8, false>(a, stream);
   }

@@ -161,7 +161,7 @@ def test_any_features(dev, m, n, k):
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 16), (3, 40), (5, 130), (4, 512), (2, 1000), (3, 1024), (2, 2056), (2, 3072),
-                                 (2, 5120), (1, 7777), (2, 8192), (1, 15360), (1, 33000), (1, 65536)])
+                                 (2, 5120), (1, 7777), (2, 8192), (2, 10001), (1, 15360), (1, 33000), (1, 65536)])
 def test_quantizer(dev, m, k, dtype):
     from convrot_mlx_amd import quantize_int8_rowwise
 
