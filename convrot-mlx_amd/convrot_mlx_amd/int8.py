@@ -46,17 +46,26 @@ def quantize_int8_rowwise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return codes if codes.shape[1] == k else codes[:, :k], scales
 
 
-def _operand(t: torch.Tensor, zero_tail: bool) -> torch.Tensor:
-    """An int8 matrix as rows the product can read: adjacent features, 16-byte aligned rows that
-    cover the features rounded up to 16 (past them zeros, with `zero_tail`); else a padded copy."""
+def _readable(t: torch.Tensor, zero_tail: bool) -> bool:
+    """Whether the product can read an int8 matrix where it lies: adjacent features, 16-byte aligned rows
+    that cover the features rounded up to 16 (past them zeros, with `zero_tail`)."""
     k = t.shape[1]
     if k % 16 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t
-    if (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= _round16(k) and t.data_ptr() % 16 == 0
+        return True
+    return (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= _round16(k) and t.data_ptr() % 16 == 0
             and (k % 16 == 0 or (not zero_tail and t.shape[0] * t.stride(0) + t.storage_offset()
-                                 <= t.untyped_storage().nbytes()))):
-        return t
+                                 <= t.untyped_storage().nbytes())))
+
+
+def _padded(t: torch.Tensor) -> torch.Tensor:
+    """A copy of an int8 matrix that the product can read."""
+    k = t.shape[1]
     return torch.nn.functional.pad(t, (0, -k % 16)) if k % 16 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _operand(t: torch.Tensor, zero_tail: bool) -> torch.Tensor:
+    """An int8 matrix as rows the product can read: itself, else a padded copy."""
+    return t if _readable(t, zero_tail) else _padded(t)
 
 
 def _scales(t: torch.Tensor | None) -> torch.Tensor | None:
@@ -156,7 +165,7 @@ def hip_w8a8_matmul(qact: torch.Tensor, qweight: torch.Tensor, xscales: torch.Te
     n = _check_product(k, qweight, wscales, bias)
     _check_scales("activation scales", xscales, m)
     nat.dtype_code(output_dtype)
-    nat.on_device(qact, qweight, xscales, wscales, bias)
+    nat.on_device(qact, qweight, xscales, wscales, bias, residual, gate)
     gr = _residual(residual, gate, inplace, m, n, output_dtype)
     return _w8a8(_operand(qact, False), _operand(qweight, True), _scales(xscales), _scales(wscales),
                  _scales(bias), k, output_dtype, gr)
@@ -169,7 +178,7 @@ def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tenso
     rounding at the end."""
     k = x.shape[-1]
     _check_product(k, qweight, wscales, bias)
-    nat.on_device(x, qweight, wscales, bias)
+    nat.on_device(x, qweight, wscales, bias, residual, gate)
     return _linear(x, _operand(qweight, True), _scales(wscales), _scales(bias), k, residual, gate, inplace)
 
 
@@ -194,32 +203,42 @@ class Int8Linear(nn.Module):
         if tuple(weight.shape) != (self.out_features, self.in_features):
             raise ValueError(f"weight must have shape {(self.out_features, self.in_features)}, got "
                              f"{tuple(weight.shape)}")
+        if bias is not None:
+            _check_scales("bias", bias, self.out_features)
         codes, self.scales = quantize_int8_rowwise(weight)
         self.qweight = codes.contiguous()
         if bias is not None:
-            self.bias = bias.to(torch.float32)
+            self.bias = bias.to(weight.device, torch.float32)
         return self
 
-    def _weight(self) -> torch.Tensor:
-        """The weight as the kernels read it: itself, or where in_features is no multiple of 16 a
-        copy with padded rows, made once per tensor version."""
-        q = self.qweight
-        if self.in_features % 16 == 0:
-            return q
-        # the source is held beside its copy, so no other tensor can take its place unseen
-        if self._padded is None or self._padded[0] is not q or self._padded[1] != q._version:
-            self._padded = (q, q._version, torch.nn.functional.pad(q, (0, -self.in_features % 16)))
-        return self._padded[2]
-
-    def forward(self, x: torch.Tensor, *, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
-                inplace: bool = False) -> torch.Tensor:
-        """linear(x); with `residual`, residual + gate * linear(x), as ConvRotLinear.forward."""
+    def _check(self, x: torch.Tensor, residual: torch.Tensor | None, *others: torch.Tensor | None) -> None:
+        """Whether x, the residual and the layer's own tensors (which may have been assigned anew) fit
+        each other and lie on one device: the kernels read as far as these shapes say."""
         if x.shape[-1] != self.in_features:
             raise ValueError(f"Int8Linear expected K={self.in_features}, got {x.shape[-1]}")
         if residual is not None and tuple(residual.shape) != (*x.shape[:-1], self.out_features):
             raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
                              f"{(*x.shape[:-1], self.out_features)}")
-        nat.on_device(x, self.qweight, self.scales, self.bias)
+        if _check_product(self.in_features, self.qweight, self.scales, self.bias) != self.out_features:
+            raise ValueError(f"W8A8 weight must have {self.out_features} rows, got {tuple(self.qweight.shape)}")
+        nat.on_device(x, self.qweight, self.scales, self.bias, residual, *others)
+
+    def _weight(self) -> torch.Tensor:
+        """The weight as the kernels read it: itself, or where its rows do not lie as they need it
+        (in_features no multiple of 16, a strided tensor) a copy with padded rows, made once per
+        tensor version."""
+        q = self.qweight
+        if _readable(q, True):
+            return q
+        # the source is held beside its copy, so no other tensor can take its place unseen
+        if self._padded is None or self._padded[0] is not q or self._padded[1] != q._version:
+            self._padded = (q, q._version, _padded(q))
+        return self._padded[2]
+
+    def forward(self, x: torch.Tensor, *, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                inplace: bool = False) -> torch.Tensor:
+        """linear(x); with `residual`, residual + gate * linear(x), as ConvRotLinear.forward."""
+        self._check(x, residual, gate)
         return _linear(x, self._weight(), _scales(self.scales), _scales(self.bias), self.in_features, residual, gate, inplace)
 
     def forward_modulated(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, eps: float = 1e-6, *,
@@ -227,23 +246,18 @@ class Int8Linear(nn.Module):
                           inplace: bool = False) -> torch.Tensor:
         """self((1 + scale) * layer_norm(x) + shift), the norm and the quantization in one kernel (the
         normalized row goes to codes unrounded); residual, gate and inplace as in forward."""
-        if x.shape[-1] != self.in_features:
-            raise ValueError(f"Int8Linear expected K={self.in_features}, got {x.shape[-1]}")
-        if residual is not None and tuple(residual.shape) != (*x.shape[:-1], self.out_features):
-            raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
-                             f"{(*x.shape[:-1], self.out_features)}")
+        self._check(x, residual, gate, shift, scale)
         k = self.in_features
         x2d = flat_rows(x)
         m = x2d.shape[0]
         gr = _residual(residual, gate, inplace, m, self.out_features, x.dtype)
         gain, sh, each, _ = norm_operands(x2d, None, None, scale, shift)
-        device = nat.require_device(x2d, gain, sh, self.qweight)
-        codes = torch.empty((m, _round16(k)), dtype=torch.int8, device=device)
-        scales = torch.empty((m,), dtype=torch.float32, device=device)
+        codes = torch.empty((m, _round16(k)), dtype=torch.int8, device=x.device)
+        scales = torch.empty((m,), dtype=torch.float32, device=x.device)
         nat.check(nat.load().convrot_layer_norm_int8(
             nat.ptr(x2d), nat.dtype_code(x.dtype), m, k, x2d.stride(0), nat.ptr(gain), nat.ptr(sh),
             nat.dtype_code(gain.dtype), 1, each, float(eps), nat.ptr(codes), codes.shape[1], nat.ptr(scales),
-            nat.stream_of(device)))
+            nat.stream_of(x.device)))
         out = _w8a8(codes, self._weight(), scales, _scales(self.scales), _scales(self.bias), k, x.dtype, gr)
         return residual if inplace else out.reshape(*x.shape[:-1], self.out_features)
 
