@@ -196,7 +196,7 @@ class Int8Linear(nn.Module):
         self.register_buffer("scales", torch.ones((out_features,), dtype=torch.float32, device=device))
         self.register_buffer("bias", torch.zeros((out_features,), dtype=torch.float32, device=device))
         self.source_has_bias = bias
-        self._padded: tuple | None = None
+        self._kept_copy: tuple | None = None
 
     def load_weight(self, weight: torch.Tensor, bias: torch.Tensor | None = None) -> Int8Linear:
         """Quantize a dense (out, in) weight into this layer."""
@@ -225,15 +225,30 @@ class Int8Linear(nn.Module):
 
     def _weight(self) -> torch.Tensor:
         """The weight as the kernels read it: itself, or where its rows do not lie as they need it
-        (in_features no multiple of 16, a strided tensor) a copy with padded rows, made once per
-        tensor version."""
+        (in_features no multiple of 16, a strided tensor) a copy with padded rows, kept until the
+        tensor or its version is another one."""
         q = self.qweight
         if _readable(q, True):
             return q
+        # Copies of their own: for a graph, which has to follow the weight from replay to replay and
+        # would outlive a kept copy, and for inference tensors, which count no versions.
+        if q.is_inference() or (q.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return _padded(q)
+        stream = torch.cuda.current_stream(q.device) if q.is_cuda else None
+        kept = self._kept_copy
         # the source is held beside its copy, so no other tensor can take its place unseen
-        if self._padded is None or self._padded[0] is not q or self._padded[1] != q._version:
-            self._padded = (q, q._version, _padded(q))
-        return self._padded[2]
+        if kept is None or kept[0] is not q or kept[1] != q._version:
+            copy = _padded(q)
+            self._kept_copy = (q, q._version, copy, stream, None if stream is None else stream.record_event())
+            return copy
+        _, _, copy, made_on, ready = kept
+        if stream != made_on:  # its writing comes first, and its memory is not given away under this call
+            stream.wait_event(ready)
+            copy.record_stream(stream)
+        return copy
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "_kept_copy": None}
 
     def forward(self, x: torch.Tensor, *, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                 inplace: bool = False) -> torch.Tensor:

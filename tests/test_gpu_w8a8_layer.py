@@ -39,3 +39,65 @@ def test_strided_weight(dev, k):
     wide[:, ::2] = layer.qweight
     layer.load_state_dict({**layer.state_dict(), "qweight": wide[:, ::2]}, assign=True)
     assert torch.equal(layer(x).cpu(), want)
+
+
+CYCLES = 100_000_000  # of a spinning kernel: some tens of milliseconds
+
+
+def test_padded_weight_on_two_streams(dev):
+    """The copy with padded rows is written on the first caller's stream; a call on another stream, which
+    that caller has not been ordered before, waits for it."""
+    for seed in range(3):
+        layer, x, want = layer_and_rows(seed, 250, 96, 40, dev)
+        a, b = torch.cuda.Stream(), torch.cuda.Stream()
+        for s in (a, b):  # workspaces, and kernels loaded
+            with torch.cuda.stream(s):
+                layer_and_rows(9, 256, 96, 40, dev)[0](torch.zeros((40, 256), dtype=BF16, device=dev))
+        with torch.cuda.stream(a):
+            torch.full((96, 256), 77, dtype=torch.int8, device=dev)  # what the copy's memory may hold before
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(CYCLES)
+            first = layer(x)
+        with torch.cuda.stream(b):
+            second = layer(x)
+        torch.cuda.synchronize()
+        assert torch.equal(first.cpu(), want) and torch.equal(second.cpu(), want)
+
+
+def test_replaced_copy_is_kept_for_its_readers(dev):
+    """A weight changed in place gets a new copy; the old one's memory stays until a delayed call on
+    another stream has read it."""
+    layer, x, want = layer_and_rows(5, 250, 96, 40, dev)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):
+        layer(x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(b):
+        torch.cuda._sleep(CYCLES)
+        late = layer(x)
+    with torch.cuda.stream(a):
+        layer.qweight.neg_()
+        layer(x)
+        spoil = [torch.full((96, 256), 77, dtype=torch.int8, device=dev) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert len(spoil) == 8 and torch.equal(late.cpu(), want)
+
+
+def test_captured_layer_follows_its_weight(dev):
+    layer, x, want = layer_and_rows(6, 250, 96, 40, dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            static = layer(x)
+    for i in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(static, layer(x))
+        if i == 0:
+            assert torch.equal(static.cpu(), want)
+        layer.qweight.neg_()  # seen by the next replay and the next eager call
+        torch.cuda.synchronize()

@@ -54,3 +54,26 @@ def test_strided_weight_is_read_in_order(k):
         w = layer._weight()
         assert w.stride(1) == 1 and w.stride(0) % 16 == 0 and w.data_ptr() % 16 == 0
         assert torch.equal(w[:, :k], view) and not w[:, k:].any()
+
+
+def test_weights_of_inference_mode():
+    with torch.inference_mode():
+        layer = Int8Linear(50, 4)
+        layer.qweight.random_(-127, 128)
+        for _ in range(2):
+            assert torch.equal(layer._weight()[:, :50], layer.qweight)
+            layer.qweight.neg_()
+
+
+def test_copies_of_a_layer_read_their_own_weight():
+    import copy
+    import pickle
+
+    layer = Int8Linear(50, 4)
+    layer.qweight.random_(-127, 128)
+    layer._weight()
+    for other in (copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))):
+        assert torch.equal(other._weight(), layer._weight())
+        other.qweight.neg_()
+        assert torch.equal(other._weight()[:, :50], -layer.qweight)
+    assert torch.equal(layer._weight()[:, :50], layer.qweight)
