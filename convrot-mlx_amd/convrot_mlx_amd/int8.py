@@ -20,6 +20,7 @@ from .norm import flat_rows, norm_operands, rows_of
 
 INT8_MAX = 127
 MAX_FEATURES = 65536
+MAX_ROW_STRIDE = 1 << 22
 
 
 def _round16(k: int) -> int:
@@ -46,14 +47,19 @@ def quantize_int8_rowwise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return codes if codes.shape[1] == k else codes[:, :k], scales
 
 
+def _row_stride(t: torch.Tensor) -> int:
+    """Bytes between an operand's rows (the stride of a single row says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else _round16(t.shape[1])
+
+
 def _readable(t: torch.Tensor, zero_tail: bool) -> bool:
     """Whether the product can read an int8 matrix where it lies: adjacent features, 16-byte aligned rows
     that cover the features rounded up to 16 (past them zeros, with `zero_tail`)."""
-    k = t.shape[1]
-    if k % 16 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return True
-    return (t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= _round16(k) and t.data_ptr() % 16 == 0
-            and (k % 16 == 0 or (not zero_tail and t.shape[0] * t.stride(0) + t.storage_offset()
+    rows, k = t.shape
+    stride = _row_stride(t)
+    return (t.stride(1) == 1 and stride % 16 == 0 and _round16(k) <= stride <= MAX_ROW_STRIDE
+            and t.data_ptr() % 16 == 0
+            and (k % 16 == 0 or (not zero_tail and (rows - 1) * stride + _round16(k) + t.storage_offset()
                                  <= t.untyped_storage().nbytes())))
 
 
@@ -97,7 +103,7 @@ def _w8a8(act, weight, xscales, wscales, bias, k: int, dtype: torch.dtype, gr: G
     stream = nat.stream_handle(act.device)
     work = _workspace(act.device, stream)
     nat.check(nat.load().convrot_w8a8_gemm(
-        act.data_ptr(), act.stride(0), xscales.data_ptr(), weight.data_ptr(), weight.stride(0), wscales.data_ptr(),
+        act.data_ptr(), _row_stride(act), xscales.data_ptr(), weight.data_ptr(), _row_stride(weight), wscales.data_ptr(),
         None if bias is None else bias.data_ptr(), m, n, k, *_residual_args(gr),
         None if work is None else work.data_ptr(), 0 if work is None else work.numel(), out.data_ptr(),
         nat.dtype_code(dtype), stream))
@@ -121,7 +127,7 @@ def _linear(x: torch.Tensor, weight: torch.Tensor, wscales, bias, k: int, residu
     if need * 4 > work_bytes or torch.cuda.is_current_stream_capturing():
         scratch = torch.empty((need,), dtype=torch.uint8, device=device)
     nat.check(lib.convrot_w8a8_linear(
-        x2d.data_ptr(), dtype, stride, weight.data_ptr(), weight.stride(0), wscales.data_ptr(),
+        x2d.data_ptr(), dtype, stride, weight.data_ptr(), _row_stride(weight), wscales.data_ptr(),
         None if bias is None else bias.data_ptr(), m, n, k, *_residual_args(gr),
         None if scratch is None else scratch.data_ptr(), need, None if work is None else work.data_ptr(), work_bytes,
         out.data_ptr(), stream))

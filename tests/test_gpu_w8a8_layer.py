@@ -101,3 +101,39 @@ def test_captured_layer_follows_its_weight(dev):
             assert torch.equal(static.cpu(), want)
         layer.qweight.neg_()  # seen by the next replay and the next eager call
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("k", [16, 64, 1040, 50])
+def test_single_rows_at_any_stride(dev, k):
+    """A single row of codes, or the weight of a single output: the stride of its row says nothing."""
+    from convrot_mlx_amd import hip_w8a8_linear, hip_w8a8_matmul
+
+    host, (qa, qw, xs, ws, bias) = operands(k, 1, 1, k, dev)
+    want = product_plain(*host, torch.float32)
+
+    def forms(t):
+        wide = torch.full((2, k + 5), 99, dtype=torch.int8, device=dev)
+        wide[0, :k] = t[0]
+        yield wide[:1, :k]  # the next row k + 5 bytes on
+        yield t.t().contiguous().t()  # [k, 1] turned: a stride of one
+        yield wide.flatten().as_strided((1, k), (7, 1))
+
+    for a in forms(qa):
+        for w in forms(qw):
+            assert torch.equal(hip_w8a8_matmul(a, w, xs, ws, bias, output_dtype=torch.float32).cpu(), want)
+    x = torch.randn((3, k), generator=torch.Generator().manual_seed(k)).to(BF16)
+    codes, scales = quantize_plain(x)
+    for w in forms(qw):
+        assert torch.equal(hip_w8a8_linear(x.to(dev), w, ws, bias).cpu(), product_plain(codes, host[1], scales, *host[3:],
+                                                                                      BF16))
+
+
+def test_rows_too_far_apart_are_copied(dev):
+    from convrot_mlx_amd import hip_w8a8_matmul
+
+    host, (qa, qw, xs, ws, bias) = operands(3, 2, 2, 64, dev)
+    far = torch.zeros(((1 << 22) + 16 + 64,), dtype=torch.int8, device=dev).as_strided((2, 64), ((1 << 22) + 16, 1))
+    for codes, swap in ((qa, False), (qw, True)):
+        far.copy_(codes)
+        got = hip_w8a8_matmul(*((qa, far) if swap else (far, qw)), xs, ws, bias, output_dtype=BF16)
+        assert torch.equal(got.cpu(), product_plain(*host, BF16))

@@ -77,3 +77,16 @@ def test_copies_of_a_layer_read_their_own_weight():
         other.qweight.neg_()
         assert torch.equal(other._weight()[:, :50], -layer.qweight)
     assert torch.equal(layer._weight()[:, :50], layer.qweight)
+
+
+def test_single_row_operands_stay_in_place():
+    from convrot_mlx_amd import int8
+
+    wide = torch.zeros((2, 69), dtype=torch.int8)
+    for t in (wide[:1, :64], torch.zeros((64, 1), dtype=torch.int8).t()):
+        assert int8._operand(t, True) is t and int8._row_stride(t) == 64
+    t = wide[:1, :50]  # the kernels read 64 bytes: of codes any, of a weight zeros
+    assert int8._operand(t, False) is t and int8._row_stride(t) == 64
+    assert int8._operand(t, True) is not t
+    end = torch.zeros(50, dtype=torch.int8)[None]  # 64 bytes would pass the end of its memory
+    assert int8._operand(end, False).shape == (1, 64)
