@@ -879,10 +879,14 @@ int convrot_w8a8_linear(const void* x, int dtype, int64_t x_stride, const int8_t
   const int64_t need = convrot_w8a8_scratch_bytes(M, K);
   convrot::Workspace rest = work;
   if (!scratch && need <= workspace_bytes / 4) {
-    // the end of the workspace, away from the partial sums that share K
-    rest.bytes = (size_t)(workspace_bytes - need) & ~(size_t)255;
-    scratch = rest.ptr + rest.bytes;
-    scratch_bytes = need;
+    // the end of the workspace, away from the partial sums that share K and never over the control
+    // block in front of them, whose words stay zero between launches
+    const size_t left = (size_t)(workspace_bytes - need) & ~(size_t)255;
+    if (left >= convrot::kW8a8PartialOffset) {
+      rest.bytes = left;
+      scratch = rest.ptr + left;
+      scratch_bytes = need;
+    }
   }
   if (!scratch || !aligned(scratch, 16) || scratch_bytes < need)
     return fail(CONVROT_ERR_INVALID, "the W8A8 linear needs a 16-byte aligned scratch buffer of %lld bytes, got %lld",

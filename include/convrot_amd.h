@@ -467,7 +467,8 @@ int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscale
  * scales between them: convrot_w8a8_scratch_bytes(M, K) bytes, 16-byte aligned,
  * of any content.  It may be NULL where convrot_w8a8_fused says that the rows
  * are quantized inside the product's launch (few rows) and out does not overlap
- * x, and where it is at most a quarter of the workspace, whose end then holds it.
+ * x, and where it is at most a quarter of the workspace and leaves its first 32 KiB
+ * (the control block) alone: the workspace's end then holds it.
  */
 int64_t convrot_w8a8_scratch_bytes(int64_t M, int64_t K);
 int convrot_w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride);

@@ -1,0 +1,24 @@
+"""CPU: where the 8-bit linear puts its codes in a caller's workspace (every call here is refused before
+any launch; addresses are never read)."""
+
+from __future__ import annotations
+
+import pytest
+
+P, FAR, BF16 = 4096, 1 << 30, 2
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from convrot_mlx_amd import _native
+
+    return _native.load()
+
+
+@pytest.mark.parametrize("nbytes", [22 * 1024, 32 * 1024, 36 * 1024, 37 * 1024])
+def test_codes_stay_off_the_control_block(lib, nbytes):
+    """40 rows of 64 features need 5280 bytes: at most a quarter of these workspaces, but what they leave is
+    less than the 32 KiB of the control block, whose counters stay zero between launches."""
+    assert lib.convrot_w8a8_scratch_bytes(40, 64) == 5280 <= nbytes // 4
+    rc = lib.convrot_w8a8_linear(P, BF16, 64, P, 64, P, None, 40, 8, 64, None, None, 0, 1, None, 0, P, nbytes, FAR, None)
+    assert rc == 1 and "scratch buffer of 5280 bytes" in lib.convrot_last_error().decode()
