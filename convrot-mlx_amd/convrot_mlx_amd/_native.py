@@ -66,6 +66,7 @@ SIGNATURES = {
     "convrot_quantize_int8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "convrot_w8a8_gemm": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,
                                  _i64, _vp, _i32, _vp]),
+    "convrot_w8a8_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "convrot_w8a8_scratch_bytes": (_i64, [_i64, _i64]),
     "convrot_w8a8_fused": (_i32, [_vp, _i32, _i64, _i64, _i64]),
     "convrot_w8a8_linear": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp,

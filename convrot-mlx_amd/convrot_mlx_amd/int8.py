@@ -96,12 +96,28 @@ def _output(gr: GatedResidual | None, m: int, n: int, dtype: torch.dtype, device
     return torch.empty((m, n), dtype=dtype, device=device)
 
 
+_CONTROL_BYTES = 32768  # of a workspace: zero before a launch
+
+
+def _product_workspace(device, stream: int, capturing: bool, m: int, n: int, k: int) -> torch.Tensor | None:
+    """Counters and partial sums of a product whose workgroups share K: the stream's, or, as a graph may be
+    replayed beside that stream and beside other graphs, memory of the graph's own."""
+    if not capturing:
+        return _workspace(device, stream)
+    need = nat.load().convrot_w8a8_workspace_bytes(m, n, k)
+    if need == 0:
+        return None
+    work = torch.empty((need,), dtype=torch.uint8, device=device)
+    work[:_CONTROL_BYTES].zero_()
+    return work
+
+
 def _w8a8(act, weight, xscales, wscales, bias, k: int, dtype: torch.dtype, gr: GatedResidual | None) -> torch.Tensor:
     """The product of operands as the kernel reads them (see _operand)."""
     m, n = act.shape[0], weight.shape[0]
     out = _output(gr, m, n, dtype, act.device)
     stream = nat.stream_handle(act.device)
-    work = _workspace(act.device, stream)
+    work = _product_workspace(act.device, stream, torch.cuda.is_current_stream_capturing(), m, n, k)
     nat.check(nat.load().convrot_w8a8_gemm(
         act.data_ptr(), _row_stride(act), xscales.data_ptr(), weight.data_ptr(), _row_stride(weight), wscales.data_ptr(),
         None if bias is None else bias.data_ptr(), m, n, k, *_residual_args(gr),
@@ -119,12 +135,13 @@ def _linear(x: torch.Tensor, weight: torch.Tensor, wscales, bias, k: int, residu
     out = _output(gr, m, n, x.dtype, device)
     lib, dtype, stride = nat.load(), nat.dtype_code(x.dtype), x2d.stride(0)
     stream = nat.stream_handle(device)
-    work = _workspace(device, stream)
+    capturing = torch.cuda.is_current_stream_capturing()
+    work = _product_workspace(device, stream, capturing, m, n, k)
     work_bytes = 0 if work is None else work.numel()
     # codes and scales between the two launches: the end of the stream's workspace holds up to a
-    # quarter of it; a graph, which may be replayed beside this stream, holds its own
+    # quarter of it; a graph holds its own
     need, scratch = m * ((k + 127) // 128 * 128 + 4), None
-    if need * 4 > work_bytes or torch.cuda.is_current_stream_capturing():
+    if need * 4 > work_bytes or capturing:
         scratch = torch.empty((need,), dtype=torch.uint8, device=device)
     nat.check(lib.convrot_w8a8_linear(
         x2d.data_ptr(), dtype, stride, weight.data_ptr(), _row_stride(weight), wscales.data_ptr(),

@@ -846,6 +846,11 @@ int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscale
                        "convrot_w8a8_gemm");
 }
 
+int64_t convrot_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxFeatures || M > 0x7ffffe00 || N > 0x7ffffe00) return 0;
+  return convrot::w8a8_workspace_bytes(M, N, K);
+}
+
 // Rows of codes in whole cache lines (rows of 2112 bytes: the product 10 % slower).
 static int64_t codes_stride_of(int64_t K) { return (K + 127) / 128 * 128; }
 

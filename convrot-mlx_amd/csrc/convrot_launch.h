@@ -192,6 +192,9 @@ hipError_t launch_w8a8_gemm(const int8_t* act, int64_t lda, const float* xscales
                             const float* wscales, const float* bias, int64_t M, int64_t N, int64_t K, void* out,
                             int out_dtype, hipStream_t stream, const GatedResidual& gr, const Workspace& work);
 
+// Workspace that launch_w8a8_gemm uses for a shape (0: none).
+int64_t w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
 // Whether a few rows are quantized inside their product's launch, and that launch.
 bool w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride);
 hipError_t launch_w8a8_fused(const void* x, int64_t x_stride, int dtype, const int8_t* weight, int64_t ldw,

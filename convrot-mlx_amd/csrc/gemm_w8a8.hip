@@ -329,6 +329,24 @@ hipError_t launch_w8a8_gemm(const int8_t* act, int64_t lda, const float* xscales
   }
 }
 
+// What a product asks of a workspace as large as the W4A4 GEMM's: with these bytes the choices above
+// come out the same.
+int64_t w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  const Workspace all{(uint8_t*)256, kSkWorkspaceBytes};  // never read here
+  const int kblocks = (int)((K + 127) / 128);
+  int64_t tiles, splits, bytes;
+  if (rows_kernel(M) && rows_fit(M, N, K)) {
+    tiles = (N + kRowsN - 1) / kRowsN, bytes = 4096;
+    splits = rows_splits(tiles, kblocks, all);
+  } else {
+    const Choice c = choose(M, N, K, all);
+    const int64_t bm = c.tile & 1023, bn = c.tile >> 10;
+    tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn), bytes = bm * bn * 4;
+    splits = c.splits;
+  }
+  return splits > 1 ? (int64_t)kW8a8PartialOffset + tiles * splits * bytes : 0;
+}
+
 bool w8a8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
   const size_t es = dtype == kF32 ? 4 : 2;
   return rows_kernel(M) && M * K * (int64_t)es <= kFusedBytes && K % 16 == 0 && ((uintptr_t)x & 15) == 0 &&

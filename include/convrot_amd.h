@@ -453,8 +453,10 @@ int convrot_quantize_int8(const void* x, int dtype, int64_t rows, int64_t featur
  * zero (the activations' may be anything).  K <= 65536.  out [M, N] contiguous.
  * workspace (may be NULL): the W4A4 / W4A16 GEMMs' (convrot_w4a4_workspace_bytes,
  * zero-filled once), which lets workgroups share the K of few tiles; the same
- * bits with and without it.
+ * bits with and without it.  convrot_w8a8_workspace_bytes(M, N, K) bytes, their first
+ * 32 KiB zero, serve a product (or convrot_w8a8_linear with a scratch buffer) as well; 0: it uses none.
  */
+int64_t convrot_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int convrot_w8a8_gemm(const int8_t* act, int64_t act_stride, const float* xscales, const int8_t* weight,
                       int64_t weight_stride, const float* wscales, const float* bias, int64_t M, int64_t N,
                       int64_t K, const void* residual, const void* gate, int64_t gate_stride,

@@ -137,3 +137,60 @@ def test_rows_too_far_apart_are_copied(dev):
         far.copy_(codes)
         got = hip_w8a8_matmul(*((qa, far) if swap else (far, qw)), xs, ws, bias, output_dtype=BF16)
         assert torch.equal(got.cpu(), product_plain(*host, BF16))
+
+
+SHARED = [(24, 1024, 12288), (4, 1024, 12288), (1, 512, 8192)]  # tiles and few rows whose workgroups share K
+
+
+@pytest.mark.parametrize("m,n,k", SHARED)
+def test_graphs_with_shared_k_side_by_side(dev, m, n, k):
+    """Two graphs captured on one stream, replayed on two others beside eager calls on it: each product has
+    counters and partial sums of its own."""
+    from convrot_mlx_amd import _native, hip_w8a8_linear, hip_w8a8_matmul, quantize_int8_rowwise
+
+    assert _native.load().convrot_w8a8_workspace_bytes(m, n, k) > 32768
+    _, (_, qw, _, ws, bias) = operands(m, 1, n, k, dev)
+    xs = [torch.randn((m, k), generator=torch.Generator().manual_seed(i)).to(BF16).to(dev) for i in range(3)]
+    want = [hip_w8a8_linear(x, qw, ws, bias).clone() for x in xs]
+    capture, others = torch.cuda.Stream(), [torch.cuda.Stream(), torch.cuda.Stream()]
+    capture.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(capture):
+        hip_w8a8_linear(xs[0], qw, ws, bias)  # the stream has a workspace
+        for x in xs[:2]:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=capture):
+                codes, scales = quantize_int8_rowwise(x)
+                outs.append([o for _ in range(8) for o in (
+                    hip_w8a8_linear(x, qw, ws, bias),
+                    hip_w8a8_matmul(codes, qw, scales, ws, bias, output_dtype=BF16))])
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for out in outs:
+            for o in out:
+                o.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, others):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(capture):
+            eager = [hip_w8a8_linear(xs[2], qw, ws, bias) for _ in range(16)]
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert all(torch.equal(o, w) for o in out)
+        assert all(torch.equal(o, want[2]) for o in eager)
+
+
+@pytest.mark.parametrize("split", [2, 3, 7, 64])
+@pytest.mark.parametrize("tile,m", [("160x128", 200), ("128x160", 150)])
+def test_shared_k_of_the_largest_tiles(dev, tuning, tile, m, split):
+    from convrot_mlx_amd import hip_w8a8_matmul
+
+    tuning.set("w8a8_tile", tile)
+    tuning.set("w8a8_split", split)
+    for n, k in ((70, 992), (200, 4112)):
+        host, (qa, qw, xs, ws, bias) = operands(m + k, m, n, k, dev)
+        want = product_plain(*host, BF16)
+        for _ in range(3):
+            assert torch.equal(hip_w8a8_matmul(qa, qw, xs, ws, bias, output_dtype=BF16).cpu(), want)
