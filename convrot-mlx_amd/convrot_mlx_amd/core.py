@@ -130,6 +130,31 @@ def _prepare(x: torch.Tensor, group_size: int, mode: int) -> tuple[torch.Tensor,
     return out, scales
 
 
+def check_vectors(shape: tuple, *vectors: torch.Tensor | None) -> None:
+    """Modulation vectors go to even groups of x's rows, in order: any [V, K], and of more axes the
+    shapes that broadcast over x of `shape` that way (x's leading axes, then ones).  Refuses the others,
+    e.g. [1, L, K] beside x [B, L, K], which would broadcast to other rows."""
+    for t in vectors:
+        if t is None or t.ndim < 3 or len(shape) < 3:
+            continue
+        lead, rows = tuple(t.shape[:-1]), tuple(shape[:-1])
+        aligned = (1,) * (len(rows) - len(lead)) + lead
+        if len(lead) <= len(rows) and all(d in (1, n) for d, n in zip(aligned, rows)):
+            repeated = False
+            for d, n in zip(aligned, rows):
+                good = d == 1 or not repeated
+                repeated |= d == 1 < n
+                if not good:
+                    break
+        else:  # [V, 1, K] of any V
+            while lead and lead[-1] == 1:
+                lead = lead[:-1]
+            good = len(lead) <= 1 or lead == rows[: len(lead)]
+        if not good:
+            raise ValueError(f"modulation vectors {tuple(t.shape)} beside x {tuple(shape)} are no even groups of rows in "
+                             f"order; pass [V, {shape[-1]}], or x's leading axes followed by ones")
+
+
 def _modulation_rows(rows: int, features: int, shift: torch.Tensor, scale: torch.Tensor):
     """shift / scale as [V, K] rows of the activation dtype, and the rows of x per vector."""
     if shift.shape[-1] != features or scale.shape[-1] != features:

@@ -289,7 +289,7 @@ class Int8Linear(nn.Module):
         x2d = flat_rows(x)
         m = x2d.shape[0]
         gr = _residual(residual, gate, inplace, m, self.out_features, x.dtype)
-        gain, sh, each, _ = norm_operands(x2d, None, None, scale, shift)
+        gain, sh, each, _ = norm_operands(x2d, None, None, scale, shift, x.shape)
         codes = torch.empty((m, _round16(k)), dtype=torch.int8, device=x.device)
         scales = torch.empty((m,), dtype=torch.float32, device=x.device)
         nat.check(nat.load().convrot_layer_norm_int8(

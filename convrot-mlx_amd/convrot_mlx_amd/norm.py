@@ -14,6 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
+from .core import check_vectors
 
 MAX_BACKWARD_FEATURES = 32768
 
@@ -34,10 +35,11 @@ def flat_rows(x: torch.Tensor) -> torch.Tensor:
     return rows_of(x)
 
 
-def norm_operands(x2d, weight, bias, scale, shift):
-    """(gain or None, shift or None, rows a vector, plus one?) of a norm's parameters: contiguous
-    rows of K, both of one type that the kernels take beside x's."""
+def norm_operands(x2d, weight, bias, scale, shift, shape):
+    """(gain or None, shift or None, rows a vector, plus one?) of a norm's parameters beside x of `shape`:
+    contiguous rows of K, both of one type that the kernels take beside x's."""
     rows, k = x2d.shape
+    check_vectors(shape, scale, shift)
     if (weight is not None or bias is not None) and (scale is not None or shift is not None):
         raise ValueError("layer norm takes weight and bias, or scale and shift")
     plus_one = scale is not None or shift is not None
@@ -71,12 +73,12 @@ def hip_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     """Layer norm over the last axis of x [..., K] (rows at any one stride), of x's type.
 
     weight, bias: [K].  Or scale, shift: [V, K] or [V, 1, K], the rows split evenly over the V
-    vectors in order, as x [B, L, K] beside scale [B, 1, K] does: (1 + scale) * u + shift.  Either
-    of a pair may be None.  With return_stats also the rows' float32 mean and 1 / sqrt(var + eps)."""
+    vectors in order, as x [B, L, K] beside scale [B, 1, K] does: (1 + scale) * u + shift (shapes that
+    broadcast to other rows, [1, L, K], are refused).  Either of a pair may be None.  With return_stats also the rows' float32 mean and 1 / sqrt(var + eps)."""
     device = nat.on_device(x, weight, bias, scale, shift)
     x2d = flat_rows(x)
     rows, k = x2d.shape
-    gain, add, each, plus_one = norm_operands(x2d, weight, bias, scale, shift)
+    gain, add, each, plus_one = norm_operands(x2d, weight, bias, scale, shift, x.shape)
     out = x.new_empty(x.shape)
     stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if return_stats else None
     mean, rstd = (None, None) if stats is None else stats.unbind(0)
@@ -109,7 +111,7 @@ def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
     for name, t in (("mean", mean), ("rstd", rstd)):
         if tuple(t.shape) != (rows,) or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous float32 {(rows,)}, got {t.dtype} {tuple(t.shape)}")
-    gain, _, each, plus_one = norm_operands(x2d, weight, None, scale, None)
+    gain, _, each, plus_one = norm_operands(x2d, weight, None, scale, None, x.shape)
     if gain is None and vectors is not None:
         if vectors < 1 or rows % vectors:
             raise ValueError(f"{rows} activation rows do not split evenly over {vectors} modulation vectors")
