@@ -207,13 +207,15 @@ def hip_fused_modulated_prepare(
 
     x: [rows, K] (or [..., K]); shift, scale: [V, K] (or [V, 1, K]) with rows
     divisible by V -- rows r*rows/V .. use vector r, as x [B, L, K] with
-    shift [B, 1, K] does.  output: "int8" (int8 codes + f32 scales), "packed"
-    (uint8 [rows, K/2] + scales) or "rotate" (rotated activation of x's dtype).
+    shift [B, 1, K] does (shapes that broadcast to other rows are refused).
+    output: "int8" (int8 codes + f32 scales), "packed" (uint8 [rows, K/2] + scales) or
+    "rotate" (rotated activation of x's dtype).
     """
     modes = {"int8": nat.PREP_INT8, "packed": nat.PREP_PACKED, "rotate": nat.PREP_ROTATE}
     if output not in modes:
         raise ValueError(f"output must be one of {sorted(modes)}, got {output!r}")
     _validate_fused(x.reshape(-1, x.shape[-1]), group_size, "modulated activation preparation")
+    check_vectors(x.shape, shift, scale)
     out, scales = _prepare_modulated(x.reshape(-1, x.shape[-1]), shift, scale, group_size, modes[output], eps)
     return out if output == "rotate" else (out, scales)
 
@@ -1167,6 +1169,7 @@ class ConvRotLinear(nn.Module):
         gate and inplace as in forward."""
         if x.shape[-1] != self.in_features:
             raise ValueError(f"ConvRotLinear expected K={self.in_features}, got {x.shape[-1]}")
+        check_vectors(x.shape, shift, scale)
         x2d = x.reshape(-1, self.in_features)
         return self._project(lambda mode: _prepare_modulated(x2d, shift, scale, self.group_size, mode, eps),
                              x.shape[:-1], x.dtype, residual, gate, inplace)

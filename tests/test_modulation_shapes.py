@@ -37,3 +37,15 @@ def test_refused(lead, vectors, name):
     kw = dict(scale=None, shift=None) | {name: t}
     with pytest.raises(ValueError, match="no even groups of rows"):
         norm.norm_operands(x.reshape(-1, K), None, None, kw["scale"], kw["shift"], x.shape)
+
+
+def test_refused_by_the_fused_preparation():
+    from convrot_mlx_amd import ConvRotLinear, hip_fused_modulated_prepare
+
+    x, t = torch.zeros(4, 5, 64), torch.zeros(1, 5, 64)
+    with pytest.raises(ValueError, match="no even groups of rows"):
+        hip_fused_modulated_prepare(x, t, t, 64)
+    with pytest.raises(ValueError, match="no even groups of rows"):
+        ConvRotLinear(64, 16, group_size=64).forward_modulated(x, t, t)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        hip_fused_modulated_prepare(x, t.transpose(0, 1), t.transpose(0, 1), 64)
