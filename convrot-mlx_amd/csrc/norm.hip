@@ -252,6 +252,10 @@ __global__ __launch_bounds__(T* TEAMS) void norm_backward_kernel(
     }
   };
 
+  // The mean, but zero past the row: of a constant row of large values (0 - mean) rstd is infinite,
+  // and zero (d there) times it no number.
+  auto centre = [&](float mu, int c, int j) { return feature_of<T, C, VEC>(t, c, VEC ? 0 : j) < K ? mu : 0.0f; };
+
   struct Rows {
     RawChunk<DT, T, C, VEC> x[R][C], d[R][C];
     float mu[R], rs[R];
@@ -297,7 +301,7 @@ __global__ __launch_bounds__(T* TEAMS) void norm_backward_kernel(
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           // features past the row: d is zero
-          u[j] = (u[j] - cur.mu[i]) * cur.rs[i];
+          u[j] = (u[j] - centre(cur.mu[i], c, j)) * cur.rs[i];
           db[c][j] += d[j];
           dg[c][j] += d[j] * u[j];
           const float h = d[j] * (C == 1 ? g1[j] : g[j]);
@@ -321,7 +325,7 @@ __global__ __launch_bounds__(T* TEAMS) void norm_backward_kernel(
         cur.x[i][c].get(u), cur.d[i][c].get(d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          u[j] = (u[j] - cur.mu[i]) * cur.rs[i];
+          u[j] = (u[j] - centre(cur.mu[i], c, j)) * cur.rs[i];
           d[j] = cur.rs[i] * (d[j] * (C == 1 ? g1[j] : g[j]) - m0 - u[j] * m1);
         }
         store_chunk<DT, T, C, VEC>((E*)dx + row * (int64_t)K, K, t, c, d);
