@@ -92,13 +92,15 @@ def hip_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
 
 def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, *,
                             weight: torch.Tensor | None = None, scale: torch.Tensor | None = None,
-                            vectors: int | None = None, param_grads: bool = True):
+                            vectors: int | None = None, param_grads: bool = True,
+                            shift_dtype: torch.dtype | None = None):
     """Gradients of hip_layer_norm from dy, its input and its stats: (dx, dgain, dshift).
 
     dgain is the gradient of weight (or scale), dshift that of bias (or shift), [K] beside a
     weight, else of scale's shape ([vectors, K] where the norm had a shift alone: pass `vectors`);
-    both are of the parameter's type (x's without one), None without param_grads.  Sums over rows
-    are float32 in a fixed order: results repeat bit for bit."""
+    both are of the weight's or scale's type (x's without one), None without param_grads.  A bias or
+    shift of another type: pass it as `shift_dtype`, and dshift is rounded to that one alone.  Sums
+    over rows are float32 in a fixed order: results repeat bit for bit."""
     nat.require_device(dy, x, mean, rstd, weight, scale)
     if dy.shape != x.shape:
         raise ValueError(f"dy {tuple(dy.shape)} must have the shape of x {tuple(x.shape)}")
@@ -120,6 +122,12 @@ def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
         vectors = gain.numel() // k
     given = scale if scale is not None else weight
     kind = x.dtype if gain is None else gain.dtype
+    gain_dtype = x.dtype if given is None else given.dtype
+    if shift_dtype is None:
+        shift_dtype = gain_dtype
+    if param_grads and kind != torch.float32 and shift_dtype != kind:
+        kind = torch.float32  # the sums as they are, each rounded once to its parameter's type
+        gain = None if gain is None else gain.to(kind)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     grads = work = None
     lib = nat.load()
@@ -136,11 +144,8 @@ def hip_layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
         return dx, None, None
     if rows == 0:
         grads.zero_()
-    if given is not None:
-        grads = grads.to(given.dtype).reshape(2, *given.shape)
-    elif vectors is None:
-        grads = grads.reshape(2, k)
-    return dx, grads[0], grads[1]
+    shape = given.shape if given is not None else (k,) if vectors is None else (vectors, k)
+    return dx, grads[0].reshape(shape).to(gain_dtype), grads[1].reshape(shape).to(shift_dtype)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -162,9 +167,10 @@ class _LayerNorm(torch.autograd.Function):
         if ctx.adaptive and scale is None:
             vectors = ctx.add[0].numel() // max(1, x.shape[-1])
         dx, dgain, dadd = hip_layer_norm_backward(dy, x, mean, rstd, weight=weight, scale=scale, vectors=vectors,
-                                                  param_grads=any(needs[1:5]))
+                                                  param_grads=any(needs[1:5]),
+                                                  shift_dtype=None if ctx.add is None else ctx.add[1])
         if dadd is not None and ctx.add is not None:
-            dadd = dadd.reshape(ctx.add[0]).to(ctx.add[1])
+            dadd = dadd.reshape(ctx.add[0])
         a = ctx.adaptive
         return (dx if needs[0] else None, dgain if needs[1] and not a else None, dadd if needs[2] and not a else None,
                 dgain if needs[3] and a else None, dadd if needs[4] and a else None, None)

@@ -54,3 +54,46 @@ def test_gradient_of_constant_rows_of_large_values(dev, rows, k, dtype):
     assert_within(dx, wdx, odx, "dx")
     assert_within(dw, wdw[0], odw[0], "dw")
     assert_within(db, wdb[0], odb[0], "db")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("form", ["bias", "weight16", "shift", "scale16", "weight32", "f64"])
+def test_each_gradient_is_rounded_to_its_own_type(dev, dtype, form):
+    """A float32 bias or shift beside 16-bit activations, alone or beside a 16-bit weight or scale: its
+    gradient is the float32 sum, and the weight's that sum in 16 bits."""
+    from convrot_mlx_amd import layer_norm
+
+    x, w, b, dy = inputs(23, 300, 640, dtype, dev, 2)
+    adaptive = form in ("shift", "scale16")
+    other = torch.float64 if form == "f64" else F32
+    gain = None if form in ("bias", "shift") else w if adaptive else (w[0] + 1).to(F32 if form == "weight32" else dtype)
+    add = (b if adaptive else b[0]).to(dtype if form == "weight32" else other)
+    leaves = [t.detach().clone().requires_grad_() for t in (gain, add) if t is not None]
+    names = ("scale", "shift") if adaptive else ("weight", "bias")
+    y = layer_norm(x, eps=EPS, **dict(zip(names[2 - len(leaves):], leaves)))
+    y.backward(dy)
+    vectors = 2 if adaptive else 1
+    g64 = torch.ones(1, 640, dtype=torch.float64) if gain is None else gain.double().cpu().reshape(vectors, 640) + adaptive
+    _, _, wdg, odg, wdb, odb = norm_grads(x.double().cpu(), g64.repeat_interleave(300 // vectors, 0)
+                                          if adaptive and gain is not None else g64, dy.double().cpu(), EPS, vectors)
+    assert leaves[-1].grad.dtype == leaves[-1].dtype
+    sums = leaves[-1].grad.reshape(vectors, 640)
+    assert_within(sums.float(), wdb, odb, "dshift") if form != "weight32" else assert_within(sums, wdb, odb, "dshift")
+    if gain is not None:
+        assert leaves[0].grad.dtype == gain.dtype
+        assert_within(leaves[0].grad.reshape(vectors, 640), wdg, odg, "dgain")
+
+
+def test_float32_shift_beyond_the_range_of_float16(dev):
+    from convrot_mlx_amd import hip_layer_norm, hip_layer_norm_backward, layer_norm
+
+    x, w, _, _ = inputs(29, 400, 64, F16, dev)
+    dy = torch.full((400, 64), 1000.0, dtype=F16, device=dev)
+    for kw in ({}, dict(weight=w[0] + 1)):
+        bias = torch.zeros(64, device=dev, requires_grad=True)
+        layer_norm(x, bias=bias, eps=EPS, **kw).backward(dy)
+        assert torch.equal(bias.grad, torch.full((64,), 400e3, device=dev))
+        _, mean, rstd = hip_layer_norm(x, eps=EPS, return_stats=True, **kw)
+        _, dgain, dshift = hip_layer_norm_backward(dy, x, mean, rstd, shift_dtype=F32, **kw)
+        assert dgain.dtype == F16 and torch.equal(dshift, bias.grad)
+        assert hip_layer_norm_backward(dy, x, mean, rstd, **kw)[2].isinf().all()  # without it, x's type
