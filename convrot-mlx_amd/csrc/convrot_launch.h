@@ -37,6 +37,10 @@ enum TuneKey : int {
 };
 int tuning(TuneKey key);
 
+// Workgroups of `threads` that one launch takes: a HIP grid has fewer than 2^32 threads an axis.
+// Operators whose rows may need more go in several launches.
+constexpr int64_t max_groups(int threads) { return 0xffffffffll / threads; }
+
 // Whether a tile forced through convrot_set_tuning is one the library builds:
 // a W4A4 INT8 tile (DMA kernels with ring depth `stages`, 0 for any, or the
 // register-staged kernel), an FP6 W4A4 tile, a W4A16 tiled-kernel tile.

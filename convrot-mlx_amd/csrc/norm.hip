@@ -168,9 +168,22 @@ struct RowArgs {
 template <int DT, int OP, int T, int C, bool VEC>
 void run_rows(const RowArgs& a, hipStream_t stream) {
   constexpr int TEAMS = T == 64 ? 4 : 1;
-  row_kernel<DT, T, C, VEC, OP><<<dim3((unsigned)((a.rows + TEAMS - 1) / TEAMS)), dim3(T * TEAMS), 0, stream>>>(
-      a.x, a.rows, (int)a.K, a.x_stride, a.gain, a.shift, a.param_dtype, a.plus_one, a.rows_per_vector, a.eps, a.out,
-      a.out_stride, a.mean, a.rstd, a.scales);
+  constexpr int64_t MOST = max_groups(T * TEAMS) * TEAMS;
+  const int64_t es = DT == kF32 ? 4 : 2, out_row = a.out_stride * (OP == kNormOut ? es : 1);
+  const int64_t param_row = a.K * (a.param_dtype == kF32 ? 4 : 2), each = a.rows_per_vector;
+  for (int64_t row = 0; row < a.rows;) {
+    // whole vectors, or rows inside one that is longer than a launch
+    const int64_t vector = each > 0 ? row / each : 0, in_vector = each > 0 ? row % each : 0;
+    int64_t n = std::min(a.rows - row, MOST), rows_per_vector = each;
+    if (each > MOST) n = rows_per_vector = std::min(n, each - in_vector);
+    else if (each > 0 && n < a.rows - row) n = n / each * each;
+    auto params = [&](const void* p) { return p ? (const char*)p + vector * param_row : nullptr; };
+    row_kernel<DT, T, C, VEC, OP><<<dim3((unsigned)((n + TEAMS - 1) / TEAMS)), dim3(T * TEAMS), 0, stream>>>(
+        (const char*)a.x + row * a.x_stride * es, n, (int)a.K, a.x_stride, params(a.gain), params(a.shift),
+        a.param_dtype, a.plus_one, rows_per_vector, a.eps, (char*)a.out + row * out_row, a.out_stride,
+        a.mean ? a.mean + row : nullptr, a.rstd ? a.rstd + row : nullptr, a.scales ? a.scales + row : nullptr);
+    row += n;
+  }
 }
 
 template <int DT, int OP>
@@ -429,10 +442,16 @@ template <int DT, int T, int C, bool VEC>
 hipError_t run_backward(const BackwardArgs& a, hipStream_t stream) {
   constexpr int TEAMS = backward_teams(T);
   const size_t lds = TEAMS > 1 && a.partial ? (size_t)a.K * 8 : 0;  // at most 16 KB
-  const int64_t vectors = a.rows / a.rows_per_vector;
-  norm_backward_kernel<DT, T, C, VEC, TEAMS><<<dim3((unsigned)(vectors * a.parts)), dim3(T * TEAMS), lds, stream>>>(
-      a.dy, a.dy_stride, a.x, a.x_stride, a.mean, a.rstd, (int)a.K, a.gain, a.param_dtype, a.plus_one,
-      a.rows_per_vector, a.parts, a.dx, a.partial);
+  const int64_t vectors = a.rows / a.rows_per_vector, most = std::max<int64_t>(1, max_groups(T * TEAMS) / a.parts);
+  const int64_t es = DT == kF32 ? 4 : 2, param_row = a.K * (a.param_dtype == kF32 ? 4 : 2);
+  for (int64_t v = 0; v < vectors; v += most) {
+    const int64_t n = std::min(most, vectors - v), row = v * a.rows_per_vector;
+    norm_backward_kernel<DT, T, C, VEC, TEAMS><<<dim3((unsigned)(n * a.parts)), dim3(T * TEAMS), lds, stream>>>(
+        (const char*)a.dy + row * a.dy_stride * es, a.dy_stride, (const char*)a.x + row * a.x_stride * es, a.x_stride,
+        a.mean + row, a.rstd + row, (int)a.K, a.gain ? (const char*)a.gain + v * param_row : nullptr, a.param_dtype,
+        a.plus_one, a.rows_per_vector, a.parts, (char*)a.dx + row * a.K * es,
+        a.partial ? a.partial + v * a.parts * 2 * a.K : nullptr);
+  }
   return hipGetLastError();
 }
 
@@ -501,9 +520,13 @@ hipError_t launch_layer_norm_backward(const void* dy, int64_t dy_stride, const v
   else if (dtype == kF16) e = vec ? pick_backward<kF16, true>(a, stream) : pick_backward<kF16, false>(a, stream);
   else e = vec ? pick_backward<kBF16, true>(a, stream) : pick_backward<kBF16, false>(a, stream);
   if (e != hipSuccess || !a.partial) return e;
-  const int64_t vectors = rows / rows_per_vector;
-  sum_parts_kernel<<<dim3((unsigned)(vectors * ((2 * K + 63) / 64))), dim3(1024), 0, stream>>>(
-      a.partial, a.parts, (int)K, dgain, dshift, param_dtype);
+  const int64_t vectors = rows / rows_per_vector, groups = (2 * K + 63) / 64, most = max_groups(1024) / groups;
+  const int64_t param_row = K * (param_dtype == kF32 ? 4 : 2);
+  for (int64_t v = 0; v < vectors; v += most) {
+    auto params = [&](void* p) { return p ? (char*)p + v * param_row : nullptr; };
+    sum_parts_kernel<<<dim3((unsigned)(std::min(most, vectors - v) * groups)), dim3(1024), 0, stream>>>(
+        a.partial + v * a.parts * 2 * K, a.parts, (int)K, params(dgain), params(dshift), param_dtype);
+  }
   return hipGetLastError();
 }
 

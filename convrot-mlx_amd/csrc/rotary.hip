@@ -45,6 +45,7 @@ struct RotaryArgs {
   int64_t table_sb;            // elements from one batch entry's table to the next, 0: shared
   float eps;
   int splits;                  // waves that share a token's heads (forward)
+  int64_t first;               // first unit (token and split) of a launch (forward)
   int64_t tokens;              // batch * length
   float* partial;              // backward: [workgroups][2][D]
 };
@@ -99,7 +100,7 @@ template <int DT, int G, bool PAIRS>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs r) {
   constexpr int HPW = 64 / G;  // heads a wave holds at a time
   const int lane = threadIdx.x & 63, c = lane % G, slot = lane / G;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t unit = r.first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const uint32_t token = (uint32_t)(unit / (uint32_t)r.splits), split = (uint32_t)(unit % (uint32_t)r.splits);
   if (token >= r.tokens) return;
   const uint32_t b = token / (uint32_t)r.length, l = token % (uint32_t)r.length;
@@ -462,16 +463,18 @@ hipError_t run_rotary(RotaryArgs r, bool interleaved, bool backward, hipStream_t
     r.splits = (int)std::min<int64_t>(steps, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, r.tokens)));
     waves *= r.splits;
   }
-  const int64_t blocks = (waves + 3) / 4;
-  if (!backward && blocks > 0x7fffffff) return hipErrorInvalidValue;
-  const unsigned grid = (unsigned)(backward ? backward_groups(r.tokens) : blocks);
-  switch (G) {
-    case 1: run_vec<DT, 1>(r, interleaved, backward, grid, s); break;
-    case 2: run_vec<DT, 2>(r, interleaved, backward, grid, s); break;
-    case 4: run_vec<DT, 4>(r, interleaved, backward, grid, s); break;
-    case 8: run_vec<DT, 8>(r, interleaved, backward, grid, s); break;
-    case 16: run_vec<DT, 16>(r, interleaved, backward, grid, s); break;
-    default: run_vec<DT, 32>(r, interleaved, backward, grid, s); break;
+  const int64_t blocks = backward ? backward_groups(r.tokens) : (waves + 3) / 4;
+  for (int64_t b = 0; b < blocks; b += max_groups(256)) {
+    r.first = 4 * b;
+    const unsigned grid = (unsigned)std::min(blocks - b, max_groups(256));
+    switch (G) {
+      case 1: run_vec<DT, 1>(r, interleaved, backward, grid, s); break;
+      case 2: run_vec<DT, 2>(r, interleaved, backward, grid, s); break;
+      case 4: run_vec<DT, 4>(r, interleaved, backward, grid, s); break;
+      case 8: run_vec<DT, 8>(r, interleaved, backward, grid, s); break;
+      case 16: run_vec<DT, 16>(r, interleaved, backward, grid, s); break;
+      default: run_vec<DT, 32>(r, interleaved, backward, grid, s); break;
+    }
   }
   return hipGetLastError();
 }
@@ -539,13 +542,18 @@ hipError_t launch_axes_table(const void* positions, int kind, int64_t rows, int 
   for (int a = 0; a < axes; ++a) ax.half[a] = dims[a] / 2, P += dims[a] / 2;
   const int64_t n = rows * P;
   if (n == 0) return hipSuccess;
-  const dim3 grid((unsigned)((n + 255) / 256)), block(256);
   const double lt = log(theta);
-  switch (kind) {
-    case CONVROT_POS_F32: axes_table_kernel<float><<<grid, block, 0, stream>>>((const float*)positions, rows, ax, P, lt, out); break;
-    case CONVROT_POS_F64: axes_table_kernel<double><<<grid, block, 0, stream>>>((const double*)positions, rows, ax, P, lt, out); break;
-    case CONVROT_POS_I32: axes_table_kernel<int><<<grid, block, 0, stream>>>((const int*)positions, rows, ax, P, lt, out); break;
-    default: axes_table_kernel<int64_t><<<grid, block, 0, stream>>>((const int64_t*)positions, rows, ax, P, lt, out); break;
+  const int64_t most = max_groups(256) * 256 / P;  // rows of a launch
+  for (int64_t row = 0; row < rows; row += most) {
+    const int64_t count = std::min(most, rows - row), at = row * axes;
+    float* o = out + row * P * 2;
+    const dim3 grid((unsigned)((count * P + 255) / 256)), block(256);
+    switch (kind) {
+      case CONVROT_POS_F32: axes_table_kernel<float><<<grid, block, 0, stream>>>((const float*)positions + at, count, ax, P, lt, o); break;
+      case CONVROT_POS_F64: axes_table_kernel<double><<<grid, block, 0, stream>>>((const double*)positions + at, count, ax, P, lt, o); break;
+      case CONVROT_POS_I32: axes_table_kernel<int><<<grid, block, 0, stream>>>((const int*)positions + at, count, ax, P, lt, o); break;
+      default: axes_table_kernel<int64_t><<<grid, block, 0, stream>>>((const int64_t*)positions + at, count, ax, P, lt, o); break;
+    }
   }
   return hipGetLastError();
 }
