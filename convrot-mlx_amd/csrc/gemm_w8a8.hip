@@ -249,6 +249,7 @@ Choice choose(int64_t M, int64_t N, int64_t K, const Workspace& work) {
     for (int s = 1; s <= most; ++s) {
       if (forced_splits > 0 ? s != std::min(forced_splits, most) : s > 1 && (kblocks < 8 * s || tiles * s > 256)) continue;
       const int64_t groups = tiles * s, rounds = groups / slots;
+      if (groups > max_groups(256)) continue;
       const float part = (float)(groups - rounds * slots) / (float)slots, blocks = (float)((kblocks + s - 1) / s);
       float t = (float)rounds * (blocks * c.full + c.fixed);
       if (part > 0.0f)  // few workgroups run at a higher clock, and alone on their CUs

@@ -139,7 +139,8 @@ struct Engine {
       const int q = d - (arr == 0 ? 0 : arr == 1 ? XS_DMAS : XS_DMAS + WS_DMAS);
       const int off = arr == 0 ? XS_OFF : arr == 1 ? WS_OFF : BIAS_OFF;
       const float* base = arr == 0 ? p.xscales + m0 : arr == 1 ? p.wscales + n0 : (p.bias ? p.bias + n0 : p.wscales);
-      const int count = arr == 0 ? p.M - m0 : (arr == 1 || p.bias) ? p.N - n0 : 0;
+      // at most the tile's: four bytes times all that follow may pass 32 bits
+      const int count = arr == 0 ? min(BM, p.M - m0) : (arr == 1 || p.bias) ? min(BN, p.N - n0) : 0;
       dma4(buffer_rsrc(base, (uint32_t)count * 4u), (uint32_t)(q * 256 + lane * 4), smem_addr + (uint32_t)(off + q * 256));
     }
   }
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER
 template <int BM, int BN, int STAGES, int PER_CU, int ODT>
 hipError_t launch_tile(const W8a8Operands& p, const W8a8Split& split, hipStream_t s) {
   const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-  if (tm * tn * split.splits > 0x7fffffff) return hipErrorInvalidValue;
+  if (tm * tn * split.splits > max_groups(256)) return hipErrorInvalidValue;
   w8a8_tile_kernel<BM, BN, STAGES, PER_CU, ODT><<<dim3((unsigned)(tm * tn * split.splits)), dim3(256), 0, s>>>(
       p, (int)tm, (int)tn, split);
   return hipGetLastError();

@@ -84,3 +84,18 @@ def test_axes_table(dev):
     table = rotary_axes_table(pos, (128,))
     for part in seams(ROWS, (2 ** 24 - 1) * 4):
         assert torch.equal(table[part], rotary_axes_table(pos[part], (128,)))
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_product_of_2_30_rows(dev, dtype):
+    """Rows whose scales lie past 4 GiB, and more tiles of 64 x 64 than a launch takes."""
+    from convrot_mlx_amd import hip_w8a8_matmul
+
+    rows = 2 ** 30 + 3000
+    gen = torch.Generator(dev).manual_seed(0)
+    act = torch.randint(-127, 128, (rows, 16), generator=gen, device=dev, dtype=torch.int8)
+    w = torch.randint(-127, 128, (3, 16), generator=gen, device=dev, dtype=torch.int8)
+    xs, ws = torch.rand((rows,), generator=gen, device=dev), torch.rand((3,), generator=gen, device=dev)
+    out = hip_w8a8_matmul(act, w, xs, ws, ws, output_dtype=dtype)
+    for part in seams(rows, 750, 3000, 2 ** 29, 2 ** 30):
+        assert torch.equal(out[part], hip_w8a8_matmul(act[part], w, xs[part], ws, ws, output_dtype=dtype))
