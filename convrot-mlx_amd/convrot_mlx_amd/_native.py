@@ -11,6 +11,7 @@ import ctypes
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_NAME = "libconvrot_amd.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
@@ -156,6 +157,43 @@ def on_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device:
         else:
             return device
     return require_device(first, *rest)
+
+
+def differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether torch differentiates a call on these tensors, in reverse or forward mode."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    # inside a level of dual tensors only (without that name: always asked)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return False
+
+
+class _WithoutGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, run, what, *tensors):
+        ctx.what = what
+        out = run()
+        if any(out is t for t in tensors):
+            ctx.mark_dirty(out)
+            return out
+        return out.data  # no view, so that it may be changed in place
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} has no gradient: run it under torch.no_grad(), or on detached tensors")
+
+
+def without_gradient(run, what: str, *tensors: torch.Tensor | None, target: torch.Tensor | None = None):
+    """run(), a call on these tensors that returns a new one, or writes into and returns `target`, one of
+    them: where torch differentiates it, backward raises an error instead of stopping there in silence."""
+    if not differentiated(*tensors):
+        return run()
+    if target is not None and target.requires_grad and target.is_leaf and torch.is_grad_enabled():
+        raise RuntimeError("a leaf tensor that requires a gradient is used in place")
+    return _WithoutGradient.apply(run, what, *tensors)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -190,8 +190,15 @@ def hip_w8a8_matmul(qact: torch.Tensor, qweight: torch.Tensor, xscales: torch.Te
     nat.dtype_code(output_dtype)
     nat.on_device(qact, qweight, xscales, wscales, bias, residual, gate)
     gr = _residual(residual, gate, inplace, m, n, output_dtype)
-    return _w8a8(_operand(qact, False), _operand(qweight, True), _scales(xscales), _scales(wscales),
-                 _scales(bias), k, output_dtype, gr)
+
+    def run():
+        out = _w8a8(_operand(qact, False), _operand(qweight, True), _scales(xscales), _scales(wscales), _scales(bias), k,
+                    output_dtype, gr)
+        return residual if inplace else out
+
+    out = nat.without_gradient(run, "hip_w8a8_matmul", xscales, wscales, bias, residual, gate,
+                               target=residual if inplace else None)
+    return out.view(m, n) if inplace else out
 
 
 def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, bias: torch.Tensor | None = None,
@@ -202,13 +209,16 @@ def hip_w8a8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tenso
     k = x.shape[-1]
     _check_product(k, qweight, wscales, bias)
     nat.on_device(x, qweight, wscales, bias, residual, gate)
-    return _linear(x, _operand(qweight, True), _scales(wscales), _scales(bias), k, residual, gate, inplace)
+    return nat.without_gradient(
+        lambda: _linear(x, _operand(qweight, True), _scales(wscales), _scales(bias), k, residual, gate, inplace),
+        "hip_w8a8_linear", x, wscales, bias, residual, gate, target=residual if inplace else None)
 
 
 class Int8Linear(nn.Module):
     """A linear layer stored and executed in 8 bits: `qweight` int8 [N, K], `scales` float32 [N]
-    (ones), `bias` float32 [N] (zeros); the output type is the input type.  The calls of
-    ConvRotLinear: forward and forward_modulated, each with residual=, gate= and inplace=."""
+    (ones), `bias` float32 [N] (zeros); the output type is the input type.  Of ConvRotLinear's calls it
+    has forward and forward_modulated, each with residual=, gate= and inplace=.  It has no gradient: a
+    backward pass that reaches it raises an error."""
 
     def __init__(self, in_features: int, out_features: int, *, bias: bool = True, device=None):
         super().__init__()
@@ -277,7 +287,10 @@ class Int8Linear(nn.Module):
                 inplace: bool = False) -> torch.Tensor:
         """linear(x); with `residual`, residual + gate * linear(x), as ConvRotLinear.forward."""
         self._check(x, residual, gate)
-        return _linear(x, self._weight(), _scales(self.scales), _scales(self.bias), self.in_features, residual, gate, inplace)
+        return nat.without_gradient(
+            lambda: _linear(x, self._weight(), _scales(self.scales), _scales(self.bias), self.in_features, residual, gate,
+                            inplace),
+            "Int8Linear", x, self.scales, self.bias, residual, gate, target=residual if inplace else None)
 
     def forward_modulated(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, eps: float = 1e-6, *,
                           residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
@@ -285,6 +298,11 @@ class Int8Linear(nn.Module):
         """self((1 + scale) * layer_norm(x) + shift), the norm and the quantization in one kernel (the
         normalized row goes to codes unrounded); residual, gate and inplace as in forward."""
         self._check(x, residual, gate, shift, scale)
+        return nat.without_gradient(lambda: self._modulated(x, shift, scale, eps, residual, gate, inplace), "Int8Linear", x,
+                                    shift, scale, self.scales, self.bias, residual, gate,
+                                    target=residual if inplace else None)
+
+    def _modulated(self, x, shift, scale, eps, residual, gate, inplace) -> torch.Tensor:
         k = self.in_features
         x2d = flat_rows(x)
         m = x2d.shape[0]

@@ -194,3 +194,21 @@ def test_shared_k_of_the_largest_tiles(dev, tuning, tile, m, split):
         want = product_plain(*host, BF16)
         for _ in range(3):
             assert torch.equal(hip_w8a8_matmul(qa, qw, xs, ws, bias, output_dtype=BF16).cpu(), want)
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_no_gradient_is_lost_in_silence(dev, inplace):
+    """A layer between trained ones keeps its result in grad mode, and the backward pass that reaches it raises."""
+    layer, x, _ = layer_and_rows(8, 64, 24, 5, dev)
+    res = torch.randn((5, 24), generator=torch.Generator().manual_seed(1)).to(BF16).to(dev)
+    shift = torch.zeros(64, dtype=BF16, device=dev)
+    for call in (lambda t, **kw: layer(t, **kw), lambda t, **kw: layer.forward_modulated(t, shift, shift, **kw)):
+        with torch.no_grad():
+            want = call(x, residual=res)
+        leaf = x.clone().requires_grad_()
+        target = res.clone()
+        got = call(leaf * 1, residual=target, inplace=inplace)
+        assert torch.equal(got, want) and (got is target) == inplace
+        with pytest.raises(RuntimeError, match="Int8Linear has no gradient"):
+            got.sum().backward()
+        assert leaf.grad is None
