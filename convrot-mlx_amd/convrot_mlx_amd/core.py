@@ -1147,7 +1147,14 @@ class ConvRotLinear(nn.Module):
         broadcasts to the output ([B, 1, N] per image, [N], or full); `inplace` writes the
         result into `residual` and returns it, the same bits as out of place.  W4A4 sums are exact
         integers; W4A16 sums are float32 in an order that the kernel of the row count has, so
-        rows of one batch need not have the bits they have alone."""
+        rows of one batch need not have the bits they have alone.  There is no gradient (here and in the
+        other calls): a backward pass that reaches them raises an error."""
+        if nat.differentiated(x, residual, gate):
+            return nat.without_gradient(lambda: self._forward(x, residual, gate, inplace), "ConvRotLinear", x, residual, gate,
+                                        target=residual if inplace else None)
+        return self._forward(x, residual, gate, inplace)
+
+    def _forward(self, x, residual, gate, inplace: bool) -> torch.Tensor:
         if x.shape[-1] != self.in_features:
             raise ValueError(f"ConvRotLinear expected K={self.in_features}, got {x.shape[-1]}")
         x2d = x.reshape(-1, self.in_features)
@@ -1171,8 +1178,10 @@ class ConvRotLinear(nn.Module):
             raise ValueError(f"ConvRotLinear expected K={self.in_features}, got {x.shape[-1]}")
         check_vectors(x.shape, shift, scale)
         x2d = x.reshape(-1, self.in_features)
-        return self._project(lambda mode: _prepare_modulated(x2d, shift, scale, self.group_size, mode, eps),
-                             x.shape[:-1], x.dtype, residual, gate, inplace)
+        return nat.without_gradient(
+            lambda: self._project(lambda mode: _prepare_modulated(x2d, shift, scale, self.group_size, mode, eps),
+                                  x.shape[:-1], x.dtype, residual, gate, inplace),
+            "ConvRotLinear", x, shift, scale, residual, gate, target=residual if inplace else None)
 
     def forward_gelu(self, x: torch.Tensor, head: torch.Tensor | None = None, *,
                      residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
@@ -1187,8 +1196,10 @@ class ConvRotLinear(nn.Module):
             raise ValueError(f"GELU producer head {tuple(head.shape)} and x {tuple(x.shape)} differ in leading shape")
         x2d = x.reshape(-1, x.shape[-1])
         h2d = None if head is None else head.reshape(-1, head_features)
-        return self._project(lambda mode: _prepare_gelu(x2d, h2d, self.group_size, mode), x.shape[:-1], x.dtype,
-                             residual, gate, inplace)
+        return nat.without_gradient(
+            lambda: self._project(lambda mode: _prepare_gelu(x2d, h2d, self.group_size, mode), x.shape[:-1], x.dtype,
+                                  residual, gate, inplace),
+            "ConvRotLinear", x, head, residual, gate, target=residual if inplace else None)
 
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, group_size={self.group_size}, "

@@ -56,6 +56,8 @@ def _readable(t: torch.Tensor, zero_tail: bool) -> bool:
     """Whether the product can read an int8 matrix where it lies: adjacent features, 16-byte aligned rows
     that cover the features rounded up to 16 (past them zeros, with `zero_tail`)."""
     rows, k = t.shape
+    if k % 16 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return True
     stride = _row_stride(t)
     return (t.stride(1) == 1 and stride % 16 == 0 and _round16(k) <= stride <= MAX_ROW_STRIDE
             and t.data_ptr() % 16 == 0
@@ -244,40 +246,46 @@ class Int8Linear(nn.Module):
             self.bias = bias.to(weight.device, torch.float32)
         return self
 
-    def _check(self, x: torch.Tensor, residual: torch.Tensor | None, *others: torch.Tensor | None) -> None:
-        """Whether x, the residual and the layer's own tensors (which may have been assigned anew) fit
-        each other and lie on one device: the kernels read as far as these shapes say."""
+    def _checked(self, x: torch.Tensor, residual: torch.Tensor | None, *others: torch.Tensor | None) -> tuple:
+        """The layer's weight, scales and bias (which may have been assigned anew), after a look whether
+        they, x and the residual fit each other and lie on one device: the kernels read as far as these
+        shapes say."""
         if x.shape[-1] != self.in_features:
             raise ValueError(f"Int8Linear expected K={self.in_features}, got {x.shape[-1]}")
         if residual is not None and tuple(residual.shape) != (*x.shape[:-1], self.out_features):
             raise ValueError(f"residual {tuple(residual.shape)} must have the output shape "
                              f"{(*x.shape[:-1], self.out_features)}")
-        if _check_product(self.in_features, self.qweight, self.scales, self.bias) != self.out_features:
-            raise ValueError(f"W8A8 weight must have {self.out_features} rows, got {tuple(self.qweight.shape)}")
-        nat.on_device(x, self.qweight, self.scales, self.bias, residual, *others)
+        q, scales, bias = self.qweight, self.scales, self.bias
+        if _check_product(self.in_features, q, scales, bias) != self.out_features:
+            raise ValueError(f"W8A8 weight must have {self.out_features} rows, got {tuple(q.shape)}")
+        nat.on_device(x, q, scales, bias, residual, *others)
+        return q, scales, bias
 
     def _weight(self) -> torch.Tensor:
         """The weight as the kernels read it: itself, or where its rows do not lie as they need it
         (in_features no multiple of 16, a strided tensor) a copy with padded rows, kept until the
         tensor or its version is another one."""
         q = self.qweight
-        if _readable(q, True):
-            return q
+        return q if _readable(q, True) else self._copied(q)
+
+    def _copied(self, q: torch.Tensor) -> torch.Tensor:
         # Copies of their own: for a graph, which has to follow the weight from replay to replay and
         # would outlive a kept copy, and for inference tensors, which count no versions.
         if q.is_inference() or (q.is_cuda and torch.cuda.is_current_stream_capturing()):
             return _padded(q)
-        stream = torch.cuda.current_stream(q.device) if q.is_cuda else None
+        stream = nat.stream_handle(q.device) if q.is_cuda else None
         kept = self._kept_copy
         # the source is held beside its copy, so no other tensor can take its place unseen
         if kept is None or kept[0] is not q or kept[1] != q._version:
             copy = _padded(q)
-            self._kept_copy = (q, q._version, copy, stream, None if stream is None else stream.record_event())
+            ready = torch.cuda.current_stream(q.device).record_event() if q.is_cuda else None
+            self._kept_copy = (q, q._version, copy, stream, ready)
             return copy
         _, _, copy, made_on, ready = kept
         if stream != made_on:  # its writing comes first, and its memory is not given away under this call
-            stream.wait_event(ready)
-            copy.record_stream(stream)
+            here = torch.cuda.current_stream(q.device)
+            here.wait_event(ready)
+            copy.record_stream(here)
         return copy
 
     def __getstate__(self) -> dict:
@@ -286,21 +294,20 @@ class Int8Linear(nn.Module):
     def forward(self, x: torch.Tensor, *, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                 inplace: bool = False) -> torch.Tensor:
         """linear(x); with `residual`, residual + gate * linear(x), as ConvRotLinear.forward."""
-        self._check(x, residual, gate)
+        q, scales, bias = self._checked(x, residual, gate)
         return nat.without_gradient(
-            lambda: _linear(x, self._weight(), _scales(self.scales), _scales(self.bias), self.in_features, residual, gate,
-                            inplace),
-            "Int8Linear", x, self.scales, self.bias, residual, gate, target=residual if inplace else None)
+            lambda: _linear(x, q if _readable(q, True) else self._copied(q), _scales(scales), _scales(bias), q.shape[1],
+                            residual, gate, inplace),
+            "Int8Linear", x, scales, bias, residual, gate, target=residual if inplace else None)
 
     def forward_modulated(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, eps: float = 1e-6, *,
                           residual: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                           inplace: bool = False) -> torch.Tensor:
         """self((1 + scale) * layer_norm(x) + shift), the norm and the quantization in one kernel (the
         normalized row goes to codes unrounded); residual, gate and inplace as in forward."""
-        self._check(x, residual, gate, shift, scale)
+        _, scales, bias = self._checked(x, residual, gate, shift, scale)
         return nat.without_gradient(lambda: self._modulated(x, shift, scale, eps, residual, gate, inplace), "Int8Linear", x,
-                                    shift, scale, self.scales, self.bias, residual, gate,
-                                    target=residual if inplace else None)
+                                    shift, scale, scales, bias, residual, gate, target=residual if inplace else None)
 
     def _modulated(self, x, shift, scale, eps, residual, gate, inplace) -> torch.Tensor:
         k = self.in_features
@@ -311,9 +318,9 @@ class Int8Linear(nn.Module):
         codes = torch.empty((m, _round16(k)), dtype=torch.int8, device=x.device)
         scales = torch.empty((m,), dtype=torch.float32, device=x.device)
         nat.check(nat.load().convrot_layer_norm_int8(
-            nat.ptr(x2d), nat.dtype_code(x.dtype), m, k, x2d.stride(0), nat.ptr(gain), nat.ptr(sh),
-            nat.dtype_code(gain.dtype), 1, each, float(eps), nat.ptr(codes), codes.shape[1], nat.ptr(scales),
-            nat.stream_of(x.device)))
+            x2d.data_ptr(), nat.dtype_code(x.dtype), m, k, x2d.stride(0), gain.data_ptr(), sh.data_ptr(),
+            nat.dtype_code(gain.dtype), 1, each, float(eps), codes.data_ptr(), codes.shape[1], scales.data_ptr(),
+            nat.stream_handle(x.device)))
         out = _w8a8(codes, self._weight(), scales, _scales(self.scales), _scales(self.bias), k, x.dtype, gr)
         return residual if inplace else out.reshape(*x.shape[:-1], self.out_features)
 

@@ -103,3 +103,27 @@ def test_every_8_bit_call(monkeypatch, call, inplace):
     assert got.requires_grad and torch.equal(got, want)
     with pytest.raises(RuntimeError, match="has no gradient"):
         got.sum().backward()
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("call", ["forward", "forward_modulated", "forward_gelu"])
+def test_every_4_bit_layer_call(monkeypatch, call, inplace):
+    from convrot_mlx_amd import ConvRotLinear, core
+
+    def project(self, prep, lead, dtype, residual, gate, inplace):
+        out = torch.ones(*lead, self.out_features)
+        if inplace:
+            residual.data.copy_(out)
+        return residual if inplace else out
+
+    monkeypatch.setattr(ConvRotLinear, "_project", project)
+    monkeypatch.setattr(core, "_linear_rows_eligible", lambda *args: False)
+    layer, x = ConvRotLinear(64, 4, group_size=64), torch.randn(5, 64, requires_grad=True)
+    args = (x.detach()[0], x.detach()[1]) if call == "forward_modulated" else ()
+    kw = dict(residual=torch.zeros(5, 4), inplace=True) if inplace else {}
+    with torch.no_grad():
+        assert not getattr(layer, call)(x, *args, **kw).requires_grad
+    got = getattr(layer, call)(x, *args, **kw)
+    assert got.requires_grad and (got == 1).all()
+    with pytest.raises(RuntimeError, match="ConvRotLinear has no gradient"):
+        got.sum().backward()
