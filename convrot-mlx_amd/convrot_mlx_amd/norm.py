@@ -179,7 +179,8 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
                scale: torch.Tensor | None = None, shift: torch.Tensor | None = None,
                eps: float = 1e-6) -> torch.Tensor:
-    """hip_layer_norm, with gradients for x and for the parameters that need them."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, scale, shift)):
+    """hip_layer_norm, with gradients for x and for the parameters that need them (reverse mode; dual
+    tensors of forward mode are refused)."""
+    if nat.differentiated(x, weight, bias, scale, shift):
         return _LayerNorm.apply(x, weight, bias, scale, shift, eps)
     return hip_layer_norm(x, weight, bias, scale=scale, shift=shift, eps=eps)

@@ -195,7 +195,8 @@ class _QkRotary(torch.autograd.Function):
 
 def qk_rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, *, q_weight: torch.Tensor | None = None,
               k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = True):
-    """hip_qk_rotary, with gradients for q, k and the norm weights (none for the table)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    """hip_qk_rotary, with gradients for q, k and the norm weights (none for the table; reverse mode, dual
+    tensors of forward mode are refused)."""
+    if nat.differentiated(q, k, q_weight, k_weight):
         return _QkRotary.apply(q, k, table, q_weight, k_weight, eps, interleaved)
     return hip_qk_rotary(q, k, table, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved)
