@@ -270,7 +270,9 @@ class DoubleStreamBlock(nn.Module):
             attn = attention(torch.cat([tq, iq], 2), torch.cat([tk, ik], 2), torch.cat([tv, iv], 2), pe)
         else:
             b, h, lt, d = tq.shape
-            if torch.is_grad_enabled() and (iq.requires_grad or tq.requires_grad):
+            # with gradients as parts that are joined, without them straight into the joint sequence
+            leaves = (iq, ik, tq, tk, *self.txt_qknorm.parameters(), *self.img_qknorm.parameters())
+            if torch.is_grad_enabled() and any(t.requires_grad for t in leaves):
                 parts = self.txt_qknorm.rotated(tq, tk, pe[:, :lt]), self.img_qknorm.rotated(iq, ik, pe[:, lt:])
                 q, k = torch.cat([parts[0][0], parts[1][0]], 2), torch.cat([parts[0][1], parts[1][1]], 2)
             else:
