@@ -97,3 +97,24 @@ def test_float32_shift_beyond_the_range_of_float16(dev):
         _, dgain, dshift = hip_layer_norm_backward(dy, x, mean, rstd, shift_dtype=F32, **kw)
         assert dgain.dtype == F16 and torch.equal(dshift, bias.grad)
         assert hip_layer_norm_backward(dy, x, mean, rstd, **kw)[2].isinf().all()  # without it, x's type
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,k", [(1, 64), (70, 8), (33, 320), (40, 1024), (20, 1500), (12, 2690), (10, 3072), (6, 5120),
+                                    (4, 6458), (3, 8200), (2, 12289), (2, 20000)])
+def test_gradient_with_a_vector_a_row(dev, rows, k, dtype):
+    """Modulation a token: every row's parameter gradients are that row's alone."""
+    from convrot_mlx_amd import hip_layer_norm, hip_layer_norm_backward
+
+    x, scale, shift, dy = inputs(rows + k, rows, k, dtype, dev, rows)
+    y, mean, rstd = hip_layer_norm(x, scale=scale, shift=shift, eps=EPS, return_stats=True)
+    g64 = 1 + scale.double().cpu()
+    want, _, _, _, _, off = norm(x.double().cpu(), g64, shift.double().cpu(), EPS)
+    assert_within(y, want, off, "y")
+    dx, ds, dh = hip_layer_norm_backward(dy, x, mean, rstd, scale=scale)
+    wdx, odx, wds, ods, wdh, odh = norm_grads(x.double().cpu(), g64, dy.double().cpu(), EPS, rows)
+    assert_within(dx, wdx, odx, "dx")
+    assert_within(ds, wds, ods, "dscale")
+    assert torch.equal(dh, dy)
+    only, none, _ = hip_layer_norm_backward(dy, x, mean, rstd, scale=scale, param_grads=False)
+    assert none is None and torch.equal(only, dx)
