@@ -266,8 +266,10 @@ __global__ __launch_bounds__(T* TEAMS) void norm_backward_kernel(
   };
 
   // The mean, but zero past the row: of a constant row of large values (0 - mean) rstd is infinite,
-  // and zero (d there) times it no number.
-  auto centre = [&](float mu, int c, int j) { return feature_of<T, C, VEC>(t, c, VEC ? 0 : j) < K ? mu : 0.0f; };
+  // and zero (d there) times it no number.  (float16 has no such values: 65504 / sqrt(eps) is finite.)
+  auto centre = [&](float mu, int c, int j) {
+    return DT == kF16 || feature_of<T, C, VEC>(t, c, VEC ? 0 : j) < K ? mu : 0.0f;
+  };
 
   struct Rows {
     RawChunk<DT, T, C, VEC> x[R][C], d[R][C];
