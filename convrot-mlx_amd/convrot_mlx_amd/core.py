@@ -151,8 +151,8 @@ def check_vectors(shape: tuple, *vectors: torch.Tensor | None) -> None:
                 lead = lead[:-1]
             good = len(lead) <= 1 or lead == rows[: len(lead)]
         if not good:
-            raise ValueError(f"modulation vectors {tuple(t.shape)} beside x {tuple(shape)} are no even groups of rows in "
-                             f"order; pass [V, {shape[-1]}], or x's leading axes followed by ones")
+            raise ValueError(f"modulation vectors {tuple(t.shape)} beside x {tuple(shape)} are no even groups of rows "
+                             f"in order; pass [V, {shape[-1]}], or x's leading axes followed by ones")
 
 
 def _modulation_rows(rows: int, features: int, shift: torch.Tensor, scale: torch.Tensor):
@@ -1150,8 +1150,8 @@ class ConvRotLinear(nn.Module):
         rows of one batch need not have the bits they have alone.  There is no gradient (here and in the
         other calls): a backward pass that reaches them raises an error."""
         if nat.differentiated(x, residual, gate):
-            return nat.without_gradient(lambda: self._forward(x, residual, gate, inplace), "ConvRotLinear", x, residual, gate,
-                                        target=residual if inplace else None)
+            return nat.without_gradient(lambda: self._forward(x, residual, gate, inplace), "ConvRotLinear", x,
+                                        residual, gate, target=residual if inplace else None)
         return self._forward(x, residual, gate, inplace)
 
     def _forward(self, x, residual, gate, inplace: bool) -> torch.Tensor:

@@ -18,7 +18,6 @@ from . import _native as nat
 from .core import GatedResidual, _f32, _gated_residual, _workspace
 from .norm import flat_rows, norm_operands, rows_of
 
-INT8_MAX = 127
 MAX_FEATURES = 65536
 MAX_ROW_STRIDE = 1 << 22
 

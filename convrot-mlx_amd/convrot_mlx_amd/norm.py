@@ -74,7 +74,8 @@ def hip_layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: to
 
     weight, bias: [K].  Or scale, shift: [V, K] or [V, 1, K], the rows split evenly over the V
     vectors in order, as x [B, L, K] beside scale [B, 1, K] does: (1 + scale) * u + shift (shapes that
-    broadcast to other rows, [1, L, K], are refused).  Either of a pair may be None.  With return_stats also the rows' float32 mean and 1 / sqrt(var + eps)."""
+    broadcast to other rows, [1, L, K], are refused).  Either of a pair may be None.  With
+    return_stats also the rows' float32 mean and 1 / sqrt(var + eps)."""
     device = nat.on_device(x, weight, bias, scale, shift)
     x2d = flat_rows(x)
     rows, k = x2d.shape

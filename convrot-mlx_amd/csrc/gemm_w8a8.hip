@@ -26,9 +26,11 @@ namespace {
 // weights at 4.6 TB/s; 8 rows 8192 -> 8192 14.3 us, 4.7 TB/s.  Against the 64 x 64
 // tile: 12.3 and 13.4 us, 7.5 and 8.8 (16 rows, 4096 -> 4096).
 constexpr int kRowsMax = 16, kRowsN = 64;
-// Rows of a fused call, which lie in LDS beside their codes.  One launch and two, in a graph:
-// 1 row 3072 -> 18432 12.9 and 15.0 us, 2 rows of 4096 -> 4096 9.0 and 9.2, 8 rows of 1024 -> 4096 6.5
-// and 6.4; an eager call saves 4 us of host time besides.
+// Rows of a fused call, which lie in LDS beside their codes.  One launch and two, in a graph, weights
+// cold: 1 row 3072 -> 18432 15.4 and 18.0 us, 2 rows of 4096 -> 4096 9.5 and 10.6, at the limit 1 row
+// 8192 -> 2048 9.7 and 11.9, 8192 -> 8192 19.0 and 20.9, 8 rows of 1024 -> 4096 6.06 and 6.15, 16 rows of
+// 512 -> 4096 5.7 and 5.8; an eager call saves 4 us of host time besides.  Rows past the limit (one of
+// 12288 in 16 bits) take two launches; one has not been tried there.
 constexpr int kFusedBytes = 16384;
 constexpr size_t kTwoPerCu = 79 * 1024;  // dynamic LDS of two workgroups a CU
 
@@ -185,9 +187,12 @@ __global__ __launch_bounds__(256) void w8a8_rows_kernel(W8a8Operands p, const vo
 
 // Time of a tile's k-block (alone on its CU, and with every CU busy, where the
 // clock drops) and what its prologue, epilogue and stores add, in microseconds,
-// fitted to 13 shapes x 16 tiles.  The tile the model picks is within 7 % of the
-// fastest measured on all of them (4608 x 3072 -> 12288: 256 x 224 165 us, the
-// others 165 to 286; 1536 x 15360 -> 3072: 160 x 128 71 us, 256 x 256 153).
+// fitted to measurements of 16-bit outputs without a residual, and used for all.  Of 15
+// shapes x 16 tiles (16-bit) the tile that the model picks is within 4 % of the fastest on 12
+// (4608 x 3072 -> 12288: 256 x 224 160 us, the others 159 to 287; 1536 x 15360 -> 3072:
+// 160 x 128 72 us, 256 x 256 153); it loses 8 % at 77 x 3072 -> 9216 (12.1 us, 128 x 64
+// 11.2), 11 % at 512 x 3072 -> 12288 (31.1, 256 x 128 28.1) and 18 % at 512 x 3072 -> 3072
+// (13.6, 128 x 64 11.5).
 struct Cost {
   int bm, bn, per_cu;
   float lone, full, fixed;
@@ -208,8 +213,11 @@ int most_splits(int64_t tiles, int kblocks, int64_t tile_bytes, const Workspace&
 }
 
 // Splits of K of the few-row kernel: while the chip is not full and a part keeps 8
-// blocks.  The exchange of partial sums costs 2 to 4 us: 16 rows 12288 -> 3072 (48
-// tiles) 21.0 us with one, 14.4 with two, 12.5 with four, 14.3 with six.
+// blocks.  The exchange of partial sums costs 2 to 4 us: 4 rows 12288 -> 3072 (48
+// tiles) 20.5 us with one, 14.1 with two, 12.4 with three, 11.9 with four (the rule's),
+// 14.5 with six; 8 rows 8192 -> 4096 (64 tiles) 14.8 with one, 10.7 with three (the
+// rule's), 12.9 with eight.  Few tiles of long rows: 4 rows 16384 -> 1024 (16 tiles) 21.6
+// with one, 9.5 with six or eight, 10.9 with the rule's twelve.
 int rows_splits(int64_t tiles, int kblocks, const Workspace& work) {
   const int forced = tuning(kTuneW8a8Split);
   const int64_t s = forced > 0 ? forced : std::min<int64_t>(192 / tiles, kblocks / 8);

@@ -5,8 +5,9 @@
 //
 // The integer sum is exact (K <= 65536: |sum| <= 2^14 K = 2^30), so the order in
 // which K is walked or split cannot change a bit.  An optional gated residual
-// follows with the rounding of each of its operations, as for the 4-bit linears
-// (convrot_device.h).
+// follows in float32 and is rounded once, dt(res[m][n] + gate[n] * that): the
+// 4-bit linears round each of its operations, to give the bits of the array
+// operations that they stand for.
 //
 // Operands: activations [M, K] and weights [N, K] as they are, row-major with
 // row strides of a multiple of 16 bytes, so 8-bit checkpoints need no layout of
