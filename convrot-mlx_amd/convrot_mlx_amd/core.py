@@ -1079,16 +1079,17 @@ class ConvRotLinear(nn.Module):
         if self.weight_layout == WEIGHT_LAYOUT_CDNA4 and q.ndim != 2:
             _check_cdna4(q, self.out_features, self.in_features)
             return q
-        key = (q.data_ptr(), q._version, tuple(q.shape), q.device)
-        if self._cdna4_cache is None or self._cdna4_cache[0] != key:
+        kept = self._cdna4_cache
+        # the source is held beside what is made of it, so no other tensor can take its place unseen
+        if kept is None or kept[2] is not q or kept[0] != q._version:
             _validate_mpp_weight_layout(q, self.in_features)
             if q.shape[1] * 2 != self.out_features:
                 raise ValueError(
                     f"MPP W4 weight must use K x packed-N layout; activation K={self.in_features}, "
                     f"weight={tuple(q.shape)}"
                 )
-            self._cdna4_cache = (key, repack_mpp_weight_for_cdna4(q))
-        return self._cdna4_cache[1]
+            self._cdna4_cache = kept = (q._version, repack_mpp_weight_for_cdna4(q), q)
+        return kept[1]
 
     def _fp6_weight(self, w: torch.Tensor, rows: int) -> torch.Tensor | None:
         """The FP6 form of the CDNA4 weight `w`, converted once and cached per tensor version
@@ -1097,16 +1098,16 @@ class ConvRotLinear(nn.Module):
         (no compact field).  The compact conversion reads a flag back from the device; under
         graph capture, where it cannot, a layer without a cached form returns None and the
         product runs on INT8 operands (the same bits)."""
-        key = (w.data_ptr(), w._version, tuple(w.shape), w.device, _fp6_weight_form)
-        if self._fp6_cache is None or self._fp6_cache[0] != key:
+        key, kept = (w._version, _fp6_weight_form), self._fp6_cache
+        if kept is None or kept[2] is not w or kept[0] != key:
             form = fp6_weight_form(rows, self.out_features)
             if form == "compact" and torch.cuda.is_current_stream_capturing():
                 return None
             w6 = fp6_weight_compact(w, self.out_features, self.in_features) if form == "compact" else None
             if w6 is None:
                 w6 = fp6_weight(w, self.out_features, self.in_features)
-            self._fp6_cache = (key, w6)
-        return self._fp6_cache[1]
+            self._fp6_cache = kept = (key, w6, w)
+        return kept[1]
 
     def _project(self, prep, lead: tuple, dtype: torch.dtype, residual, gate, inplace: bool) -> torch.Tensor:
         """Run the prepared activation `prep(mode)` through this layer's GEMM, then the
