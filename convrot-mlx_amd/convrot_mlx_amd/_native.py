@@ -206,6 +206,21 @@ def stream_handle(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
+def made_here(device: torch.device) -> tuple:
+    """Where a tensor that is kept between calls was just written: the current stream, and an event behind it."""
+    return stream_handle(device), torch.cuda.current_stream(device).record_event()
+
+
+def use_here(t: torch.Tensor, made: tuple) -> torch.Tensor:
+    """A kept tensor for a call on the current stream: behind its writing, and its memory not given away under
+    the call.  (A capture begins behind a synchronization, and cannot wait for what lies before it.)"""
+    if stream_handle(t.device) != made[0] and not torch.cuda.is_current_stream_capturing():
+        here = torch.cuda.current_stream(t.device)
+        here.wait_event(made[1])
+        t.record_stream(here)
+    return t
+
+
 def stream_of(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 

@@ -1088,8 +1088,11 @@ class ConvRotLinear(nn.Module):
                     f"MPP W4 weight must use K x packed-N layout; activation K={self.in_features}, "
                     f"weight={tuple(q.shape)}"
                 )
-            self._cdna4_cache = kept = (q._version, repack_mpp_weight_for_cdna4(q), q)
-        return kept[1]
+            packed = repack_mpp_weight_for_cdna4(q)
+            if not torch.cuda.is_current_stream_capturing():  # else it is there when the graph has run
+                self._cdna4_cache = (q._version, packed, q, nat.made_here(q.device))
+            return packed
+        return nat.use_here(kept[1], kept[3])
 
     def _fp6_weight(self, w: torch.Tensor, rows: int) -> torch.Tensor | None:
         """The FP6 form of the CDNA4 weight `w`, converted once and cached per tensor version
@@ -1106,8 +1109,13 @@ class ConvRotLinear(nn.Module):
             w6 = fp6_weight_compact(w, self.out_features, self.in_features) if form == "compact" else None
             if w6 is None:
                 w6 = fp6_weight(w, self.out_features, self.in_features)
-            self._fp6_cache = kept = (key, w6, w)
-        return kept[1]
+            if not torch.cuda.is_current_stream_capturing():
+                self._fp6_cache = (key, w6, w, nat.made_here(w.device))
+            return w6
+        return nat.use_here(kept[1], kept[3])
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "_cdna4_cache": None, "_fp6_cache": None}
 
     def _project(self, prep, lead: tuple, dtype: torch.dtype, residual, gate, inplace: bool) -> torch.Tensor:
         """Run the prepared activation `prep(mode)` through this layer's GEMM, then the

@@ -272,20 +272,13 @@ class Int8Linear(nn.Module):
         # would outlive a kept copy, and for inference tensors, which count no versions.
         if q.is_inference() or (q.is_cuda and torch.cuda.is_current_stream_capturing()):
             return _padded(q)
-        stream = nat.stream_handle(q.device) if q.is_cuda else None
         kept = self._kept_copy
         # the source is held beside its copy, so no other tensor can take its place unseen
         if kept is None or kept[0] is not q or kept[1] != q._version:
             copy = _padded(q)
-            ready = torch.cuda.current_stream(q.device).record_event() if q.is_cuda else None
-            self._kept_copy = (q, q._version, copy, stream, ready)
+            self._kept_copy = (q, q._version, copy, nat.made_here(q.device) if q.is_cuda else None)
             return copy
-        _, _, copy, made_on, ready = kept
-        if stream != made_on:  # its writing comes first, and its memory is not given away under this call
-            here = torch.cuda.current_stream(q.device)
-            here.wait_event(ready)
-            copy.record_stream(here)
-        return copy
+        return nat.use_here(kept[2], kept[3]) if q.is_cuda else kept[2]
 
     def __getstate__(self) -> dict:
         return {**self.__dict__, "_kept_copy": None}

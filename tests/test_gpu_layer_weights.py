@@ -37,3 +37,69 @@ def test_weights_assigned_one_after_the_other(dev, backend):
         layer.load_nk_weight(qw, ws)
         places.add(layer.qweight.data_ptr())
         assert torch.equal(layer(x), w)
+
+
+CYCLES = 100_000_000  # of a spinning kernel: some tens of milliseconds
+
+
+@pytest.mark.parametrize("backend", ["hip-w4a4", "mpp-w4a4", "mpp-w4a16"])
+def test_forms_made_on_another_stream(dev, backend, fp6_form):
+    """A form made by a call on one stream is read by a call on another only once it is written."""
+    fp6_form("full")
+    x = torch.randn((M, K), generator=torch.Generator(dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for seed in range(3):
+        state = packed(seed, dev)
+        want = layer_of(backend, *state, dev)(x)
+        layer = layer_of(backend, *state, dev)
+        for s in (a, b):  # each stream's workspace
+            with torch.cuda.stream(s):
+                layer_of(backend, *state, dev)(x)
+        with torch.cuda.stream(a):
+            for size in (K * N // 2, K * N * 3 // 4):  # what the forms' memory may hold before
+                torch.full((size,), 77, dtype=torch.uint8, device=dev)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(CYCLES)
+            first = layer(x)
+        with torch.cuda.stream(b):
+            second = layer(x)
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want)
+
+
+@pytest.mark.parametrize("backend", ["hip-w4a4", "mpp-w4a4", "mpp-w4a16"])
+def test_forms_made_under_capture_are_the_graphs(dev, backend, fp6_form):
+    """A layer first called under capture: its forms are written when the graph runs, so an eager call before
+    that makes its own."""
+    fp6_form("full")
+    x = torch.randn((M, K), generator=torch.Generator(dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    state = packed(5, dev)
+    want = layer_of(backend, *state, dev)(x)
+    layer = layer_of(backend, *state, dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer_of(backend, *state, dev)(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            static = layer(x)
+        eager = layer(x)
+        side.synchronize()
+        assert torch.equal(eager, want)
+        for _ in range(3):
+            static.zero_()
+            graph.replay()
+            side.synchronize()
+            assert torch.equal(static, want) and torch.equal(layer(x), want)
+
+
+def test_copies_of_a_layer(dev):
+    import copy
+    import pickle
+
+    x = torch.randn((M, K), generator=torch.Generator(dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    layer = layer_of("mpp-w4a4", *packed(6, dev), dev)
+    want = layer(x)
+    for other in (copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))):
+        assert torch.equal(other(x), want)
