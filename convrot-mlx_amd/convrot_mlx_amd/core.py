@@ -1079,9 +1079,10 @@ class ConvRotLinear(nn.Module):
         if self.weight_layout == WEIGHT_LAYOUT_CDNA4 and q.ndim != 2:
             _check_cdna4(q, self.out_features, self.in_features)
             return q
-        kept = self._cdna4_cache
-        # the source is held beside what is made of it, so no other tensor can take its place unseen
-        if kept is None or kept[2] is not q or kept[0] != q._version:
+        kept, version = self._cdna4_cache, None if q.is_inference() else q._version
+        # the source is held beside what is made of it, so no other tensor can take its place unseen;
+        # tensors of inference mode count no versions: theirs is made at each call
+        if kept is None or kept[2] is not q or version is None or kept[0] != version:
             _validate_mpp_weight_layout(q, self.in_features)
             if q.shape[1] * 2 != self.out_features:
                 raise ValueError(
@@ -1089,8 +1090,9 @@ class ConvRotLinear(nn.Module):
                     f"weight={tuple(q.shape)}"
                 )
             packed = repack_mpp_weight_for_cdna4(q)
-            if not torch.cuda.is_current_stream_capturing():  # else it is there when the graph has run
-                self._cdna4_cache = (q._version, packed, q, nat.made_here(q.device))
+            # under capture it is there only when the graph has run
+            if version is not None and not torch.cuda.is_current_stream_capturing():
+                self._cdna4_cache = (version, packed, q, nat.made_here(q.device))
             return packed
         return nat.use_here(kept[1], kept[3])
 
@@ -1100,7 +1102,10 @@ class ConvRotLinear(nn.Module):
         weight) or the FP6 operand blocks (0.75 byte), which also hold a weight with a -8 code
         (no compact field).  The compact conversion reads a flag back from the device; under
         graph capture, where it cannot, a layer without a cached form returns None and the
-        product runs on INT8 operands (the same bits)."""
+        product runs on INT8 operands (the same bits); so does a weight made in inference mode,
+        whose changes no version tells."""
+        if w.is_inference():
+            return None
         key, kept = (w._version, _fp6_weight_form), self._fp6_cache
         if kept is None or kept[2] is not w or kept[0] != key:
             form = fp6_weight_form(rows, self.out_features)

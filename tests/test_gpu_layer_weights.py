@@ -103,3 +103,18 @@ def test_copies_of_a_layer(dev):
     want = layer(x)
     for other in (copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))):
         assert torch.equal(other(x), want)
+
+
+@pytest.mark.parametrize("backend", ["hip-w4a4", "mpp-w4a4", "hip-w4a16", "mpp-w4a16"])
+def test_weights_of_inference_mode(dev, backend):
+    x = torch.randn((M, K), generator=torch.Generator(dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    states = [packed(seed, dev) for seed in (7, 8)]
+    want = [layer_of(backend, *s, dev)(x) for s in states]
+    with torch.inference_mode():
+        layer, other = (layer_of(backend, *s, dev) for s in states)
+        assert layer.qweight.is_inference()
+        for _ in range(2):
+            assert torch.equal(layer(x), want[0])
+        layer.qweight.copy_(other.qweight), layer.scales.copy_(other.scales)
+        assert torch.equal(layer(x), want[1])
+    assert torch.equal(layer(x), want[1])
