@@ -349,6 +349,7 @@ int64_t w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     splits = rows_splits(tiles, kblocks, all);
   } else {
     const Choice c = choose(M, N, K, all);
+    if (c.tile == 0) return 0;  // more tiles than a launch takes, whichever it is
     const int64_t bm = c.tile & 1023, bn = c.tile >> 10;
     tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn), bytes = bm * bn * 4;
     splits = c.splits;

@@ -34,3 +34,12 @@ def test_workspace_bytes_of_a_product(lib):
     for m, n, k in ((1, 18432, 3072), (77, 9216, 3072), (4608, 12288, 3072), (3, 64, 128), (0, 64, 128), (4, 64, 0),
                     (4, 64, 65552)):
         assert lib.convrot_w8a8_workspace_bytes(m, n, k) == 0
+
+
+def test_workspace_bytes_of_what_no_launch_takes(lib):
+    assert lib.convrot_w8a8_workspace_bytes(0x7ffffe00, 0x7ffffe00, 64) == 0
+    try:
+        assert lib.convrot_set_tuning(b"w8a8_tile", b"64x64") == 0
+        assert lib.convrot_w8a8_workspace_bytes(1 << 30, 1 << 20, 64) == 0
+    finally:
+        lib.convrot_set_tuning(b"w8a8_tile", None)
