@@ -84,6 +84,16 @@ SIGNATURES = {
     "convrot_qk_rotary_workspace_bytes": (_i64, [_i32]),
     "convrot_qk_rotary_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64,
                                           _i32, _vp, _i32, _i64, _vp, _vp, _i32, _f32, _i32, _vp, _i64, _vp]),
+    "convrot_quantize_fp8": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "convrot_quantize_fp8_weight": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "convrot_fp8_gemm": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64,
+                                _i64, _vp, _i64, _vp, _i32, _vp]),
+    "convrot_fp8_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "convrot_fp8_scratch_bytes": (_i64, [_i64, _i64]),
+    "convrot_fp8_linear": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64,
+                                  _vp, _i64, _vp, _i64, _vp, _vp]),
+    "convrot_fp8_grouped_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+                                          _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "convrot_last_error": (ctypes.c_char_p, []),
     "convrot_set_tuning": (_i32, [ctypes.c_char_p, ctypes.c_char_p]),
     "convrot_version": (ctypes.c_char_p, []),
@@ -206,6 +216,25 @@ def stream_handle(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on(device: torch.device):
+    """`device` as the current one for the length of a call (a launch goes to the current device, whatever
+    device its stream belongs to); nothing where it is that already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
 def made_here(device: torch.device) -> tuple:
     """Where a tensor that is kept between calls was just written: the current stream, and an event behind it."""
     return stream_handle(device), torch.cuda.current_stream(device).record_event()
@@ -252,7 +281,8 @@ def set_tuning(name: str, value: str | None) -> None:
     linear_rows_cfg (1/2/3/5/16), w4a4_midm_cfg (10 * row tiles + weight tiles),
     fp6_split (1/2/4: parts of each 256x256 FP6 tile past the whole rounds),
     w8a8_tile ("BMxBN", 256x256 to 64x64),
-    w8a8_split (workgroups that share a W8A8 tile's K)."""
+    w8a8_split (workgroups that share a W8A8 tile's K), fp8_tile ("BMxBN", 256x256 to 32x64),
+    fp8_split (workgroups that share an FP8 tile's K)."""
     check(load().convrot_set_tuning(name.encode(), None if value is None else str(value).encode()))
 
 

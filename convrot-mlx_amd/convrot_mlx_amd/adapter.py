@@ -18,6 +18,7 @@ import torch
 from torch import nn
 
 from .core import CONVROT_GROUP_SIZE, ConvRotLinear, eligible_linear, quantize_convrot_weight
+from .fp8 import Fp8Linear
 from .int8 import Int8Linear
 
 
@@ -60,18 +61,27 @@ def replace_convrot_linears(
     return names
 
 
-def replace_int8_linears(model: nn.Module, *, select=None, convert: bool = True) -> list[str]:
-    """Replace Linears of `model` with Int8Linear layers in place; return the replaced names in
-    `named_modules` order.  `select(name, linear)` says which (all by default): used before
-    replace_convrot_linears it keeps the layers that 4 bits hurt at 8, the rest follow at 4.
-    convert=False installs zero weights and unit scales, ready for load_state_dict."""
+def _replace_linears(model: nn.Module, kind, select, convert: bool) -> list[str]:
     selected = [(name, module) for name, module in model.named_modules()
                 if name and isinstance(module, nn.Linear) and (select is None or select(name, module))]
     for name, dense in selected:
         out_features, in_features = dense.weight.shape
-        layer = Int8Linear(in_features, out_features, bias=dense.bias is not None, device=dense.weight.device)
+        layer = kind(in_features, out_features, bias=dense.bias is not None, device=dense.weight.device)
         if convert:
             with torch.no_grad():
                 layer.load_weight(dense.weight.detach(), None if dense.bias is None else dense.bias.detach())
         _set_submodule(model, name, layer)
     return [name for name, _ in selected]
+
+
+def replace_fp8_linears(model: nn.Module, *, select=None, convert: bool = True) -> list[str]:
+    """Replace Linears of `model` with Fp8Linear layers in place, as replace_int8_linears does."""
+    return _replace_linears(model, Fp8Linear, select, convert)
+
+
+def replace_int8_linears(model: nn.Module, *, select=None, convert: bool = True) -> list[str]:
+    """Replace Linears of `model` with Int8Linear layers in place; return the replaced names in
+    `named_modules` order.  `select(name, linear)` says which (all by default): used before
+    replace_convrot_linears it keeps the layers that 4 bits hurt at 8, the rest follow at 4.
+    convert=False installs zero weights and unit scales, ready for load_state_dict."""
+    return _replace_linears(model, Int8Linear, select, convert)

@@ -12,6 +12,7 @@
 #include <atomic>
 
 #include "convrot_launch.h"
+#include "fp8_device.h"
 
 namespace convrot {
 namespace {
@@ -99,7 +100,8 @@ int convrot_set_tuning(const char* name, const char* value) {
                 {"gemm_persist", kTuneGemmPersist},   {"gemm_mfma32", kTuneGemmMfma32},
                 {"fp6_tile", kTuneFp6Tile},           {"linear_rows_cfg", kTuneRowsCfg},
                 {"w4a4_midm_cfg", kTuneMidmCfg},      {"fp6_split", kTuneFp6Split},
-                {"w8a8_tile", kTuneW8a8Tile},         {"w8a8_split", kTuneW8a8Split}};
+                {"w8a8_tile", kTuneW8a8Tile},         {"w8a8_split", kTuneW8a8Split},
+                {"fp8_tile", kTuneFp8Tile},           {"fp8_split", kTuneFp8Split}};
   int key = -1;
   for (const auto& n : kNames)
     if (strcmp(n.name, name) == 0) key = n.key;
@@ -118,12 +120,14 @@ int convrot_set_tuning(const char* name, const char* value) {
       }
       case kTuneFp6Tile:
       case kTuneW8a8Tile:
+      case kTuneFp8Tile:
       case kTuneW4a16Tile: {
         int bm = 0, bn = 0;
         char tail = 0;
         good = sscanf(value, "%dx%d%c", &bm, &bn, &tail) == 2 &&
                (key == kTuneFp6Tile    ? fp6_tile_known(bm, bn)
                 : key == kTuneW8a8Tile ? w8a8_tile_known(bm, bn)
+                : key == kTuneFp8Tile  ? fp8_tile_known(bm, bn)
                                        : w4a16_tile_known(bm, bn));
         v = bm | bn << 10;
         break;
@@ -145,6 +149,7 @@ int convrot_set_tuning(const char* name, const char* value) {
         good = v == 1 || v == 2 || v == 4;
         break;
       case kTuneW8a8Split:
+      case kTuneFp8Split:
         v = atoi(value);
         good = v >= 1 && v <= 64;
         break;
@@ -1032,6 +1037,209 @@ int convrot_qk_rotary_backward(const void* dq, const void* dk, const void* q, co
                                                           k_weight_grad, strides, (float*)workspace,
                                                           (hipStream_t)stream),
                        "convrot_qk_rotary_backward");
+}
+
+// ---- linears in 8-bit floating point
+
+namespace {
+
+constexpr int64_t kMaxXsRow = int64_t(1) << 21;  // floats between rows' scales: a tile's offsets stay below 2^32
+
+int64_t blocks_of(int64_t K) { return (K + convrot::kBlock - 1) / convrot::kBlock; }
+
+int check_fp8_codes(const uint8_t* codes, int64_t stride, int64_t features, const float* scales) {
+  if (!codes || !scales) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (stride < features || stride % 16 || !aligned(codes, 16) || !aligned(scales, 4))
+    return fail(CONVROT_ERR_INVALID, "codes need 16-byte aligned rows of at least %lld bytes, got a stride of %lld",
+                (long long)features, (long long)stride);
+  if (stride > kMaxInt8Stride)
+    return fail(CONVROT_ERR_UNSUPPORTED, "row strides of codes are limited to %lld bytes", (long long)kMaxInt8Stride);
+  return ok();
+}
+
+// Checks of an FP8 product but for its activations; CONVROT_OK when the launch may proceed (M == 0 or
+// N == 0 included).
+int check_fp8(int64_t M, int64_t N, int64_t K, const uint8_t* weight, int64_t weight_stride, const float* wscales,
+              int64_t wscales_stride, const void* out, int out_dtype) {
+  if (!valid_dtype(out_dtype)) return fail(CONVROT_ERR_INVALID, "unsupported output dtype code %d", out_dtype);
+  if (M < 0 || N < 0 || K <= 0)
+    return fail(CONVROT_ERR_INVALID, "invalid GEMM shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+  if (K > kMaxFeatures)
+    return fail(CONVROT_ERR_UNSUPPORTED, "FP8 GEMM supports K up to %lld, got %lld", (long long)kMaxFeatures, (long long)K);
+  // 2^31 - 1 less what rounding a dimension up to whole tiles adds
+  if (M > 0x7ffffe00 || N > 0x7ffffe00) return fail(CONVROT_ERR_UNSUPPORTED, "GEMM dimension too large");
+  if (M == 0 || N == 0) return ok();
+  if (!weight || !wscales || !out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (weight_stride < (K + 15) / 16 * 16 || weight_stride % 16 || !aligned(weight, 16) || !aligned(out, 16))
+    return fail(CONVROT_ERR_INVALID,
+                "FP8 operands need 16-byte aligned rows that cover K rounded up to 16 (K=%lld, weight stride %lld)",
+                (long long)K, (long long)weight_stride);
+  if (weight_stride > kMaxInt8Stride)
+    return fail(CONVROT_ERR_UNSUPPORTED, "FP8 row strides are limited to %lld bytes", (long long)kMaxInt8Stride);
+  if (wscales_stride < blocks_of(K) || !aligned(wscales, 4))
+    return fail(CONVROT_ERR_INVALID, "weight scales need rows of %lld floats, got a stride of %lld",
+                (long long)blocks_of(K), (long long)wscales_stride);
+  return ok();
+}
+
+int check_fp8_work(const void* residual, const void* gate, int64_t rows_per_gate, const void* workspace,
+                   int64_t workspace_bytes) {
+  if (gate && !residual) return fail(CONVROT_ERR_INVALID, "a gate needs a residual");
+  if (gate && rows_per_gate <= 0)
+    return fail(CONVROT_ERR_INVALID, "rows_per_gate must be positive, got %lld", (long long)rows_per_gate);
+  if (workspace_bytes < 0 || (workspace_bytes > 0 && !workspace))
+    return fail(CONVROT_ERR_INVALID, "invalid workspace (%lld bytes)", (long long)workspace_bytes);
+  if (workspace && !aligned(workspace, 256)) return fail(CONVROT_ERR_INVALID, "workspace must be 256-byte aligned");
+  return ok();
+}
+
+// Codes and scales of rows in a scratch buffer: [rows][K rounded up to 128], then [blocks][rows rounded up to 4].
+struct Fp8Scratch {
+  uint8_t* codes;
+  float* scales;
+  int64_t stride, xs_block;
+};
+int64_t fp8_scratch_bytes(int64_t rows, int64_t K) {
+  return rows <= 0 || K <= 0 ? 0 : rows * blocks_of(K) * convrot::kBlock + blocks_of(K) * ((rows + 3) / 4 * 4) * 4;
+}
+Fp8Scratch fp8_scratch(void* scratch, int64_t rows, int64_t K) {
+  const int64_t stride = blocks_of(K) * convrot::kBlock;
+  return {(uint8_t*)scratch, (float*)((uint8_t*)scratch + rows * stride), stride, (rows + 3) / 4 * 4};
+}
+int check_fp8_scratch(const void* scratch, int64_t bytes, int64_t rows, int64_t K) {
+  if (!scratch || !aligned(scratch, 16) || bytes < fp8_scratch_bytes(rows, K))
+    return fail(CONVROT_ERR_INVALID, "the FP8 linear needs a 16-byte aligned scratch buffer of %lld bytes, got %lld",
+                (long long)fp8_scratch_bytes(rows, K), (long long)bytes);
+  return ok();
+}
+
+}  // namespace
+
+int convrot_quantize_fp8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride, uint8_t* codes,
+                         int64_t codes_stride, float* scales, int64_t scales_row, int64_t scales_block, void* stream) {
+  if (int rc = check_rows("8-bit quantization", x, dtype, rows, features, x_stride, kMaxFeatures)) return rc;
+  if (rows == 0 || features == 0) return ok();
+  if (int rc = check_fp8_codes(codes, codes_stride, features, scales)) return rc;
+  if (scales_row < 1 || scales_block < 1)
+    return fail(CONVROT_ERR_INVALID, "invalid strides of scales (%lld, %lld)", (long long)scales_row, (long long)scales_block);
+  return launch_status(convrot::launch_quantize_fp8(x, dtype, rows, features, x_stride, codes, codes_stride, scales,
+                                                    scales_row, scales_block, (hipStream_t)stream),
+                       "convrot_quantize_fp8");
+}
+
+int convrot_quantize_fp8_weight(const void* w, int dtype, int64_t N, int64_t K, int64_t w_stride, uint8_t* codes,
+                                int64_t codes_stride, float* scales, void* stream) {
+  if (int rc = check_rows("8-bit quantization", w, dtype, N, K, w_stride, kMaxFeatures)) return rc;
+  if (N == 0 || K == 0) return ok();
+  if (int rc = check_fp8_codes(codes, codes_stride, K, scales)) return rc;
+  return launch_status(convrot::launch_quantize_fp8_weight(w, dtype, N, K, w_stride, codes, codes_stride, scales,
+                                                           (hipStream_t)stream),
+                       "convrot_quantize_fp8_weight");
+}
+
+int convrot_fp8_gemm(const uint8_t* act, int64_t act_stride, const float* xscales, int64_t xscales_row,
+                     int64_t xscales_block, const uint8_t* weight, int64_t weight_stride, const float* wscales,
+                     int64_t wscales_stride, const float* bias, int64_t M, int64_t N, int64_t K, const void* residual,
+                     const void* gate, int64_t gate_stride, int64_t rows_per_gate, void* workspace,
+                     int64_t workspace_bytes, void* out, int out_dtype, void* stream) {
+  if (int rc = check_fp8(M, N, K, weight, weight_stride, wscales, wscales_stride, out, out_dtype)) return rc;
+  if (int rc = check_fp8_work(residual, gate, rows_per_gate, workspace, workspace_bytes)) return rc;
+  if (M == 0 || N == 0) return ok();
+  if (!act || !xscales) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (act_stride < (K + 15) / 16 * 16 || act_stride % 16 || !aligned(act, 16) || !aligned(xscales, 4))
+    return fail(CONVROT_ERR_INVALID,
+                "FP8 operands need 16-byte aligned rows that cover K rounded up to 16 (K=%lld, activation stride %lld)",
+                (long long)K, (long long)act_stride);
+  if (act_stride > kMaxInt8Stride)
+    return fail(CONVROT_ERR_UNSUPPORTED, "FP8 row strides are limited to %lld bytes", (long long)kMaxInt8Stride);
+  if (xscales_row < 0 || xscales_block < 0 || xscales_row > kMaxXsRow)
+    return fail(CONVROT_ERR_UNSUPPORTED, "strides of activation scales (%lld, %lld) are not supported",
+                (long long)xscales_row, (long long)xscales_block);
+  convrot::GatedResidual gr{};
+  if (residual)
+    if (int rc = check_residual(residual, gate, gate_stride, rows_per_gate, M, N, &gr)) return rc;
+  const convrot::Fp8Operands p{act, weight, act_stride, weight_stride, xscales, wscales, bias, xscales_row,
+                               xscales_block, wscales_stride, out, (int)M, (int)N, (int)K, gr, {}, 0, 0};
+  const convrot::Workspace work{(uint8_t*)workspace, workspace ? (size_t)workspace_bytes : 0};
+  return launch_status(convrot::launch_fp8_gemm(p, out_dtype, (hipStream_t)stream, work), "convrot_fp8_gemm");
+}
+
+int64_t convrot_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > kMaxFeatures || M > 0x7ffffe00 || N > 0x7ffffe00) return 0;
+  return convrot::fp8_workspace_bytes(M, N, K);
+}
+
+int64_t convrot_fp8_scratch_bytes(int64_t rows, int64_t K) { return fp8_scratch_bytes(rows, K); }
+
+int convrot_fp8_linear(const void* x, int dtype, int64_t x_stride, const uint8_t* weight, int64_t weight_stride,
+                       const float* wscales, int64_t wscales_stride, const float* bias, int64_t M, int64_t N,
+                       int64_t K, const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate,
+                       void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* out,
+                       void* stream) {
+  if (int rc = check_rows("8-bit quantization", x, dtype, M, K, x_stride, kMaxFeatures)) return rc;
+  if (int rc = check_fp8(M, N, K, weight, weight_stride, wscales, wscales_stride, out, dtype)) return rc;
+  if (int rc = check_fp8_work(residual, gate, rows_per_gate, workspace, workspace_bytes)) return rc;
+  if (M == 0 || N == 0) return ok();
+  if (int rc = check_fp8_scratch(scratch, scratch_bytes, M, K)) return rc;
+  const Fp8Scratch c = fp8_scratch(scratch, M, K);
+  convrot::GatedResidual gr{};
+  if (residual)
+    if (int rc = check_residual(residual, gate, gate_stride, rows_per_gate, M, N, &gr)) return rc;
+  const convrot::Fp8Operands p{c.codes, weight, c.stride, weight_stride, c.scales, wscales, bias, 1,
+                               c.xs_block, wscales_stride, out, (int)M, (int)N, (int)K, gr, {}, 0, 0};
+  const convrot::Workspace work{(uint8_t*)workspace, workspace ? (size_t)workspace_bytes : 0};
+  hipError_t e = convrot::launch_quantize_fp8(x, dtype, M, K, x_stride, c.codes, c.stride, c.scales, 1, c.xs_block,
+                                              (hipStream_t)stream);
+  if (e == hipSuccess) e = convrot::launch_fp8_gemm(p, dtype, (hipStream_t)stream, work);
+  return launch_status(e, "convrot_fp8_linear");
+}
+
+namespace {
+
+constexpr int64_t kMaxExperts = 65536;
+
+// Checks of rows grouped by expert; `x_rows` is the number of rows of the activations.
+int check_groups(const int32_t* offsets, int64_t experts, const int32_t* index, int64_t choices, int64_t x_rows,
+                 int64_t rows) {
+  if (experts < 1 || experts > kMaxExperts)
+    return fail(CONVROT_ERR_UNSUPPORTED, "grouped products support 1 to %lld experts, got %lld", (long long)kMaxExperts,
+                (long long)experts);
+  if (x_rows < 0 || rows < 0 || choices < 1 || choices > 0x7fffffff)
+    return fail(CONVROT_ERR_INVALID, "invalid groups of %lld rows of %lld (%lld choices)", (long long)rows,
+                (long long)x_rows, (long long)choices);
+  if (!index && x_rows != rows)
+    return fail(CONVROT_ERR_INVALID, "%lld sorted rows, but %lld are grouped", (long long)x_rows, (long long)rows);
+  if (rows > 0 && !offsets) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(offsets, 4) || !aligned(index, 4)) return fail(CONVROT_ERR_INVALID, "offsets and index must be aligned");
+  return ok();
+}
+
+}  // namespace
+
+int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const uint8_t* weight,
+                               int64_t weight_stride, int64_t weight_expert, const float* wscales,
+                               int64_t wscales_stride, int64_t wscales_expert, const int32_t* offsets, int64_t experts,
+                               const int32_t* index, int64_t choices, int64_t rows, int64_t N, int64_t K,
+                               void* scratch, int64_t scratch_bytes, void* out, void* stream) {
+  if (int rc = check_rows("8-bit quantization", x, dtype, x_rows, K, x_stride, kMaxFeatures)) return rc;
+  if (int rc = check_fp8(rows, N, K, weight, weight_stride, wscales, wscales_stride, out, dtype)) return rc;
+  if (int rc = check_groups(offsets, experts, index, choices, x_rows, rows)) return rc;
+  if (weight_expert < 0 || weight_expert % 16 || wscales_expert < 0)
+    return fail(CONVROT_ERR_INVALID, "experts' weights must be 16-byte aligned (%lld bytes apart)", (long long)weight_expert);
+  if (rows == 0 || N == 0) return ok();
+  if (x_rows > 0)
+    if (int rc = check_fp8_scratch(scratch, scratch_bytes, x_rows, K)) return rc;
+  const Fp8Scratch c = fp8_scratch(scratch, x_rows, K);
+  if (index && (x_rows * c.stride > convrot::kMaxExtent || x_rows == 0))
+    return fail(CONVROT_ERR_UNSUPPORTED, "rows read through an index support 1 to 2^32 codes, got %lld rows of %lld",
+                (long long)x_rows, (long long)c.stride);
+  const convrot::Fp8Operands p{c.codes, weight, c.stride, weight_stride, c.scales, wscales, nullptr, 1, c.xs_block,
+                               wscales_stride, out, (int)rows, (int)N, (int)K, {},
+                               {offsets, index, (int)experts, (int)choices, x_rows}, weight_expert, wscales_expert};
+  hipError_t e = convrot::launch_quantize_fp8(x, dtype, x_rows, K, x_stride, c.codes, c.stride, c.scales, 1, c.xs_block,
+                                              (hipStream_t)stream);
+  if (e == hipSuccess) e = convrot::launch_fp8_gemm(p, dtype, (hipStream_t)stream, convrot::Workspace{});
+  return launch_status(e, "convrot_fp8_grouped_linear");
 }
 
 }  // extern "C"

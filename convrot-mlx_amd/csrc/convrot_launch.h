@@ -33,6 +33,8 @@ enum TuneKey : int {
   kTuneFp6Split,         // FP6 256x256 tiles past the whole rounds: as 1, 2 or 4 workgroups
   kTuneW8a8Tile,         // W8A8 tile: bm | bn << 10
   kTuneW8a8Split,        // workgroups that share a W8A8 tile's K
+  kTuneFp8Tile,          // FP8 tile: bm | bn << 10
+  kTuneFp8Split,         // workgroups that share an FP8 tile's K
   kTuneCount
 };
 int tuning(TuneKey key);
@@ -48,6 +50,7 @@ bool w4a4_tile_known(int bm, int bn, int wm, int wn, int stages);
 bool fp6_tile_known(int bm, int bn);
 bool w4a16_tile_known(int bm, int bn);
 bool w8a8_tile_known(int bm, int bn);
+bool fp8_tile_known(int bm, int bn);
 
 // The FP6 W4A4 tile the plan (and the fp6_tile override) picks for M x N on operand
 // blocks, and on compact weights, where each 256 x 256 tile past the whole rounds
@@ -254,5 +257,22 @@ hipError_t launch_qk_rotary_backward(const RotaryShape& shape, const void* dq, c
                                      hipStream_t stream);
 hipError_t launch_axes_table(const void* positions, int kind, int64_t rows, int axes, const int* dims, double theta,
                              float* out, hipStream_t stream);
+
+// ---- linears in 8-bit floating point (gemm_fp8.hip), their quantizers (fp8_quant.hip), and the
+// products of rows grouped by expert
+
+// Codes [rows, K] (rows codes_stride bytes apart, zeros from K to the end of the last block of 128 as
+// far as they reach), the scale of block b of row m at float m * xs_row + b * xs_block.
+hipError_t launch_quantize_fp8(const void* x, int dtype, int64_t rows, int64_t K, int64_t x_stride, uint8_t* codes,
+                               int64_t codes_stride, float* scales, int64_t xs_row, int64_t xs_block,
+                               hipStream_t stream);
+hipError_t launch_quantize_fp8_weight(const void* w, int dtype, int64_t N, int64_t K, int64_t w_stride, uint8_t* codes,
+                                      int64_t codes_stride, float* scales, hipStream_t stream);
+
+struct Fp8Operands;  // fp8_device.h
+hipError_t launch_fp8_gemm(const Fp8Operands& p, int out_dtype, hipStream_t stream, const Workspace& work);
+
+// Workspace that launch_fp8_gemm uses for a shape (0: none), in the places of the W8A8 product's.
+int64_t fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 }  // namespace convrot

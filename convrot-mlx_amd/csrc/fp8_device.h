@@ -1,0 +1,74 @@
+// What the kernels of 8-bit floating point share: e4m3 codes with a float32 scale
+// for each block of 128, and the operands of their products.
+//
+// A block whose largest magnitude is a has the scale s = 2^p, the smallest power of
+// two with a / s <= 448, the type's largest value.  Dividing by a power of two is
+// exact, so the code is x / s rounded once (to the nearest, ties to even), whatever
+// order or precision the scale is applied in; against s = a / 448 the codes lose at
+// most a bit of range at the low end (values below 2^-6 s lose mantissa bits), none
+// of their precision.
+#pragma once
+
+#include "w8a8_device.h"
+
+namespace convrot {
+
+constexpr int kBlock = 128;                      // features (and of a weight, outputs) under one scale
+constexpr uint32_t kPastEnd = 0xffffff00u;       // buffer offset past every operand: reads zero
+constexpr int64_t kMaxExtent = 0xfffff000ll;     // bytes of an operand that is addressed as one buffer
+
+struct Fp8Scale {
+  float inverse, scale;
+};
+// From the bits of a block's largest magnitude (infinity lies above every number, NaN above
+// infinity).  Below 2^-100: a block of zeros; not finite: the scale NaN (every product of the block
+// is NaN).
+__device__ __forceinline__ Fp8Scale fp8_scale(uint32_t most) {
+  if (most >= 0x7f800000u) return {0.0f, __builtin_nanf("")};
+  if (most < (27u << 23)) return {0.0f, 0.0f};
+  // a = m 2^e with m in [1, 2): 448 = 1.75 * 2^8
+  const uint32_t p = (most >> 23) - 8u + ((most & 0x7fffffu) > 0x600000u ? 1u : 0u);  // biased
+  return {__builtin_bit_cast(float, (254u - p) << 23), __builtin_bit_cast(float, p << 23)};
+}
+// Four codes of values over the scale; in a block that is not finite any value is 0 (the scale is NaN).
+__device__ __forceinline__ uint32_t fp8_codes4(const float* v, float inverse) {
+  float t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = inverse == 0.0f ? 0.0f : v[j] * inverse;
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], w, true);
+}
+
+// Rows grouped by expert: expert e has rows offsets[e] .. offsets[e + 1] - 1 of `rows`; those from
+// offsets[experts] on have none and give zeros.  With `index`, sorted row s is row index[s] / choices
+// of the activations.
+struct Groups {
+  const int* offsets = nullptr;
+  const int* index = nullptr;
+  int experts = 0, choices = 1;
+  int64_t act_rows = 0;
+};
+
+struct Fp8Operands {
+  const uint8_t* act;
+  const uint8_t* weight;
+  int64_t lda, ldw;
+  const float *xscales, *wscales, *bias;
+  int64_t xs_row, xs_block;  // floats between the scales of rows, of blocks
+  int64_t ws_row;            // floats between the scales of blocks of outputs
+  void* out;
+  int M, N, K;
+  GatedResidual gr;
+  Groups g;
+  int64_t weight_expert, ws_expert;  // bytes and floats between experts
+};
+
+// The tiled product of one output type (gemm_fp8_tile.h, one source a type); `tile` is one of FP8_TILES.
+template <int ODT>
+hipError_t launch_fp8_tile(int tile, const Fp8Operands& p, const W8a8Split& split, hipStream_t stream);
+
+// The tiles built: BM, BN, waves along each, ring stages, workgroups a CU.
+#define FP8_TILES(X) \
+  X(256, 256, 4, 2, 2, 1) X(256, 128, 4, 2, 3, 1) X(128, 128, 2, 2, 2, 2) X(64, 128, 2, 2, 3, 2) X(32, 64, 1, 4, 5, 2)
+
+}  // namespace convrot

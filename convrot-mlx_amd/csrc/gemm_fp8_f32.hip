@@ -1,0 +1,6 @@
+// The tiled products of 8-bit floating point with float32 outputs.
+#include "gemm_fp8_tile.h"
+
+namespace convrot {
+template hipError_t launch_fp8_tile<kF32>(int tile, const Fp8Operands& p, const W8a8Split& split, hipStream_t stream);
+}

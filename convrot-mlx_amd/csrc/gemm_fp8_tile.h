@@ -1,0 +1,431 @@
+// Products of e4m3 codes with a float32 scale for each block of 128, for gfx950:
+//
+//   out[m][n] = dt( sum_b (xs[m][b] ws[n / 128][b]) * (sum_{k in block b} act[m][k] w[n][k]) + bias[n] )
+//
+// with an optional gated residual in float32 before the one rounding, for rows of one
+// weight, and for rows grouped by expert (fp8_device.h), sorted or read through an index.
+//
+// The codes of one block go through one MFMA of K = 128 (v_mfma_f32_16x16x128_f8f6f4,
+// from zero); its 4 results a lane are multiplied by their scales and added in float32
+// by the vector unit (4 FMAs of 4 cycles beside 32 cycles of the MFMA: hidden while two
+// waves share a SIMD).  So the sums of different blocks are added at float32, and the
+// scales may be any numbers.
+//
+// What the FP8 form keeps of a sum: the 16 products of features 16 i .. 16 i + 15 are
+// aligned to the largest of them and lose what lies more than 13 bits below its leading
+// one (measured with single products; sums of different sixteens are float32's own), up
+// to 15 * 2^-13 of the largest product, 1.5e-5 of a sum of normal values: a sixteenth of
+// float16's own rounding.  Float32 outputs get their products added at float32 instead,
+// on bf16 MFMAs (codes are exact in bf16), at half the rate.
+//
+// Operands: codes row-major, rows of 16-byte aligned strides that cover K rounded up to
+// 16, zeros from K on.  Each 1 KB piece of a block (8 rows x 128 bytes: whole cache
+// lines) goes by one wave instruction straight into an LDS ring of STAGES blocks; the
+// 16-byte chunks of a row are permuted by its row number, so that the fragment reads (16
+// rows x 16 bytes) meet no bank twice.  Beside the codes of a block lie the scales of its
+// rows; the weights' scales of all blocks lie in LDS from the start.
+#pragma once
+
+#include <type_traits>
+
+#include "convrot_launch.h"
+#include "gemm_groups.h"
+#include "gemm_w8a8_tile.h"
+
+namespace convrot {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kMaxBlocks = 512;  // K up to 65536
+
+template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU>
+struct Fp8Engine {
+  static constexpr int NW = WM * WN, THREADS = NW * 64;
+  static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  static constexpr int APW = BM / 8 / NW, BPW = BN / 8 / NW, LPW = APW + BPW + 1;  // DMAs a wave and block
+  static constexpr int XS_OFF = (BM + BN) * 128, STAGE_BYTES = XS_OFF + NW * 256;
+  static constexpr int RING = STAGES * STAGE_BYTES, STAGING = NW * TM * (TN * 2 + 16);  // 16-bit epilogue
+  // weights' scales of the tile's blocks of outputs (WS of them: the tile lies in one, or covers two)
+  static constexpr int WS = BN > kBlock ? BN / kBlock : 1;
+  static constexpr int WS_OFF = RING > STAGING ? RING : STAGING;
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BM <= NW * 64, "whole pieces a wave");
+  static_assert(kBlock % TN == 0 && (BN % kBlock == 0 || kBlock % BN == 0), "a wave's corner under one scale");
+  static_assert((STAGES - 1) * LPW <= 63, "vmcnt counts at most 63 DMAs");
+  static constexpr int smem_bytes(int blocks) { return WS_OFF + WS * ((blocks * 4 + 255) / 256 * 256); }
+
+  uint8_t* smem;
+  uint32_t smem_addr;
+  int lane, wave, wm, wn;
+  i32x4_sgpr ra, rw;
+  uint32_t va[APW], vw[BPW], vx;
+  bool past_a[2], past_w[2];  // lane's chunk of the last block lies past the row's end, in even and odd pieces
+  uint32_t tail;              // the block that rows end in, ~0 where they fill it
+  const float* xs_base;
+  int64_t xs_block;
+  uint32_t xs_bytes;
+
+  __device__ __forceinline__ explicit Fp8Engine(uint8_t* s) : smem(s) {
+    smem_addr = (uint32_t)(uintptr_t)s;
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wm = wave / WN;
+    wn = wave % WN;
+  }
+
+  // Sorted row m's row of the activations, -1 for none.
+  __device__ __forceinline__ static int64_t source(const Fp8Operands& p, int m, int row_end) {
+    if (m >= row_end) return -1;
+    const int i = p.g.index[m];
+    const uint32_t t = (uint32_t)i / (uint32_t)p.g.choices;
+    return i < 0 || t >= p.g.act_rows ? -1 : (int64_t)t;
+  }
+
+  template <bool GATHER>
+  __device__ __forceinline__ void set_tile(const Fp8Operands& p, int expert, int m0, int row_end, int n0) {
+    const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u, rest = k16 & 127u;
+    tail = rest ? k16 >> 7 : ~0u;
+    const int mrows = min(BM, row_end - m0), nrows = min(BN, p.N - n0);
+    const int rl = lane >> 3, c = lane & 7;
+    rw = buffer_rsrc(p.weight + (int64_t)expert * p.weight_expert + (int64_t)n0 * p.ldw,
+                     (uint32_t)(nrows - 1) * (uint32_t)p.ldw + k16);
+#pragma unroll
+    for (int i = 0; i < BPW; ++i) {
+      const int piece = wave * BPW + i;
+      vw[i] = (uint32_t)(8 * piece + rl) * (uint32_t)p.ldw + 16u * (uint32_t)(c ^ rl ^ (piece & 1));
+    }
+    xs_block = p.xs_block;
+    const int xr = wave * 64 + lane;  // the row whose scale this lane moves
+    if constexpr (GATHER) {
+      ra = buffer_rsrc(p.act, (uint32_t)((p.g.act_rows - 1) * p.lda) + k16);
+#pragma unroll
+      for (int i = 0; i < APW; ++i) {
+        const int piece = wave * APW + i;
+        const int64_t t = source(p, m0 + 8 * piece + rl, row_end);
+        va[i] = t < 0 ? kPastEnd : (uint32_t)(t * p.lda) + 16u * (uint32_t)(c ^ rl ^ (piece & 1));
+      }
+      const int64_t t = xr < BM ? source(p, m0 + xr, row_end) : -1;
+      vx = t < 0 ? kPastEnd : (uint32_t)(t * p.xs_row) * 4u;
+      xs_base = p.xscales;
+      xs_bytes = (uint32_t)((p.g.act_rows - 1) * p.xs_row) * 4u + 4u;
+    } else {
+      ra = buffer_rsrc(p.act + (int64_t)m0 * p.lda, (uint32_t)(mrows - 1) * (uint32_t)p.lda + k16);
+#pragma unroll
+      for (int i = 0; i < APW; ++i) {
+        const int piece = wave * APW + i;
+        va[i] = 8 * piece + rl < mrows
+                    ? (uint32_t)(8 * piece + rl) * (uint32_t)p.lda + 16u * (uint32_t)(c ^ rl ^ (piece & 1))
+                    : kPastEnd;
+      }
+      vx = xr < mrows ? (uint32_t)xr * (uint32_t)p.xs_row * 4u : kPastEnd;
+      xs_base = p.xscales + (int64_t)m0 * p.xs_row;
+      xs_bytes = (uint32_t)(mrows - 1) * (uint32_t)p.xs_row * 4u + 4u;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      past_a[e] = 16u * (uint32_t)(c ^ rl ^ ((wave * APW + e) & 1)) >= rest;
+      past_w[e] = 16u * (uint32_t)(c ^ rl ^ ((wave * BPW + e) & 1)) >= rest;
+    }
+  }
+
+  // The weights' scales of the tile into LDS, block b of output block j at float j * stride + b.
+  __device__ __forceinline__ void issue_ws(const Fp8Operands& p, int expert, int n0) const {
+    const int blocks = (p.K + kBlock - 1) / kBlock, pieces = (blocks + 63) / 64;
+    const int nb = min(WS, (p.N + kBlock - 1) / kBlock - n0 / kBlock);
+    const float* base = p.wscales + (int64_t)expert * p.ws_expert + (int64_t)(n0 / kBlock) * p.ws_row;
+    for (int d = wave; d < nb * pieces; d += NW) {
+      const int j = d / pieces, at = d - j * pieces;
+      dma4(buffer_rsrc(base + j * p.ws_row, (uint32_t)blocks * 4u), (uint32_t)(at * 256 + lane * 4),
+           smem_addr + (uint32_t)(WS_OFF + d * 256));
+    }
+  }
+
+  __device__ __forceinline__ void issue(uint32_t kb, int stage) const {
+    const uint32_t base = smem_addr + (uint32_t)(stage * STAGE_BYTES), k = kb * 128u;
+    const bool last = kb == tail;
+#pragma unroll
+    for (int i = 0; i < APW; ++i) {
+      uint32_t off = va[i] == kPastEnd ? kPastEnd : va[i] + k;
+      if (last) off = past_a[i & 1] ? kPastEnd : off;
+      dma16(ra, off, base + (uint32_t)(wave * APW + i) * 1024u);
+    }
+#pragma unroll
+    for (int i = 0; i < BPW; ++i) {
+      uint32_t off = vw[i] + k;
+      if (last) off = past_w[i & 1] ? kPastEnd : off;
+      dma16(rw, off, base + (uint32_t)BM * 128u + (uint32_t)(wave * BPW + i) * 1024u);
+    }
+    dma4(buffer_rsrc(xs_base + (int64_t)kb * xs_block, xs_bytes), vx, base + (uint32_t)XS_OFF + (uint32_t)wave * 256u);
+  }
+
+  __device__ __forceinline__ i32x8 fragment(const uint8_t* row) const {
+    const int r = lane & 15, q = lane >> 4, sw = chunk_swizzle(r);
+    const i32x4 lo = *(const i32x4*)(row + ((2 * q) ^ sw) * 16), hi = *(const i32x4*)(row + ((2 * q + 1) ^ sw) * 16);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+
+  // The 32 codes of a fragment as bf16 (exact).
+  struct Wide {
+    bf16x8 v[4];
+  };
+  __device__ __forceinline__ static Wide widen(const i32x8& c) {
+    Wide w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      i32x4 t;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        t[2 * h] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * i + h], 1.0f, false));
+        t[2 * h + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * i + h], 1.0f, true));
+      }
+      w.v[i] = __builtin_bit_cast(bf16x8, t);
+    }
+    return w;
+  }
+
+  // acc += the scaled products of one block.  WIDE: on bf16 MFMAs, whose sums are float32's own (what
+  // the FP8 form keeps of a sum is stated above).
+  template <bool WIDE>
+  __device__ __forceinline__ void block(int stage, float ws, f32x4 (&acc)[FN][FM]) const {
+    const uint8_t* base = smem + stage * STAGE_BYTES;
+    const uint8_t* sa = base + (wm * TM + (lane & 15)) * 128;
+    const uint8_t* sw = base + BM * 128 + (wn * TN + (lane & 15)) * 128;
+    const float* xs = (const float*)(base + XS_OFF) + wm * TM + (lane & 15);
+    using Frag = std::conditional_t<WIDE, Wide, i32x8>;
+    Frag a[FM];
+    float s[FM];
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      if constexpr (WIDE) a[fm] = widen(fragment(sa + fm * 2048));
+      else a[fm] = fragment(sa + fm * 2048);
+      s[fm] = xs[fm * 16] * ws;
+    }
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int fn = 0; fn < FN; ++fn) {
+      Frag w;
+      if constexpr (WIDE) w = widen(fragment(sw + fn * 2048));
+      else w = fragment(sw + fn * 2048);
+#pragma unroll
+      for (int fm = 0; fm < FM; ++fm) {
+        f32x4 part = zero;
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], a[fm].v[i], part, 0, 0, 0);
+        } else {
+          part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a[fm], zero, 0, 0, 0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[fn][fm][j] = __builtin_fmaf(part[j], s[fm], acc[fn][fm][j]);
+      }
+    }
+  }
+
+  // acc += the products of blocks kb0 .. kb0 + n - 1, n >= 1.
+  template <bool WIDE>
+  __device__ __forceinline__ void run(uint32_t kb0, int n, int ws_stride, f32x4 (&acc)[FN][FM]) {
+    const uint32_t last = kb0 + (uint32_t)n - 1;
+    const float* ws = (const float*)(smem + WS_OFF) + (WS > 1 ? wn * TN / kBlock * ws_stride : 0);
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) issue(min(kb0 + s, last), s);
+    int st = 0;
+    for (uint32_t kb = kb0; kb <= last; ++kb) {
+      wait_vmcnt<(STAGES - 2) * LPW>();
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): this wave is done with the stage before
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      // into the stage that every wave is done with (past the last block: the last one again)
+      issue(min(kb + STAGES - 1, last), st == 0 ? STAGES - 1 : st - 1);
+      block<WIDE>(st, ws[kb], acc);
+      st = st + 1 == STAGES ? 0 : st + 1;
+    }
+    wait_vmcnt<0>();  // the DMAs past the last block have landed before the ring is reused
+  }
+};
+
+// Bias of outputs n .. n + 3 (0 without one, or past N).
+__device__ __forceinline__ void load_bias4(const Fp8Operands& p, int n, float (&b)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = p.bias && n + j < p.N ? p.bias[n + j] : 0.0f;
+}
+
+// The wave's corner of the tile: bias, gated residual, rounding, store; rows m0 .. row_end - 1.  16-bit
+// outputs (and residuals) go through the wave's part of LDS in whole aligned chunks of 16 bytes.
+template <class E, int ODT, bool ALIGNED>
+__device__ __forceinline__ void fp8_epilogue16(const E& e, const f32x4 (&acc)[E::FN][E::FM], const Fp8Operands& p, int m0,
+                                               int row_end, int n0) {
+  constexpr int FM = E::FM, FN = E::FN, TM = E::TM, TN = E::TN, RS = TN * 2 + 16;
+  const int lane = e.lane, mw = m0 + e.wm * TM, nw = n0 + e.wn * TN;
+  uint8_t* region = e.smem + e.wave * (TM * RS);
+  const bool residual = p.gr.residual != nullptr;
+  const bool one_gate = residual && mw / p.gr.rows_per_gate == (min(mw + TM, row_end) - 1) / p.gr.rows_per_gate;
+  if (residual) {
+    move_corner<TM, TN, ALIGNED, false>(region, (uint16_t*)p.gr.residual, lane, mw, nw, row_end, p.N);
+    wave_lds_fence();
+  }
+  uint8_t* at[FM];
+#pragma unroll
+  for (int fm = 0; fm < FM; ++fm) {
+    const int row = fm * 16 + (lane & 15);
+    at[fm] = region + row * RS + (ALIGNED ? 0 : 2 * (int)(((int64_t)(mw + row) * p.N + nw) & 7));
+  }
+  static_for<FN>([&](auto frag) __attribute__((always_inline)) {
+    constexpr int fn = frag.value;
+    const int nl = fn * 16 + 4 * (lane >> 4);
+    float b[4], g[4];
+    load_bias4(p, nw + nl, b);
+    if (one_gate && mw < row_end) load_gate4<ODT>(p.gr, mw, nw + nl, p.N, g);
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      float o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = acc[fn][fm][r] + b[r];
+      uint16_t* q = (uint16_t*)(at[fm] + nl * 2);
+      if (residual) {
+        const int m = mw + fm * 16 + (lane & 15);
+        if (!one_gate && m < row_end) load_gate4<ODT>(p.gr, m, nw + nl, p.N, g);
+        float res[4];
+        if constexpr (ALIGNED) {
+          load_elem4<ODT>(q, 0, res);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) res[r] = load_elem<ODT>(q, r);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = res[r] + g[r] * o[r];
+      }
+      if constexpr (ALIGNED) {
+        store_out4<ODT>(q, 0, o[0], o[1], o[2], o[3]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) store_out<ODT>(q, r, o[r]);
+      }
+    }
+  });
+  wave_lds_fence();
+  move_corner<TM, TN, ALIGNED, true>(region, (uint16_t*)p.out, lane, mw, nw, row_end, p.N);
+}
+
+template <class E>
+__device__ __forceinline__ void fp8_epilogue32(const E& e, const f32x4 (&acc)[E::FN][E::FM], const Fp8Operands& p, int m0,
+                                               int row_end, int n0) {
+  const int lane = e.lane, mw = m0 + e.wm * E::TM, nw = n0 + e.wn * E::TN;
+  const W8a8Operands q{nullptr, nullptr, 0, 0, nullptr, nullptr, nullptr, p.out, row_end, p.N, p.K, p.gr};
+  static_for<E::FN>([&](auto frag) __attribute__((always_inline)) {
+    constexpr int fn = frag.value;
+    const int n = nw + fn * 16 + 4 * (lane >> 4);
+    if (n >= p.N) return;
+    float b[4];
+    load_bias4(p, n, b);
+#pragma unroll
+    for (int fm = 0; fm < E::FM; ++fm) {
+      const int m = mw + fm * 16 + (lane & 15);
+      if (m >= row_end) continue;
+      float o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = acc[fn][fm][r] + b[r];
+      store4<kF32>(q, m, n, (p.N & 3) == 0, o);
+    }
+  });
+}
+
+// KIND 0: rows of one weight (their K may be shared between workgroups), 1: sorted rows of experts, 2:
+// rows of experts read through the index.
+template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, int ODT, int KIND>
+__global__ __launch_bounds__(WM* WN * 64) __attribute__((amdgpu_waves_per_eu(PER_CU* WM* WN / 4, PER_CU* WM* WN / 4)))
+void fp8_tile_kernel(Fp8Operands p, int tiles_m, int tiles_n, W8a8Split split) {
+  using E = Fp8Engine<BM, BN, WM, WN, STAGES, PER_CU>;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  E e(smem);
+  if constexpr (KIND != 0) tiles_m = group_tile_rows<BM>(p.g, p.M);
+  // tiles that one XCD (one L2) runs are neighbours, in groups of kGroupM tile rows
+  const int tiles = tiles_m * tiles_n, per_xcd = tiles / kXcds;
+  const int part = KIND == 0 && split.splits > 1 ? blockIdx.x / tiles : 0;
+  int t = blockIdx.x - part * tiles;
+  if (KIND != 0 && t >= tiles) return;
+  if (t < per_xcd * kXcds) t = (t % kXcds) * per_xcd + t / kXcds;
+  const int group = t / (kGroupM * tiles_n), first_m = group * kGroupM;
+  const int group_rows = min(kGroupM, tiles_m - first_m), in_group = t - group * kGroupM * tiles_n;
+  const int tile_row = first_m + in_group % group_rows, n0 = (in_group / group_rows) * BN;
+  GroupTile at{0, tile_row * BM, p.M};
+  if constexpr (KIND != 0) {
+    at = group_tile<BM>(p.g, p.M, tile_row);
+    if (at.expert < 0) return;
+  }
+  const int m0 = at.row0, row_end = at.row_end;
+
+  f32x4 acc[E::FN][E::FM];
+#pragma unroll
+  for (int a = 0; a < E::FN; ++a)
+#pragma unroll
+    for (int b = 0; b < E::FM; ++b) acc[a][b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  const int kblocks = (p.K + kBlock - 1) / kBlock, ws_stride = (kblocks + 63) / 64 * 64;
+  if (KIND == 0 || at.expert < p.g.experts) {
+    e.issue_ws(p, at.expert, n0);
+    e.template set_tile<KIND == 2>(p, at.expert, m0, row_end, n0);
+    if (KIND != 0 || split.splits == 1) {
+      e.template run<ODT == kF32>(0, kblocks, ws_stride, acc);
+    } else {
+      e.template run<ODT == kF32>((uint32_t)(part * split.kblocks), min(split.kblocks, kblocks - part * split.kblocks), ws_stride, acc);
+      // partials [tile][part][fragment][thread], added in the parts' order by the last workgroup to arrive
+      __shared__ int last;
+      constexpr uint32_t BYTES = BM * BN * 4, STEP = E::THREADS * 16u;
+      const __amdgpu_buffer_rsrc_t r =
+          partial_rsrc(split.partials + (size_t)t * split.splits * BYTES, (uint32_t)split.splits * BYTES);
+      const uint32_t mine = threadIdx.x * 16u;
+      static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+        for (int fm = 0; fm < E::FM; ++fm)
+          store_partial(r, (uint32_t)part * BYTES + (uint32_t)(fn.value * E::FM + fm) * STEP + mine,
+                        __builtin_bit_cast(i32x4, acc[fn.value][fm]));
+      });
+      if (!last_to_arrive(split.counters + t, split.splits, &last)) return;
+      static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+        for (int fm = 0; fm < E::FM; ++fm) acc[fn.value][fm] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      });
+      for (int q = 0; q < split.splits; ++q)
+        static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+          for (int fm = 0; fm < E::FM; ++fm)
+            acc[fn.value][fm] += __builtin_bit_cast(
+                f32x4, load_partial(r, (uint32_t)q * BYTES + (uint32_t)(fn.value * E::FM + fm) * STEP + mine));
+        });
+    }
+  }
+  __syncthreads();  // every wave is done with the ring before it stages outputs
+  if constexpr (ODT == kF32) fp8_epilogue32<E>(e, acc, p, m0, row_end, n0);
+  else if ((p.N & 7) == 0) fp8_epilogue16<E, ODT, true>(e, acc, p, m0, row_end, n0);
+  else fp8_epilogue16<E, ODT, false>(e, acc, p, m0, row_end, n0);
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, int ODT, int KIND>
+hipError_t launch_fp8_tile_k(const Fp8Operands& p, const W8a8Split& split, hipStream_t s) {
+  using E = Fp8Engine<BM, BN, WM, WN, STAGES, PER_CU>;
+  static_assert(E::smem_bytes(kMaxBlocks) <= 160 * 1024 - 64, "LDS of one CU");
+  const int64_t tm = KIND == 0 ? ((int64_t)p.M + BM - 1) / BM : most_tile_rows(p.M, p.g.experts, BM);
+  const int64_t tn = ((int64_t)p.N + BN - 1) / BN, groups = tm * tn * split.splits;
+  if (groups > max_groups(E::THREADS) || groups > 0x7fffffff) return hipErrorInvalidValue;
+  fp8_tile_kernel<BM, BN, WM, WN, STAGES, PER_CU, ODT, KIND>
+      <<<dim3((unsigned)groups), dim3(E::THREADS), E::smem_bytes((p.K + kBlock - 1) / kBlock), s>>>(p, (int)tm, (int)tn,
+                                                                                                  split);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+template <int ODT>
+hipError_t launch_fp8_tile(int tile, const Fp8Operands& p, const W8a8Split& split, hipStream_t stream) {
+  switch (tile) {
+#define FP8_CASE(BM, BN, WM, WN, STAGES, PER_CU)                                                                \
+  case tile_code(BM, BN):                                                                                       \
+    if (!p.g.offsets) return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, ODT, 0>(p, split, stream);       \
+    if (!p.g.index) return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, ODT, 1>(p, split, stream);         \
+    return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, ODT, 2>(p, split, stream);
+    FP8_TILES(FP8_CASE)
+#undef FP8_CASE
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace convrot

@@ -1,0 +1,74 @@
+// Output tiles of products whose rows are grouped by expert, shared by the grouped kernels.
+#pragma once
+
+#include "fp8_device.h"
+
+namespace convrot {
+
+// offsets[i], within 0 .. rows whatever the caller's array holds; the first group begins at row 0.
+__device__ __forceinline__ int group_start(const Groups& g, int i, int rows) {
+  return i == 0 ? 0 : min(max(g.offsets[i], 0), rows);
+}
+
+struct GroupTile {
+  int expert;        // -1: no such tile; g.experts: rows of no expert
+  int row0, row_end; // the tile's first row, and where its group ends
+};
+
+// Rows of tiles of BM rows: the experts' in order, then those of the rows behind the last one.  Every
+// wave finds its own: 64 experts a step, their tiles summed over the lanes.
+template <int BM>
+__device__ __forceinline__ int group_tile_rows(const Groups& g, int rows) {
+  const int lane = threadIdx.x & 63;
+  int total = 0;
+  for (int e0 = 0; e0 <= g.experts; e0 += 64) {
+    const int e = e0 + lane;
+    int n = 0;
+    if (e <= g.experts) {
+      const int a = group_start(g, e, rows), b = e < g.experts ? group_start(g, e + 1, rows) : rows;
+      n = b > a ? (b - a + BM - 1) / BM : 0;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d);
+    total += n;
+  }
+  return __builtin_amdgcn_readfirstlane(total);
+}
+
+template <int BM>
+__device__ __forceinline__ GroupTile group_tile(const Groups& g, int rows, int tile_row) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int e0 = 0; e0 <= g.experts; e0 += 64) {
+    const int e = e0 + lane;
+    int a = 0, b = 0;
+    if (e <= g.experts) {
+      a = group_start(g, e, rows);
+      b = e < g.experts ? group_start(g, e + 1, rows) : rows;
+    }
+    const int n = b > a ? (b - a + BM - 1) / BM : 0;
+    int upto = n;  // tiles of this lane's expert and those before it
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    const int first = before + upto - n;
+    const uint64_t hit = __ballot(tile_row >= first && tile_row < first + n);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      const int r0 = __builtin_amdgcn_readlane(a, src) + (tile_row - __builtin_amdgcn_readlane(first, src)) * BM;
+      return {e0 + src, r0, __builtin_amdgcn_readlane(b, src)};
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return {-1, 0, 0};
+}
+
+// Most rows of tiles that any split of `rows` over the experts (and none) makes.
+inline int64_t most_tile_rows(int64_t rows, int64_t experts, int bm) {
+  const int64_t bound = rows / bm + experts + 1;
+  return rows < bound ? rows : bound;
+}
+
+}  // namespace convrot

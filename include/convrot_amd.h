@@ -560,6 +560,61 @@ int convrot_qk_rotary_backward(const void* dq, const void* dk, const void* q, co
                                const void* k_weight, int weight_dtype, float eps, int interleaved, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/*
+ * Linears in 8-bit floating point: e4m3 codes (one byte, the OCP "fn" form without infinities) with a
+ * float32 scale for each block of 128 features of a row, and of 128 x 128 of a weight.
+ *
+ * convrot_quantize_fp8: scale = 2^p, the smallest power of two with (largest |x| of the block) / scale
+ * <= 448; code = x / scale rounded to the nearest, ties to even.  A block whose largest magnitude is
+ * below 2^-100 counts as zero (scale 0), one that holds a NaN or an infinity gets the scale NaN.
+ * codes: rows codes_stride bytes apart (a multiple of 16, at least features), zeros from `features` to
+ * the end of the last block as far as they reach.  The scale of block b of row m goes to float
+ * m * scales_row + b * scales_block.  features <= 65536.
+ * convrot_quantize_fp8_weight: the same with one scale for each 128 x 128 of w [N, K], scales
+ * [ceil(N / 128)][ceil(K / 128)].
+ */
+int convrot_quantize_fp8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride, uint8_t* codes,
+                         int64_t codes_stride, float* scales, int64_t scales_row, int64_t scales_block, void* stream);
+int convrot_quantize_fp8_weight(const void* w, int dtype, int64_t N, int64_t K, int64_t w_stride, uint8_t* codes,
+                                int64_t codes_stride, float* scales, void* stream);
+
+/*
+ * out[m][n] = dt( sum_b (xs[m][b] ws[n / 128][b]) * (sum_{k in block b} act[m][k] weight[n][k]) + bias[n] ),
+ * sums in float32; then, with a residual, dt(residual[m][n] + gate * that), rounded once.  Any scales.
+ * act, weight: rows 16-byte aligned, of strides that are multiples of 16 and cover K rounded up to 16,
+ * zeros from K on.  xscales at m * xscales_row + b * xscales_block; wscales rows wscales_stride floats
+ * apart; bias float32 [N] or NULL.  residual, gate and workspace as in convrot_w8a8_gemm (the same
+ * workspace serves both); convrot_fp8_workspace_bytes says how much of it one product uses.
+ * convrot_fp8_linear: the same from x [M, K] of `dtype`, quantized into `scratch`
+ * (convrot_fp8_scratch_bytes, 16-byte aligned, any content).
+ */
+int convrot_fp8_gemm(const uint8_t* act, int64_t act_stride, const float* xscales, int64_t xscales_row,
+                     int64_t xscales_block, const uint8_t* weight, int64_t weight_stride, const float* wscales,
+                     int64_t wscales_stride, const float* bias, int64_t M, int64_t N, int64_t K, const void* residual,
+                     const void* gate, int64_t gate_stride, int64_t rows_per_gate, void* workspace,
+                     int64_t workspace_bytes, void* out, int out_dtype, void* stream);
+int64_t convrot_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int64_t convrot_fp8_scratch_bytes(int64_t rows, int64_t K);
+int convrot_fp8_linear(const void* x, int dtype, int64_t x_stride, const uint8_t* weight, int64_t weight_stride,
+                       const float* wscales, int64_t wscales_stride, const float* bias, int64_t M, int64_t N,
+                       int64_t K, const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate,
+                       void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* out,
+                       void* stream);
+
+/*
+ * The linears of a mixture of experts on such codes: sorted rows offsets[e] .. offsets[e + 1] - 1 (int32
+ * [experts + 1] on the device, from 0, not decreasing, at most `rows`) times weight e,
+ * weight + e * weight_expert bytes, scales wscales + e * wscales_expert floats.  Rows from
+ * offsets[experts] on give zeros.  Sorted row s is row s of x [x_rows = rows, K], or, with an index (int32
+ * [rows]), row index[s] / choices of x [x_rows, K] (out of range: a row of zeros), x_rows * K rounded
+ * up to 128 at most 2^32 - 4096.  scratch: convrot_fp8_scratch_bytes(x_rows, K).  out [rows, N].
+ */
+int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const uint8_t* weight,
+                               int64_t weight_stride, int64_t weight_expert, const float* wscales,
+                               int64_t wscales_stride, int64_t wscales_expert, const int32_t* offsets, int64_t experts,
+                               const int32_t* index, int64_t choices, int64_t rows, int64_t N, int64_t K,
+                               void* scratch, int64_t scratch_bytes, void* out, void* stream);
+
 /* Thread-local message of the last failed call on this thread ("" if none). */
 const char* convrot_last_error(void);
 
@@ -587,6 +642,8 @@ const char* convrot_last_error(void);
  *   fp6_tile         "BMxBN"              FP6 W4A4 tile: 256x256, 256x224, 128x256, 128x192 or 128x128
  *   w8a8_tile        "BMxBN"              W8A8 tile (256x256 .. 64x64), for few rows too
  *   w8a8_split       "1" .. "64"          workgroups that share a W8A8 tile's K (with a workspace)
+ *   fp8_tile         "BMxBN"              FP8 tile (256x256 .. 32x64)
+ *   fp8_split        "1" .. "64"          workgroups that share an FP8 tile's K (with a workspace)
  * Returns CONVROT_ERR_INVALID for an unknown name, a malformed value or a
  * tile the library does not build.
  */
