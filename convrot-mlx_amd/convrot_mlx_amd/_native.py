@@ -94,6 +94,12 @@ SIGNATURES = {
                                   _vp, _i64, _vp, _i64, _vp, _vp]),
     "convrot_fp8_grouped_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
                                           _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "convrot_expert_plan_workspace_bytes": (_i64, [_i64, _i64]),
+    "convrot_expert_plan": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "convrot_gather_rows": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "convrot_combine_rows": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "convrot_combine_rows_backward": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp,
+                                             _vp]),
     "convrot_last_error": (ctypes.c_char_p, []),
     "convrot_set_tuning": (_i32, [ctypes.c_char_p, ctypes.c_char_p]),
     "convrot_version": (ctypes.c_char_p, []),

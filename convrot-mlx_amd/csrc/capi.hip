@@ -1242,4 +1242,95 @@ int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t
   return launch_status(e, "convrot_fp8_grouped_linear");
 }
 
+// ---- what lies around the linears of a mixture of experts
+
+namespace {
+
+constexpr int64_t kMaxPlanExperts = 1024;  // one thread of the ordering workgroup each
+
+int check_token_rows(const char* what, const void* y, int dtype, int64_t rows, int64_t features, int64_t stride,
+                     int64_t tokens, int64_t choices) {
+  if (int rc = check_rows(what, y, dtype, rows, features, stride, kMaxRows)) return rc;
+  if (tokens < 0 || choices < 1 || tokens * choices > kMaxRows || choices > kMaxRows)
+    return fail(CONVROT_ERR_INVALID, "%s: invalid shape of %lld tokens of %lld choices", what, (long long)tokens,
+                (long long)choices);
+  return ok();
+}
+
+}  // namespace
+
+int64_t convrot_expert_plan_workspace_bytes(int64_t count, int64_t experts) {
+  if (count <= 0 || count > kMaxRows || experts < 1 || experts > kMaxPlanExperts) return 0;
+  return convrot::expert_plan_workspace_bytes(count, (int)experts);
+}
+
+int convrot_expert_plan(const void* ids, int ids_bits, int64_t count, int64_t experts, int32_t* offsets, int32_t* order,
+                        int32_t* slots, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (ids_bits != 32 && ids_bits != 64) return fail(CONVROT_ERR_INVALID, "expert numbers have 32 or 64 bits, got %d", ids_bits);
+  if (experts < 1 || experts > kMaxPlanExperts)
+    return fail(CONVROT_ERR_UNSUPPORTED, "the order by expert supports 1 to %lld experts, got %lld",
+                (long long)kMaxPlanExperts, (long long)experts);
+  if (count < 0 || count > kMaxRows)
+    return fail(CONVROT_ERR_UNSUPPORTED, "the order by expert supports at most 2^31-1 choices, got %lld", (long long)count);
+  if (!offsets || (count > 0 && (!ids || !order || !slots))) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(ids, ids_bits / 8) || !aligned(offsets, 4) || !aligned(order, 4) || !aligned(slots, 4))
+    return fail(CONVROT_ERR_INVALID, "expert numbers and their order must be aligned to their types");
+  const int64_t need = convrot_expert_plan_workspace_bytes(count, experts);
+  if (need > 0 && (!workspace || !aligned(workspace, 4) || workspace_bytes < need))
+    return fail(CONVROT_ERR_INVALID, "the order by expert needs a workspace of %lld bytes, got %lld", (long long)need,
+                (long long)workspace_bytes);
+  return launch_status(convrot::launch_expert_plan(ids, ids_bits == 64, count, (int)experts, offsets, order, slots,
+                                                   (int*)workspace, (hipStream_t)stream),
+                       "convrot_expert_plan");
+}
+
+int convrot_gather_rows(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const int32_t* index,
+                        int64_t choices, int64_t rows, int64_t features, void* out, void* stream) {
+  if (int rc = check_rows("gathered rows", x, dtype, x_rows, features, x_stride, kMaxRows)) return rc;
+  if (rows < 0 || rows > kMaxRows || choices < 1 || choices > kMaxRows)
+    return fail(CONVROT_ERR_INVALID, "invalid shape of %lld gathered rows (%lld choices)", (long long)rows, (long long)choices);
+  if (rows == 0 || features == 0) return ok();
+  if (!index || !out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(index, 4) || !aligned(out, dtype == CONVROT_DTYPE_F32 ? 4 : 2))
+    return fail(CONVROT_ERR_INVALID, "index and out must be aligned to their types");
+  return launch_status(convrot::launch_gather_rows(x, dtype, x_rows, x_stride, index, (int)choices, rows, features, out,
+                                                   (hipStream_t)stream),
+                       "convrot_gather_rows");
+}
+
+int convrot_combine_rows(const void* y, int dtype, int64_t y_rows, int64_t y_stride, const int32_t* slots,
+                         const float* weights, int64_t tokens, int64_t choices, int64_t features, void* out,
+                         void* stream) {
+  if (int rc = check_token_rows("combined rows", y, dtype, y_rows, features, y_stride, tokens, choices)) return rc;
+  if (tokens == 0 || features == 0) return ok();
+  if (!slots || !out) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(slots, 4) || !aligned(weights, 4) || !aligned(out, dtype == CONVROT_DTYPE_F32 ? 4 : 2))
+    return fail(CONVROT_ERR_INVALID, "slots, weights and out must be aligned to their types");
+  return launch_status(convrot::launch_combine_rows(y, dtype, y_rows, y_stride, slots, weights, tokens, (int)choices,
+                                                    features, out, (hipStream_t)stream),
+                       "convrot_combine_rows");
+}
+
+int convrot_combine_rows_backward(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int dtype,
+                                  int64_t y_rows, const int32_t* order, const int32_t* slots, const float* weights,
+                                  int64_t tokens, int64_t choices, int64_t features, void* dy, float* dweights,
+                                  void* stream) {
+  if (int rc = check_token_rows("the gradient of combined rows", dout, dtype, tokens, features, dout_stride, tokens,
+                                choices))
+    return rc;
+  if (y_rows != tokens * choices)
+    return fail(CONVROT_ERR_INVALID, "%lld rows for %lld choices", (long long)y_rows, (long long)(tokens * choices));
+  if (dweights)
+    if (int rc = check_rows("the gradient of combined rows", y, dtype, y_rows, features, y_stride, kMaxRows)) return rc;
+  if (tokens == 0 || (!dy && !dweights)) return ok();
+  if (!slots || (dy && !order)) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(order, 4) || !aligned(slots, 4) || !aligned(weights, 4) || !aligned(dweights, 4) ||
+      !aligned(dy, dtype == CONVROT_DTYPE_F32 ? 4 : 2))
+    return fail(CONVROT_ERR_INVALID, "order, slots, weights and gradients must be aligned to their types");
+  return launch_status(convrot::launch_combine_rows_backward(dout, dout_stride, y, y_stride, dtype, y_rows, order, slots,
+                                                             weights, tokens, (int)choices, features, dy, dweights,
+                                                             (hipStream_t)stream),
+                       "convrot_combine_rows_backward");
+}
+
 }  // extern "C"

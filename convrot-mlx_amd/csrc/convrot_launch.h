@@ -275,4 +275,19 @@ hipError_t launch_fp8_gemm(const Fp8Operands& p, int out_dtype, hipStream_t stre
 // Workspace that launch_fp8_gemm uses for a shape (0: none), in the places of the W8A8 product's.
 int64_t fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
+// ---- the linears of a mixture of experts: what lies around them (experts.hip)
+
+int64_t expert_plan_workspace_bytes(int64_t count, int experts);
+hipError_t launch_expert_plan(const void* ids, bool ids64, int64_t count, int experts, int* offsets, int* order,
+                              int* slots, int* workspace, hipStream_t stream);
+hipError_t launch_gather_rows(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const int* index, int choices,
+                              int64_t rows, int64_t features, void* out, hipStream_t stream);
+hipError_t launch_combine_rows(const void* y, int dtype, int64_t y_rows, int64_t y_stride, const int* slots,
+                               const float* weights, int64_t tokens, int choices, int64_t features, void* out,
+                               hipStream_t stream);
+hipError_t launch_combine_rows_backward(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride,
+                                        int dtype, int64_t y_rows, const int* order, const int* slots,
+                                        const float* weights, int64_t tokens, int choices, int64_t features, void* dy,
+                                        float* dweights, hipStream_t stream);
+
 }  // namespace convrot

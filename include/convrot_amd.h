@@ -615,6 +615,32 @@ int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t
                                const int32_t* index, int64_t choices, int64_t rows, int64_t N, int64_t K,
                                void* scratch, int64_t scratch_bytes, void* out, void* stream);
 
+/*
+ * What lies around the experts' linears.
+ * convrot_expert_plan: a stable order of `count` choices (a token's choices beside each other) by their
+ * expert, ids int32 or int64 (ids_bits), choices outside 0 .. experts - 1 last: order[s] is the choice at
+ * sorted place s, slots its inverse, offsets [experts + 1] each expert's first place.  experts <= 1024.
+ * workspace: convrot_expert_plan_workspace_bytes bytes of any content (none needed where that is 0).
+ * convrot_gather_rows: out[s] = x[index[s] / choices] (out of range: zeros), out [rows, features].
+ * convrot_combine_rows: out[t] = sum over c of weights[t][c] * y[slots[t][c]] (weights NULL: 1), in float32,
+ * the choices in order, rounded once; a slot outside 0 .. y_rows - 1 adds nothing.
+ * convrot_combine_rows_backward: dy[s] = weights[t][c] * dout[t] for s = slots[t][c] with order[s] = t * choices + c, dy
+ * [y_rows, features], and dweights[t][c] = <dout[t], y[slots[t][c]]> (either may be NULL; y is read for
+ * dweights alone); y_rows = tokens * choices.  Sums in a fixed order.
+ */
+int64_t convrot_expert_plan_workspace_bytes(int64_t count, int64_t experts);
+int convrot_expert_plan(const void* ids, int ids_bits, int64_t count, int64_t experts, int32_t* offsets, int32_t* order,
+                        int32_t* slots, void* workspace, int64_t workspace_bytes, void* stream);
+int convrot_gather_rows(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const int32_t* index,
+                        int64_t choices, int64_t rows, int64_t features, void* out, void* stream);
+int convrot_combine_rows(const void* y, int dtype, int64_t y_rows, int64_t y_stride, const int32_t* slots,
+                         const float* weights, int64_t tokens, int64_t choices, int64_t features, void* out,
+                         void* stream);
+int convrot_combine_rows_backward(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int dtype,
+                                  int64_t y_rows, const int32_t* order, const int32_t* slots, const float* weights,
+                                  int64_t tokens, int64_t choices, int64_t features, void* dy, float* dweights,
+                                  void* stream);
+
 /* Thread-local message of the last failed call on this thread ("" if none). */
 const char* convrot_last_error(void);
 
