@@ -94,6 +94,10 @@ SIGNATURES = {
                                   _vp, _i64, _vp, _i64, _vp, _vp]),
     "convrot_fp8_grouped_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
                                           _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "convrot_grouped_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp,
+                                      _vp]),
+    "convrot_grouped_linear_rows_grad": (_i32, [_vp, _i32, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "convrot_grouped_linear_weight_grad": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
     "convrot_expert_plan_workspace_bytes": (_i64, [_i64, _i64]),
     "convrot_expert_plan": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
     "convrot_gather_rows": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp]),
@@ -288,7 +292,7 @@ def set_tuning(name: str, value: str | None) -> None:
     fp6_split (1/2/4: parts of each 256x256 FP6 tile past the whole rounds),
     w8a8_tile ("BMxBN", 256x256 to 64x64),
     w8a8_split (workgroups that share a W8A8 tile's K), fp8_tile ("BMxBN", 256x256 to 32x64),
-    fp8_split (workgroups that share an FP8 tile's K)."""
+    fp8_split (workgroups that share an FP8 tile's K), grouped_tile ("BMxBN", 256x256 to 32x64)."""
     check(load().convrot_set_tuning(name.encode(), None if value is None else str(value).encode()))
 
 

@@ -15,15 +15,17 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .fp8 import _check_weight, _operand, _row_stride, _weight_scales
+from .fp8 import CODES, MAX_FEATURES, Fp8Buffers, _check_weight, _operand, _row_stride, _weight_scales, quantize_fp8_weight
 from .norm import rows_of
 
 MAX_PLAN_EXPERTS = 1024
 MAX_EXPERTS = 65536
 MAX_GATHERED_BYTES = (1 << 32) - 4096
+MAX_STRIDE = 1 << 21
 
 
 class ExpertPlan(NamedTuple):
@@ -226,3 +228,169 @@ def combine_rows(rows: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor | N
     if nat.differentiated(rows, weights):
         return _CombineRows.apply(rows, weights, plan)
     return hip_combine_rows(rows, plan, weights)
+
+
+# ------------------------------------------------------------------ 16 bits, with gradients
+
+
+def _operand16(t: torch.Tensor) -> torch.Tensor:
+    """[.., K] in 16 bits as the products read it, itself or a copy: adjacent features, rows (and experts) 16-byte
+    aligned, zeros from K to the next multiple of 8."""
+    k = t.shape[-1]
+    if k % 8 == 0 and t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        stride = _stride16(t)
+        if (t.stride(-1) == 1 and stride % 8 == 0 and k <= stride <= MAX_STRIDE
+                and (t.ndim == 2 or t.shape[0] == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= 0))):
+            return t
+    padded = t.new_zeros((*t.shape[:-1], (k + 7) // 8 * 8))
+    padded[..., :k] = t
+    return padded
+
+
+def _stride16(t: torch.Tensor) -> int:
+    """Elements between rows (the stride of a single row says nothing)."""
+    return t.stride(-2) if t.shape[-2] > 1 else (t.shape[-1] + 7) // 8 * 8
+
+
+def _expert_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _check_grouped(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gather: bool) -> _Rows:
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"experts' linears take float16 or bfloat16, got {x.dtype}")
+    if weight.ndim != 3 or weight.dtype != x.dtype:
+        raise ValueError(f"experts' weights must be {x.dtype} [E, N, K], got {weight.dtype} {tuple(weight.shape)}")
+    _, n, k = weight.shape
+    if not (1 <= n <= MAX_FEATURES and 1 <= k <= MAX_FEATURES):
+        raise ValueError(f"experts' linears support 1 to {MAX_FEATURES} features, got N={n} K={k}")
+    r = _grouped_rows(x, weight.shape[0], plan, gather)
+    if x.shape[1] != k:
+        raise ValueError(f"experts' weights take K={k} features, got {x.shape[1]}")
+    nat.on_device(x, weight, r.offsets, r.index)
+    return r
+
+
+def hip_grouped_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, gather: bool = False) -> torch.Tensor:
+    """Sorted rows x [R, K] (or with `gather` tokens' rows x [T, K], read in the plan's order), float16 or
+    bfloat16, each times its expert's weight of [E, N, K] -> [R, N]; float32 sums, rounded once.  Rows of no
+    expert give zeros.  Features no multiple of 8 copy operands into padded rows."""
+    r = _check_grouped(x, weight, plan, gather)
+    experts, n, k = weight.shape
+    x, w = _operand16(x), _operand16(weight)
+    if r.index is not None and x.shape[0] * _stride16(x) * 2 > MAX_GATHERED_BYTES:
+        x, r = _operand16(_gather_rows(x[:, :k], r.index, r.choices)), r._replace(index=None, choices=1)
+    out = torch.empty((r.rows, n), dtype=x.dtype, device=x.device)
+    with nat.on(x.device):
+        nat.check(nat.load().convrot_grouped_linear(
+            x.data_ptr(), nat.dtype_code(x.dtype), x.shape[0], _stride16(x), w.data_ptr(), _stride16(w), _expert_stride(w),
+            r.offsets.data_ptr(), experts, nat.address(r.index), r.choices, r.rows, n, k, out.data_ptr(),
+            nat.stream_handle(x.device)))
+    return out
+
+
+def hip_grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *,
+                                gather: bool = False, rows_grad: bool = True, weight_grad: bool = True):
+    """Gradients of hip_grouped_linear from dy [R, N]: (dx of x's shape, dweight [E, N, K]), either None where not
+    wanted; float32 sums in a fixed order, rounded once (with `gather` a token's dx is the float32 sum of its
+    choices' gradients, each rounded)."""
+    r = _check_grouped(x, weight, plan, gather)
+    experts, n, k = weight.shape
+    if tuple(dy.shape) != (r.rows, n) or dy.dtype != x.dtype:
+        raise ValueError(f"dy must be {x.dtype} {(r.rows, n)}, got {dy.dtype} {tuple(dy.shape)}")
+    if gather and rows_grad:
+        _combine_checks(dy, plan, None)
+    nat.on_device(dy, x)
+    lib, code, device = nat.load(), nat.dtype_code(x.dtype), x.device
+    g = _operand16(dy)
+    dx = dw = None
+    if rows_grad:
+        w = _operand16(weight)
+        dx = torch.empty((r.rows, k), dtype=x.dtype, device=device)
+        with nat.on(device):
+            nat.check(lib.convrot_grouped_linear_rows_grad(
+                g.data_ptr(), code, _stride16(g), w.data_ptr(), _stride16(w), _expert_stride(w), r.offsets.data_ptr(),
+                experts, r.rows, n, k, dx.data_ptr(), nat.stream_handle(device)))
+        if gather:
+            dx = hip_combine_rows(dx, plan)
+    if weight_grad:
+        rows = _operand16(_gather_rows(x, r.index, r.choices) if gather else x)
+        wide = k if n * k % 8 == 0 or experts == 1 else (k + 7) // 8 * 8  # every expert's gradient 16-byte aligned
+        dw = torch.empty((experts, n, wide), dtype=x.dtype, device=device)
+        with nat.on(device):
+            nat.check(lib.convrot_grouped_linear_weight_grad(
+                g.data_ptr(), code, _stride16(g), rows.data_ptr(), _stride16(rows), r.offsets.data_ptr(), experts, r.rows, n,
+                wide, dw.data_ptr(), nat.stream_handle(device)))
+        dw = dw[..., :k].contiguous()
+    return dx, dw
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, plan, gather):
+        ctx.save_for_backward(x, weight, *plan)
+        ctx.gather = gather
+        return hip_grouped_linear(x, weight, plan, gather=gather)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, *plan = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        dx, dw = hip_grouped_linear_backward(dy, x, weight, ExpertPlan(*plan), gather=ctx.gather, rows_grad=needs[0],
+                                             weight_grad=needs[1])
+        return dx, dw, None, None
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, gather: bool = False) -> torch.Tensor:
+    """hip_grouped_linear, with gradients for the rows and the weights (reverse mode; dual tensors of forward
+    mode are refused)."""
+    if nat.differentiated(x, weight):
+        return _GroupedLinear.apply(x, weight, plan, gather)
+    return hip_grouped_linear(x, weight, plan, gather=gather)
+
+
+class ExpertLinear(nn.Module):
+    """The dense linears of E experts: `weight` [E, N, K] (no bias), called on rows sorted by an ExpertPlan, or
+    with gather=True on the tokens' rows.  Parameters start as torch's Linear starts its weight."""
+
+    def __init__(self, experts: int, in_features: int, out_features: int, *, device=None, dtype=torch.bfloat16):
+        super().__init__()
+        self.weight = nn.Parameter(torch.empty((experts, out_features, in_features), device=device, dtype=dtype))
+        nn.init.uniform_(self.weight, -in_features ** -0.5, in_features ** -0.5)
+
+    def forward(self, x: torch.Tensor, plan: ExpertPlan, *, gather: bool = False) -> torch.Tensor:
+        return grouped_linear(x, self.weight, plan, gather=gather)
+
+    def extra_repr(self) -> str:
+        experts, n, k = self.weight.shape
+        return f"experts={experts}, in_features={k}, out_features={n}"
+
+
+class Fp8ExpertLinear(Fp8Buffers):
+    """The linears of E experts stored and executed in 8-bit floating point: `qweight` float8_e4m3fn [E, N, K],
+    `scales` float32 [E, ceil(N / 128), ceil(K / 128)] (ones); no bias and no gradient: a backward pass that reaches
+    it raises an error."""
+
+    def __init__(self, experts: int, in_features: int, out_features: int, *, device=None):
+        super().__init__()
+        blocks = (out_features + 127) // 128, (in_features + 127) // 128
+        self.register_buffer("qweight", torch.zeros((experts, out_features, in_features), dtype=torch.uint8,
+                                                    device=device).view(CODES))
+        self.register_buffer("scales", torch.ones((experts, *blocks), dtype=torch.float32, device=device))
+
+    def load_weight(self, weight: torch.Tensor) -> Fp8ExpertLinear:
+        """Quantize dense weights [E, N, K] into this layer."""
+        if weight.shape != self.qweight.shape:
+            raise ValueError(f"weight must have shape {tuple(self.qweight.shape)}, got {tuple(weight.shape)}")
+        self.qweight, self.scales = quantize_fp8_weight(weight)
+        return self
+
+    def forward(self, x: torch.Tensor, plan: ExpertPlan, *, gather: bool = False) -> torch.Tensor:
+        return hip_fp8_grouped_linear(x, self.qweight, self.scales, plan, gather=gather)
+
+    def extra_repr(self) -> str:
+        experts, n, k = self.qweight.shape
+        return f"experts={experts}, in_features={k}, out_features={n}"

@@ -212,7 +212,21 @@ def hip_fp8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor
         "hip_fp8_linear", x, wscales, bias, residual, gate, target=residual if inplace else None)
 
 
-class Fp8Linear(nn.Module):
+class Fp8Buffers(nn.Module):
+    """A module whose buffers hold codes and their float32 scales (and bias)."""
+
+    def _apply(self, fn, recurse=True):
+        # .half(), .bfloat16() and .to(dtype) cast parameters and buffers of floating types: the codes and
+        # their scales stay what they are and only move
+        kept = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
+
+class Fp8Linear(Fp8Buffers):
     """A linear layer stored and executed in 8-bit floating point: `qweight` float8_e4m3fn [N, K], `scales`
     float32 [ceil(N / 128), ceil(K / 128)] (ones), `bias` float32 [N] (zeros); the output type is the input
     type.  It has forward and forward_modulated, each with residual=, gate= and inplace=, and no gradient: a
@@ -229,16 +243,6 @@ class Fp8Linear(nn.Module):
                                                   device=device))
         self.register_buffer("bias", torch.zeros((out_features,), dtype=torch.float32, device=device))
         self.source_has_bias = bias
-
-    def _apply(self, fn, recurse=True):
-        # .half(), .bfloat16() and .to(dtype) cast parameters and buffers of floating types: the codes and
-        # their scales stay what they are and only move
-        kept = {name: self._buffers[name] for name in ("qweight", "scales", "bias")}
-        super()._apply(fn, recurse)
-        for name, t in kept.items():
-            if self._buffers[name].dtype != t.dtype:
-                self._buffers[name] = t.to(self._buffers[name].device)
-        return self
 
     def load_weight(self, weight: torch.Tensor, bias: torch.Tensor | None = None) -> Fp8Linear:
         """Quantize a dense (out, in) weight into this layer."""

@@ -12,7 +12,7 @@
 #include <atomic>
 
 #include "convrot_launch.h"
-#include "fp8_device.h"
+#include "gemm_groups.h"
 
 namespace convrot {
 namespace {
@@ -101,7 +101,8 @@ int convrot_set_tuning(const char* name, const char* value) {
                 {"fp6_tile", kTuneFp6Tile},           {"linear_rows_cfg", kTuneRowsCfg},
                 {"w4a4_midm_cfg", kTuneMidmCfg},      {"fp6_split", kTuneFp6Split},
                 {"w8a8_tile", kTuneW8a8Tile},         {"w8a8_split", kTuneW8a8Split},
-                {"fp8_tile", kTuneFp8Tile},           {"fp8_split", kTuneFp8Split}};
+                {"fp8_tile", kTuneFp8Tile},           {"fp8_split", kTuneFp8Split},
+                {"grouped_tile", kTuneGroupedTile}};
   int key = -1;
   for (const auto& n : kNames)
     if (strcmp(n.name, name) == 0) key = n.key;
@@ -121,6 +122,7 @@ int convrot_set_tuning(const char* name, const char* value) {
       case kTuneFp6Tile:
       case kTuneW8a8Tile:
       case kTuneFp8Tile:
+      case kTuneGroupedTile:
       case kTuneW4a16Tile: {
         int bm = 0, bn = 0;
         char tail = 0;
@@ -128,6 +130,7 @@ int convrot_set_tuning(const char* name, const char* value) {
                (key == kTuneFp6Tile    ? fp6_tile_known(bm, bn)
                 : key == kTuneW8a8Tile ? w8a8_tile_known(bm, bn)
                 : key == kTuneFp8Tile  ? fp8_tile_known(bm, bn)
+                : key == kTuneGroupedTile ? grouped_tile_known(bm, bn)
                                        : w4a16_tile_known(bm, bn));
         v = bm | bn << 10;
         break;
@@ -1331,6 +1334,87 @@ int convrot_combine_rows_backward(const void* dout, int64_t dout_stride, const v
                                                              weights, tokens, (int)choices, features, dy, dweights,
                                                              (hipStream_t)stream),
                        "convrot_combine_rows_backward");
+}
+
+// ---- grouped products in 16 bits
+
+namespace {
+
+// Checks of the operands of `rows` rows in 16 bits: [.., features], 16-byte aligned rows that cover them
+// rounded up to 8.
+int check_rows16(const char* what, const void* p, int64_t stride, int64_t features) {
+  if (!p) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (!aligned(p, 16) || stride % 8 || stride < (features + 7) / 8 * 8)
+    return fail(CONVROT_ERR_INVALID, "%s needs 16-byte aligned rows that cover %lld features rounded up to 8, got a stride of %lld",
+                what, (long long)features, (long long)stride);
+  if (stride * 2 > kMaxInt8Stride)
+    return fail(CONVROT_ERR_UNSUPPORTED, "row strides are limited to %lld elements", (long long)(kMaxInt8Stride / 2));
+  return ok();
+}
+
+int check_grouped(int dtype, const int32_t* offsets, int64_t experts, const int32_t* index, int64_t choices,
+                  int64_t x_rows, int64_t rows, int64_t N, int64_t K) {
+  if (dtype != CONVROT_DTYPE_F16 && dtype != CONVROT_DTYPE_BF16)
+    return fail(CONVROT_ERR_INVALID, "grouped products take float16 or bfloat16, got dtype code %d", dtype);
+  if (N < 1 || K < 1 || rows < 0)
+    return fail(CONVROT_ERR_INVALID, "invalid grouped product rows=%lld N=%lld K=%lld", (long long)rows, (long long)N,
+                (long long)K);
+  if (N > kMaxFeatures || K > kMaxFeatures)
+    return fail(CONVROT_ERR_UNSUPPORTED, "grouped products support up to %lld features, got N=%lld K=%lld",
+                (long long)kMaxFeatures, (long long)N, (long long)K);
+  if (rows > 0x7ffffe00) return fail(CONVROT_ERR_UNSUPPORTED, "GEMM dimension too large");
+  return check_groups(offsets, experts, index, choices, x_rows, rows);
+}
+
+}  // namespace
+
+int convrot_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* weight,
+                           int64_t weight_stride, int64_t weight_expert, const int32_t* offsets, int64_t experts,
+                           const int32_t* index, int64_t choices, int64_t rows, int64_t N, int64_t K, void* out,
+                           void* stream) {
+  if (int rc = check_grouped(dtype, offsets, experts, index, choices, x_rows, rows, N, K)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_rows16("x", x, x_stride, K)) return rc;
+  if (int rc = check_rows16("weight", weight, weight_stride, K)) return rc;
+  if (weight_expert < 0 || weight_expert % 8 || !out || !aligned(out, 16))
+    return fail(CONVROT_ERR_INVALID, "experts' weights and out must be 16-byte aligned");
+  if (index && (x_rows == 0 || (x_rows - 1) * x_stride * 2 + (K + 7) / 8 * 16 > convrot::kMaxExtent))
+    return fail(CONVROT_ERR_UNSUPPORTED, "rows read through an index support 1 to 2^32 bytes, got %lld rows %lld apart",
+                (long long)x_rows, (long long)x_stride);
+  const convrot::GroupedOperands p{(const uint16_t*)x, (const uint16_t*)weight, x_stride, weight_stride, weight_expert,
+                                   (uint16_t*)out, (int)rows, (int)N, (int)K,
+                                   {offsets, index, (int)experts, (int)choices, x_rows}};
+  return launch_status(convrot::launch_grouped(index ? 1 : 0, p, dtype, (hipStream_t)stream), "convrot_grouped_linear");
+}
+
+int convrot_grouped_linear_rows_grad(const void* dy, int dtype, int64_t dy_stride, const void* weight,
+                                     int64_t weight_stride, int64_t weight_expert, const int32_t* offsets,
+                                     int64_t experts, int64_t rows, int64_t N, int64_t K, void* dx, void* stream) {
+  if (int rc = check_grouped(dtype, offsets, experts, nullptr, 1, rows, rows, N, K)) return rc;
+  if (rows == 0) return ok();
+  if (int rc = check_rows16("dy", dy, dy_stride, N)) return rc;
+  if (int rc = check_rows16("weight", weight, weight_stride, K)) return rc;
+  if (weight_expert < 0 || weight_expert % 8 || !dx || !aligned(dx, 16))
+    return fail(CONVROT_ERR_INVALID, "experts' weights and dx must be 16-byte aligned");
+  const convrot::GroupedOperands p{(const uint16_t*)dy, (const uint16_t*)weight, dy_stride, weight_stride, weight_expert,
+                                   (uint16_t*)dx, (int)rows, (int)K, (int)N, {offsets, nullptr, (int)experts, 1, rows}};
+  return launch_status(convrot::launch_grouped(2, p, dtype, (hipStream_t)stream), "convrot_grouped_linear_rows_grad");
+}
+
+int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_stride, const void* x, int64_t x_stride,
+                                       const int32_t* offsets, int64_t experts, int64_t rows, int64_t N, int64_t K,
+                                       void* dw, void* stream) {
+  if (int rc = check_grouped(dtype, offsets, experts, nullptr, 1, rows, rows, N, K)) return rc;
+  if (!dw || !aligned(dw, 16) || (experts > 1 && N * K % 8))
+    return fail(CONVROT_ERR_INVALID, "dw must be 16-byte aligned, each expert's too (N=%lld K=%lld)", (long long)N, (long long)K);
+  if (!offsets) return fail(CONVROT_ERR_INVALID, "null pointer argument");
+  if (rows > 0) {
+    if (int rc = check_rows16("dy", dy, dy_stride, N)) return rc;
+    if (int rc = check_rows16("x", x, x_stride, K)) return rc;
+  }
+  const convrot::GroupedOperands p{(const uint16_t*)dy, (const uint16_t*)x, dy_stride, x_stride, 0, (uint16_t*)dw, (int)rows,
+                                   (int)N, (int)K, {offsets, nullptr, (int)experts, 1, rows}};
+  return launch_status(convrot::launch_grouped(3, p, dtype, (hipStream_t)stream), "convrot_grouped_linear_weight_grad");
 }
 
 }  // extern "C"

@@ -35,6 +35,7 @@ enum TuneKey : int {
   kTuneW8a8Split,        // workgroups that share a W8A8 tile's K
   kTuneFp8Tile,          // FP8 tile: bm | bn << 10
   kTuneFp8Split,         // workgroups that share an FP8 tile's K
+  kTuneGroupedTile,      // tile of the grouped 16-bit products: bm | bn << 10
   kTuneCount
 };
 int tuning(TuneKey key);
@@ -51,6 +52,8 @@ bool fp6_tile_known(int bm, int bn);
 bool w4a16_tile_known(int bm, int bn);
 bool w8a8_tile_known(int bm, int bn);
 bool fp8_tile_known(int bm, int bn);
+bool grouped_tile_known(int bm, int bn);         // of rows
+bool grouped_weight_tile_known(int bm, int bn);  // of the weights' gradient
 
 // The FP6 W4A4 tile the plan (and the fp6_tile override) picks for M x N on operand
 // blocks, and on compact weights, where each 256 x 256 tile past the whole rounds
@@ -274,6 +277,9 @@ hipError_t launch_fp8_gemm(const Fp8Operands& p, int out_dtype, hipStream_t stre
 
 // Workspace that launch_fp8_gemm uses for a shape (0: none), in the places of the W8A8 product's.
 int64_t fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
+struct GroupedOperands;  // gemm_groups.h
+hipError_t launch_grouped(int kind, const GroupedOperands& p, int dtype, hipStream_t stream);
 
 // ---- the linears of a mixture of experts: what lies around them (experts.hip)
 

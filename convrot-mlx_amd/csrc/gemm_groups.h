@@ -71,4 +71,24 @@ inline int64_t most_tile_rows(int64_t rows, int64_t experts, int bm) {
   return rows < bound ? rows : bound;
 }
 
+// What a launch computes: KIND 0 forward on sorted rows, 1 on rows read through the index, 2 the rows' gradient,
+// 3 the weights'.
+struct GroupedOperands {
+  const uint16_t *rows, *other;  // x (or dy); the weights, or (KIND 3) x beside dy
+  int64_t ld_rows, ld_other;     // elements between rows
+  int64_t expert;                // elements between experts' weights
+  uint16_t* out;
+  int R;                         // sorted rows
+  int N, C;                      // columns of the output, length contracted (KIND 3: rows and columns of a weight, N x C)
+  Groups g;
+};
+
+// The tiled product of one type (gemm_grouped_tile.h, one source a type).
+template <int DT>
+hipError_t launch_grouped_tile(int tile, int kind, const GroupedOperands& p, hipStream_t stream);
+
+// The tiles built: BM, BN, ring stages, workgroups a CU; for rows, and for the weights' gradient.
+#define GROUPED_TILES(X) X(256, 256, 2, 1) X(128, 128, 2, 2) X(64, 128, 3, 2) X(32, 64, 6, 2)
+#define GROUPED_WEIGHT_TILES(X) X(256, 256, 2, 1) X(128, 128, 2, 2)
+
 }  // namespace convrot

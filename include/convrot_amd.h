@@ -616,6 +616,28 @@ int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t
                                void* scratch, int64_t scratch_bytes, void* out, void* stream);
 
 /*
+ * The experts' linears in 16 bits (float16 or bfloat16; float32 sums, one rounding), groups as in
+ * convrot_fp8_grouped_linear:
+ *   out[s] = x[row(s)] W_e^T        (rows of no expert: zeros; x through an index: at most 2^32 - 4096 bytes)
+ *   dx[s]  = dy[s] W_e              (rows of no expert: zeros)
+ *   dw[e]  = sum over expert e's rows s of dy[s]^T x[s]   (an expert without rows: zeros)
+ * x, dy and weight: 16-byte aligned rows, strides (elements) that are multiples of 8 and cover the features
+ * rounded up to 8, zeros from there on; weight e at weight + e * weight_expert elements.  out [rows, N],
+ * dx [rows, K], dw [experts, N, K] contiguous (several experts' dw: N K a multiple of 8).  Up to 65536
+ * features.  The weights' gradient reads sorted rows of x (convrot_gather_rows makes them).
+ */
+int convrot_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* weight,
+                           int64_t weight_stride, int64_t weight_expert, const int32_t* offsets, int64_t experts,
+                           const int32_t* index, int64_t choices, int64_t rows, int64_t N, int64_t K, void* out,
+                           void* stream);
+int convrot_grouped_linear_rows_grad(const void* dy, int dtype, int64_t dy_stride, const void* weight,
+                                     int64_t weight_stride, int64_t weight_expert, const int32_t* offsets,
+                                     int64_t experts, int64_t rows, int64_t N, int64_t K, void* dx, void* stream);
+int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_stride, const void* x, int64_t x_stride,
+                                       const int32_t* offsets, int64_t experts, int64_t rows, int64_t N, int64_t K,
+                                       void* dw, void* stream);
+
+/*
  * What lies around the experts' linears.
  * convrot_expert_plan: a stable order of `count` choices (a token's choices beside each other) by their
  * expert, ids int32 or int64 (ids_bits), choices outside 0 .. experts - 1 last: order[s] is the choice at
@@ -670,6 +692,8 @@ const char* convrot_last_error(void);
  *   w8a8_split       "1" .. "64"          workgroups that share a W8A8 tile's K (with a workspace)
  *   fp8_tile         "BMxBN"              FP8 tile (256x256 .. 32x64)
  *   fp8_split        "1" .. "64"          workgroups that share an FP8 tile's K (with a workspace)
+ *   grouped_tile     "BMxBN"              tile of the grouped 16-bit products (256x256 .. 32x64; the weights'
+ *                                         gradient takes 256x256 and 128x128 alone)
  * Returns CONVROT_ERR_INVALID for an unknown name, a malformed value or a
  * tile the library does not build.
  */

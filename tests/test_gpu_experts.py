@@ -280,3 +280,306 @@ def test_fp8_rows_past_32_bits(dev):
             want, spread = plain.product(v[None], plain.weight_values(q[e], ws[e]), False)
             assert_within(got[at][None], want, spread)
         assert int(got.any(1).sum()) == len(rows)
+
+
+# ------------------------------------------------------------------ the products in 16 bits
+
+
+def product16(a, b, length):
+    """a [M, C] b [N, C]^T in 64 bits, and what float32 sums may add: a chain of at most `length` additions."""
+    return a @ b.t().contiguous(), U * (length + 8) * (a.abs() @ b.abs().t().contiguous())
+
+
+GROUPS16 = [(1, 1, 1, 8, 8), (3, 2, 5, 70, 144), (8, 2, 16, 256, 512), (40, 1, 3, 130, 61), (64, 4, 70, 96, 256),
+            (129, 2, 4, 300, 400), (700, 1, 2, 264, 72), (300, 3, 9, 515, 333), (16, 2, 300, 64, 136), (600, 2, 2, 520, 264)]
+
+
+def check_products(dev, tokens, choices, experts, n, k, dtype, gather, seed=0):
+    from convrot_mlx_amd import expert_plan, hip_grouped_linear, hip_grouped_linear_backward
+
+    ids = choose(n + seed, tokens, choices, experts)
+    plan = expert_plan(ids.to(dev), experts)
+    w = normal(n, experts, n, k).to(dtype).to(dev)
+    x = normal(k, tokens if gather else tokens * choices, k).to(dtype).to(dev)
+    dy = normal(k + 1, tokens * choices, n).to(dtype).to(dev)
+    at = plan.offsets.tolist()
+    dy[at[-1]:] = float("nan")  # rows of no expert reach nothing but themselves
+    got = hip_grouped_linear(x, w, plan, gather=gather)
+    dx, dw = hip_grouped_linear_backward(dy, x, w, plan, gather=gather)
+    assert got.dtype == dtype and got.shape == (tokens * choices, n) and dx.shape == x.shape and dw.shape == w.shape
+    rows = (x[plan.order.long() // choices] if gather else x).double()
+    want_dx, off_dx = torch.zeros((tokens * choices, k), dtype=torch.float64, device=dev), torch.zeros((tokens * choices, k), dtype=torch.float64, device=dev)
+    for e in range(experts):
+        r = slice(at[e], at[e + 1])
+        we, g = w[e].double(), dy[r].double()
+        if at[e + 1] == at[e]:
+            assert not dw[e].any()
+            continue
+        assert_within(got[r], *product16(rows[r], we, k), f"forward {e}")
+        want_dx[r], off_dx[r] = product16(g, we.t().contiguous(), n)
+        count = at[e + 1] - at[e]
+        assert_within(dw[e], *product16(g.t().contiguous(), rows[r].t().contiguous(), count), f"weights {e}")
+    assert not got[at[-1]:].any()
+    if gather:  # each choice's gradient is rounded, then they are added at float32
+        slots = plan.slots.long()
+        each, off = want_dx[slots], off_dx[slots]
+        half = {BF16: 2.0 ** -8, F16: 2.0 ** -11}[dtype]
+        tiny = {BF16: 2.0 ** -133, F16: 2.0 ** -25}[dtype]
+        assert_within(dx, each.sum(1), (half * (each.abs() + off) + off + tiny).sum(1) + U * choices * each.abs().sum(1), "rows")
+    else:
+        assert_within(dx, want_dx, off_dx, "rows")
+        assert not dx[at[-1]:].any()
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens,choices,experts,n,k", GROUPS16)
+def test_products(dev, tokens, choices, experts, n, k, dtype, gather):
+    check_products(dev, tokens, choices, experts, n, k, dtype, gather)
+
+
+@pytest.mark.parametrize("tile", ["256x256", "128x128", "64x128", "32x64"])
+@pytest.mark.parametrize("tokens,choices,experts,n,k", [(500, 2, 5, 270, 400), (600, 1, 2, 520, 264), (30, 1, 4, 64, 64)])
+def test_every_tile(dev, tuning, tile, tokens, choices, experts, n, k):
+    tuning.set("grouped_tile", tile)
+    for gather in (False, True):
+        check_products(dev, tokens, choices, experts, n, k, BF16, gather, seed=1)
+
+
+def test_operands_of_other_layouts(dev):
+    from convrot_mlx_amd import ExpertPlan, expert_plan, hip_grouped_linear, hip_grouped_linear_backward
+
+    plan = expert_plan(choose(3, 30, 2, 4).to(dev), 4)
+    for n, k in ((72, 128), (33, 41)):
+        w, x, dy = (normal(i, *s).to(F16).to(dev) for i, s in enumerate(((4, n, k), (60, k), (60, n))))
+        want = hip_grouped_linear(x, w, plan)
+        dx, dw = hip_grouped_linear_backward(dy, x, w, plan)
+        for other in (torch.cat([w, w], 2)[..., :k], torch.cat([w, w], 1)[:, :n], w.transpose(0, 1).contiguous().transpose(0, 1),
+                      w.transpose(1, 2).contiguous().transpose(1, 2)):
+            assert torch.equal(hip_grouped_linear(x, other, plan), want)
+            got = hip_grouped_linear_backward(dy, x, other, plan)
+            assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+        for view in (lambda t: torch.cat([t, t], 1)[:, t.shape[1]:], lambda t: t.t().contiguous().t(),
+                     lambda t: torch.cat([t.flatten(), t.flatten()])[t.numel():].view(t.shape)):
+            assert torch.equal(hip_grouped_linear(view(x), w, ExpertPlan(plan.offsets)), want)
+            got = hip_grouped_linear_backward(view(dy), view(x), w, plan)
+            assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+        one = hip_grouped_linear_backward(dy, x, w, plan, rows_grad=False)
+        assert one[0] is None and torch.equal(one[1], dw)
+        one = hip_grouped_linear_backward(dy, x, w, plan, weight_grad=False)
+        assert one[1] is None and torch.equal(one[0], dx)
+        same = w[:1].expand(4, -1, -1)  # one weight for all: experts 0 elements apart
+        assert torch.equal(hip_grouped_linear(x, same, plan), hip_grouped_linear(x, same.contiguous(), plan))
+
+
+def test_not_finite_rows(dev):
+    """A row's NaN or infinity reaches its own outputs, its own gradient and its expert's weight gradient alone."""
+    from convrot_mlx_amd import ExpertPlan, hip_grouped_linear, hip_grouped_linear_backward
+
+    offsets = torch.tensor([0, 37, 37, 100], dtype=torch.int32, device=dev)
+    plan = ExpertPlan(offsets)
+    w, x, dy = (normal(i, *s).to(BF16).to(dev) for i, s in enumerate(((3, 72, 136), (120, 136), (120, 72))))
+    want = hip_grouped_linear(x, w, plan), *hip_grouped_linear_backward(dy, x, w, plan)
+    x[36, 5], x[110], dy[36, 3], dy[119] = float("nan"), float("inf"), float("inf"), float("nan")
+    got = hip_grouped_linear(x, w, plan), *hip_grouped_linear_backward(dy, x, w, plan)
+    keep = [i for i in range(120) if i != 36]
+    for a, b in zip(got[:2], want[:2]):
+        assert torch.equal(a[keep], b[keep]) and not torch.isfinite(a[36]).any()
+    assert torch.equal(got[2][1:], want[2][1:]) and got[2][0].isnan().any()
+
+
+def test_offsets_and_indices_of_any_content(dev):
+    from convrot_mlx_amd import ExpertPlan, hip_grouped_linear, hip_grouped_linear_backward
+
+    w, x, dy = (normal(i, *s).to(BF16).to(dev) for i, s in enumerate(((3, 40, 128), (50, 128), (50, 40))))
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    for offsets in (i32(-5, 10, 2 ** 31 - 1, 60), i32(0, 50, 10, 20), i32(7, -1, -1, 50), i32(0, 0, 0, 0)):
+        plan = ExpertPlan(offsets)
+        assert hip_grouped_linear(x, w, plan).shape == (50, 40)
+        dx, dw = hip_grouped_linear_backward(dy, x, w, plan)
+        assert dx.shape == x.shape and dw.shape == w.shape
+    assert not hip_grouped_linear(x, w, plan).any() and not dx.any() and not dw.any()
+    order = torch.arange(100, dtype=torch.int32, device=dev)
+    order[3], order[40], order[99] = -1, 2 ** 31 - 1, 100
+    got = hip_grouped_linear(x, w, ExpertPlan(i32(0, 30, 60, 100), order), gather=True)
+    want = hip_grouped_linear(x, w, ExpertPlan(i32(0, 30, 60, 100), torch.arange(100, dtype=torch.int32, device=dev)), gather=True)
+    keep = [i for i in range(100) if i not in (3, 40, 99)]
+    assert torch.equal(got[keep], want[keep]) and not got[[3, 40, 99]].any()
+
+
+def test_no_rows_in_16_bits(dev):
+    from convrot_mlx_amd import expert_plan, hip_grouped_linear, hip_grouped_linear_backward
+
+    plan = expert_plan(torch.zeros((0, 2), dtype=torch.int32, device=dev), 3)
+    w, x = torch.ones((3, 40, 24), dtype=BF16, device=dev), torch.zeros((0, 24), dtype=BF16, device=dev)
+    for gather in (False, True):
+        assert hip_grouped_linear(x, w, plan, gather=gather).shape == (0, 40)
+        dx, dw = hip_grouped_linear_backward(torch.zeros((0, 40), dtype=BF16, device=dev), x, w, plan, gather=gather)
+        assert dx.shape == (0, 24) and dw.shape == w.shape and not dw.any()
+
+
+def test_rows_past_32_bits(dev):
+    """Tokens, sorted rows and gradients past 4 GiB."""
+    from convrot_mlx_amd import ExpertPlan, hip_grouped_linear, hip_grouped_linear_backward
+
+    k, tokens = 4096, (1 << 19) + 100
+    w = normal(1, 2, 32, k, std=0.05).to(BF16).to(dev)
+    x = torch.zeros((tokens, k), dtype=BF16, device=dev)
+    dy = torch.zeros((tokens, 32), dtype=BF16, device=dev)
+    rows = [0, 5, tokens // 2, 1 << 19, tokens - 1]
+    some, g = normal(2, len(rows), k).to(BF16).to(dev), normal(3, len(rows), 32).to(BF16).to(dev)
+    x[rows], dy[rows] = some, g
+    order = torch.arange(tokens - 1, -1, -1, dtype=torch.int32, device=dev)
+    third = tokens // 3
+    plan = ExpertPlan(torch.tensor([0, third, tokens], dtype=torch.int32, device=dev), order)
+    for gather in (True, False):
+        got = hip_grouped_linear(x, w, plan, gather=gather)
+        for row, v in zip(rows, some):
+            at = tokens - 1 - row if gather else row
+            assert_within(got[at][None], *product16(v[None].double(), w[int(at >= third)].double(), k))
+        assert int(got.any(1).sum()) == len(rows)
+    dx, dw = hip_grouped_linear_backward(dy, x, w, plan)
+    for e in range(2):
+        mine = [i for i, r in enumerate(rows) if int(r >= third) == e]
+        assert_within(dw[e], *product16(g[mine].double().t().contiguous(), some[mine].double().t().contiguous(), len(rows)))
+        assert_within(dx[[rows[i] for i in mine]], *product16(g[mine].double(), w[e].double().t().contiguous(), 32))
+    assert int(dx.any(1).sum()) == len(rows)
+
+
+# ------------------------------------------------------------------ together
+
+
+def mixture(x, ids, weights, up, down):
+    """A mixture's feed-forward layer on rows x [T, K]: up and down are called on sorted rows."""
+    from convrot_mlx_amd import combine_rows, expert_plan
+
+    plan = expert_plan(ids, up.experts)
+    h = up(x, plan, gather=True)
+    return combine_rows(down(torch.nn.functional.silu(h), plan), plan, weights)
+
+
+def layers(dev, experts, k, hidden, dtype=BF16):
+    from convrot_mlx_amd import ExpertLinear
+
+    torch.manual_seed(0)
+    up, down = ExpertLinear(experts, k, hidden, device=dev, dtype=dtype), ExpertLinear(experts, hidden, k, device=dev, dtype=dtype)
+    up.experts = experts
+    return up, down
+
+
+@pytest.mark.parametrize("tokens", [1, 37, 300])
+def test_a_mixture_and_its_gradients(dev, tokens):
+    """The layer as a user builds it, against the same in 64 bits, and its gradients against the formula's there.
+    Every 16-bit tensor between the products is off by at most half a unit (2^-9 of its value, bf16): the
+    relative errors of h, silu(h), the rows, and (backward) three more roundings add up."""
+    k, hidden, experts, choices = 136, 264, 6, 2
+    up, down = layers(dev, experts, k, hidden)
+    ids = choose(tokens, tokens, choices, experts).to(dev)
+    x = normal(1, tokens, k).to(BF16).to(dev).requires_grad_()
+    wts = torch.rand((tokens, choices), generator=torch.Generator().manual_seed(2)).to(dev).requires_grad_()
+    out = mixture(x, ids, wts, up, down)
+    dout = normal(3, tokens, k).to(BF16).to(dev)
+    leaves = (x, wts, up.weight, down.weight)
+    grads = torch.autograd.grad(out, leaves, dout)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    xd, wd, ud, dd = wide
+    ref = torch.zeros((tokens, k), dtype=torch.float64, device=dev)
+    for e in range(experts):
+        for c in range(choices):
+            at = (ids[:, c] == e).nonzero()[:, 0]
+            if len(at):
+                h = torch.nn.functional.silu(xd[at] @ ud[e].t().contiguous())
+                ref = ref.index_add(0, at, wd[at, c, None] * (h @ dd[e].t().contiguous()))
+    want = torch.autograd.grad(ref, wide, dout.double(), allow_unused=True)
+    for got, w in zip((out, *grads), (ref.detach(), *want)):
+        w = torch.zeros_like(got, dtype=torch.float64) if w is None else w
+        off = (got.detach().double() - w).norm() / w.norm().clamp_min(1e-30)
+        assert off <= 8 * 2.0 ** -8, off  # at most eight roundings of half a unit each, in any of these tensors
+
+
+def test_a_mixture_at_8_bits(dev):
+    """The same layer with its experts quantized: the layer's own calls, and near the 16-bit one."""
+    from convrot_mlx_amd import Fp8ExpertLinear, combine_rows, expert_plan, hip_fp8_grouped_linear
+
+    k, hidden, experts, tokens = 256, 384, 5, 70
+    up, down = layers(dev, experts, k, hidden)
+    ids = choose(5, tokens, 2, experts).to(dev)
+    x, wts = normal(1, tokens, k).to(BF16).to(dev), torch.rand((tokens, 2), device=dev)
+    q_up = Fp8ExpertLinear(experts, k, hidden, device=dev).load_weight(up.weight.detach())
+    q_down = Fp8ExpertLinear(experts, hidden, k, device=dev).load_weight(down.weight.detach())
+    q_up.experts = experts
+    got = mixture(x, ids, wts, q_up, q_down)
+    plan = expert_plan(ids, experts)
+    h = hip_fp8_grouped_linear(x, q_up.qweight, q_up.scales, plan, gather=True)
+    y = hip_fp8_grouped_linear(torch.nn.functional.silu(h), q_down.qweight, q_down.scales, plan)
+    assert torch.equal(got, combine_rows(y, plan, wts))
+    near = mixture(x, ids, wts, up, down).detach().double()
+    # codes are off by 2^-4 of a value at most: two operands of each of two products
+    assert (got.double() - near).norm() <= 4 * 2.0 ** -4 * near.norm()
+    moved = torch.nn.ModuleList([q_up]).half()[0]
+    assert moved.qweight.dtype == FP8 and moved.scales.dtype == F32
+    with pytest.raises(RuntimeError, match="has no gradient"):
+        q_up(x.requires_grad_(), plan, gather=True).sum().backward()
+
+
+def test_a_mixture_in_graphs(dev):
+    """Forward and backward captured and replayed, on new inputs in the same memory, beside eager calls and on
+    another stream."""
+    from convrot_mlx_amd import Fp8ExpertLinear
+
+    k, hidden, experts, tokens = 136, 264, 6, 4200
+    up, down = layers(dev, experts, k, hidden)
+    q_up = Fp8ExpertLinear(experts, k, hidden, device=dev).load_weight(up.weight.detach())
+    q_down = Fp8ExpertLinear(experts, hidden, k, device=dev).load_weight(down.weight.detach())
+    q_up.experts = experts
+    x, ids = normal(1, tokens, k).to(BF16).to(dev).requires_grad_(), choose(2, tokens, 2, experts).to(dev)
+    wts, dout = torch.rand((tokens, 2), device=dev).requires_grad_(), normal(3, tokens, k).to(BF16).to(dev)
+
+    def train():
+        out = mixture(x, ids, wts, up, down)
+        return [out.detach(), *torch.autograd.grad(out, (x, wts, up.weight, down.weight), dout)]
+
+    def serve():
+        with torch.no_grad():
+            return [mixture(x, ids, wts, q_up, q_down)]
+
+    side = torch.cuda.Stream()
+    for step in (train, serve):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step()
+        for i in range(4):
+            with torch.no_grad():
+                x.copy_(normal(10 + i, tokens, k))
+                ids.copy_(choose(10 + i, tokens, 2, experts))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(held, step()):
+                assert torch.equal(a, b)
+
+
+def test_gradients_against_differences(dev):
+    """The product is linear in the rows and in the weights: a difference along a direction is the gradient's
+    product with it, up to the roundings of the outputs."""
+    from convrot_mlx_amd import expert_plan, grouped_linear
+
+    plan = expert_plan(choose(4, 50, 2, 3).to(dev), 3)
+    w, x, dy = (normal(i, *s).to(F16).to(dev) for i, s in enumerate(((3, 40, 72), (50, 72), (100, 40))))
+    dy[int(plan.offsets[-1]):] = 0
+    wg, xg = w.clone().requires_grad_(), x.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(grouped_linear(xg, wg, plan, gather=True), (xg, wg), dy)
+    for t, grad, call in ((x, dx, lambda v: grouped_linear(v, w, plan, gather=True)), (w, dw, lambda v: grouped_linear(x, v, plan, gather=True))):
+        v = torch.randint(-1, 2, t.shape, generator=torch.Generator().manual_seed(9)).to(F16).to(dev)
+        a, b = call(t + v).double(), call(t - v).double()  # t and v: sums within half a unit of float16
+        slope = ((a - b) / 2 * dy.double()).sum()
+        want = (grad.double() * v.double()).sum()
+        size = ((a.abs() + b.abs()) * dy.double().abs()).sum()
+        # the outputs' roundings; the gradient's; and those of t + v and t - v, through the gradient
+        bound = size + (grad.double() * v.double()).abs().sum() + 2 * (grad.double().abs() * (t.double().abs() + 1)).sum()
+        assert abs(slope - want) <= 2.0 ** -11 * bound
