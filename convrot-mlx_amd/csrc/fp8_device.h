@@ -17,6 +17,24 @@ constexpr int kBlock = 128;                      // features (and of a weight, o
 constexpr uint32_t kPastEnd = 0xffffff00u;       // buffer offset past every operand: reads zero
 constexpr int64_t kMaxExtent = 0xfffff000ll;     // bytes of an operand that is addressed as one buffer
 
+// A buffer resource for the loads below: its words may have been written by the vector unit
+// (v_readfirstlane, where the compiler cannot see that a value is uniform), after which a load may read them 5
+// wait states later at the earliest.  The compiler puts those before its own loads, not before inline asm.
+__device__ __forceinline__ i32x4_sgpr dma_rsrc(const void* base, uint32_t bytes) {
+  i32x4_sgpr r = buffer_rsrc(base, bytes);
+  asm volatile("s_nop 4" : "+s"(r));
+  return r;
+}
+// dma16 and dma4 with the wait state that a load to LDS needs behind the write of its address into M0.
+__device__ __forceinline__ void load_lds16(i32x4_sgpr rsrc, uint32_t voffset, uint32_t lds_addr) {
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)
+               : "memory");
+}
+__device__ __forceinline__ void load_lds4(i32x4_sgpr rsrc, uint32_t voffset, uint32_t lds_addr) {
+  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)
+               : "memory");
+}
+
 struct Fp8Scale {
   float inverse, scale;
 };
@@ -67,8 +85,15 @@ struct Fp8Operands {
 template <int ODT>
 hipError_t launch_fp8_tile(int tile, const Fp8Operands& p, const W8a8Split& split, hipStream_t stream);
 
-// The tiles built: BM, BN, waves along each, ring stages, workgroups a CU.
+constexpr int kMaxFp8SplitTile = 128 * 128;  // tiles up to this size may share their K between workgroups
+
+// The tiles built: BM, BN, waves along each, ring stages, workgroups a CU, and whether the MFMAs run in slots
+// (run_slots of gemm_fp8_tile.h).  In slots and not, in us: 256 x 256 (8192 x 8192 -> 8192) 468 and 540, 32 x 64 (1 row
+// 4096 -> 12288) 11.8 and 12.5, 64 x 64 (128 rows 4096 -> 4096) 12.8 and 13.3; 128 x 128 and 64 x 128, whose LDS traffic
+// bounds them, 640 and 573 (8192 x 8192 -> 8192), 29.0 and 27.0 (1024 x 4096 -> 4096).  With 8 waves 128 x 128 takes
+// 26 us there, with 4 29.9.
 #define FP8_TILES(X) \
-  X(256, 256, 4, 2, 2, 1) X(256, 128, 4, 2, 3, 1) X(128, 128, 2, 2, 2, 2) X(64, 128, 2, 2, 3, 2) X(32, 64, 1, 4, 5, 2)
+  X(256, 256, 4, 2, 2, 1, true) X(128, 128, 2, 4, 2, 2, false) X(64, 128, 2, 4, 3, 2, false) X(64, 64, 2, 2, 4, 2, true) \
+  X(32, 64, 1, 4, 5, 2, true)
 
 }  // namespace convrot

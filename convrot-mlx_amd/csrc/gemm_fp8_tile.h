@@ -39,7 +39,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxBlocks = 512;  // K up to 65536
 
-template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU>
+template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, bool IN_SLOTS>
 struct Fp8Engine {
   static constexpr int NW = WM * WN, THREADS = NW * 64;
   static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
@@ -87,7 +87,7 @@ struct Fp8Engine {
     tail = rest ? k16 >> 7 : ~0u;
     const int mrows = min(BM, row_end - m0), nrows = min(BN, p.N - n0);
     const int rl = lane >> 3, c = lane & 7;
-    rw = buffer_rsrc(p.weight + (int64_t)expert * p.weight_expert + (int64_t)n0 * p.ldw,
+    rw = dma_rsrc(p.weight + (int64_t)expert * p.weight_expert + (int64_t)n0 * p.ldw,
                      (uint32_t)(nrows - 1) * (uint32_t)p.ldw + k16);
 #pragma unroll
     for (int i = 0; i < BPW; ++i) {
@@ -97,7 +97,7 @@ struct Fp8Engine {
     xs_block = p.xs_block;
     const int xr = wave * 64 + lane;  // the row whose scale this lane moves
     if constexpr (GATHER) {
-      ra = buffer_rsrc(p.act, (uint32_t)((p.g.act_rows - 1) * p.lda) + k16);
+      ra = dma_rsrc(p.act, (uint32_t)((p.g.act_rows - 1) * p.lda) + k16);
 #pragma unroll
       for (int i = 0; i < APW; ++i) {
         const int piece = wave * APW + i;
@@ -109,7 +109,7 @@ struct Fp8Engine {
       xs_base = p.xscales;
       xs_bytes = (uint32_t)((p.g.act_rows - 1) * p.xs_row) * 4u + 4u;
     } else {
-      ra = buffer_rsrc(p.act + (int64_t)m0 * p.lda, (uint32_t)(mrows - 1) * (uint32_t)p.lda + k16);
+      ra = dma_rsrc(p.act + (int64_t)m0 * p.lda, (uint32_t)(mrows - 1) * (uint32_t)p.lda + k16);
 #pragma unroll
       for (int i = 0; i < APW; ++i) {
         const int piece = wave * APW + i;
@@ -135,7 +135,7 @@ struct Fp8Engine {
     const float* base = p.wscales + (int64_t)expert * p.ws_expert + (int64_t)(n0 / kBlock) * p.ws_row;
     for (int d = wave; d < nb * pieces; d += NW) {
       const int j = d / pieces, at = d - j * pieces;
-      dma4(buffer_rsrc(base + j * p.ws_row, (uint32_t)blocks * 4u), (uint32_t)(at * 256 + lane * 4),
+      load_lds4(dma_rsrc(base + j * p.ws_row, (uint32_t)blocks * 4u), (uint32_t)(at * 256 + lane * 4),
            smem_addr + (uint32_t)(WS_OFF + d * 256));
     }
   }
@@ -147,21 +147,32 @@ struct Fp8Engine {
     for (int i = 0; i < APW; ++i) {
       uint32_t off = va[i] == kPastEnd ? kPastEnd : va[i] + k;
       if (last) off = past_a[i & 1] ? kPastEnd : off;
-      dma16(ra, off, base + (uint32_t)(wave * APW + i) * 1024u);
+      load_lds16(ra, off, base + (uint32_t)(wave * APW + i) * 1024u);
     }
 #pragma unroll
     for (int i = 0; i < BPW; ++i) {
       uint32_t off = vw[i] + k;
       if (last) off = past_w[i & 1] ? kPastEnd : off;
-      dma16(rw, off, base + (uint32_t)BM * 128u + (uint32_t)(wave * BPW + i) * 1024u);
+      load_lds16(rw, off, base + (uint32_t)BM * 128u + (uint32_t)(wave * BPW + i) * 1024u);
     }
-    dma4(buffer_rsrc(xs_base + (int64_t)kb * xs_block, xs_bytes), vx, base + (uint32_t)XS_OFF + (uint32_t)wave * 256u);
+    load_lds4(dma_rsrc(xs_base + (int64_t)kb * xs_block, xs_bytes), vx, base + (uint32_t)XS_OFF + (uint32_t)wave * 256u);
   }
 
   __device__ __forceinline__ i32x8 fragment(const uint8_t* row) const {
     const int r = lane & 15, q = lane >> 4, sw = chunk_swizzle(r);
     const i32x4 lo = *(const i32x4*)(row + ((2 * q) ^ sw) * 16), hi = *(const i32x4*)(row + ((2 * q + 1) ^ sw) * 16);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+
+  __device__ __forceinline__ i32x8 a_fragment(int stage, int fm) const {
+    return fragment(smem + stage * STAGE_BYTES + (wm * TM + fm * 16 + (lane & 15)) * 128);
+  }
+  __device__ __forceinline__ i32x8 w_fragment(int stage, int fn) const {
+    return fragment(smem + stage * STAGE_BYTES + BM * 128 + (wn * TN + fn * 16 + (lane & 15)) * 128);
+  }
+  // The scale of the lane's row of fragment fm.
+  __device__ __forceinline__ float xscale(int stage, int fm) const {
+    return *(const float*)(smem + stage * STAGE_BYTES + XS_OFF + (wm * TM + fm * 16 + (lane & 15)) * 4);
   }
 
   // The 32 codes of a fragment as bf16 (exact).
@@ -183,29 +194,25 @@ struct Fp8Engine {
     return w;
   }
 
-  // acc += the scaled products of one block.  WIDE: on bf16 MFMAs, whose sums are float32's own (what
-  // the FP8 form keeps of a sum is stated above).
+  // acc += the scaled products of one block.  WIDE (float32 outputs): on bf16 MFMAs, whose sums are float32's own.
   template <bool WIDE>
   __device__ __forceinline__ void block(int stage, float ws, f32x4 (&acc)[FN][FM]) const {
-    const uint8_t* base = smem + stage * STAGE_BYTES;
-    const uint8_t* sa = base + (wm * TM + (lane & 15)) * 128;
-    const uint8_t* sw = base + BM * 128 + (wn * TN + (lane & 15)) * 128;
-    const float* xs = (const float*)(base + XS_OFF) + wm * TM + (lane & 15);
     using Frag = std::conditional_t<WIDE, Wide, i32x8>;
+    const auto as = [](const i32x8& c) __attribute__((always_inline)) {
+      if constexpr (WIDE) return widen(c);
+      else return c;
+    };
     Frag a[FM];
     float s[FM];
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
-      if constexpr (WIDE) a[fm] = widen(fragment(sa + fm * 2048));
-      else a[fm] = fragment(sa + fm * 2048);
-      s[fm] = xs[fm * 16] * ws;
+      a[fm] = as(a_fragment(stage, fm));
+      s[fm] = xscale(stage, fm) * ws;
     }
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int fn = 0; fn < FN; ++fn) {
-      Frag w;
-      if constexpr (WIDE) w = widen(fragment(sw + fn * 2048));
-      else w = fragment(sw + fn * 2048);
+      const Frag w = as(w_fragment(stage, fn));
 #pragma unroll
       for (int fm = 0; fm < FM; ++fm) {
         f32x4 part = zero;
@@ -221,11 +228,9 @@ struct Fp8Engine {
     }
   }
 
-  // acc += the products of blocks kb0 .. kb0 + n - 1, n >= 1.
   template <bool WIDE>
-  __device__ __forceinline__ void run(uint32_t kb0, int n, int ws_stride, f32x4 (&acc)[FN][FM]) {
+  __device__ __forceinline__ void run_blocks(uint32_t kb0, int n, const float* ws, f32x4 (&acc)[FN][FM]) const {
     const uint32_t last = kb0 + (uint32_t)n - 1;
-    const float* ws = (const float*)(smem + WS_OFF) + (WS > 1 ? wn * TN / kBlock * ws_stride : 0);
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) issue(min(kb0 + s, last), s);
     int st = 0;
@@ -239,6 +244,85 @@ struct Fp8Engine {
       block<WIDE>(st, ws[kb], acc);
       st = st + 1 == STAGES ? 0 : st + 1;
     }
+  }
+
+  // The same for 16-bit outputs, with the instructions in an order of their own.  Slot (fn, fm) of a block is an MFMA, and beside it the FMAs of the MFMA LAG slots
+  // before, whose results are there by then, and a fragment read: of the next fn's weights, and in the last
+  // fn of the next block's activations, each into the registers that its slot has just used.  Before that
+  // last fn the wave has read all of its block: a barrier there frees the block's stage, which the DMA of
+  // block kb + STAGES fills, and publishes block kb + 1.  (Left to the compiler's order, every MFMA is waited for by
+  // its FMAs, and the other waves of the SIMD have to fill the gap: with two of them, of 256 x 256 tiles, they
+  // do not.)
+  __device__ __forceinline__ void run_slots(uint32_t kb0, int n, const float* ws, f32x4 (&acc)[FN][FM]) const {
+    constexpr int LAG = FM - 1, SLOTS = FN * FM;
+    const uint32_t last = kb0 + (uint32_t)n - 1;
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) issue(min(kb0 + s, last), s);
+    wait_vmcnt<(STAGES - 1) * LPW>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    i32x8 a[FM], w[2];
+    float xs[FM], s[FM], wsv = ws[kb0];
+    f32x4 part[FM];
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    w[0] = w_fragment(0, 0);
+#pragma unroll
+    for (int fm = 0; fm < FM; ++fm) {
+      a[fm] = a_fragment(0, fm);
+      xs[fm] = xscale(0, fm);
+      s[fm] = 0.0f;
+      part[fm] = zero;
+    }
+    int st = 0;
+    for (uint32_t kb = kb0; kb <= last; ++kb) {
+      const int nst = st + 1 == STAGES ? 0 : st + 1;
+      // weights of fn = 0 lie in w[0] at the start of a block, so an odd FN would need them to change places
+      static_assert(FN == 1 || FN % 2 == 0, "fragments in turn");
+      static_for<SLOTS>([&](auto slot) __attribute__((always_inline)) {
+        constexpr int t = slot.value, fn = t / FM, fm = t % FM;
+        if constexpr (fn == FN - 1 && fm == 0) {
+          wait_vmcnt<(STAGES - 2) * LPW>();
+          __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          // past the last block: the last one again, into stages nothing reads
+          issue(min(kb + STAGES, last), st);
+        }
+        if constexpr (fm == 0 && FN > 1) w[(fn + 1) & 1] = fn + 1 < FN ? w_fragment(st, fn + 1) : w_fragment(nst, 0);
+        const f32x4 now = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[FN > 1 ? fn & 1 : 0], a[fm], zero, 0, 0, 0, 0, 0, 0);
+        // the MFMA of LAG slots before (of the block before, in the first ones)
+        constexpr int of = (fm + FM - LAG) % FM, on = t >= LAG ? (t - LAG) / FM : FN - 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[on][of][j] = __builtin_fmaf(part[of][j], s[of], acc[on][of][j]);
+        if constexpr (fn == 0) {
+          if constexpr (LAG > 0 && fm < LAG) s[of] = xs[of] * wsv;
+          if constexpr (fm == 0) s[0] = xs[0] * wsv;
+        }
+        part[fm] = now;
+        if constexpr (fn == FN - 1) {
+          if constexpr (fm == 0) wsv = ws[min(kb + 1, last)];
+          a[fm] = a_fragment(nst, fm);
+          xs[fm] = xscale(nst, fm);
+          if constexpr (FN == 1 && fm == FM - 1) w[0] = w_fragment(nst, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      st = nst;
+    }
+#pragma unroll
+    for (int i = 0; i < LAG; ++i) {
+      const int of = FM - LAG + i;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[FN - 1][of][j] = __builtin_fmaf(part[of][j], s[of], acc[FN - 1][of][j]);
+    }
+  }
+
+  // acc += the products of blocks kb0 .. kb0 + n - 1, n >= 1.
+  template <bool WIDE>
+  __device__ __forceinline__ void run(uint32_t kb0, int n, int ws_stride, f32x4 (&acc)[FN][FM]) const {
+    const float* ws = (const float*)(smem + WS_OFF) + (WS > 1 ? wn * TN / kBlock * ws_stride : 0);
+    if constexpr (IN_SLOTS && !WIDE) run_slots(kb0, n, ws, acc);
+    else run_blocks<WIDE>(kb0, n, ws, acc);
     wait_vmcnt<0>();  // the DMAs past the last block have landed before the ring is reused
   }
 };
@@ -260,7 +344,7 @@ __device__ __forceinline__ void fp8_epilogue16(const E& e, const f32x4 (&acc)[E:
   const bool residual = p.gr.residual != nullptr;
   const bool one_gate = residual && mw / p.gr.rows_per_gate == (min(mw + TM, row_end) - 1) / p.gr.rows_per_gate;
   if (residual) {
-    move_corner<TM, TN, ALIGNED, false>(region, (uint16_t*)p.gr.residual, lane, mw, nw, row_end, p.N);
+    move_corner<TM, TN, ALIGNED, false, (FM * FN > 16 ? 4 : 16)>(region, (uint16_t*)p.gr.residual, lane, mw, nw, row_end, p.N);
     wave_lds_fence();
   }
   uint8_t* at[FM];
@@ -329,86 +413,167 @@ __device__ __forceinline__ void fp8_epilogue32(const E& e, const f32x4 (&acc)[E:
   });
 }
 
-// KIND 0: rows of one weight (their K may be shared between workgroups), 1: sorted rows of experts, 2:
-// rows of experts read through the index.
-template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, int ODT, int KIND>
-__global__ __launch_bounds__(WM* WN * 64) __attribute__((amdgpu_waves_per_eu(PER_CU* WM* WN / 4, PER_CU* WM* WN / 4)))
-void fp8_tile_kernel(Fp8Operands p, int tiles_m, int tiles_n, W8a8Split split) {
-  using E = Fp8Engine<BM, BN, WM, WN, STAGES, PER_CU>;
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  E e(smem);
-  if constexpr (KIND != 0) tiles_m = group_tile_rows<BM>(p.g, p.M);
-  // tiles that one XCD (one L2) runs are neighbours, in groups of kGroupM tile rows
-  const int tiles = tiles_m * tiles_n, per_xcd = tiles / kXcds;
-  const int part = KIND == 0 && split.splits > 1 ? blockIdx.x / tiles : 0;
-  int t = blockIdx.x - part * tiles;
-  if (KIND != 0 && t >= tiles) return;
+// Where a launch's t-th tile lies: tiles that one XCD (one L2) runs are neighbours, in groups of kGroupM tile rows.
+struct TilePlace {
+  int row, column;
+};
+__device__ __forceinline__ TilePlace place_of(int t, int tiles, int tiles_m, int tiles_n) {
+  const int per_xcd = tiles / kXcds;
   if (t < per_xcd * kXcds) t = (t % kXcds) * per_xcd + t / kXcds;
   const int group = t / (kGroupM * tiles_n), first_m = group * kGroupM;
   const int group_rows = min(kGroupM, tiles_m - first_m), in_group = t - group * kGroupM * tiles_n;
-  const int tile_row = first_m + in_group % group_rows, n0 = (in_group / group_rows) * BN;
-  GroupTile at{0, tile_row * BM, p.M};
-  if constexpr (KIND != 0) {
-    at = group_tile<BM>(p.g, p.M, tile_row);
-    if (at.expert < 0) return;
-  }
-  const int m0 = at.row0, row_end = at.row_end;
+  return {first_m + in_group % group_rows, in_group / group_rows};
+}
 
-  f32x4 acc[E::FN][E::FM];
-#pragma unroll
-  for (int a = 0; a < E::FN; ++a)
-#pragma unroll
-    for (int b = 0; b < E::FM; ++b) acc[a][b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  const int kblocks = (p.K + kBlock - 1) / kBlock, ws_stride = (kblocks + 63) / 64 * 64;
-  if (KIND == 0 || at.expert < p.g.experts) {
-    e.issue_ws(p, at.expert, n0);
-    e.template set_tile<KIND == 2>(p, at.expert, m0, row_end, n0);
-    if (KIND != 0 || split.splits == 1) {
-      e.template run<ODT == kF32>(0, kblocks, ws_stride, acc);
-    } else {
-      e.template run<ODT == kF32>((uint32_t)(part * split.kblocks), min(split.kblocks, kblocks - part * split.kblocks), ws_stride, acc);
-      // partials [tile][part][fragment][thread], added in the parts' order by the last workgroup to arrive
-      __shared__ int last;
-      constexpr uint32_t BYTES = BM * BN * 4, STEP = E::THREADS * 16u;
-      const __amdgpu_buffer_rsrc_t r =
-          partial_rsrc(split.partials + (size_t)t * split.splits * BYTES, (uint32_t)split.splits * BYTES);
-      const uint32_t mine = threadIdx.x * 16u;
-      static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
-#pragma unroll
-        for (int fm = 0; fm < E::FM; ++fm)
-          store_partial(r, (uint32_t)part * BYTES + (uint32_t)(fn.value * E::FM + fm) * STEP + mine,
-                        __builtin_bit_cast(i32x4, acc[fn.value][fm]));
-      });
-      if (!last_to_arrive(split.counters + t, split.splits, &last)) return;
-      static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
-#pragma unroll
-        for (int fm = 0; fm < E::FM; ++fm) acc[fn.value][fm] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-      });
-      for (int q = 0; q < split.splits; ++q)
-        static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
-#pragma unroll
-          for (int fm = 0; fm < E::FM; ++fm)
-            acc[fn.value][fm] += __builtin_bit_cast(
-                f32x4, load_partial(r, (uint32_t)q * BYTES + (uint32_t)(fn.value * E::FM + fm) * STEP + mine));
-        });
-    }
-  }
+// What the rows of a launch are. KIND 0: rows of one weight (their K may be shared between workgroups), 1: sorted rows of
+// experts, 2: rows of experts read through the index.
+template <int BM, int KIND>
+__device__ __forceinline__ int tile_rows_of(const Fp8Operands& p, int tiles_m) {
+  return KIND == 0 ? tiles_m : group_tile_rows<BM>(p.g, p.M);
+}
+template <int BM, int KIND>
+__device__ __forceinline__ GroupTile rows_at(const Fp8Operands& p, int row) {
+  return KIND == 0 ? GroupTile{0, row * BM, p.M} : group_tile<BM>(p.g, p.M, row);
+}
+
+template <class E, int ODT>
+__device__ __forceinline__ void fp8_epilogue(const E& e, const f32x4 (&acc)[E::FN][E::FM], const Fp8Operands& p, int m0,
+                                             int row_end, int n0) {
   __syncthreads();  // every wave is done with the ring before it stages outputs
   if constexpr (ODT == kF32) fp8_epilogue32<E>(e, acc, p, m0, row_end, n0);
   else if ((p.N & 7) == 0) fp8_epilogue16<E, ODT, true>(e, acc, p, m0, row_end, n0);
   else fp8_epilogue16<E, ODT, false>(e, acc, p, m0, row_end, n0);
 }
 
-template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, int ODT, int KIND>
+template <class E>
+__device__ __forceinline__ void clear(f32x4 (&acc)[E::FN][E::FM]) {
+#pragma unroll
+  for (int a = 0; a < E::FN; ++a)
+#pragma unroll
+    for (int b = 0; b < E::FM; ++b) acc[a][b] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// A whole tile: rows m0 .. (m0 + BM or) row_end - 1 of an expert, outputs n0 ..
+template <class E, int ODT, int KIND>
+__device__ __forceinline__ void fp8_tile(uint8_t* smem, const Fp8Operands& p, int expert, int m0, int row_end, int n0) {
+  E e(smem);
+  f32x4 acc[E::FN][E::FM];
+  clear<E>(acc);
+  const int kblocks = (p.K + kBlock - 1) / kBlock;
+  if (KIND == 0 || expert < p.g.experts) {
+    e.issue_ws(p, expert, n0);
+    e.template set_tile<KIND == 2>(p, expert, m0, row_end, n0);
+    e.template run<ODT == kF32>(0, kblocks, (kblocks + 63) / 64 * 64, acc);
+  }
+  fp8_epilogue<E, ODT>(e, acc, p, m0, row_end, n0);
+}
+
+// Tiles of 256 x 256.  The last round of them, of `slots` workgroups, runs as halves or quarters while that
+// gives each CU at most one: 8800 x 8192 -> 4096 (560 tiles, 48 past two rounds) TAILWITH us, with whole ones
+// TAILWITHOUT.
+template <int ODT, int KIND>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_large_kernel(Fp8Operands p,
+                                                                                                 int tiles_m,
+                                                                                                 int tiles_n, int slots) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  tiles_m = tile_rows_of<256, KIND>(p, tiles_m);
+  const int tiles = tiles_m * tiles_n;
+  const LastRound last = last_round(tiles, slots);
+  const int t = blockIdx.x;
+  if (t < last.whole) {
+    const TilePlace at = place_of(t, last.whole, tiles_m, tiles_n);
+    const GroupTile r = rows_at<256, KIND>(p, at.row);
+    if (r.expert < 0) return;
+    fp8_tile<Fp8Engine<256, 256, 4, 2, 2, 1, true>, ODT, KIND>(smem, p, r.expert, r.row0, r.row_end, at.column * 256);
+    return;
+  }
+  const int u = t - last.whole, tile = last.whole + u / last.parts, part = u % last.parts;
+  if (tile >= tiles) return;
+  // in the order of the whole ones, without the XCDs' turns
+  const int group = tile / (kGroupM * tiles_n), first_m = group * kGroupM;
+  const int group_rows = min(kGroupM, tiles_m - first_m), in_group = tile - group * kGroupM * tiles_n;
+  const GroupTile r = rows_at<256, KIND>(p, first_m + in_group % group_rows);
+  if (r.expert < 0) return;
+  const int n0 = in_group / group_rows * 256 + (part & 1) * 128, m0 = r.row0 + (part >> 1) * 128;
+  if (n0 >= p.N || m0 >= r.row_end) return;
+  if (last.parts == 2)
+    fp8_tile<Fp8Engine<256, 128, 4, 2, 2, 1, false>, ODT, KIND>(smem, p, r.expert, m0, r.row_end, n0);
+  else
+    fp8_tile<Fp8Engine<128, 128, 2, 4, 2, 1, false>, ODT, KIND>(smem, p, r.expert, m0, r.row_end, n0);
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, bool IN_SLOTS, int ODT, int KIND>
+__global__ __launch_bounds__(WM* WN * 64) __attribute__((amdgpu_waves_per_eu(PER_CU* WM* WN / 4, PER_CU* WM* WN / 4)))
+void fp8_tile_kernel(Fp8Operands p, int tiles_m, int tiles_n, W8a8Split split) {
+  using E = Fp8Engine<BM, BN, WM, WN, STAGES, PER_CU, IN_SLOTS>;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  tiles_m = tile_rows_of<BM, KIND>(p, tiles_m);
+  const int tiles = tiles_m * tiles_n;
+  const int part = KIND == 0 && split.splits > 1 ? blockIdx.x / tiles : 0, t = blockIdx.x - part * tiles;
+  if (KIND != 0 && t >= tiles) return;
+  const TilePlace at = place_of(t, tiles, tiles_m, tiles_n);
+  const GroupTile r = rows_at<BM, KIND>(p, at.row);
+  if (r.expert < 0) return;
+  const int n0 = at.column * BN;
+  if constexpr (KIND != 0) {
+    fp8_tile<E, ODT, KIND>(smem, p, r.expert, r.row0, r.row_end, n0);
+  } else {
+    E e(smem);
+    f32x4 acc[E::FN][E::FM];
+    clear<E>(acc);
+    const int kblocks = (p.K + kBlock - 1) / kBlock, kb0 = part * split.kblocks;
+    e.issue_ws(p, 0, n0);
+    e.template set_tile<false>(p, 0, r.row0, r.row_end, n0);
+    e.template run<ODT == kF32>((uint32_t)kb0, min(split.kblocks, kblocks - kb0), (kblocks + 63) / 64 * 64, acc);
+    if (split.splits > 1) {
+      // partials [tile][part][fragment][thread], added in the parts' order by the last workgroup to arrive
+      __shared__ int last;
+      constexpr uint32_t BYTES = BM * BN * 4, STEP = E::THREADS * 16u;
+      const int slot = at.row * tiles_n + at.column;
+      const __amdgpu_buffer_rsrc_t rp =
+          partial_rsrc(split.partials + (size_t)slot * split.splits * BYTES, (uint32_t)split.splits * BYTES);
+      const uint32_t mine = threadIdx.x * 16u;
+      static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+        for (int fm = 0; fm < E::FM; ++fm)
+          store_partial(rp, (uint32_t)part * BYTES + (uint32_t)(fn.value * E::FM + fm) * STEP + mine,
+                        __builtin_bit_cast(i32x4, acc[fn.value][fm]));
+      });
+      if (!last_to_arrive(split.counters + slot, split.splits, &last)) return;
+      clear<E>(acc);
+      for (int q = 0; q < split.splits; ++q)
+        static_for<E::FN>([&](auto fn) __attribute__((always_inline)) {
+#pragma unroll
+          for (int fm = 0; fm < E::FM; ++fm)
+            acc[fn.value][fm] += __builtin_bit_cast(
+                f32x4, load_partial(rp, (uint32_t)q * BYTES + (uint32_t)(fn.value * E::FM + fm) * STEP + mine));
+        });
+    }
+    fp8_epilogue<E, ODT>(e, acc, p, r.row0, r.row_end, n0);
+  }
+}
+
+template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, bool IN_SLOTS, int ODT, int KIND>
 hipError_t launch_fp8_tile_k(const Fp8Operands& p, const W8a8Split& split, hipStream_t s) {
-  using E = Fp8Engine<BM, BN, WM, WN, STAGES, PER_CU>;
+  using E = Fp8Engine<BM, BN, WM, WN, STAGES, PER_CU, IN_SLOTS>;
   static_assert(E::smem_bytes(kMaxBlocks) <= 160 * 1024 - 64, "LDS of one CU");
   const int64_t tm = KIND == 0 ? ((int64_t)p.M + BM - 1) / BM : most_tile_rows(p.M, p.g.experts, BM);
-  const int64_t tn = ((int64_t)p.N + BN - 1) / BN, groups = tm * tn * split.splits;
-  if (groups > max_groups(E::THREADS) || groups > 0x7fffffff) return hipErrorInvalidValue;
-  fp8_tile_kernel<BM, BN, WM, WN, STAGES, PER_CU, ODT, KIND>
-      <<<dim3((unsigned)groups), dim3(E::THREADS), E::smem_bytes((p.K + kBlock - 1) / kBlock), s>>>(p, (int)tm, (int)tn,
-                                                                                                  split);
+  const int64_t tn = ((int64_t)p.N + BN - 1) / BN;
+  const size_t lds = (size_t)E::smem_bytes((p.K + kBlock - 1) / kBlock);
+  if constexpr (BM == 256) {
+    const int slots = device_cus();
+    // (what experts make of the bound's tiles is known on the device alone)
+    if (tm * tn > 0x7fff0000 || slots < 1) return hipErrorInvalidValue;
+    const LastRound last = last_round((int)(tm * tn), slots);
+    const int64_t groups = KIND == 0 ? last.whole + (tm * tn - last.whole) * last.parts : tm * tn + slots;
+    if (groups > max_groups(E::THREADS)) return hipErrorInvalidValue;
+    fp8_large_kernel<ODT, KIND><<<dim3((unsigned)groups), dim3(E::THREADS), lds, s>>>(p, (int)tm, (int)tn, slots);
+  } else {
+    const int64_t groups = tm * tn * split.splits;
+    if (groups > max_groups(E::THREADS) || groups > 0x7fffffff) return hipErrorInvalidValue;
+    fp8_tile_kernel<BM, BN, WM, WN, STAGES, PER_CU, IN_SLOTS, ODT, KIND>
+        <<<dim3((unsigned)groups), dim3(E::THREADS), lds, s>>>(p, (int)tm, (int)tn, split);
+  }
   return hipGetLastError();
 }
 
@@ -417,11 +582,11 @@ hipError_t launch_fp8_tile_k(const Fp8Operands& p, const W8a8Split& split, hipSt
 template <int ODT>
 hipError_t launch_fp8_tile(int tile, const Fp8Operands& p, const W8a8Split& split, hipStream_t stream) {
   switch (tile) {
-#define FP8_CASE(BM, BN, WM, WN, STAGES, PER_CU)                                                                \
+#define FP8_CASE(BM, BN, WM, WN, STAGES, PER_CU, SLOTS)                                                         \
   case tile_code(BM, BN):                                                                                       \
-    if (!p.g.offsets) return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, ODT, 0>(p, split, stream);       \
-    if (!p.g.index) return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, ODT, 1>(p, split, stream);         \
-    return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, ODT, 2>(p, split, stream);
+    if (!p.g.offsets) return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, SLOTS, ODT, 0>(p, split, stream);       \
+    if (!p.g.index) return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, SLOTS, ODT, 1>(p, split, stream);         \
+    return launch_fp8_tile_k<BM, BN, WM, WN, STAGES, PER_CU, SLOTS, ODT, 2>(p, split, stream);
     FP8_TILES(FP8_CASE)
 #undef FP8_CASE
     default: return hipErrorInvalidValue;

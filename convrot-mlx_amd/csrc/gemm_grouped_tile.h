@@ -132,9 +132,9 @@ struct Side {
   __device__ __forceinline__ i32x4_sgpr rsrc(uint32_t kb) const {
     if constexpr (ACROSS) {
       const int left = min(64, count - (int)kb * 64);
-      return buffer_rsrc(base + (int64_t)kb * step, (uint32_t)(left - 1) * row_bytes + bytes);
+      return dma_rsrc(base + (int64_t)kb * step, (uint32_t)(left - 1) * row_bytes + bytes);
     } else {
-      return buffer_rsrc(base, bytes);
+      return dma_rsrc(base, bytes);
     }
   }
   __device__ __forceinline__ void issue(i32x4_sgpr r, uint32_t kb, int i, int wave, uint32_t lds) const {
@@ -143,7 +143,7 @@ struct Side {
       o = o == kPastEnd ? kPastEnd : o + kb * 128u;
       if (kb == tail) o = past[i & 1] ? kPastEnd : o;
     }
-    dma16(r, o, lds + (uint32_t)(wave * PW + i) * 1024u);
+    load_lds16(r, o, lds + (uint32_t)(wave * PW + i) * 1024u);
   }
 
   // The address of this lane's part of fragment 0 of the wave's corner at `first`, k-step 0; of
@@ -165,12 +165,12 @@ struct Side {
       // the corner begins at a multiple of its size, so f and the swizzle's bits lie apart from it
       const uint32_t a = (at ^ (uint32_t)(F * 32)) + (uint32_t)(KS * 8 * ROW);
       typedef __attribute__((address_space(3))) s16x4* P;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(a));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(a + 4 * ROW));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)a);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(uintptr_t)(a + 4 * ROW));
       return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       typedef __attribute__((address_space(3))) i32x4* P;
-      return *(P)((at ^ (uint32_t)(KS * 16)) + (uint32_t)(F * 2048));
+      return *(P)(uintptr_t)((at ^ (uint32_t)(KS * 16)) + (uint32_t)(F * 2048));
     }
   }
 };

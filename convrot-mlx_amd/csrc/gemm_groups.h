@@ -65,6 +65,17 @@ __device__ __forceinline__ GroupTile group_tile(const Groups& g, int rows, int t
   return {-1, 0, 0};
 }
 
+// How `tiles` large tiles run on `slots` CUs: whole ones in whole rounds, and those of the last round as 4 or 2
+// parts each while that gives a CU at most one workgroup.
+struct LastRound {
+  int whole, parts;
+};
+__host__ __device__ __forceinline__ LastRound last_round(int tiles, int slots) {
+  const int rest = tiles % slots;
+  const int parts = rest == 0 ? 1 : rest * 4 <= slots ? 4 : rest * 2 <= slots ? 2 : 1;
+  return {parts == 1 ? tiles : tiles - rest, parts};
+}
+
 // Most rows of tiles that any split of `rows` over the experts (and none) makes.
 inline int64_t most_tile_rows(int64_t rows, int64_t experts, int bm) {
   const int64_t bound = rows / bm + experts + 1;

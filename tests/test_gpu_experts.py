@@ -186,7 +186,7 @@ def test_fp8_products(dev, tokens, choices, experts, n, k, dtype, gather):
     assert not got[at[-1]:].any()
 
 
-@pytest.mark.parametrize("tile", ["256x256", "256x128", "128x128", "64x128", "32x64"])
+@pytest.mark.parametrize("tile", ["256x256", "128x128", "64x128", "64x64", "32x64"])
 def test_fp8_every_tile(dev, tuning, tile):
     from convrot_mlx_amd import expert_plan, hip_fp8_grouped_linear
 
