@@ -175,8 +175,9 @@ struct Side {
   }
 };
 
-template <int BM, int BN, int STAGES, int DT, bool ACROSS_A, bool ACROSS_B>
+template <int BM_, int BN_, int STAGES, int DT, bool ACROSS_A, bool ACROSS_B>
 struct Engine16 {
+  static constexpr int BM = BM_, BN = BN_;
   using A = Side<BM, ACROSS_A>;
   using B = Side<BN, ACROSS_B>;
   static constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 16, FN = TN / 16, LPW = A::PW + B::PW;
@@ -309,26 +310,21 @@ __device__ __forceinline__ void store_tile(const E& e, const f32x4 (&acc)[E::FN]
   move_corner<TM, TN, ALIGNED, true>(region, (uint16_t*)out, lane, mw, nw, row_end, N);
 }
 
-template <int BM, int BN, int STAGES, int PER_CU, int DT, int KIND>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER_CU))) void grouped_kernel(
-    GroupedOperands p, int tiles_i, int tiles_j) {
-  using E = Engine16<BM, BN, STAGES, DT, KIND == 3, KIND >= 2>;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES];
+// One tile: output rows m0 .. (m0 + BM or) row_end - 1, columns n0 .., of an expert (whose rows, with KIND 3, are
+// the contracted ones).
+template <class E, int DT, int KIND>
+__device__ __forceinline__ void grouped_tile(uint8_t* smem, const GroupedOperands& p, int expert, int m0, int row_end,
+                                             int n0) {
   E e(smem);
   f32x4 acc[E::FN][E::FM];
 #pragma unroll
   for (int i = 0; i < E::FN; ++i)
 #pragma unroll
     for (int j = 0; j < E::FM; ++j) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  int m0, n0, row_end, columns;
+  int columns = p.N;
   uint16_t* out = p.out;
   if constexpr (KIND == 3) {
-    // the tiles of one expert run behind each other on all XCDs, each XCD on neighbours
-    const int tiles = tiles_i * tiles_j, per_xcd = tiles / kXcds, expert = blockIdx.x / tiles;
-    int t = blockIdx.x - expert * tiles;
-    if (t < per_xcd * kXcds) t = (t % kXcds) * per_xcd + t / kXcds;
-    m0 = t / tiles_j * BM, n0 = t % tiles_j * BN;
-    row_end = p.N, columns = p.C;
+    columns = p.C;
     out += (int64_t)expert * p.N * p.C;
     const int a = group_start(p.g, expert, p.R), b = group_start(p.g, expert + 1, p.R);
     if (b > a) {
@@ -336,35 +332,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER
       e.b.set_across(p.other + (int64_t)a * p.ld_other + n0, p.ld_other, p.C - n0, b - a, e.lane, e.wave);
       e.run((b - a + 63) / 64, acc);
     }
-  } else {
-    tiles_i = group_tile_rows<BM>(p.g, p.R);
-    // tiles that one XCD (one L2) runs are neighbours, in groups of kGroupM tile rows
-    const int tiles = tiles_i * tiles_j, per_xcd = tiles / kXcds;
-    int t = blockIdx.x;
-    if (t >= tiles) return;
-    if (t < per_xcd * kXcds) t = (t % kXcds) * per_xcd + t / kXcds;
-    const int group = t / (kGroupM * tiles_j), first = group * kGroupM;
-    const int group_rows = min(kGroupM, tiles_i - first), in_group = t - group * kGroupM * tiles_j;
-    const GroupTile at = group_tile<BM>(p.g, p.R, first + in_group % group_rows);
-    if (at.expert < 0) return;
-    m0 = at.row0, row_end = at.row_end, n0 = in_group / group_rows * BN, columns = p.N;
-    if (at.expert < p.g.experts) {
-      const int rows = min(BM, row_end - m0);
-      if constexpr (KIND == 1) {
-        e.a.set_gather(p.rows, p.ld_rows, p.g.act_rows, p.C, e.lane, e.wave, [&](int r) __attribute__((always_inline)) {
-          if (r >= rows) return (int64_t)-1;
-          const int i = p.g.index[m0 + r];
-          const uint32_t token = (uint32_t)i / (uint32_t)p.g.choices;
-          return i < 0 || token >= p.g.act_rows ? (int64_t)-1 : (int64_t)token;
-        });
-      } else {
-        e.a.set_along(p.rows + (int64_t)m0 * p.ld_rows, p.ld_rows, rows, p.C, e.lane, e.wave);
-      }
-      const uint16_t* w = p.other + at.expert * p.expert;
-      if constexpr (KIND == 2) e.b.set_across(w + n0, p.ld_other, p.N - n0, p.C, e.lane, e.wave);
-      else e.b.set_along(w + (int64_t)n0 * p.ld_other, p.ld_other, min(BN, p.N - n0), p.C, e.lane, e.wave);
-      e.run((p.C + 63) / 64, acc);
+  } else if (expert < p.g.experts) {
+    const int rows = min(E::BM, row_end - m0);
+    if constexpr (KIND == 1) {
+      e.a.set_gather(p.rows, p.ld_rows, p.g.act_rows, p.C, e.lane, e.wave, [&](int r) __attribute__((always_inline)) {
+        if (r >= rows) return (int64_t)-1;
+        const int i = p.g.index[m0 + r];
+        const uint32_t token = (uint32_t)i / (uint32_t)p.g.choices;
+        return i < 0 || token >= p.g.act_rows ? (int64_t)-1 : (int64_t)token;
+      });
+    } else {
+      e.a.set_along(p.rows + (int64_t)m0 * p.ld_rows, p.ld_rows, rows, p.C, e.lane, e.wave);
     }
+    const uint16_t* w = p.other + expert * p.expert;
+    if constexpr (KIND == 2) e.b.set_across(w + n0, p.ld_other, p.N - n0, p.C, e.lane, e.wave);
+    else e.b.set_along(w + (int64_t)n0 * p.ld_other, p.ld_other, min(E::BN, p.N - n0), p.C, e.lane, e.wave);
+    e.run((p.C + 63) / 64, acc);
   }
   __syncthreads();  // every wave is done with the ring before it stages outputs
   // chunks are aligned where every row of the array is
@@ -372,13 +355,87 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER
   else store_tile<E, DT, false>(e, acc, out, m0, row_end, n0, columns);
 }
 
+// Where the t-th tile of a launch lies.  The first `turns` of them go to the XCDs (and their L2s) in runs of
+// neighbours.  Of rows: in groups of kGroupM tile rows; of the weights' gradient: one expert behind the other, each
+// on all XCDs, as experts of many rows take longer.
+template <int BM, int KIND>
+__device__ __forceinline__ GroupTile grouped_place(const GroupedOperands& p, int t, int turns, int tiles_i, int tiles_j,
+                                                   int* column) {
+  if constexpr (KIND == 3) {
+    const int tiles = tiles_i * tiles_j, per_xcd = tiles / kXcds, expert = t / tiles;
+    t -= expert * tiles;
+    if (t < per_xcd * kXcds && (expert + 1) * tiles <= turns) t = (t % kXcds) * per_xcd + t / kXcds;
+    *column = t % tiles_j;
+    return {expert, t / tiles_j * BM, p.N};
+  } else {
+    const int per_xcd = turns / kXcds;
+    if (t < per_xcd * kXcds) t = (t % kXcds) * per_xcd + t / kXcds;
+    const int group = t / (kGroupM * tiles_j), first = group * kGroupM;
+    const int group_rows = min(kGroupM, tiles_i - first), in_group = t - group * kGroupM * tiles_j;
+    *column = in_group / group_rows;
+    return group_tile<BM>(p.g, p.R, first + in_group % group_rows);
+  }
+}
+
+template <int BM, int BN, int STAGES, int PER_CU, int DT, int KIND>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER_CU))) void grouped_kernel(
+    GroupedOperands p, int tiles_i, int tiles_j) {
+  using E = Engine16<BM, BN, STAGES, DT, KIND == 3, KIND >= 2>;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES];
+  if constexpr (KIND != 3) tiles_i = group_tile_rows<BM>(p.g, p.R);
+  const int tiles = tiles_i * tiles_j * (KIND == 3 ? p.g.experts : 1), t = blockIdx.x;
+  if (t >= tiles) return;
+  int column;
+  const GroupTile at = grouped_place<BM, KIND>(p, t, tiles, tiles_i, tiles_j, &column);
+  if (at.expert < 0) return;
+  grouped_tile<E, DT, KIND>(smem, p, at.expert, at.row0, at.row_end, column * BN);
+}
+
+// Tiles of 256 x 256, the last round of them in halves or quarters (last_round of gemm_groups.h).
+template <int DT, int KIND>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void grouped_large_kernel(GroupedOperands p,
+                                                                                                     int tiles_i,
+                                                                                                     int tiles_j,
+                                                                                                     int slots) {
+  constexpr bool AA = KIND == 3, AB = KIND >= 2;
+  using E = Engine16<256, 256, 2, DT, AA, AB>;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES];
+  if constexpr (KIND != 3) tiles_i = group_tile_rows<256>(p.g, p.R);
+  const int tiles = tiles_i * tiles_j * (KIND == 3 ? p.g.experts : 1), t = blockIdx.x;
+  const LastRound last = last_round(tiles, slots);
+  int column;
+  if (t < last.whole) {
+    const GroupTile at = grouped_place<256, KIND>(p, t, last.whole, tiles_i, tiles_j, &column);
+    if (at.expert < 0) return;
+    grouped_tile<E, DT, KIND>(smem, p, at.expert, at.row0, at.row_end, column * 256);
+    return;
+  }
+  const int u = t - last.whole, tile = last.whole + u / last.parts, part = u % last.parts;
+  if (tile >= tiles) return;
+  const GroupTile at = grouped_place<256, KIND>(p, tile, 0, tiles_i, tiles_j, &column);
+  if (at.expert < 0) return;
+  const int m0 = at.row0 + (part >> 1) * 128, n0 = column * 256 + (part & 1) * 128;
+  if (m0 >= at.row_end || n0 >= (KIND == 3 ? p.C : p.N)) return;
+  if (last.parts == 2)
+    grouped_tile<Engine16<256, 128, 3, DT, AA, AB>, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
+  else
+    grouped_tile<Engine16<128, 128, 4, DT, AA, AB>, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
+}
+
 template <int BM, int BN, int STAGES, int PER_CU, int DT, int KIND>
 hipError_t launch_grouped_k(const GroupedOperands& p, hipStream_t s) {
   const int64_t ti = KIND == 3 ? ((int64_t)p.N + BM - 1) / BM : most_tile_rows(p.R, p.g.experts, BM);
   const int64_t tj = ((int64_t)(KIND == 3 ? p.C : p.N) + BN - 1) / BN;
-  const int64_t groups = ti * tj * (KIND == 3 ? p.g.experts : 1);
-  if (groups > max_groups(256)) return hipErrorInvalidValue;
-  grouped_kernel<BM, BN, STAGES, PER_CU, DT, KIND><<<dim3((unsigned)groups), dim3(256), 0, s>>>(p, (int)ti, (int)tj);
+  const int64_t tiles = ti * tj * (KIND == 3 ? p.g.experts : 1), slots = device_cus();
+  if (tiles > max_groups(256) - slots || tiles > 0x7fff0000 || slots < 1) return hipErrorInvalidValue;
+  if constexpr (BM == 256) {
+    // (what experts make of the bound's tiles is known on the device alone)
+    const LastRound last = last_round((int)tiles, (int)slots);
+    const int64_t groups = KIND == 3 ? last.whole + (tiles - last.whole) * last.parts : tiles + slots;
+    grouped_large_kernel<DT, KIND><<<dim3((unsigned)groups), dim3(256), 0, s>>>(p, (int)ti, (int)tj, (int)slots);
+  } else {
+    grouped_kernel<BM, BN, STAGES, PER_CU, DT, KIND><<<dim3((unsigned)tiles), dim3(256), 0, s>>>(p, (int)ti, (int)tj);
+  }
   return hipGetLastError();
 }
 

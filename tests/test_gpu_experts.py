@@ -338,7 +338,7 @@ def test_products(dev, tokens, choices, experts, n, k, dtype, gather):
     check_products(dev, tokens, choices, experts, n, k, dtype, gather)
 
 
-@pytest.mark.parametrize("tile", ["256x256", "128x128", "64x128", "32x64"])
+@pytest.mark.parametrize("tile", ["256x256", "128x128", "64x128", "64x64", "32x128", "32x64"])
 @pytest.mark.parametrize("tokens,choices,experts,n,k", [(500, 2, 5, 270, 400), (600, 1, 2, 520, 264), (30, 1, 4, 64, 64)])
 def test_every_tile(dev, tuning, tile, tokens, choices, experts, n, k):
     tuning.set("grouped_tile", tile)
