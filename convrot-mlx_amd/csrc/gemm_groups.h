@@ -100,7 +100,7 @@ hipError_t launch_grouped_tile(int tile, int kind, const GroupedOperands& p, hip
 
 // The tiles built: BM, BN, ring stages, workgroups a CU; for rows, and for the weights' gradient.
 #define GROUPED_TILES(X) \
-  X(256, 256, 2, 1) X(128, 128, 2, 2) X(64, 128, 3, 2) X(64, 64, 4, 2) X(32, 128, 3, 2) X(32, 64, 6, 2)
+  X(256, 256, 2, 1) X(128, 128, 2, 2) X(64, 128, 3, 2) X(64, 64, 5, 2) X(32, 128, 4, 2) X(32, 64, 6, 2)
 #define GROUPED_WEIGHT_TILES(X) X(256, 256, 2, 1) X(128, 128, 2, 2)
 
 }  // namespace convrot
