@@ -10,13 +10,24 @@ namespace {
 // ---- order by expert
 //
 // A stable counting sort of `count` choices by their expert (those of none last, as if of
-// expert E).  A workgroup of 16 waves takes kPlanChoices of them, each wave a run of them 64 at a
+// expert E).  A workgroup of 16 waves takes `each` of them, each wave a run of them 64 at a
 // time: first it counts its experts' choices in LDS, then, after sums over waves and experts, it
 // places them: a choice's rank among its 64 is the number of lower lanes with the same expert, found
 // bit by bit with ballots.  So the order never depends on which wave was first.  With several
 // workgroups a launch before counts for each, and a workgroup adds the counts of those before it.
-// Bound by latency: 64 choices of 64 experts 4 us, 36864 in two launches 9 us.
-constexpr int kPlanWaves = 16, kPlanChoices = 8192;
+// Bound by latency: in a graph 1024 choices of 64 experts 6.1 us, 4096 in two launches 9.6, 36864 11.2 (with 8192 a
+// workgroup 29), a million of 256 experts 37.
+constexpr int kPlanWaves = 16, kPlanAlone = 2048, kPlanEach = 1024, kPlanGroups = 64;
+
+// Workgroups and the choices of each: one up to kPlanAlone choices, then at most kPlanGroups.
+struct PlanSplit {
+  int64_t each, groups;
+};
+PlanSplit plan_split(int64_t count) {
+  if (count <= kPlanAlone) return {kPlanAlone, 1};
+  const int64_t runs = (count + kPlanEach - 1) / kPlanEach, each = (runs + kPlanGroups - 1) / kPlanGroups * kPlanEach;
+  return {each, (count + each - 1) / each};
+}
 
 template <typename I>
 __device__ __forceinline__ int expert_of(const I* ids, int64_t i, int experts) {
@@ -25,12 +36,13 @@ __device__ __forceinline__ int expert_of(const I* ids, int64_t i, int experts) {
 }
 
 template <typename I>
-__global__ __launch_bounds__(256) void plan_count_kernel(const I* __restrict__ ids, int64_t count, int experts,
-                                                         int* __restrict__ counts) {
+__global__ __launch_bounds__(256) void plan_count_kernel(const I* __restrict__ ids, int64_t count, int64_t each,
+                                                         int experts, int* __restrict__ counts) {
   extern __shared__ int hist[];
   for (int e = threadIdx.x; e <= experts; e += 256) hist[e] = 0;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kPlanChoices, i1 = min(count, i0 + kPlanChoices);
+  const int64_t i0 = (int64_t)blockIdx.x * each, i1 = min(count, i0 + each);
+#pragma unroll 4
   for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) atomicAdd(&hist[expert_of(ids, i, experts)], 1);
   __syncthreads();
   int* mine = counts + (int64_t)blockIdx.x * (experts + 1);
@@ -39,7 +51,8 @@ __global__ __launch_bounds__(256) void plan_count_kernel(const I* __restrict__ i
 
 template <typename I>
 __global__ __launch_bounds__(kPlanWaves * 64) void plan_place_kernel(const I* __restrict__ ids, int64_t count,
-                                                                     int experts, const int* __restrict__ counts,
+                                                                     int64_t choices, int experts,
+                                                                     const int* __restrict__ counts,
                                                                      int* __restrict__ offsets, int* __restrict__ order,
                                                                      int* __restrict__ slots) {
   extern __shared__ int hist[];  // [waves][experts + 1]: counts, then places of the next choice
@@ -47,8 +60,8 @@ __global__ __launch_bounds__(kPlanWaves * 64) void plan_place_kernel(const I* __
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, stride = experts + 1;
   for (int i = tid; i < kPlanWaves * stride; i += kPlanWaves * 64) hist[i] = 0;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kPlanChoices;
-  const int n = (int)min((int64_t)kPlanChoices, count - i0);
+  const int64_t i0 = (int64_t)blockIdx.x * choices;
+  const int n = (int)min(choices, count - i0);
   const int each = ((n + kPlanWaves - 1) / kPlanWaves + 63) / 64 * 64;  // a wave's run
   const int a = min(n, wave * each), b = min(n, a + each);
   int* mine = hist + wave * stride;
@@ -63,6 +76,7 @@ __global__ __launch_bounds__(kPlanWaves * 64) void plan_place_kernel(const I* __
     total = here;
     if (counts) {
       total = 0;
+#pragma unroll 8
       for (unsigned g = 0; g < gridDim.x; ++g) {
         const int c = counts[(int64_t)g * stride + tid];
         total += c;
@@ -93,11 +107,15 @@ __global__ __launch_bounds__(kPlanWaves * 64) void plan_place_kernel(const I* __
       at += c;
     }
   }
+  int none = 0;  // choices of no expert before this workgroup
+  if (counts && wave == 0) {
+    none = (unsigned)lane < blockIdx.x ? counts[(int64_t)lane * stride + experts] : 0;  // at most 64 workgroups
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) none += __shfl_xor(none, d);
+  }
   if (tid == 0) {
     if (blockIdx.x == 0) offsets[experts] = all;
-    int at = all;  // choices of no expert
-    if (counts)
-      for (unsigned g = 0; g < blockIdx.x; ++g) at += counts[(int64_t)g * stride + experts];
+    int at = all + none;
     for (int w = 0; w < kPlanWaves; ++w) {
       const int c = hist[w * stride + experts];
       hist[w * stride + experts] = at;
@@ -131,14 +149,15 @@ __global__ __launch_bounds__(kPlanWaves * 64) void plan_place_kernel(const I* __
 template <typename I>
 hipError_t plan_t(const void* ids, int64_t count, int experts, int* offsets, int* order, int* slots, int* work,
                   hipStream_t s) {
-  const unsigned groups = (unsigned)((count + kPlanChoices - 1) / kPlanChoices);
+  const PlanSplit p = plan_split(count);
   const size_t lds = (size_t)(experts + 1) * sizeof(int);
-  if (groups > 1) {
-    plan_count_kernel<I><<<dim3(groups), dim3(256), lds, s>>>((const I*)ids, count, experts, work);
+  const bool alone = p.groups == 1;
+  if (!alone) {
+    plan_count_kernel<I><<<dim3((unsigned)p.groups), dim3(256), lds, s>>>((const I*)ids, count, p.each, experts, work);
     if (hipError_t e = hipGetLastError()) return e;
   }
-  plan_place_kernel<I><<<dim3(groups ? groups : 1), dim3(kPlanWaves * 64), kPlanWaves * lds, s>>>(
-      (const I*)ids, count, experts, groups > 1 ? work : nullptr, offsets, order, slots);
+  plan_place_kernel<I><<<dim3((unsigned)p.groups), dim3(kPlanWaves * 64), kPlanWaves * lds, s>>>(
+      (const I*)ids, count, p.each, experts, alone ? nullptr : work, offsets, order, slots);
   return hipGetLastError();
 }
 
@@ -382,7 +401,7 @@ hipError_t combine_backward_t(const void* dout, int64_t dout_stride, const void*
 }  // namespace
 
 int64_t expert_plan_workspace_bytes(int64_t count, int experts) {
-  const int64_t groups = (count + kPlanChoices - 1) / kPlanChoices;
+  const int64_t groups = plan_split(count).groups;
   return groups > 1 ? groups * (experts + 1) * (int64_t)sizeof(int) : 0;
 }
 
