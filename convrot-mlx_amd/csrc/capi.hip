@@ -1183,18 +1183,30 @@ int convrot_fp8_linear(const void* x, int dtype, int64_t x_stride, const uint8_t
   if (int rc = check_fp8(M, N, K, weight, weight_stride, wscales, wscales_stride, out, dtype)) return rc;
   if (int rc = check_fp8_work(residual, gate, rows_per_gate, workspace, workspace_bytes)) return rc;
   if (M == 0 || N == 0) return ok();
-  if (int rc = check_fp8_scratch(scratch, scratch_bytes, M, K)) return rc;
-  const Fp8Scratch c = fp8_scratch(scratch, M, K);
   convrot::GatedResidual gr{};
   if (residual)
     if (int rc = check_residual(residual, gate, gate_stride, rows_per_gate, M, N, &gr)) return rc;
+  const convrot::Workspace work{(uint8_t*)workspace, workspace ? (size_t)workspace_bytes : 0};
+  // a fused launch's workgroups all read x: none may write into it
+  const int64_t es = dtype == CONVROT_DTYPE_F32 ? 4 : 2;
+  const uintptr_t xa = (uintptr_t)x, oa = (uintptr_t)out;
+  const bool apart = oa + (uintptr_t)(M * N * es) <= xa || xa + (uintptr_t)(((M - 1) * x_stride + K) * es) <= oa;
+  const bool fused = apart && convrot::fp8_fused(x, dtype, M, K, x_stride);
+  if (!fused)
+    if (int rc = check_fp8_scratch(scratch, scratch_bytes, M, K)) return rc;
+  const Fp8Scratch c = fused ? Fp8Scratch{} : fp8_scratch(scratch, M, K);
   const convrot::Fp8Operands p{c.codes, weight, c.stride, weight_stride, c.scales, wscales, bias, 1,
                                c.xs_block, wscales_stride, out, (int)M, (int)N, (int)K, gr, {}, 0, 0};
-  const convrot::Workspace work{(uint8_t*)workspace, workspace ? (size_t)workspace_bytes : 0};
+  if (fused)
+    return launch_status(convrot::launch_fp8_fused(p, x, x_stride, dtype, (hipStream_t)stream, work), "convrot_fp8_linear");
   hipError_t e = convrot::launch_quantize_fp8(x, dtype, M, K, x_stride, c.codes, c.stride, c.scales, 1, c.xs_block,
                                               (hipStream_t)stream);
   if (e == hipSuccess) e = convrot::launch_fp8_gemm(p, dtype, (hipStream_t)stream, work);
   return launch_status(e, "convrot_fp8_linear");
+}
+
+int convrot_fp8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
+  return M > 0 && K > 0 && valid_dtype(dtype) && convrot::fp8_fused(x, dtype, M, K, x_stride) ? 1 : 0;
 }
 
 namespace {

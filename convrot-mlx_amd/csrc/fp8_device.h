@@ -57,6 +57,26 @@ __device__ __forceinline__ uint32_t fp8_codes4(const float* v, float inverse) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], w, true);
 }
 
+// The 32 codes of a lane's part of a fragment as bf16 (exact).
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+struct WideCodes {
+  bf16x8 v[4];
+};
+__device__ __forceinline__ WideCodes widen_codes(const i32x8& c) {
+  WideCodes w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    i32x4 t;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      t[2 * h] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * i + h], 1.0f, false));
+      t[2 * h + 1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * i + h], 1.0f, true));
+    }
+    w.v[i] = __builtin_bit_cast(bf16x8, t);
+  }
+  return w;
+}
+
 // Rows grouped by expert: expert e has rows offsets[e] .. offsets[e + 1] - 1 of `rows`; those from
 // offsets[experts] on have none and give zeros.  With `index`, sorted row s is row index[s] / choices
 // of the activations.

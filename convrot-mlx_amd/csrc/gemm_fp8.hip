@@ -1,12 +1,191 @@
 // Products in 8-bit floating point for gfx950 (the product and its numerics are stated
-// in gemm_fp8_tile.h): the choice of tile.
+// in gemm_fp8_tile.h): the kernel for a few token rows, and the choice of kernel.
 #include <algorithm>
 
 #include "convrot_launch.h"
 #include "fp8_device.h"
+#include "row_device.h"
 
 namespace convrot {
 namespace {
+
+// ---- few rows
+//
+// Up to 16 token rows: the weights' bytes bound it, each read once.  A workgroup owns 64 output channels, each of
+// its 4 waves 16 of them and, for itself (no barrier in the loop), a ring of STAGES blocks of 128 features in LDS
+// that it keeps full by loads straight to LDS; the rows' codes and scales of its part of K lie in LDS from the
+// start.  Where the channels make too few workgroups for the chip, several share K, and the last to arrive adds
+// their sums in the parts' order.  With FUSED the rows come as they are and each workgroup quantizes its part of
+// them itself (as convrot_quantize_fp8 does, block by block): one launch instead of two, while the first weights
+// are on their way.  Measured with the 32 x 64 tile and two launches: ROWSNOTE
+constexpr int kRowsMax = 16, kRowsN = 64;
+// Bytes of a fused call's rows, which lie in LDS beside their codes, and which every workgroup quantizes: of one row,
+// and of several.  Fused and not, in us: 2 x 4096 -> 12288 10.6 and 13.1, 4 x 4096 -> 12288 12.7 and 12.7, 8 x 2048 ->
+// 24576 16.8 and 13.1, 1 x 15360 -> 5120 17.8 and 20.4.
+constexpr int64_t kFusedRowBytes = 32768, kFusedBytes = 16384;
+constexpr size_t kTwoPerCu = 79 * 1024;    // dynamic LDS of two workgroups a CU
+
+__device__ __forceinline__ uint32_t max_of_16(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppHalfMirror, 0xf, 0xf, true));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppMirror, 0xf, 0xf, true));
+}
+
+// LDS of the few-row kernel, in bytes from its start: the rings, the codes [block][row][128], the scales of
+// rows [block][row] and of the weights [block], and (fused) the rows as they are.
+struct RowsLds {
+  uint32_t codes, xs, ws, raw, end;
+};
+__host__ __device__ __forceinline__ RowsLds rows_lds(int stages, int rows, int blocks, int raw_size) {
+  const auto whole = [](uint32_t n) { return (n + 1023u) & ~1023u; };  // whole wave loads
+  RowsLds l;
+  l.codes = (uint32_t)stages * 8192u;
+  l.xs = l.codes + whole((uint32_t)(rows * blocks) * 128u);
+  l.ws = l.xs + whole((uint32_t)(rows * blocks) * 4u);
+  l.raw = l.ws + whole((uint32_t)blocks * 4u);
+  l.end = l.raw + whole((uint32_t)(rows * blocks) * 128u * (uint32_t)raw_size);
+  return l;
+}
+
+template <int DT, bool FUSED, int STAGES>
+__global__ __launch_bounds__(256) void fp8_few_rows_kernel(Fp8Operands p, const void* __restrict__ x, int64_t x_stride,
+                                                           W8a8Split split, int tiles) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  __shared__ int last;
+  constexpr uint32_t ES = DT == kF32 ? 4 : 2;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
+  const int kblocks = (p.K + kBlock - 1) / kBlock, kb0 = part * split.kblocks, n = min(split.kblocks, kblocks - kb0);
+  const uint32_t k16 = (uint32_t)(p.K + 15) & ~15u, k0 = (uint32_t)kb0 * 128u, M = (uint32_t)p.M;
+  const RowsLds at = rows_lds(STAGES, p.M, n, FUSED ? (int)ES : 0);
+  const uint32_t base = (uint32_t)(uintptr_t)smem;
+
+  // the weights' scales, and the rows: as they are, 16-byte chunks of [row][n 128], or their codes and scales
+  const i32x4_sgpr rs = dma_rsrc(p.wscales + (int64_t)(tile * kRowsN / kBlock) * p.ws_row + kb0, (uint32_t)n * 4u);
+  for (uint32_t i0 = wave * 64u; i0 < (uint32_t)n; i0 += 256u) load_lds4(rs, (i0 + lane) * 4u, base + at.ws + i0 * 4u);
+  if constexpr (FUSED) {
+    const uint32_t per_row = (uint32_t)n * 8u * ES, chunks = M * per_row;
+    const i32x4_sgpr rx = dma_rsrc(x, (uint32_t)(((int64_t)(p.M - 1) * x_stride + p.K) * ES));
+    for (uint32_t i0 = wave * 64u; i0 < chunks; i0 += 256u) {
+      const uint32_t i = i0 + (uint32_t)lane, r = M == 1 ? 0u : i / per_row, b = k0 * ES + (i - r * per_row) * 16u;
+      load_lds16(rx, i < chunks && b < (uint32_t)p.K * ES ? r * (uint32_t)x_stride * ES + b : kPastEnd,
+                 base + at.raw + i0 * 16u);
+    }
+  } else {
+    const uint32_t per_block = M * 8u, chunks = (uint32_t)n * per_block;
+    const i32x4_sgpr ra = dma_rsrc(p.act, (uint32_t)(p.M - 1) * (uint32_t)p.lda + k16);
+    for (uint32_t i0 = wave * 64u; i0 < chunks; i0 += 256u) {
+      const uint32_t i = i0 + (uint32_t)lane, b = i / per_block, r = (i - b * per_block) >> 3;
+      const uint32_t k = k0 + b * 128u + (((i & 7u) ^ (uint32_t)chunk_swizzle((int)r)) << 4);
+      load_lds16(ra, i < chunks && k < k16 ? r * (uint32_t)p.lda + k : kPastEnd, base + at.codes + i0 * 16u);
+    }
+    const i32x4_sgpr rx = dma_rsrc(p.xscales, (uint32_t)((p.M - 1) * p.xs_row + (kblocks - 1) * p.xs_block) * 4u + 4u);
+    for (uint32_t i0 = wave * 64u; i0 < M * (uint32_t)n; i0 += 256u) {
+      const uint32_t i = i0 + (uint32_t)lane, b = i / M, r = i - b * M;
+      load_lds4(rx, i < M * (uint32_t)n ? (r * (uint32_t)p.xs_row + (kb0 + b) * (uint32_t)p.xs_block) * 4u : kPastEnd,
+                base + at.xs + i0 * 4u);
+    }
+  }
+
+  // the wave's 16 weight rows (none past N)
+  const int nw = tile * kRowsN + wave * 16, nrows = min(16, p.N - nw);
+  const i32x4_sgpr rw = dma_rsrc(p.weight + (int64_t)(nrows > 0 ? nw : 0) * p.ldw,
+                                 nrows > 0 ? (uint32_t)(nrows - 1) * (uint32_t)p.ldw + k16 : 0u);
+  const int rl = lane >> 3, c = lane & 7;
+  const uint32_t rest = k16 & 127u, tail_kb = rest ? k16 >> 7 : ~0u, lastkb = (uint32_t)(kb0 + n - 1);
+  const uint32_t ring = base + (uint32_t)wave * (STAGES * 2048u);
+  uint32_t vw[2];
+  bool past[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t cw = 16u * (uint32_t)(c ^ rl ^ j);
+    vw[j] = (uint32_t)(8 * j + rl) * (uint32_t)p.ldw + cw;
+    past[j] = cw >= rest;
+  }
+  auto issue = [&](uint32_t kb, int stage) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t off = vw[j] + kb * 128u;
+      if (kb == tail_kb) off = past[j] ? kPastEnd : off;
+      load_lds16(rw, off, ring + (uint32_t)(stage * 2048 + j * 1024));
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) issue(min((uint32_t)(kb0 + s), lastkb), s);
+  wait_vmcnt<2 * STAGES>();  // the rows, but not the ring
+  __syncthreads();
+  if constexpr (FUSED) {
+    typedef typename Elem<DT>::T T;
+    // 16 lanes a block of a row, 8 features a lane
+    const uint32_t sub = (uint32_t)tid & 15u, total = M * (uint32_t)n;
+    for (uint32_t i = (uint32_t)tid >> 4; i < total; i += 16u) {  // uniform over the 16 lanes
+      const uint32_t r = M == 1 ? 0u : i / (uint32_t)n, b = i - r * (uint32_t)n;
+      float v[8];
+      load8<DT>((const T*)(smem + at.raw) + (i * 128u + sub * 8u), v);
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+      const Fp8Scale sc = fp8_scale(max_of_16(most));
+      const uint2 w = {fp8_codes4(v, sc.inverse), fp8_codes4(v + 4, sc.inverse)};
+      const uint32_t row = b * M + r, chunk = (sub >> 1) ^ (uint32_t)chunk_swizzle((int)r);
+      *(uint2*)(smem + at.codes + row * 128u + (chunk << 4) + (sub & 1u) * 8u) = w;
+      if (sub == 0) ((float*)(smem + at.xs))[row] = sc.scale;
+    }
+    __syncthreads();
+  }
+
+  const int q = lane >> 4, r = lane & 15, ra = min(r, p.M - 1);  // columns past M: some row's, never stored
+  const auto fragment = [&](const uint8_t* row, int swizzle) {
+    const i32x4 lo = *(const i32x4*)(row + ((2 * q) ^ swizzle) * 16);
+    const i32x4 hi = *(const i32x4*)(row + ((2 * q + 1) ^ swizzle) * 16);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  const uint8_t* wr = smem + wave * (STAGES * 2048) + r * 128;
+  const uint8_t* ar = smem + at.codes + ra * 128;
+  const float *xs = (const float*)(smem + at.xs) + ra, *ws = (const float*)(smem + at.ws);
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  int st = 0;
+  for (int i = 0; i < n; ++i) {
+    wait_vmcnt<2 * (STAGES - 1)>();
+    const auto w = fragment(wr + st * 2048, chunk_swizzle(r));
+    const auto a = fragment(ar + (uint32_t)i * M * 128u, chunk_swizzle(ra));
+    const float s = xs[(uint32_t)i * M] * ws[i];
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (DT == kF32) {
+      const WideCodes wide = widen_codes(w), act = widen_codes(a);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide.v[j], act.v[j], sum, 0, 0, 0);
+    } else {
+      sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, sum, 0, 0, 0, 0, 0, 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
+    issue(min((uint32_t)(kb0 + i + STAGES), lastkb), st);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = __builtin_fmaf(sum[j], s, acc[j]);
+    st = st + 1 == STAGES ? 0 : st + 1;
+  }
+  wait_vmcnt<0>();
+
+  if (split.splits > 1) {
+    const __amdgpu_buffer_rsrc_t rp =
+        partial_rsrc(split.partials + (size_t)tile * split.splits * 4096, (uint32_t)split.splits * 4096u);
+    store_partial(rp, (uint32_t)(part * 4096 + tid * 16), __builtin_bit_cast(i32x4, acc));
+    if (!last_to_arrive(split.counters + tile, split.splits, &last)) return;
+    acc = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < split.splits; ++s)
+      acc += __builtin_bit_cast(f32x4, load_partial(rp, (uint32_t)(s * 4096 + tid * 16)));
+  }
+  const int nn = nw + 4 * q;
+  if (r >= p.M || nn >= p.N) return;
+  float o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = acc[j] + (p.bias ? p.bias[min(nn + j, p.N - 1)] : 0.0f);
+  const W8a8Operands out{nullptr, nullptr, 0, 0, nullptr, nullptr, nullptr, p.out, p.M, p.N, p.K, p.gr};
+  store4<DT>(out, r, nn, (p.N & 3) == 0, o);
+}
+
+// ---- choice of kernel
 
 // Time of a tile's block of 128 features (few tiles, and with every CU busy), and what its prologue and
 // epilogue add, in microseconds, fitted to 16-bit products without a residual on weights from memory.
@@ -98,9 +277,45 @@ int grouped_tile(const Fp8Operands& p) {
   return best;
 }
 
+// Workgroups that share the K of the few-row kernel's tiles: while the chip is not full, up to 8, and a part keeps 12
+// blocks.  1 row 15360 -> 5120 (80 tiles) 19.8 us with one, 17.7 with three (the rule's), 20.3 with eight; 16384 ->
+// 1024 (16 tiles) 20.0 with one, 10.5 with eight (the rule's), 13.8 with sixteen; 4096 -> 1024 7.1 with one, 8.1 with
+// two (the rule's), but for 16 rows, on the short ring, 11.2 and 10.6.
+int rows_splits(int64_t tiles, int kblocks, const Workspace& work) {
+  const int forced = tuning(kTuneFp8Split);
+  const int64_t s = forced > 0 ? forced : std::min<int64_t>({256 / tiles, kblocks / 12, 8});
+  return (int)std::max<int64_t>(1, std::min<int64_t>(s, most_splits(tiles, kblocks, 4096, work)));
+}
+
+// Whether the few-row kernel takes a product: its rows' codes beside the ring, two workgroups a CU.
+bool few_rows(const Fp8Operands& p) {
+  return tuning(kTuneFp8Tile) <= 0 && p.M <= kRowsMax &&
+         rows_lds(4, p.M, (p.K + kBlock - 1) / kBlock, 0).end <= kTwoPerCu;
+}
+
+template <int DT, bool FUSED>
+hipError_t launch_few_rows(const Fp8Operands& p, const void* x, int64_t x_stride, const Workspace& work,
+                           hipStream_t s) {
+  const int64_t tiles = ((int64_t)p.N + kRowsN - 1) / kRowsN;
+  const int kblocks = (p.K + kBlock - 1) / kBlock;
+  const W8a8Split split = make_split(rows_splits(tiles, kblocks, work), kblocks, work);
+  const int raw = FUSED ? (DT == kF32 ? 4 : 2) : 0;
+  const dim3 grid((unsigned)(tiles * split.splits));
+  // two workgroups a CU where the rows leave room beside the deep ring, else beside the short one
+  const uint32_t deep = rows_lds(8, p.M, split.kblocks, raw).end, flat = rows_lds(4, p.M, split.kblocks, raw).end;
+  if (deep <= kTwoPerCu || flat > kTwoPerCu)
+    fp8_few_rows_kernel<DT, FUSED, 8><<<grid, dim3(256), deep, s>>>(p, x, x_stride, split, (int)tiles);
+  else
+    fp8_few_rows_kernel<DT, FUSED, 4><<<grid, dim3(256), flat, s>>>(p, x, x_stride, split, (int)tiles);
+  return hipGetLastError();
+}
+
 template <int DT>
 hipError_t launch_t(const Fp8Operands& p, const Workspace& work, hipStream_t s) {
   const int kblocks = (p.K + 127) / 128;
+  // (scales far apart: the tiles walk to them block by block)
+  if (!p.g.offsets && few_rows(p) && (p.M - 1) * p.xs_row + (int64_t)kblocks * p.xs_block < (int64_t(1) << 29))
+    return launch_few_rows<DT, false>(p, nullptr, 0, work, s);
   if (p.g.offsets) return launch_fp8_tile<DT>(grouped_tile(p), p, make_split(1, kblocks, work), s);
   const Choice c = choose(p.M, p.N, p.K, work);
   return launch_fp8_tile<DT>(c.tile, p, make_split(c.splits, kblocks, work), s);
@@ -124,12 +339,38 @@ hipError_t launch_fp8_gemm(const Fp8Operands& p, int out_dtype, hipStream_t stre
   }
 }
 
-int64_t fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  const Workspace all{(uint8_t*)256, kSkWorkspaceBytes};  // never read here
+bool fp8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
+  const int64_t es = dtype == kF32 ? 4 : 2;
+  return tuning(kTuneFp8Tile) <= 0 && M <= kRowsMax && M * K * es <= (M == 1 ? kFusedRowBytes : kFusedBytes) &&
+         K * es % 16 == 0 && ((uintptr_t)x & 15) == 0 &&
+         (M == 1 || (x_stride * es % 16 == 0 && x_stride < (int64_t(1) << 24)));
+}
+
+hipError_t launch_fp8_fused(const Fp8Operands& p, const void* x, int64_t x_stride, int dtype, hipStream_t stream,
+                            const Workspace& work) {
+  switch (dtype) {
+    case kF32: return launch_few_rows<kF32, true>(p, x, x_stride, work, stream);
+    case kF16: return launch_few_rows<kF16, true>(p, x, x_stride, work, stream);
+    default: return launch_few_rows<kBF16, true>(p, x, x_stride, work, stream);
+  }
+}
+
+static int64_t fp8_tile_workspace_bytes(int64_t M, int64_t N, int64_t K, const Workspace& all) {
   const Choice c = choose(M, N, K, all);
   if (c.tile == 0 || c.splits <= 1) return 0;
   const int64_t bm = c.tile & 1023, bn = c.tile >> 10, tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
   return (int64_t)kW8a8PartialOffset + tiles * c.splits * bm * bn * 4;
+}
+
+int64_t fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  const Workspace all{(uint8_t*)256, kSkWorkspaceBytes};  // never read here
+  if (M <= kRowsMax && tuning(kTuneFp8Tile) <= 0) {
+    // the few-row kernel, if it takes the product (the tiles may need more: the larger of both)
+    const int64_t tiles = (N + kRowsN - 1) / kRowsN, splits = rows_splits(tiles, (int)((K + 127) / 128), all);
+    const int64_t rows = splits > 1 ? (int64_t)kW8a8PartialOffset + tiles * splits * 4096 : 0;
+    return std::max(rows, fp8_tile_workspace_bytes(M, N, K, all));
+  }
+  return fp8_tile_workspace_bytes(M, N, K, all);
 }
 
 }  // namespace convrot

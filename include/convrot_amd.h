@@ -586,7 +586,8 @@ int convrot_quantize_fp8_weight(const void* w, int dtype, int64_t N, int64_t K, 
  * apart; bias float32 [N] or NULL.  residual, gate and workspace as in convrot_w8a8_gemm (the same
  * workspace serves both); convrot_fp8_workspace_bytes says how much of it one product uses.
  * convrot_fp8_linear: the same from x [M, K] of `dtype`, quantized into `scratch`
- * (convrot_fp8_scratch_bytes, 16-byte aligned, any content).
+ * (convrot_fp8_scratch_bytes, 16-byte aligned, any content), which may be NULL where convrot_fp8_fused says that
+ * the rows are quantized inside the product's launch (few rows) and out does not overlap x.
  */
 int convrot_fp8_gemm(const uint8_t* act, int64_t act_stride, const float* xscales, int64_t xscales_row,
                      int64_t xscales_block, const uint8_t* weight, int64_t weight_stride, const float* wscales,
@@ -595,6 +596,7 @@ int convrot_fp8_gemm(const uint8_t* act, int64_t act_stride, const float* xscale
                      int64_t workspace_bytes, void* out, int out_dtype, void* stream);
 int64_t convrot_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int64_t convrot_fp8_scratch_bytes(int64_t rows, int64_t K);
+int convrot_fp8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride);
 int convrot_fp8_linear(const void* x, int dtype, int64_t x_stride, const uint8_t* weight, int64_t weight_stride,
                        const float* wscales, int64_t wscales_stride, const float* bias, int64_t M, int64_t N,
                        int64_t K, const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate,

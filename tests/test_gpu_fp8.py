@@ -149,6 +149,48 @@ def test_shared_k(dev, tuning, tile, m, split):
         assert torch.equal(hip_fp8_linear(x.to(dev), q, ws), first)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("split", [None, 1, 3])
+@pytest.mark.parametrize("m,k", [(1, 4096), (1, 16384), (2, 1032), (5, 72), (7, 2304), (16, 512), (16, 1096), (16, 4160)])
+def test_few_rows(dev, tuning, m, k, split, dtype):
+    """Rows quantized inside the product's launch, in a launch of their own (longer or unaligned rows), and as
+    codes: the same bits."""
+    from convrot_mlx_amd import hip_fp8_linear, hip_fp8_matmul, quantize_fp8_blockwise
+
+    if split:
+        tuning.set("fp8_split", split)
+    n = 330
+    q, ws = weight(k, n, k, dev)
+    bias, x = normal(n, n).to(dev), normal(m, m, k).to(dtype)
+    want, spread = plain.product(plain.row_values(*plain.codes(x)).to(dev), plain.weight_values(q, ws), dtype == F32)
+    x = x.to(dev)
+    got = hip_fp8_linear(x, q, ws, bias)
+    # (the parts' sums are added in float32: up to `parts` more roundings)
+    assert_within(got, want + bias.double(), 2 * spread + U * (bias.abs().double() + want.abs()))
+    codes, scales = quantize_fp8_blockwise(x)
+    assert torch.equal(hip_fp8_matmul(codes, q, scales, ws, bias, output_dtype=dtype), got)
+    apart = torch.full((m, k + 9), float("nan"), dtype=dtype, device=dev)
+    apart[:, 1:k + 1] = x
+    assert torch.equal(hip_fp8_linear(apart[:, 1:k + 1], q, ws, bias), got)
+    apart = torch.full((2 * m, k), float("nan"), dtype=dtype, device=dev)
+    apart[::2] = x
+    assert torch.equal(hip_fp8_linear(apart[::2], q, ws, bias), got)
+
+
+def test_few_rows_in_place_of_their_residual(dev):
+    """A residual that is the input itself, written in place: no workgroup may read what another has written."""
+    from convrot_mlx_amd import hip_fp8_linear
+
+    for m in (1, 8):
+        q, ws = weight(3, 2048, 2048, dev)
+        x = normal(m, m, 2048).to(BF16).to(dev)
+        want = hip_fp8_linear(x, q, ws, residual=x)
+        for _ in range(3):
+            got = x.clone()
+            assert hip_fp8_linear(got, q, ws, residual=got, inplace=True) is got
+            assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("k", [50, 64, 200])
 def test_strided_and_unaligned_operands(dev, k):
     from convrot_mlx_amd import hip_fp8_matmul
