@@ -454,6 +454,11 @@ template <int ODT, int KIND>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_large_kernel(Fp8Operands p,
                                                                                                  int tiles_m,
                                                                                                  int tiles_n, int slots) {
+  using E = Fp8Engine<256, 256, 4, 2, 2, 1, true>;
+  using Half = Fp8Engine<256, 128, 4, 2, 2, 1, false>;
+  using Quarter = Fp8Engine<128, 128, 2, 4, 2, 1, false>;
+  static_assert(Half::WS_OFF <= E::WS_OFF && Half::WS <= E::WS && Quarter::WS_OFF <= E::WS_OFF && Quarter::WS <= E::WS,
+                "the parts lie in the LDS of a whole tile");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   tiles_m = tile_rows_of<256, KIND>(p, tiles_m);
   const int tiles = tiles_m * tiles_n;
@@ -463,7 +468,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const TilePlace at = place_of(t, last.whole, tiles_m, tiles_n);
     const GroupTile r = rows_at<256, KIND>(p, at.row);
     if (r.expert < 0) return;
-    fp8_tile<Fp8Engine<256, 256, 4, 2, 2, 1, true>, ODT, KIND>(smem, p, r.expert, r.row0, r.row_end, at.column * 256);
+    fp8_tile<E, ODT, KIND>(smem, p, r.expert, r.row0, r.row_end, at.column * 256);
     return;
   }
   const int u = t - last.whole, tile = last.whole + u / last.parts, part = u % last.parts;
@@ -475,10 +480,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   if (r.expert < 0) return;
   const int n0 = in_group / group_rows * 256 + (part & 1) * 128, m0 = r.row0 + (part >> 1) * 128;
   if (n0 >= p.N || m0 >= r.row_end) return;
-  if (last.parts == 2)
-    fp8_tile<Fp8Engine<256, 128, 4, 2, 2, 1, false>, ODT, KIND>(smem, p, r.expert, m0, r.row_end, n0);
-  else
-    fp8_tile<Fp8Engine<128, 128, 2, 4, 2, 1, false>, ODT, KIND>(smem, p, r.expert, m0, r.row_end, n0);
+  if (last.parts == 2) fp8_tile<Half, ODT, KIND>(smem, p, r.expert, m0, r.row_end, n0);
+  else fp8_tile<Quarter, ODT, KIND>(smem, p, r.expert, m0, r.row_end, n0);
 }
 
 template <int BM, int BN, int WM, int WN, int STAGES, int PER_CU, bool IN_SLOTS, int ODT, int KIND>

@@ -399,7 +399,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                                                                                                      int slots) {
   constexpr bool AA = KIND == 3, AB = KIND >= 2;
   using E = Engine16<256, 256, 2, DT, AA, AB>;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES];
+  using Half = Engine16<256, 128, 3, DT, AA, AB>;
+  using Quarter = Engine16<128, 128, 4, DT, AA, AB>;
+  constexpr int PARTS = Half::SMEM_BYTES > Quarter::SMEM_BYTES ? Half::SMEM_BYTES : Quarter::SMEM_BYTES;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES > PARTS ? E::SMEM_BYTES : PARTS];
   if constexpr (KIND != 3) tiles_i = group_tile_rows<256>(p.g, p.R);
   const int tiles = tiles_i * tiles_j * (KIND == 3 ? p.g.experts : 1), t = blockIdx.x;
   const LastRound last = last_round(tiles, slots);
@@ -416,10 +419,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   if (at.expert < 0) return;
   const int m0 = at.row0 + (part >> 1) * 128, n0 = column * 256 + (part & 1) * 128;
   if (m0 >= at.row_end || n0 >= (KIND == 3 ? p.C : p.N)) return;
-  if (last.parts == 2)
-    grouped_tile<Engine16<256, 128, 3, DT, AA, AB>, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
-  else
-    grouped_tile<Engine16<128, 128, 4, DT, AA, AB>, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
+  if (last.parts == 2) grouped_tile<Half, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
+  else grouped_tile<Quarter, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
 }
 
 template <int BM, int BN, int STAGES, int PER_CU, int DT, int KIND>

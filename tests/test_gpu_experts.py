@@ -206,6 +206,28 @@ def test_fp8_every_tile(dev, tuning, tile):
         assert not got[at[-1]:].any()
 
 
+@pytest.mark.parametrize("tokens,n", [(2500, 2000), (2500, 7690), (300, 1000)])
+def test_fp8_last_round_in_parts(dev, tuning, tokens, n):
+    """Large tiles whose last round runs as halves (80 of 256 CUs; 341, 85 past a round) and as quarters."""
+    from convrot_mlx_amd import expert_plan, hip_fp8_grouped_linear, hip_fp8_linear
+
+    tuning.set("fp8_tile", "256x256")
+    experts, k = 2, 272
+    plan = expert_plan(choose(n, tokens, 1, experts).to(dev), experts)
+    q, ws = fp8_weight(n, experts, n, k, dev)
+    x = normal(n, tokens, k).to(BF16)
+    values = plain.row_values(*plain.codes(x)).to(dev)
+    assert_within(hip_fp8_linear(x.to(dev), q[1], ws[1]), *plain.product(values, plain.weight_values(q[1], ws[1]), False))
+    for gather in (False, True):
+        got = hip_fp8_grouped_linear(x.to(dev), q, ws, plan, gather=gather)
+        rows = values[plan.order.long()] if gather else values
+        at = plan.offsets.tolist()
+        for e in range(experts):
+            want, spread = plain.product(rows[at[e]: at[e + 1]], plain.weight_values(q[e], ws[e]), False)
+            assert_within(got[at[e]: at[e + 1]], want, spread, f"expert {e}")
+        assert not got[at[-1]:].any()
+
+
 def test_fp8_operands_of_other_layouts(dev):
     from convrot_mlx_amd import ExpertPlan, expert_plan, hip_fp8_grouped_linear
 
@@ -344,6 +366,15 @@ def test_every_tile(dev, tuning, tile, tokens, choices, experts, n, k):
     tuning.set("grouped_tile", tile)
     for gather in (False, True):
         check_products(dev, tokens, choices, experts, n, k, BF16, gather, seed=1)
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("n,k", [(2000, 1960), (264, 7690), (7690, 264)])
+def test_last_round_in_parts(dev, tuning, n, k, gather):
+    """Large tiles whose last round runs as halves (80 to 128 of 256 CUs, behind a whole round of 256 too) or as
+    quarters, of outputs and of both gradients."""
+    tuning.set("grouped_tile", "256x256")
+    check_products(dev, 1250, 2, 2, n, k, BF16, gather)
 
 
 def test_operands_of_other_layouts(dev):
