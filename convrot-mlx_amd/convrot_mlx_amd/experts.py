@@ -49,8 +49,8 @@ def expert_plan(ids: torch.Tensor, experts: int) -> ExpertPlan:
     count = ids.numel()
     lib = nat.load()
     offsets = torch.empty((experts + 1,), dtype=torch.int32, device=device)
-    places = torch.empty((2, count), dtype=torch.int32, device=device)
-    order, slots = places[0], places[1].view(ids.shape if ids.ndim == 2 else (count, 1))
+    order = torch.empty((count,), dtype=torch.int32, device=device)
+    slots = torch.empty(ids.shape if ids.ndim == 2 else (count, 1), dtype=torch.int32, device=device)
     with nat.on(device):
         need = lib.convrot_expert_plan_workspace_bytes(count, experts)
         work = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
@@ -317,13 +317,11 @@ def hip_grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch
             dx = hip_combine_rows(dx, plan)
     if weight_grad:
         rows = _operand16(_gather_rows(x, r.index, r.choices) if gather else x)
-        wide = k if n * k % 8 == 0 or experts == 1 else (k + 7) // 8 * 8  # every expert's gradient 16-byte aligned
-        dw = torch.empty((experts, n, wide), dtype=x.dtype, device=device)
+        dw = torch.empty((experts, n, k), dtype=x.dtype, device=device)
         with nat.on(device):
             nat.check(lib.convrot_grouped_linear_weight_grad(
                 g.data_ptr(), code, _stride16(g), rows.data_ptr(), _stride16(rows), r.offsets.data_ptr(), experts, r.rows, n,
-                wide, dw.data_ptr(), nat.stream_handle(device)))
-        dw = dw[..., :k].contiguous()
+                k, dw.data_ptr(), nat.stream_handle(device)))
     return dx, dw
 
 

@@ -313,8 +313,8 @@ __device__ __forceinline__ void load_bias4(const Fp8Operands& p, int n, float (&
 }
 
 // The wave's corner of the tile: bias, gated residual, rounding, store; rows m0 .. row_end - 1.  16-bit
-// outputs (and residuals) go through the wave's part of LDS in whole aligned chunks of 16 bytes.
-template <class E, int ODT, bool ALIGNED>
+// outputs (and residuals) go through the wave's part of LDS in chunks of 16 bytes.
+template <class E, int ODT>
 __device__ __forceinline__ void fp8_epilogue16(const E& e, const f32x4 (&acc)[E::FN][E::FM], const Fp8Operands& p, int m0,
                                                int row_end, int n0) {
   constexpr int FM = E::FM, FN = E::FN, TM = E::TM, TN = E::TN, RS = TN * 2 + 16;
@@ -323,14 +323,8 @@ __device__ __forceinline__ void fp8_epilogue16(const E& e, const f32x4 (&acc)[E:
   const bool residual = p.gr.residual != nullptr;
   const bool one_gate = residual && mw / p.gr.rows_per_gate == (min(mw + TM, row_end) - 1) / p.gr.rows_per_gate;
   if (residual) {
-    move_corner<TM, TN, ALIGNED, false, (FM * FN > 16 ? 4 : 16)>(region, (uint16_t*)p.gr.residual, lane, mw, nw, row_end, p.N);
+    move_rows<TM, TN, false, (FM * FN > 16 ? 4 : 16)>(region, (uint16_t*)p.gr.residual, lane, mw, nw, row_end, p.N);
     wave_lds_fence();
-  }
-  uint8_t* at[FM];
-#pragma unroll
-  for (int fm = 0; fm < FM; ++fm) {
-    const int row = fm * 16 + (lane & 15);
-    at[fm] = region + row * RS + (ALIGNED ? 0 : 2 * (int)(((int64_t)(mw + row) * p.N + nw) & 7));
   }
   static_for<FN>([&](auto frag) __attribute__((always_inline)) {
     constexpr int fn = frag.value;
@@ -343,30 +337,20 @@ __device__ __forceinline__ void fp8_epilogue16(const E& e, const f32x4 (&acc)[E:
       float o[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[r] = acc[fn][fm][r] + b[r];
-      uint16_t* q = (uint16_t*)(at[fm] + nl * 2);
+      uint16_t* q = (uint16_t*)(region + (fm * 16 + (lane & 15)) * RS + nl * 2);
       if (residual) {
         const int m = mw + fm * 16 + (lane & 15);
         if (!one_gate && m < row_end) load_gate4<ODT>(p.gr, m, nw + nl, p.N, g);
         float res[4];
-        if constexpr (ALIGNED) {
-          load_elem4<ODT>(q, 0, res);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) res[r] = load_elem<ODT>(q, r);
-        }
+        load_elem4<ODT>(q, 0, res);
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = res[r] + g[r] * o[r];
       }
-      if constexpr (ALIGNED) {
-        store_out4<ODT>(q, 0, o[0], o[1], o[2], o[3]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) store_out<ODT>(q, r, o[r]);
-      }
+      store_out4<ODT>(q, 0, o[0], o[1], o[2], o[3]);
     }
   });
   wave_lds_fence();
-  move_corner<TM, TN, ALIGNED, true>(region, (uint16_t*)p.out, lane, mw, nw, row_end, p.N);
+  move_rows<TM, TN, true>(region, (uint16_t*)p.out, lane, mw, nw, row_end, p.N);
 }
 
 template <class E>
@@ -420,8 +404,7 @@ __device__ __forceinline__ void fp8_epilogue(const E& e, const f32x4 (&acc)[E::F
                                              int row_end, int n0) {
   __syncthreads();  // every wave is done with the ring before it stages outputs
   if constexpr (ODT == kF32) fp8_epilogue32<E>(e, acc, p, m0, row_end, n0);
-  else if ((p.N & 7) == 0) fp8_epilogue16<E, ODT, true>(e, acc, p, m0, row_end, n0);
-  else fp8_epilogue16<E, ODT, false>(e, acc, p, m0, row_end, n0);
+  else fp8_epilogue16<E, ODT>(e, acc, p, m0, row_end, n0);
 }
 
 template <class E>

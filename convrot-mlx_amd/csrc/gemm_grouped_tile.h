@@ -277,37 +277,25 @@ struct Engine16 {
   }
 };
 
-// The wave's corner of the tile of a [.., N] array: rounded, then by its part of LDS in whole aligned
-// chunks of 16 bytes; rows below row_end.
-template <class E, int DT, bool ALIGNED>
+// The wave's corner of the tile of a [.., N] array: rounded, then by its part of LDS in chunks of 16 bytes; rows
+// below row_end.
+template <class E, int DT>
 __device__ __forceinline__ void store_tile(const E& e, const f32x4 (&acc)[E::FN][E::FM], void* out, int m0, int row_end,
                                            int n0, int N) {
   constexpr int FM = E::FM, FN = E::FN, TM = E::TM, TN = E::TN, RS = TN * 2 + 16;
   const int lane = e.lane, mw = m0 + e.wm * TM, nw = n0 + e.wn * TN;
   uint8_t* region = e.smem + e.wave * (TM * RS);
-  uint8_t* at[FM];
-#pragma unroll
-  for (int fm = 0; fm < FM; ++fm) {
-    const int row = fm * 16 + (lane & 15);
-    at[fm] = region + row * RS + (ALIGNED ? 0 : 2 * (int)(((int64_t)(mw + row) * N + nw) & 7));
-  }
   static_for<FN>([&](auto frag) __attribute__((always_inline)) {
     constexpr int fn = frag.value;
     const int nl = fn * 16 + 4 * (lane >> 4);
 #pragma unroll
     for (int fm = 0; fm < FM; ++fm) {
       const f32x4 v = acc[fn][fm];
-      uint16_t* q = (uint16_t*)(at[fm] + nl * 2);
-      if constexpr (ALIGNED) {
-        store_out4<DT>(q, 0, v[0], v[1], v[2], v[3]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) store_out<DT>(q, r, v[r]);
-      }
+      store_out4<DT>((uint16_t*)(region + (fm * 16 + (lane & 15)) * RS + nl * 2), 0, v[0], v[1], v[2], v[3]);
     }
   });
   wave_lds_fence();
-  move_corner<TM, TN, ALIGNED, true>(region, (uint16_t*)out, lane, mw, nw, row_end, N);
+  move_rows<TM, TN, true>(region, (uint16_t*)out, lane, mw, nw, row_end, N);
 }
 
 // One tile: output rows m0 .. (m0 + BM or) row_end - 1, columns n0 .., of an expert (whose rows, with KIND 3, are
@@ -350,9 +338,7 @@ __device__ __forceinline__ void grouped_tile(uint8_t* smem, const GroupedOperand
     e.run((p.C + 63) / 64, acc);
   }
   __syncthreads();  // every wave is done with the ring before it stages outputs
-  // chunks are aligned where every row of the array is
-  if ((columns & 7) == 0) store_tile<E, DT, true>(e, acc, out, m0, row_end, n0, columns);
-  else store_tile<E, DT, false>(e, acc, out, m0, row_end, n0, columns);
+  store_tile<E, DT>(e, acc, out, m0, row_end, n0, columns);
 }
 
 // Where the t-th tile of a launch lies.  The first `turns` of them go to the XCDs (and their L2s) in runs of

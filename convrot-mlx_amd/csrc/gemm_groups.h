@@ -76,6 +76,54 @@ __host__ __device__ __forceinline__ LastRound last_round(int tiles, int slots) {
   return {parts == 1 ? tiles : tiles - rest, parts};
 }
 
+// A wave's TM x TN corner of a 16-bit [.., N] array between memory and its LDS rows (TN * 2 + 16 bytes apart), 16 bytes a
+// lane and step; rows below row_end.  A row of any N begins anywhere: the hardware takes 16 bytes at any address, which
+// for odd N costs less than shifting the rows in LDS to whole aligned chunks with part chunks at both ends of every
+// corner's row (STORENOTE).  BATCH loads of a lane are in flight at a time.
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+template <int TM, int TN, bool STORE, int BATCH = 16>
+__device__ __forceinline__ void move_rows(uint8_t* region, uint16_t* base, int lane, int mw, int nw, int row_end, int N) {
+  constexpr int RS = TN * 2 + 16, CPR = TN / 8, NIT = TM * CPR / 64;
+  static_assert(TM * CPR % 64 == 0, "whole steps");
+  const int cols = min(TN, N - nw), rows = min(TM, row_end - mw);
+  if constexpr (!STORE) {
+    for (int b0 = 0; b0 < NIT; b0 += BATCH) {
+      u32x4 v[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int c = (b0 + i) * 64 + lane, row = c / CPR, first = c % CPR * 8;
+        v[i] = (u32x4){0, 0, 0, 0};
+        if (row < rows && first + 8 <= cols)
+          v[i] = *(const u32x4_at2*)(base + (int64_t)(mw + row) * N + nw + first);
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int c = (b0 + i) * 64 + lane;
+        if (c < TM * CPR) *(u32x4*)(region + c / CPR * RS + c % CPR * 16) = v[i];
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (int it = 0; it < NIT; ++it) {
+      const int c = it * 64 + lane, row = c / CPR, first = c % CPR * 8;
+      if (row < rows && first + 8 <= cols)
+        *(u32x4_at2*)(base + (int64_t)(mw + row) * N + nw + first) = *(const u32x4*)(region + row * RS + first * 2);
+    }
+  }
+  // the last columns where N is no multiple of 8, 8 lanes a row
+  const int last = cols & ~7;
+  if (last < cols && last >= 0) {
+    for (int row = lane >> 3; row < rows; row += 8) {
+      const int col = last + (lane & 7);
+      if (col >= cols) continue;
+      uint16_t* at = (uint16_t*)(region + row * RS) + col;
+      uint16_t* g = base + (int64_t)(mw + row) * N + nw + col;
+      if constexpr (STORE) *g = *at;
+      else *at = *g;
+    }
+  }
+}
+
 // Most rows of tiles that any split of `rows` over the experts (and none) makes.
 inline int64_t most_tile_rows(int64_t rows, int64_t experts, int bm) {
   const int64_t bound = rows / bm + experts + 1;

@@ -242,12 +242,13 @@ __device__ __forceinline__ void wave_lds_fence() {
 // LDS rows, 16 aligned bytes a lane: row r's first column sits at element
 // (m N + nw) % 8 of its LDS row, so that aligned chunks of the array are aligned
 // in LDS whatever N is.  ALIGNED: N % 8 == 0 (that element is 0, no part chunks).
-// BATCH loads of a lane are in flight at a time.
-template <int TM, int TN, bool ALIGNED, bool STORE, int BATCH = 16>
+template <int TM, int TN, bool ALIGNED, bool STORE>
 __device__ __forceinline__ void move_corner(uint8_t* region, uint16_t* base, int lane, int mw, int nw, int M, int N) {
   constexpr int RS = TN * 2 + 16, CPR = ALIGNED ? TN / 8 : TN / 8 + 1, NIT = (TM * CPR + 63) / 64;
   const int cols = min(TN, N - nw), rows = min(TM, M - mw);
   if constexpr (!STORE) {
+    // 16 loads in flight at a time
+    constexpr int BATCH = 16;
     for (int b0 = 0; b0 < NIT; b0 += BATCH) {
       u32x4 v[BATCH];
 #pragma unroll
