@@ -90,7 +90,7 @@ SIGNATURES = {
                                 _i64, _vp, _i64, _vp, _i32, _vp]),
     "convrot_fp8_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "convrot_fp8_scratch_bytes": (_i64, [_i64, _i64]),
-    "convrot_fp8_fused": (_i32, [_vp, _i32, _i64, _i64, _i64]),
+    "convrot_fp8_fused": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64]),
     "convrot_fp8_linear": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64,
                                   _vp, _i64, _vp, _i64, _vp, _vp]),
     "convrot_fp8_grouped_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64,

@@ -185,9 +185,9 @@ def hip_combine_rows_backward(dout: torch.Tensor, rows: torch.Tensor | None, pla
     if dout.ndim != 2 or dout.shape[0] != tokens:
         raise ValueError(f"dout {tuple(dout.shape)} must have a row for each of {tokens} tokens")
     if weights is not None:
-        _combine_checks(rows, plan, weights)
-        if rows.dtype != dout.dtype or rows.shape[1] != dout.shape[1]:
+        if rows.dtype != dout.dtype or rows.ndim != 2 or rows.shape[1] != dout.shape[1]:
             raise ValueError(f"dout {dout.dtype} {tuple(dout.shape)} must match rows {rows.dtype} {tuple(rows.shape)}")
+        _combine_checks(rows, plan, weights)
     elif order.shape[0] != slots.numel():
         raise ValueError(f"the plan's order has {order.shape[0]} rows, its slots {slots.numel()}")
     nat.dtype_code(dout.dtype)
@@ -269,7 +269,6 @@ def _check_grouped(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, gath
     r = _grouped_rows(x, weight.shape[0], plan, gather)
     if x.shape[1] != k:
         raise ValueError(f"experts' weights take K={k} features, got {x.shape[1]}")
-    nat.on_device(x, weight, r.offsets, r.index)
     return r
 
 
@@ -278,6 +277,7 @@ def hip_grouped_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, 
     bfloat16, each times its expert's weight of [E, N, K] -> [R, N]; float32 sums, rounded once.  Rows of no
     expert give zeros.  Features no multiple of 8 copy operands into padded rows."""
     r = _check_grouped(x, weight, plan, gather)
+    nat.on_device(x, weight, r.offsets, r.index)
     experts, n, k = weight.shape
     x, w = _operand16(x), _operand16(weight)
     if r.index is not None and x.shape[0] * _stride16(x) * 2 > MAX_GATHERED_BYTES:
@@ -300,9 +300,9 @@ def hip_grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch
     experts, n, k = weight.shape
     if tuple(dy.shape) != (r.rows, n) or dy.dtype != x.dtype:
         raise ValueError(f"dy must be {x.dtype} {(r.rows, n)}, got {dy.dtype} {tuple(dy.shape)}")
+    nat.on_device(dy, x, weight, r.offsets, r.index)
     if gather and rows_grad:
         _combine_checks(dy, plan, None)
-    nat.on_device(dy, x)
     lib, code, device = nat.load(), nat.dtype_code(x.dtype), x.device
     g = _operand16(dy)
     dx = dw = None

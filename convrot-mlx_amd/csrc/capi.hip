@@ -1191,7 +1191,7 @@ int convrot_fp8_linear(const void* x, int dtype, int64_t x_stride, const uint8_t
   const int64_t es = dtype == CONVROT_DTYPE_F32 ? 4 : 2;
   const uintptr_t xa = (uintptr_t)x, oa = (uintptr_t)out;
   const bool apart = oa + (uintptr_t)(M * N * es) <= xa || xa + (uintptr_t)(((M - 1) * x_stride + K) * es) <= oa;
-  const bool fused = apart && convrot::fp8_fused(x, dtype, M, K, x_stride);
+  const bool fused = apart && convrot::fp8_fused(x, dtype, M, N, K, x_stride);
   if (!fused)
     if (int rc = check_fp8_scratch(scratch, scratch_bytes, M, K)) return rc;
   const Fp8Scratch c = fused ? Fp8Scratch{} : fp8_scratch(scratch, M, K);
@@ -1205,8 +1205,8 @@ int convrot_fp8_linear(const void* x, int dtype, int64_t x_stride, const uint8_t
   return launch_status(e, "convrot_fp8_linear");
 }
 
-int convrot_fp8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
-  return M > 0 && K > 0 && valid_dtype(dtype) && convrot::fp8_fused(x, dtype, M, K, x_stride) ? 1 : 0;
+int convrot_fp8_fused(const void* x, int dtype, int64_t M, int64_t N, int64_t K, int64_t x_stride) {
+  return M > 0 && N > 0 && K > 0 && valid_dtype(dtype) && convrot::fp8_fused(x, dtype, M, N, K, x_stride) ? 1 : 0;
 }
 
 namespace {

@@ -276,7 +276,7 @@ struct Fp8Operands;  // fp8_device.h
 hipError_t launch_fp8_gemm(const Fp8Operands& p, int out_dtype, hipStream_t stream, const Workspace& work);
 
 // Whether a few rows are quantized inside their product's launch, and that launch.
-bool fp8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride);
+bool fp8_fused(const void* x, int dtype, int64_t M, int64_t N, int64_t K, int64_t x_stride);
 hipError_t launch_fp8_fused(const Fp8Operands& p, const void* x, int64_t x_stride, int dtype, hipStream_t stream,
                             const Workspace& work);
 

@@ -4,6 +4,7 @@
 
 #include "convrot_launch.h"
 #include "fp8_device.h"
+#include "gemm_groups.h"
 #include "row_device.h"
 
 namespace convrot {
@@ -261,7 +262,8 @@ Choice choose(int64_t M, int64_t N, int64_t K, const Workspace& work) {
 }
 
 // The tile of grouped rows.  How they spread over the experts is known on the device alone: taken as even, each
-// expert's last tile half full.
+// expert's last tile half full: over 89 sizes (1 to 14000 rows, 1 to 64 experts) the tile taken is 1 % slower than the
+// best of the five on average, 21 % at worst.
 int grouped_tile(const Fp8Operands& p) {
   const int forced = tuning(kTuneFp8Tile);
   if (forced > 0) return forced;
@@ -270,6 +272,7 @@ int grouped_tile(const Fp8Operands& p) {
   int best = 0;
   float best_time = 0.0f;
   for (const Cost& c : kCosts) {
+    if (most_tile_rows(p.M, p.g.experts, c.bm) * ((p.N + c.bn - 1) / c.bn) > max_groups(512) - 1024) continue;
     const float rows = std::max(1.0f, each / (float)c.bm + 0.5f) * (float)met;
     const float t = time_of(c, (int64_t)(rows * (float)((p.N + c.bn - 1) / c.bn)), (float)kblocks);
     if (best == 0 || t < best_time) best_time = t, best = tile_code(c.bm, c.bn);
@@ -287,9 +290,13 @@ int rows_splits(int64_t tiles, int kblocks, const Workspace& work) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(s, most_splits(tiles, kblocks, 4096, work)));
 }
 
-// Whether the few-row kernel takes a product: its rows' codes beside the ring, two workgroups a CU.
+// Whether the few-row kernel takes a product: its workgroups in one launch, its rows' codes beside the ring, two
+// workgroups a CU.
+bool few_rows_shape(int64_t M, int64_t N) {
+  return tuning(kTuneFp8Tile) <= 0 && M <= kRowsMax && (N + kRowsN - 1) / kRowsN <= max_groups(256);
+}
 bool few_rows(const Fp8Operands& p) {
-  return tuning(kTuneFp8Tile) <= 0 && p.M <= kRowsMax &&
+  return few_rows_shape(p.M, p.N) &&
          rows_lds(4, p.M, (p.K + kBlock - 1) / kBlock, 0).end <= kTwoPerCu;
 }
 
@@ -339,9 +346,9 @@ hipError_t launch_fp8_gemm(const Fp8Operands& p, int out_dtype, hipStream_t stre
   }
 }
 
-bool fp8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride) {
+bool fp8_fused(const void* x, int dtype, int64_t M, int64_t N, int64_t K, int64_t x_stride) {
   const int64_t es = dtype == kF32 ? 4 : 2;
-  return tuning(kTuneFp8Tile) <= 0 && M <= kRowsMax && M * K * es <= (M == 1 ? kFusedRowBytes : kFusedBytes) &&
+  return few_rows_shape(M, N) && M * K * es <= (M == 1 ? kFusedRowBytes : kFusedBytes) &&
          K * es % 16 == 0 && ((uintptr_t)x & 15) == 0 &&
          (M == 1 || (x_stride * es % 16 == 0 && x_stride < (int64_t(1) << 24)));
 }
@@ -364,7 +371,7 @@ static int64_t fp8_tile_workspace_bytes(int64_t M, int64_t N, int64_t K, const W
 
 int64_t fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   const Workspace all{(uint8_t*)256, kSkWorkspaceBytes};  // never read here
-  if (M <= kRowsMax && tuning(kTuneFp8Tile) <= 0) {
+  if (few_rows_shape(M, N)) {
     // the few-row kernel, if it takes the product (the tiles may need more: the larger of both)
     const int64_t tiles = (N + kRowsN - 1) / kRowsN, splits = rows_splits(tiles, (int)((K + 127) / 128), all);
     const int64_t rows = splits > 1 ? (int64_t)kW8a8PartialOffset + tiles * splits * 4096 : 0;

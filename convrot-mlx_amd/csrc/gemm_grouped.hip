@@ -55,6 +55,9 @@ int choose(int kind, const GroupedOperands& p) {
   float best_time = 0.0f;
   for (const Cost& c : kCosts) {
     if (kind == 3 && !grouped_weight_tile_known(c.bm, c.bn)) continue;
+    const int64_t most = kind == 3 ? over(p.N, c.bm) * p.g.experts * over(p.C, c.bn)
+                                   : most_tile_rows(p.R, p.g.experts, c.bm) * over(p.N, c.bn);
+    if (most > max_groups(256) - 1024) continue;  // no launch so large
     const float rows = kind == 3 ? (float)(over(p.N, c.bm) * p.g.experts) : tile_rows(p.R, p.g.experts, c.bm);
     const float blocks = kind == 3 ? (float)p.R / (float)met / 64.0f + 0.5f : (float)over(p.C, 64);
     const int64_t groups = (int64_t)(rows * (float)over(kind == 3 ? p.C : p.N, c.bn));
@@ -87,7 +90,8 @@ bool grouped_weight_tile_known(int bm, int bn) {
 
 hipError_t launch_grouped(int kind, const GroupedOperands& p, int dtype, hipStream_t stream) {
   const int tile = choose(kind, p);
-  return dtype == kF16 ? launch_grouped_tile<kF16>(tile, kind, p, stream) : launch_grouped_tile<kBF16>(tile, kind, p, stream);
+  if (dtype == kF16) return launch_grouped_tile<kF16>(tile, kind, p, stream);
+  return launch_grouped_tile<kBF16>(tile, kind, p, stream);
 }
 
 }  // namespace convrot

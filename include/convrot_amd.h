@@ -596,7 +596,7 @@ int convrot_fp8_gemm(const uint8_t* act, int64_t act_stride, const float* xscale
                      int64_t workspace_bytes, void* out, int out_dtype, void* stream);
 int64_t convrot_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int64_t convrot_fp8_scratch_bytes(int64_t rows, int64_t K);
-int convrot_fp8_fused(const void* x, int dtype, int64_t M, int64_t K, int64_t x_stride);
+int convrot_fp8_fused(const void* x, int dtype, int64_t M, int64_t N, int64_t K, int64_t x_stride);
 int convrot_fp8_linear(const void* x, int dtype, int64_t x_stride, const uint8_t* weight, int64_t weight_stride,
                        const float* wscales, int64_t wscales_stride, const float* bias, int64_t M, int64_t N,
                        int64_t K, const void* residual, const void* gate, int64_t gate_stride, int64_t rows_per_gate,
@@ -625,8 +625,8 @@ int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t
  *   dw[e]  = sum over expert e's rows s of dy[s]^T x[s]   (an expert without rows: zeros)
  * x, dy and weight: 16-byte aligned rows, strides (elements) that are multiples of 8 and cover the features
  * rounded up to 8, zeros from there on; weight e at weight + e * weight_expert elements.  out [rows, N],
- * dx [rows, K], dw [experts, N, K] contiguous (several experts' dw: N K a multiple of 8).  Up to 65536
- * features.  The weights' gradient reads sorted rows of x (convrot_gather_rows makes them).
+ * dx [rows, K], dw [experts, N, K] contiguous, 16-byte aligned.  Up to 65536 features.  The weights'
+ * gradient reads sorted rows of x (convrot_gather_rows makes them).
  */
 int convrot_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* weight,
                            int64_t weight_stride, int64_t weight_expert, const int32_t* offsets, int64_t experts,
