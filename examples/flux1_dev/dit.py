@@ -223,7 +223,7 @@ def project(linear: nn.Module, x: torch.Tensor, *, gelu: bool = False, head: tor
     gated residual move into a ConvRotLinear's preparation and epilogue when their flags are
     set; otherwise they are the torch ops FLUX uses."""
     convrot = hasattr(linear, "forward_gelu")
-    quantized = hasattr(linear, "forward_modulated")  # a ConvRotLinear or Int8Linear
+    quantized = hasattr(linear, "forward_modulated")  # a ConvRotLinear, Int8Linear or Fp8Linear
     kw = dict(residual=residual, gate=gate) if fused_residual and quantized and residual is not None else {}
     if gelu and fused_gelu and convrot:
         out = linear.forward_gelu(x, head=head, **kw)
@@ -432,14 +432,14 @@ def time_step(model, inputs, steps: int) -> tuple[torch.Tensor, float, float]:
 
 
 def linear_weight_bytes(model: nn.Module) -> dict:
-    """Device bytes the model's Linears hold: dense weights and biases, an Int8Linear's qweight,
+    """Device bytes the model's Linears hold: dense weights and biases, an Int8Linear's or Fp8Linear's qweight,
     scales and bias, or a ConvRotLinear's qweight, scales and bias plus the derived forms it caches (the FP6 operand weight, and the
     CDNA4 repack of a K x packed-N qweight), and the weight count they serve."""
-    from convrot_mlx_amd import ConvRotLinear, Int8Linear
+    from convrot_mlx_amd import ConvRotLinear, Fp8Linear, Int8Linear
 
     stored = derived = weights = 0
     for m in model.modules():
-        if isinstance(m, Int8Linear):
+        if isinstance(m, (Fp8Linear, Int8Linear)):
             weights += m.qweight.numel()
             stored += sum(t.numel() * t.element_size() for t in (m.qweight, m.scales, m.bias))
             continue
@@ -616,11 +616,11 @@ def keep_at_8_bits(name: str, linear: nn.Module) -> bool:
 
 def int8_figure(p: FluxParams | None = None, img_tokens: int = 1024, txt_tokens: int = 512, group_size: int = 64,
                 steps: int = 5) -> dict:
-    """One denoising step: dense bf16 against every Linear at 8 bits (Int8Linear), and against a
-    mixed model (keep_at_8_bits, the rest W4A4), both with the norms inside the linears'
-    preparations, gated residuals in their epilogues, and head norms and rotary positions in one
-    kernel."""
-    from convrot_mlx_amd import replace_convrot_linears, replace_int8_linears
+    """One denoising step: dense bf16 against every Linear at 8 bits (Int8Linear, and Fp8Linear), and
+    against a mixed model (keep_at_8_bits, the rest W4A4), all with gated residuals in the linears'
+    epilogues and head norms and rotary positions in one kernel, and with the norms inside the linears'
+    preparations (Fp8Linear: in front of them)."""
+    from convrot_mlx_amd import replace_convrot_linears, replace_fp8_linears, replace_int8_linears
 
     p = p or FluxParams()
     dev = torch.device("cuda:0")
@@ -649,6 +649,7 @@ def int8_figure(p: FluxParams | None = None, img_tokens: int = 1024, txt_tokens:
     for name, convert, rotary in (
             ("dense_bf16_fused_rotary", lambda model: [], True),
             ("w8a8", lambda model: [len(replace_int8_linears(model))], True),
+            ("fp8", lambda model: [len(replace_fp8_linears(model))], True),
             ("w8a8_torch_rotary", lambda model: [len(replace_int8_linears(model))], False),
             ("w8a8_and_w4a4", mixed, True)):
         out, t = run(convert, rotary)

@@ -177,6 +177,29 @@ def test_few_rows(dev, tuning, m, k, split, dtype):
     assert torch.equal(hip_fp8_linear(apart[::2], q, ws, bias), got)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,k", [(40, 72), (330, 1032), (200, 4160), (4096, 512)])
+@pytest.mark.parametrize("m", [17, 32, 33, 48, 50, 65, 77, 96])
+def test_17_to_96_rows(dev, m, n, k, dtype):
+    from convrot_mlx_amd import hip_fp8_linear, hip_fp8_matmul, quantize_fp8_blockwise
+
+    q, ws = weight(k, n, k, dev)
+    bias, x, res, gate = normal(n, n).to(dev), normal(m, m, k).to(dtype), normal(2, m, n).to(dtype).to(dev), normal(3, 1, n).to(dtype).to(dev)
+    want, spread = plain.product(plain.row_values(*plain.codes(x)).to(dev), plain.weight_values(q, ws), False)
+    want, spread = want + bias.double(), spread + U * (bias.abs().double() + want.abs())
+    x = x.to(dev)
+    got = hip_fp8_linear(x, q, ws, bias)
+    assert_within(got, want, spread)
+    codes, scales = quantize_fp8_blockwise(x)
+    assert torch.equal(hip_fp8_matmul(codes, q, scales.contiguous(), ws, bias, output_dtype=dtype), got)
+    full = res.double() + gate.double() * want
+    gated = hip_fp8_linear(x, q, ws, bias, residual=res, gate=gate)
+    assert_within(gated, full, gate.double().abs() * spread + U * ((gate.double() * want).abs() + full.abs()))
+    into = res.clone()
+    assert hip_fp8_linear(x, q, ws, bias, residual=into, gate=gate, inplace=True) is into
+    assert torch.equal(into, gated)
+
+
 def test_few_rows_in_place_of_their_residual(dev):
     """A residual that is the input itself, written in place: no workgroup may read what another has written."""
     from convrot_mlx_amd import hip_fp8_linear
