@@ -224,7 +224,7 @@ float time_of(const Cost& c, int64_t groups, float blocks) {
   const float part = (float)(groups - rounds * slots) / (float)slots;
   float t = (float)rounds * (blocks * c.full + c.fixed);
   if (part > 0.0f && part <= 0.5f && c.bm == 256)  // in quarters or halves
-    t += part <= 0.25f ? blocks * 0.65f + 5.0f : blocks * 0.95f + 6.0f;
+    t += part <= 0.25f ? blocks * 0.59f + 5.0f : blocks * 0.87f + 6.0f;
   else if (part > 0.0f) {
     // few workgroups run at a higher clock, and of two a CU the first ones alone
     const float crowd = c.per_cu == 1 ? part : std::max(0.0f, 2.0f * part - 1.0f);

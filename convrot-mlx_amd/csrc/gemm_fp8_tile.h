@@ -431,17 +431,28 @@ __device__ __forceinline__ void fp8_tile(uint8_t* smem, const Fp8Operands& p, in
 }
 
 // Tiles of 256 x 256.  The last round of them, of `slots` workgroups, runs as halves or quarters while that
-// gives each CU at most one: 8800 x 8192 -> 4096 (560 tiles, 48 past two rounds) 284 us, with whole ones
-// 313 to 318.
+// gives each CU at most one: 8800 x 8192 -> 4096 (560 tiles, 48 past two rounds) 272 us, with whole ones 313 to 318.
+// Alone on their CUs the parts take deeper rings, and their MFMAs run in slots: 1536 x 15360 -> 5120 (120 tiles, as
+// halves) 130 us (1860 TFLOP/s), with rings of 2 and no slots 148, with either 146 and 141; 1536 x 4096 -> 2560 (60,
+// as quarters) 23.8 and 25.5.
+struct LargeTiles {
+  using Whole = Fp8Engine<256, 256, 4, 2, 2, 1, true>;
+  using Half = Fp8Engine<256, 128, 4, 2, 3, 1, true>;
+  using Quarter = Fp8Engine<128, 128, 2, 4, 4, 1, true>;
+  static constexpr int smem_bytes(int blocks) {
+    const int w = Whole::smem_bytes(blocks), h = Half::smem_bytes(blocks), q = Quarter::smem_bytes(blocks);
+    return w > h ? (w > q ? w : q) : (h > q ? h : q);
+  }
+  static_assert(Half::THREADS == Whole::THREADS && Quarter::THREADS == Whole::THREADS, "one launch");
+};
+
 template <int ODT, int KIND>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_large_kernel(Fp8Operands p,
                                                                                                  int tiles_m,
                                                                                                  int tiles_n, int slots) {
-  using E = Fp8Engine<256, 256, 4, 2, 2, 1, true>;
-  using Half = Fp8Engine<256, 128, 4, 2, 2, 1, false>;
-  using Quarter = Fp8Engine<128, 128, 2, 4, 2, 1, false>;
-  static_assert(Half::WS_OFF <= E::WS_OFF && Half::WS <= E::WS && Quarter::WS_OFF <= E::WS_OFF && Quarter::WS <= E::WS,
-                "the parts lie in the LDS of a whole tile");
+  using E = LargeTiles::Whole;
+  using Half = LargeTiles::Half;
+  using Quarter = LargeTiles::Quarter;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   tiles_m = tile_rows_of<256, KIND>(p, tiles_m);
   const int tiles = tiles_m * tiles_n;
@@ -526,13 +537,15 @@ hipError_t launch_fp8_tile_k(const Fp8Operands& p, const W8a8Split& split, hipSt
   const int64_t tn = ((int64_t)p.N + BN - 1) / BN;
   const size_t lds = (size_t)E::smem_bytes((p.K + kBlock - 1) / kBlock);
   if constexpr (BM == 256) {
+    static_assert(LargeTiles::smem_bytes(kMaxBlocks) <= 160 * 1024 - 64, "LDS of one CU");
+    const size_t most = (size_t)LargeTiles::smem_bytes((p.K + kBlock - 1) / kBlock);
     const int slots = device_cus();
     // (what experts make of the bound's tiles is known on the device alone)
     if (tm * tn > 0x7fff0000 || slots < 1) return hipErrorInvalidValue;
     const LastRound last = last_round((int)(tm * tn), slots);
     const int64_t groups = KIND == 0 ? last.whole + (tm * tn - last.whole) * last.parts : tm * tn + slots;
     if (groups > max_groups(E::THREADS)) return hipErrorInvalidValue;
-    fp8_large_kernel<ODT, KIND><<<dim3((unsigned)groups), dim3(E::THREADS), lds, s>>>(p, (int)tm, (int)tn, slots);
+    fp8_large_kernel<ODT, KIND><<<dim3((unsigned)groups), dim3(E::THREADS), most, s>>>(p, (int)tm, (int)tn, slots);
   } else {
     const int64_t groups = tm * tn * split.splits;
     if (groups > max_groups(E::THREADS) || groups > 0x7fffffff) return hipErrorInvalidValue;
