@@ -98,7 +98,8 @@ SIGNATURES = {
     "convrot_grouped_linear": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp,
                                       _vp]),
     "convrot_grouped_linear_rows_grad": (_i32, [_vp, _i32, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
-    "convrot_grouped_linear_weight_grad": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "convrot_grouped_linear_weight_grad": (_i32, [_vp, _i32, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp,
+                                                  _vp]),
     "convrot_expert_plan_workspace_bytes": (_i64, [_i64, _i64]),
     "convrot_expert_plan": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
     "convrot_gather_rows": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp]),

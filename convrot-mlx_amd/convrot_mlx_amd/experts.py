@@ -316,12 +316,14 @@ def hip_grouped_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch
         if gather:
             dx = hip_combine_rows(dx, plan)
     if weight_grad:
-        rows = _operand16(_gather_rows(x, r.index, r.choices) if gather else x)
+        rows = _operand16(x)
+        if r.index is not None and rows.shape[0] * _stride16(rows) * 2 > MAX_GATHERED_BYTES:
+            rows, r = _operand16(_gather_rows(x, r.index, r.choices)), r._replace(index=None, choices=1)
         dw = torch.empty((experts, n, k), dtype=x.dtype, device=device)
         with nat.on(device):
             nat.check(lib.convrot_grouped_linear_weight_grad(
-                g.data_ptr(), code, _stride16(g), rows.data_ptr(), _stride16(rows), r.offsets.data_ptr(), experts, r.rows, n,
-                k, dw.data_ptr(), nat.stream_handle(device)))
+                g.data_ptr(), code, _stride16(g), rows.data_ptr(), rows.shape[0], _stride16(rows), r.offsets.data_ptr(),
+                experts, nat.address(r.index), r.choices, r.rows, n, k, dw.data_ptr(), nat.stream_handle(device)))
     return dx, dw
 
 

@@ -1413,19 +1413,24 @@ int convrot_grouped_linear_rows_grad(const void* dy, int dtype, int64_t dy_strid
   return launch_status(convrot::launch_grouped(2, p, dtype, (hipStream_t)stream), "convrot_grouped_linear_rows_grad");
 }
 
-int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_stride, const void* x, int64_t x_stride,
-                                       const int32_t* offsets, int64_t experts, int64_t rows, int64_t N, int64_t K,
-                                       void* dw, void* stream) {
-  if (int rc = check_grouped(dtype, offsets, experts, nullptr, 1, rows, rows, N, K)) return rc;
+int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_stride, const void* x, int64_t x_rows,
+                                       int64_t x_stride, const int32_t* offsets, int64_t experts, const int32_t* index,
+                                       int64_t choices, int64_t rows, int64_t N, int64_t K, void* dw, void* stream) {
+  if (int rc = check_grouped(dtype, offsets, experts, index, choices, x_rows, rows, N, K)) return rc;
   if (!dw || !aligned(dw, 16)) return fail(CONVROT_ERR_INVALID, "dw must be 16-byte aligned");
   if (!offsets) return fail(CONVROT_ERR_INVALID, "null pointer argument");
   if (rows > 0) {
     if (int rc = check_rows16("dy", dy, dy_stride, N)) return rc;
     if (int rc = check_rows16("x", x, x_stride, K)) return rc;
+    if (index && (x_rows == 0 || (x_rows - 1) * x_stride * 2 + (K + 7) / 8 * 16 > convrot::kMaxExtent))
+      return fail(CONVROT_ERR_UNSUPPORTED, "rows read through an index support 1 to 2^32 bytes, got %lld rows %lld apart",
+                  (long long)x_rows, (long long)x_stride);
   }
   const convrot::GroupedOperands p{(const uint16_t*)dy, (const uint16_t*)x, dy_stride, x_stride, 0, (uint16_t*)dw, (int)rows,
-                                   (int)N, (int)K, {offsets, nullptr, (int)experts, 1, rows}};
-  return launch_status(convrot::launch_grouped(3, p, dtype, (hipStream_t)stream), "convrot_grouped_linear_weight_grad");
+                                   (int)N, (int)K, {offsets, index, (int)experts, (int)choices, x_rows},
+                                   convrot::Divisor((uint32_t)choices)};
+  return launch_status(convrot::launch_grouped(index && rows > 0 ? 4 : 3, p, dtype, (hipStream_t)stream),
+                       "convrot_grouped_linear_weight_grad");
 }
 
 }  // extern "C"

@@ -44,7 +44,7 @@ float tile_rows(int64_t rows, int64_t experts, int bm) {
 
 int choose(int kind, const GroupedOperands& p) {
   const int forced = tuning(kTuneGroupedTile);
-  if (forced > 0 && (kind != 3 || grouped_weight_tile_known(forced & 1023, forced >> 10))) return forced;
+  if (forced > 0 && (kind < 3 || grouped_weight_tile_known(forced & 1023, forced >> 10))) return forced;
   const int64_t met = std::max<int64_t>(1, std::min<int64_t>(p.g.experts, p.R));
   const float weights = (float)(met * p.N) * (float)p.C * 2.0f / 5.5e6f;  // from or to memory, at 5.5 TB/s
   // rows that do not begin on 128 bytes take two requests a block (1384 and 1408 features, 2060 rows of 16 experts ->
@@ -54,15 +54,15 @@ int choose(int kind, const GroupedOperands& p) {
   int best = 0;
   float best_time = 0.0f;
   for (const Cost& c : kCosts) {
-    if (kind == 3 && !grouped_weight_tile_known(c.bm, c.bn)) continue;
-    const int64_t most = kind == 3 ? over(p.N, c.bm) * p.g.experts * over(p.C, c.bn)
+    if (kind >= 3 && !grouped_weight_tile_known(c.bm, c.bn)) continue;
+    const int64_t most = kind >= 3 ? over(p.N, c.bm) * p.g.experts * over(p.C, c.bn)
                                    : most_tile_rows(p.R, p.g.experts, c.bm) * over(p.N, c.bn);
     if (most > max_groups(256) - 1024) continue;  // no launch so large
-    const float rows = kind == 3 ? (float)(over(p.N, c.bm) * p.g.experts) : tile_rows(p.R, p.g.experts, c.bm);
-    const float blocks = kind == 3 ? (float)p.R / (float)met / 64.0f + 0.5f : (float)over(p.C, 64);
-    const int64_t groups = (int64_t)(rows * (float)over(kind == 3 ? p.C : p.N, c.bn));
+    const float rows = kind >= 3 ? (float)(over(p.N, c.bm) * p.g.experts) : tile_rows(p.R, p.g.experts, c.bm);
+    const float blocks = kind >= 3 ? (float)p.R / (float)met / 64.0f + 0.5f : (float)over(p.C, 64);
+    const int64_t groups = (int64_t)(rows * (float)over(kind >= 3 ? p.C : p.N, c.bn));
     float t = time_of(c, groups, blocks), read = weights;
-    if (kind != 3) {
+    if (kind < 3) {
       // every tile row of an expert reads its weights, and few workgroups do not keep the memory busy (16 choices of 8
       // experts, 5424 -> 5376: 336 of 32 x 128 110 us, 672 of 32 x 64 86)
       read *= 1.0f + 0.57f * (std::min(8.0f, rows / (float)met) - 1.0f);

@@ -12,6 +12,10 @@
 //   rows      A = dy (along)   B = w (across: c is its row)
 //   weights   A = dy (across)  B = x (across), c runs over the expert's rows
 //
+// Rows of x through the index: forward by the offsets of a tile's rows, in the weights' gradient by scalar loads of 16
+// numbers a wave and block, a block ahead (4608 tokens of 2 choices, 8 experts, 4096 -> 2048: 178 us, on gathered rows 163
+// and 25 for the gather, which also holds them in memory).
+//
 // An operand "across" is loaded as it lies, 64 rows of c, and transposed on the way from LDS to
 // the registers (ds_read_b64_tr_b16: 16 lanes read a 4 x 16 block and get its columns), so
 // nothing is transposed in memory.
@@ -51,12 +55,20 @@ __device__ __forceinline__ void mfma_drain(f32x4 (&acc)[FN][FM]) {
     for (int fm = 0; fm < FM; ++fm) asm volatile("" : "+a"(acc[fn][fm]));
 }
 
-// One operand of a tile of T rows (or, across, columns) by the workgroup's 4 waves.
-template <int T, bool ACROSS>
+struct RowNumbers {
+  int v[16];
+};
+
+// One operand of a tile of T rows (or, across, columns) by the workgroup's 4 waves.  GATHER: across, its rows of c
+// read through an index.
+template <int T, bool ACROSS, bool GATHER = false>
 struct Side {
+  static_assert(ACROSS || !GATHER, "rows along are gathered by their offsets");
+  typedef const __attribute__((address_space(4))) int* Index;  // scalar loads
   static constexpr int PW = T / 32;             // 1 KB pieces a wave and block
   static constexpr int ROW = ACROSS ? T * 2 : 128;  // bytes of an LDS row
   static constexpr int RPP = 1024 / ROW, CPR = ROW / 16;  // rows a piece, chunks a row
+  static_assert(!GATHER || PW * RPP == 16, "16 rows of c a wave");
   static_assert(T % 32 == 0 && (!ACROSS || (T & (T - 1)) == 0), "tile");
 
   const uint16_t* base;
@@ -67,6 +79,9 @@ struct Side {
   bool past[2];      // along: the lane's chunk of the last block lies past the row's end
   uint32_t tail;     // along: the block that rows end in, ~0 where they fill it
   int count;         // length of c
+  Index index;       // GATHER: of row 0 of c
+  Divisor choices;
+  uint32_t numbers;  // those below it name a row
 
   // Which unit of 32 bytes of a row of c lies at unit u.
   __device__ __forceinline__ static int unit_swizzle(int row) {
@@ -116,6 +131,46 @@ struct Side {
     }
   }
 
+  // the same, row c of it row index[c] / choices of the `total` rows at p
+  __device__ __forceinline__ void set_gather_across(const uint16_t* p, int64_t ld, int columns, int length, int lane,
+                                                    int wave, const int* rows, const Divisor& d, int each, int64_t total) {
+    base = p;
+    count = length;
+    index = (Index)(uintptr_t)rows;
+    choices = d;
+    numbers = (uint32_t)min(total * each, (int64_t)1 << 31);
+    row_bytes = (uint32_t)ld * 2u;
+    const uint32_t width = whole(min(columns, T));
+    bytes = (uint32_t)(total - 1) * row_bytes + width;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int row = (wave * PW + i) * RPP + lane / CPR, c = lane % CPR;
+      const uint32_t at = (uint32_t)((((c >> 1) ^ unit_swizzle(row)) * 2 + (c & 1)) * 16);
+      off[i] = at < width ? at : kPastEnd;
+    }
+  }
+  // GATHER: the index of the wave's 16 rows of block kb, -1 past the last one.
+  __device__ __forceinline__ RowNumbers fetch(uint32_t kb, int wave) const {
+    RowNumbers o{};
+    if constexpr (GATHER) {
+      const int c0 = (int)kb * 64 + wave * 16;
+      if (c0 + 16 <= count) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o.v[j] = index[c0 + j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o.v[j] = c0 + j < count ? index[min(c0 + j, count - 1)] : -1;
+      }
+    }
+    return o;
+  }
+  // The offset of a row from its number in the index.
+  __device__ __forceinline__ uint32_t row_offset(int n) const {
+    const uint32_t o = choices.divide((uint32_t)n) * row_bytes;
+    return __builtin_amdgcn_readfirstlane((uint32_t)n < numbers ? o : kNoRow);
+  }
+  static constexpr uint32_t kNoRow = 0xfffff000u;  // with a column's offset still past every operand
+
   // bytes of `n` elements in whole chunks (rows are padded to them: a chunk cut by the range check would
   // lose elements of its last word)
   __device__ __forceinline__ static uint32_t whole(int n) { return ((uint32_t)n * 2u + 15u) & ~15u; }
@@ -130,16 +185,28 @@ struct Side {
   }
 
   __device__ __forceinline__ i32x4_sgpr rsrc(uint32_t kb) const {
-    if constexpr (ACROSS) {
+    if constexpr (GATHER) {
+      return dma_rsrc(base, bytes);
+    } else if constexpr (ACROSS) {
       const int left = min(64, count - (int)kb * 64);
       return dma_rsrc(base + (int64_t)kb * step, (uint32_t)(left - 1) * row_bytes + bytes);
     } else {
       return dma_rsrc(base, bytes);
     }
   }
-  __device__ __forceinline__ void issue(i32x4_sgpr r, uint32_t kb, int i, int wave, uint32_t lds) const {
+  __device__ __forceinline__ void issue(i32x4_sgpr r, uint32_t kb, int i, int wave, uint32_t lds,
+                                        const RowNumbers& rows) const {
     uint32_t o = off[i];
-    if constexpr (!ACROSS) {
+    if constexpr (GATHER) {
+      const int mine = (threadIdx.x & 63) / CPR;
+      uint32_t row = row_offset(rows.v[i * RPP]);
+#pragma unroll
+      for (int j = 1; j < RPP; ++j) {
+        const uint32_t other = row_offset(rows.v[i * RPP + j]);
+        row = mine == j ? other : row;
+      }
+      o = o == kPastEnd ? kPastEnd : row + o;
+    } else if constexpr (!ACROSS) {
       o = o == kPastEnd ? kPastEnd : o + kb * 128u;
       if (kb == tail) o = past[i & 1] ? kPastEnd : o;
     }
@@ -175,11 +242,11 @@ struct Side {
   }
 };
 
-template <int BM_, int BN_, int STAGES, int DT, bool ACROSS_A, bool ACROSS_B>
+template <int BM_, int BN_, int STAGES, int DT, bool ACROSS_A, bool ACROSS_B, bool GATHER_B = false>
 struct Engine16 {
   static constexpr int BM = BM_, BN = BN_;
   using A = Side<BM, ACROSS_A>;
-  using B = Side<BN, ACROSS_B>;
+  using B = Side<BN, ACROSS_B, GATHER_B>;
   static constexpr int TM = BM / 2, TN = BN / 2, FM = TM / 16, FN = TN / 16, LPW = A::PW + B::PW;
   static constexpr int STAGE_BYTES = (BM + BN) * 128, RING = STAGES * STAGE_BYTES;
   static constexpr int STAGING = 4 * TM * (TN * 2 + 16);  // the epilogue's
@@ -208,10 +275,10 @@ struct Engine16 {
     i32x4_sgpr a, b;
   };
   __device__ __forceinline__ Rsrc rsrc(uint32_t kb) const { return {a.rsrc(kb), b.rsrc(kb)}; }
-  __device__ __forceinline__ void issue(const Rsrc& r, uint32_t kb, int stage, int idx) const {
+  __device__ __forceinline__ void issue(const Rsrc& r, uint32_t kb, int stage, int idx, const RowNumbers& rows) const {
     const uint32_t base = smem_addr + (uint32_t)(stage * STAGE_BYTES);
-    if (idx < A::PW) a.issue(r.a, kb, idx, wave, base);
-    else b.issue(r.b, kb, idx - A::PW, wave, base + (uint32_t)BM * 128u);
+    if (idx < A::PW) a.issue(r.a, kb, idx, wave, base, rows);
+    else b.issue(r.b, kb, idx - A::PW, wave, base + (uint32_t)BM * 128u, rows);
   }
 
   // n fillers spread over the first `span` MFMA slots: those after slot t are filler(t) .. filler(t + 1) - 1.
@@ -228,8 +295,9 @@ struct Engine16 {
     for (int s = 0; s < STAGES; ++s) {
       const uint32_t kb = min((uint32_t)s, last);
       const Rsrc r = rsrc(kb);
+      const RowNumbers rows = b.fetch(kb, wave);
 #pragma unroll
-      for (int i = 0; i < LPW; ++i) issue(r, kb, s, i);
+      for (int i = 0; i < LPW; ++i) issue(r, kb, s, i, rows);
     }
     // fragment i of a k-step, B's first (every MFMA of the first row needs them)
     auto read = [&](auto i, auto ks, uint32_t stage, i32x4(&bf)[FN], i32x4(&af)[FM]) __attribute__((always_inline)) {
@@ -246,6 +314,7 @@ struct Engine16 {
     int st = 0;
     for (uint32_t kb = 0; kb <= last; ++kb) {
       const int nst = st + 1 == STAGES ? 0 : st + 1;
+      RowNumbers rows = b.fetch(min(kb + STAGES, last), wave);  // arrives beside the first k-step
       const uint32_t here = smem_addr + (uint32_t)(st * STAGE_BYTES), next = smem_addr + (uint32_t)(nst * STAGE_BYTES);
       static_for<SLOTS>([&](auto slot) __attribute__((always_inline)) {
         constexpr int t = slot.value, lo = filler(t, READS, SPAN0), hi = filler(t + 1, READS, SPAN0);
@@ -256,6 +325,10 @@ struct Engine16 {
       });
       wait_vmcnt<(STAGES - 2) * LPW>();
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+      if constexpr (GATHER_B) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) asm volatile("" : "+s"(rows.v[j]));
+      }
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       // past the last block: the last one again, into stages nothing reads
@@ -265,7 +338,7 @@ struct Engine16 {
         constexpr int t = slot.value, lo = filler(t, READS, SPAN1), hi = filler(t + 1, READS, SPAN1);
         constexpr int dlo = filler(t, LPW, SPAN_DMA), dhi = filler(t + 1, LPW, SPAN_DMA);
         mfma_16<DT>(acc[t % FN][t / FN], b1[t % FN], a1[t / FN]);
-        static_for<dhi - dlo>([&](auto f) __attribute__((always_inline)) { issue(r, nkb, st, dlo + f.value); });
+        static_for<dhi - dlo>([&](auto f) __attribute__((always_inline)) { issue(r, nkb, st, dlo + f.value, rows); });
         static_for<hi - lo>([&](auto f) __attribute__((always_inline)) {
           read(std::integral_constant<int, lo + f.value>{}, K0, next, b0, a0);
         });
@@ -298,7 +371,7 @@ __device__ __forceinline__ void store_tile(const E& e, const f32x4 (&acc)[E::FN]
   move_rows<TM, TN, true>(region, (uint16_t*)out, lane, mw, nw, row_end, N);
 }
 
-// One tile: output rows m0 .. (m0 + BM or) row_end - 1, columns n0 .., of an expert (whose rows, with KIND 3, are
+// One tile: output rows m0 .. (m0 + BM or) row_end - 1, columns n0 .., of an expert (whose rows, with KIND 3 and 4, are
 // the contracted ones).
 template <class E, int DT, int KIND>
 __device__ __forceinline__ void grouped_tile(uint8_t* smem, const GroupedOperands& p, int expert, int m0, int row_end,
@@ -311,13 +384,18 @@ __device__ __forceinline__ void grouped_tile(uint8_t* smem, const GroupedOperand
     for (int j = 0; j < E::FM; ++j) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   int columns = p.N;
   uint16_t* out = p.out;
-  if constexpr (KIND == 3) {
+  if constexpr (KIND >= 3) {
     columns = p.C;
     out += (int64_t)expert * p.N * p.C;
-    const int a = group_start(p.g, expert, p.R), b = group_start(p.g, expert + 1, p.R);
+    const int a = __builtin_amdgcn_readfirstlane(group_start(p.g, expert, p.R));
+    const int b = __builtin_amdgcn_readfirstlane(group_start(p.g, expert + 1, p.R));
     if (b > a) {
       e.a.set_across(p.rows + (int64_t)a * p.ld_rows + m0, p.ld_rows, p.N - m0, b - a, e.lane, e.wave);
-      e.b.set_across(p.other + (int64_t)a * p.ld_other + n0, p.ld_other, p.C - n0, b - a, e.lane, e.wave);
+      if constexpr (KIND == 4)
+        e.b.set_gather_across(p.other + n0, p.ld_other, p.C - n0, b - a, e.lane, e.wave, p.g.index + a, p.choices,
+                              p.g.choices, p.g.act_rows);
+      else
+        e.b.set_across(p.other + (int64_t)a * p.ld_other + n0, p.ld_other, p.C - n0, b - a, e.lane, e.wave);
       e.run((b - a + 63) / 64, acc);
     }
   } else if (expert < p.g.experts) {
@@ -347,7 +425,7 @@ __device__ __forceinline__ void grouped_tile(uint8_t* smem, const GroupedOperand
 template <int BM, int KIND>
 __device__ __forceinline__ GroupTile grouped_place(const GroupedOperands& p, int t, int turns, int tiles_i, int tiles_j,
                                                    int* column) {
-  if constexpr (KIND == 3) {
+  if constexpr (KIND >= 3) {
     const int tiles = tiles_i * tiles_j, per_xcd = tiles / kXcds, expert = t / tiles;
     t -= expert * tiles;
     if (t < per_xcd * kXcds && (expert + 1) * tiles <= turns) t = (t % kXcds) * per_xcd + t / kXcds;
@@ -366,10 +444,10 @@ __device__ __forceinline__ GroupTile grouped_place(const GroupedOperands& p, int
 template <int BM, int BN, int STAGES, int PER_CU, int DT, int KIND>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_CU, PER_CU))) void grouped_kernel(
     GroupedOperands p, int tiles_i, int tiles_j) {
-  using E = Engine16<BM, BN, STAGES, DT, KIND == 3, KIND >= 2>;
+  using E = Engine16<BM, BN, STAGES, DT, KIND >= 3, KIND >= 2, KIND == 4>;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES];
-  if constexpr (KIND != 3) tiles_i = group_tile_rows<BM>(p.g, p.R);
-  const int tiles = tiles_i * tiles_j * (KIND == 3 ? p.g.experts : 1), t = blockIdx.x;
+  if constexpr (KIND < 3) tiles_i = group_tile_rows<BM>(p.g, p.R);
+  const int tiles = tiles_i * tiles_j * (KIND >= 3 ? p.g.experts : 1), t = blockIdx.x;
   if (t >= tiles) return;
   int column;
   const GroupTile at = grouped_place<BM, KIND>(p, t, tiles, tiles_i, tiles_j, &column);
@@ -383,14 +461,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                                                                                                      int tiles_i,
                                                                                                      int tiles_j,
                                                                                                      int slots) {
-  constexpr bool AA = KIND == 3, AB = KIND >= 2;
-  using E = Engine16<256, 256, 2, DT, AA, AB>;
-  using Half = Engine16<256, 128, 3, DT, AA, AB>;
-  using Quarter = Engine16<128, 128, 4, DT, AA, AB>;
+  constexpr bool AA = KIND >= 3, AB = KIND >= 2, GB = KIND == 4;
+  using E = Engine16<256, 256, 2, DT, AA, AB, GB>;
+  using Half = Engine16<256, 128, 3, DT, AA, AB, GB>;
+  using Quarter = Engine16<128, 128, 4, DT, AA, AB, GB>;
   constexpr int PARTS = Half::SMEM_BYTES > Quarter::SMEM_BYTES ? Half::SMEM_BYTES : Quarter::SMEM_BYTES;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[E::SMEM_BYTES > PARTS ? E::SMEM_BYTES : PARTS];
-  if constexpr (KIND != 3) tiles_i = group_tile_rows<256>(p.g, p.R);
-  const int tiles = tiles_i * tiles_j * (KIND == 3 ? p.g.experts : 1), t = blockIdx.x;
+  if constexpr (KIND < 3) tiles_i = group_tile_rows<256>(p.g, p.R);
+  const int tiles = tiles_i * tiles_j * (KIND >= 3 ? p.g.experts : 1), t = blockIdx.x;
   const LastRound last = last_round(tiles, slots);
   int column;
   if (t < last.whole) {
@@ -404,21 +482,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   const GroupTile at = grouped_place<256, KIND>(p, tile, 0, tiles_i, tiles_j, &column);
   if (at.expert < 0) return;
   const int m0 = at.row0 + (part >> 1) * 128, n0 = column * 256 + (part & 1) * 128;
-  if (m0 >= at.row_end || n0 >= (KIND == 3 ? p.C : p.N)) return;
+  if (m0 >= at.row_end || n0 >= (KIND >= 3 ? p.C : p.N)) return;
   if (last.parts == 2) grouped_tile<Half, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
   else grouped_tile<Quarter, DT, KIND>(smem, p, at.expert, m0, at.row_end, n0);
 }
 
 template <int BM, int BN, int STAGES, int PER_CU, int DT, int KIND>
 hipError_t launch_grouped_k(const GroupedOperands& p, hipStream_t s) {
-  const int64_t ti = KIND == 3 ? ((int64_t)p.N + BM - 1) / BM : most_tile_rows(p.R, p.g.experts, BM);
-  const int64_t tj = ((int64_t)(KIND == 3 ? p.C : p.N) + BN - 1) / BN;
-  const int64_t tiles = ti * tj * (KIND == 3 ? p.g.experts : 1), slots = device_cus();
+  const int64_t ti = KIND >= 3 ? ((int64_t)p.N + BM - 1) / BM : most_tile_rows(p.R, p.g.experts, BM);
+  const int64_t tj = ((int64_t)(KIND >= 3 ? p.C : p.N) + BN - 1) / BN;
+  const int64_t tiles = ti * tj * (KIND >= 3 ? p.g.experts : 1), slots = device_cus();
   if (tiles > max_groups(256) - slots || tiles > 0x7fff0000 || slots < 1) return hipErrorInvalidValue;
   if constexpr (BM == 256) {
     // (what experts make of the bound's tiles is known on the device alone)
     const LastRound last = last_round((int)tiles, (int)slots);
-    const int64_t groups = KIND == 3 ? last.whole + (tiles - last.whole) * last.parts : tiles + slots;
+    const int64_t groups = KIND >= 3 ? last.whole + (tiles - last.whole) * last.parts : tiles + slots;
     grouped_large_kernel<DT, KIND><<<dim3((unsigned)groups), dim3(256), 0, s>>>(p, (int)ti, (int)tj, (int)slots);
   } else {
     grouped_kernel<BM, BN, STAGES, PER_CU, DT, KIND><<<dim3((unsigned)tiles), dim3(256), 0, s>>>(p, (int)ti, (int)tj);
@@ -430,13 +508,14 @@ hipError_t launch_grouped_k(const GroupedOperands& p, hipStream_t s) {
 
 template <int DT>
 hipError_t launch_grouped_tile(int tile, int kind, const GroupedOperands& p, hipStream_t stream) {
-  switch (tile << 2 | kind) {
+  switch (tile << 3 | kind) {
 #define GROUPED_CASE(BM, BN, STAGES, PER_CU, KIND) \
-  case tile_code(BM, BN) << 2 | KIND: return launch_grouped_k<BM, BN, STAGES, PER_CU, DT, KIND>(p, stream);
+  case tile_code(BM, BN) << 3 | KIND: return launch_grouped_k<BM, BN, STAGES, PER_CU, DT, KIND>(p, stream);
 #define GROUPED_ROWS(BM, BN, STAGES, PER_CU)                                              \
   GROUPED_CASE(BM, BN, STAGES, PER_CU, 0) GROUPED_CASE(BM, BN, STAGES, PER_CU, 1) \
   GROUPED_CASE(BM, BN, STAGES, PER_CU, 2)
-#define GROUPED_WEIGHTS(BM, BN, STAGES, PER_CU) GROUPED_CASE(BM, BN, STAGES, PER_CU, 3)
+#define GROUPED_WEIGHTS(BM, BN, STAGES, PER_CU) \
+  GROUPED_CASE(BM, BN, STAGES, PER_CU, 3) GROUPED_CASE(BM, BN, STAGES, PER_CU, 4)
     GROUPED_TILES(GROUPED_ROWS)
     GROUPED_WEIGHT_TILES(GROUPED_WEIGHTS)
     default: return hipErrorInvalidValue;

@@ -130,16 +130,29 @@ inline int64_t most_tile_rows(int64_t rows, int64_t experts, int bm) {
   return rows < bound ? rows : bound;
 }
 
+// n / d for 0 <= n < 2^31 by a product: d in 1 .. 2^31 - 1.
+struct Divisor {
+  uint32_t factor = 1;
+  int shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t d) {
+    while ((uint64_t(1) << shift) < d) ++shift;
+    factor = (uint32_t)((((uint64_t(1) << shift) - d) << 32) / d) + 1;
+  }
+  __device__ __forceinline__ uint32_t divide(uint32_t n) const { return (__umulhi(factor, n) + n) >> shift; }
+};
+
 // What a launch computes: KIND 0 forward on sorted rows, 1 on rows read through the index, 2 the rows' gradient,
-// 3 the weights'.
+// 3 the weights' on sorted rows, 4 on rows of x read through the index.
 struct GroupedOperands {
-  const uint16_t *rows, *other;  // x (or dy); the weights, or (KIND 3) x beside dy
+  const uint16_t *rows, *other;  // x (or dy); the weights, or (KIND 3, 4) x beside dy
   int64_t ld_rows, ld_other;     // elements between rows
   int64_t expert;                // elements between experts' weights
   uint16_t* out;
   int R;                         // sorted rows
-  int N, C;                      // columns of the output, length contracted (KIND 3: rows and columns of a weight, N x C)
+  int N, C;                      // columns of the output, length contracted (KIND 3, 4: rows and columns of a weight, N x C)
   Groups g;
+  Divisor choices;               // KIND 4: g.choices
 };
 
 // The tiled product of one type (gemm_grouped_tile.h, one source a type).

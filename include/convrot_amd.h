@@ -622,11 +622,10 @@ int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t
  * convrot_fp8_grouped_linear:
  *   out[s] = x[row(s)] W_e^T        (rows of no expert: zeros; x through an index: at most 2^32 - 4096 bytes)
  *   dx[s]  = dy[s] W_e              (rows of no expert: zeros)
- *   dw[e]  = sum over expert e's rows s of dy[s]^T x[s]   (an expert without rows: zeros)
+ *   dw[e]  = sum over expert e's rows s of dy[s]^T x[row(s)]   (an expert without rows: zeros)
  * x, dy and weight: 16-byte aligned rows, strides (elements) that are multiples of 8 and cover the features
  * rounded up to 8, zeros from there on; weight e at weight + e * weight_expert elements.  out [rows, N],
- * dx [rows, K], dw [experts, N, K] contiguous, 16-byte aligned.  Up to 65536 features.  The weights'
- * gradient reads sorted rows of x (convrot_gather_rows makes them).
+ * dx [rows, K], dw [experts, N, K] contiguous, 16-byte aligned.  Up to 65536 features.
  */
 int convrot_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* weight,
                            int64_t weight_stride, int64_t weight_expert, const int32_t* offsets, int64_t experts,
@@ -635,9 +634,9 @@ int convrot_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t x_s
 int convrot_grouped_linear_rows_grad(const void* dy, int dtype, int64_t dy_stride, const void* weight,
                                      int64_t weight_stride, int64_t weight_expert, const int32_t* offsets,
                                      int64_t experts, int64_t rows, int64_t N, int64_t K, void* dx, void* stream);
-int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_stride, const void* x, int64_t x_stride,
-                                       const int32_t* offsets, int64_t experts, int64_t rows, int64_t N, int64_t K,
-                                       void* dw, void* stream);
+int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_stride, const void* x, int64_t x_rows,
+                                       int64_t x_stride, const int32_t* offsets, int64_t experts, const int32_t* index,
+                                       int64_t choices, int64_t rows, int64_t N, int64_t K, void* dw, void* stream);
 
 /*
  * What lies around the experts' linears.

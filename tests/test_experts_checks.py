@@ -73,7 +73,7 @@ def rows_grad(lib, **kw):
 
 
 def weight_grad(lib, **kw):
-    a = dict(dy=P, dtype=BF16, ldy=8, x=P, ldx=64, offsets=P, experts=3, rows=8, n=8, k=64, out=P) | kw
+    a = dict(dy=P, dtype=BF16, ldy=8, x=P, xrows=4, ldx=64, offsets=P, experts=3, index=P, choices=2, rows=8, n=8, k=64, out=P) | kw
     return lib.convrot_grouped_linear_weight_grad(*a.values(), None)
 
 
@@ -84,7 +84,9 @@ def weight_grad(lib, **kw):
     (rows_grad, dict(offsets=None), 1, "null"), (rows_grad, dict(experts=0), 2, "experts"), (rows_grad, dict(n=0), 1, "invalid"),
     (weight_grad, dict(dtype=F32), 1, "float16 or bfloat16"), (weight_grad, dict(x=None), 1, "null"),
     (weight_grad, dict(ldx=56), 1, "x needs"), (weight_grad, dict(out=P + 2), 1, "dw must"), (weight_grad, dict(out=None), 1, "dw must"),
-    (weight_grad, dict(rows=0, offsets=None), 1, "null"), (weight_grad, dict(k=70000), 2, "features"),
+    (weight_grad, dict(rows=0, offsets=None), 1, "null"), (weight_grad, dict(index=None), 1, "sorted rows, but"),
+    (weight_grad, dict(choices=0), 1, "invalid groups"), (weight_grad, dict(xrows=0), 2, "through an index"),
+    (weight_grad, dict(xrows=1 << 26, rows=1 << 27), 2, "through an index"), (weight_grad, dict(k=70000), 2, "features"),
 ])
 def test_gradients(lib, call, kw, code, text):
     refused(lib, call(lib, **kw), code, text)

@@ -368,6 +368,15 @@ def test_every_tile(dev, tuning, tile, tokens, choices, experts, n, k):
         check_products(dev, tokens, choices, experts, n, k, BF16, gather, seed=1)
 
 
+@pytest.mark.parametrize("tile", [None, "256x256", "128x128"])
+@pytest.mark.parametrize("tokens,choices", [(200, 5), (150, 7), (20, 64), (333, 3), (1, 1)])
+def test_rows_read_through_the_index(dev, tuning, tile, tokens, choices):
+    """Every number of choices a token: the rows of a block of the weights' gradient come through the index."""
+    if tile:
+        tuning.set("grouped_tile", tile)
+    check_products(dev, tokens, choices, 4, 136, 264, BF16, True, seed=3)
+
+
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("n,k", [(2000, 1960), (264, 7690), (7690, 264)])
 def test_last_round_in_parts(dev, tuning, n, k, gather):
@@ -436,6 +445,20 @@ def test_offsets_and_indices_of_any_content(dev):
     want = hip_grouped_linear(x, w, ExpertPlan(i32(0, 30, 60, 100), torch.arange(100, dtype=torch.int32, device=dev)), gather=True)
     keep = [i for i in range(100) if i not in (3, 40, 99)]
     assert torch.equal(got[keep], want[keep]) and not got[[3, 40, 99]].any()
+
+
+def test_gradient_of_weights_with_indices_out_of_range(dev):
+    from convrot_mlx_amd import ExpertPlan, hip_grouped_linear_backward
+
+    w, x, dy = (normal(i, *s).to(BF16).to(dev) for i, s in enumerate(((3, 40, 128), (50, 128), (100, 40))))
+    offsets = torch.tensor((0, 30, 60, 100), dtype=torch.int32, device=dev)
+    order = torch.randperm(100, generator=torch.Generator().manual_seed(5)).int().to(dev)
+    without = dy.clone()
+    without[[3, 40, 99]] = 0
+    _, want = hip_grouped_linear_backward(without, x, w, ExpertPlan(offsets, order), gather=True, rows_grad=False)
+    order[3], order[40], order[99] = -1, 2 ** 31 - 1, 100
+    _, got = hip_grouped_linear_backward(dy, x, w, ExpertPlan(offsets, order), gather=True, rows_grad=False)
+    assert torch.equal(got, want)
 
 
 def test_no_rows_in_16_bits(dev):
