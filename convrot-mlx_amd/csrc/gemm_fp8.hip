@@ -18,7 +18,9 @@ namespace {
 // start.  Where the channels make too few workgroups for the chip, several share K, and the last to arrive adds
 // their sums in the parts' order.  With FUSED the rows come as they are and each workgroup quantizes its part of
 // them itself (as convrot_quantize_fp8 does, block by block): one launch instead of two, while the first weights
-// are on their way.  Measured with the 32 x 64 tile and two launches: ROWSNOTE
+// are on their way.  Here and on the 32 x 64 tile in us, from
+// codes: 1 row 4096 -> 12288 10.1 (5.0 TB/s) and 12.0, 8 rows 10.4 and 12.1, 16 rows 1024 -> 4096 4.2 and 5.3, 1 row
+// 15360 -> 5120 17.8 and 21.0; from 16-bit rows: 10.0 and 14.4 (1 row 4096 -> 12288), 4.2 and 7.6 (1 row 1024 -> 4096).
 constexpr int kRowsMax = 16, kRowsN = 64;
 // Bytes of a fused call's rows, which lie in LDS beside their codes, and which every workgroup quantizes: of one row,
 // and of several.  Fused and not, in us: 2 x 4096 -> 12288 10.6 and 13.1, 4 x 4096 -> 12288 12.7 and 12.7, 8 x 2048 ->
