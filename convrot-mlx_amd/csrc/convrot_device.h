@@ -293,6 +293,16 @@ __device__ __forceinline__ i32x4_sgpr buffer_rsrc(const void* base, uint32_t byt
                       __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
 }
 
+// The same for loads right behind it: its words may have been written by the vector unit
+// (v_readfirstlane, where the compiler cannot see that a value is uniform, or chose lanes' selects), after
+// which a load may read them 5 wait states later at the earliest.  The compiler puts those before its own
+// loads, not before inline asm; a load that came too early read stale words of the address, a memory fault.
+__device__ __forceinline__ i32x4_sgpr dma_rsrc(const void* base, uint32_t bytes) {
+  i32x4_sgpr r = buffer_rsrc(base, bytes);
+  asm volatile("s_nop 4" : "+s"(r));
+  return r;
+}
+
 // One wave-wide 16-byte-per-lane load from a buffer straight into LDS at
 // lds_addr + 16 * lane (buffer_load_dwordx4 ... lds, address in M0).  Issued
 // through asm so the compiler does not add conservative vmcnt waits before

@@ -17,14 +17,6 @@ constexpr int kBlock = 128;                      // features (and of a weight, o
 constexpr uint32_t kPastEnd = 0xffffff00u;       // buffer offset past every operand: reads zero
 constexpr int64_t kMaxExtent = 0xfffff000ll;     // bytes of an operand that is addressed as one buffer
 
-// A buffer resource for the loads below: its words may have been written by the vector unit
-// (v_readfirstlane, where the compiler cannot see that a value is uniform), after which a load may read them 5
-// wait states later at the earliest.  The compiler puts those before its own loads, not before inline asm.
-__device__ __forceinline__ i32x4_sgpr dma_rsrc(const void* base, uint32_t bytes) {
-  i32x4_sgpr r = buffer_rsrc(base, bytes);
-  asm volatile("s_nop 4" : "+s"(r));
-  return r;
-}
 // dma16 and dma4 with the wait state that a load to LDS needs behind the write of its address into M0.
 __device__ __forceinline__ void load_lds16(i32x4_sgpr rsrc, uint32_t voffset, uint32_t lds_addr) {
   asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)

@@ -597,7 +597,7 @@ struct DmaEngine {
       const int off = (arr == 0 ? EPI_OFF : arr == 1 ? WS_OFF : BIAS_OFF) + epi_buf * EPI_BYTES;
       const float* base = arr == 0 ? xscales + m0 : arr == 1 ? wscales + n0 : (bias ? bias + n0 : wscales);
       const int count = arr == 0 ? M - m0 : (arr == 1 || bias) ? N - n0 : 0;
-      const i32x4_sgpr r = buffer_rsrc(base, (uint32_t)count * 4u);
+      const i32x4_sgpr r = dma_rsrc(base, (uint32_t)count * 4u);
       dma4(r, (uint32_t)(q * 256 + lane * 4), smem_addr + (uint32_t)(off + q * 256));
     }
   }
@@ -1522,7 +1522,7 @@ struct Fp6Engine {
       const int off = arr == 0 ? EPI_OFF : arr == 1 ? WS_OFF : BIAS_OFF;
       const float* base = arr == 0 ? xscales + m0 : arr == 1 ? wscales + n0 : (bias ? bias + n0 : wscales);
       const int count = arr == 0 ? M - m0 : (arr == 1 || bias) ? N - n0 : 0;
-      const i32x4_sgpr r = buffer_rsrc(base, (uint32_t)count * 4u);
+      const i32x4_sgpr r = dma_rsrc(base, (uint32_t)count * 4u);
       dma4(r, (uint32_t)(q * 256 + lane * 4), smem_addr + (uint32_t)(off + q * 256));
     }
   }

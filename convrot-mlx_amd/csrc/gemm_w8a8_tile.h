@@ -142,7 +142,7 @@ struct Engine {
       const float* base = arr == 0 ? p.xscales + m0 : arr == 1 ? p.wscales + n0 : (p.bias ? p.bias + n0 : p.wscales);
       // at most the tile's: four bytes times all that follow may pass 32 bits
       const int count = arr == 0 ? min(BM, p.M - m0) : (arr == 1 || p.bias) ? min(BN, p.N - n0) : 0;
-      dma4(buffer_rsrc(base, (uint32_t)count * 4u), (uint32_t)(q * 256 + lane * 4), smem_addr + (uint32_t)(off + q * 256));
+      dma4(dma_rsrc(base, (uint32_t)count * 4u), (uint32_t)(q * 256 + lane * 4), smem_addr + (uint32_t)(off + q * 256));
     }
   }
 
