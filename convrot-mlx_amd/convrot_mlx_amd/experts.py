@@ -93,6 +93,11 @@ def _grouped_rows(x: torch.Tensor, experts: int, plan: ExpertPlan, gather: bool)
     rows = index.shape[0]
     if rows % max(1, tokens) or (tokens == 0 and rows):
         raise ValueError(f"{rows} sorted rows are no whole number of choices of {tokens} tokens")
+    if plan.slots is not None:  # says how many choices a token has: x of another number of tokens is no input of this plan
+        slots = _plan_tensor("slots", plan.slots, 2)
+        if slots.shape[0] != tokens or slots.numel() != rows:
+            raise ValueError(f"the plan orders {tuple(slots.shape)} choices, {slots.shape[0]} tokens' ({rows} rows), got x of "
+                             f"{tokens} rows (sorted rows are taken without gather)")
     return _Rows(offsets, index, max(1, rows // max(1, tokens)), rows)
 
 

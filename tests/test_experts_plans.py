@@ -1,0 +1,39 @@
+"""CPU: what the experts' calls make of a plan that does not fit their rows, before any launch."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from convrot_mlx_amd import ExpertPlan, grouped_linear, hip_fp8_grouped_linear, hip_grouped_linear, hip_grouped_linear_backward
+
+FP8 = torch.float8_e4m3fn
+BF16 = torch.bfloat16
+
+
+def ints(*values):
+    return torch.tensor(values, dtype=torch.int32)
+
+
+PLAN = ExpertPlan(ints(0, 2, 4), ints(0, 2, 1, 3), ints(0, 2, 1, 3).view(2, 2))  # 2 tokens of 2 choices
+
+
+@pytest.mark.parametrize("plan,rows", [(PLAN, 4), (PLAN, 1), (PLAN._replace(slots=PLAN.slots.view(4, 1)), 2),
+                                       (PLAN._replace(slots=PLAN.slots.view(1, 4)), 2),
+                                       (PLAN._replace(slots=ints(0, 1).view(2, 1)), 2)])
+def test_rows_of_another_number_of_tokens(plan, rows):
+    """Sorted rows are a whole number of choices of any divisor's tokens: the plan's slots say which it is."""
+    x, w = torch.zeros(rows, 16, dtype=BF16), torch.zeros(2, 8, 16, dtype=BF16)
+    codes = torch.zeros(2, 8, 16, dtype=torch.uint8).view(FP8)
+    for call in (lambda: hip_grouped_linear(x, w, plan, gather=True), lambda: grouped_linear(x, w, plan, gather=True),
+                 lambda: hip_fp8_grouped_linear(x, codes, torch.ones(2, 1, 1), plan, gather=True),
+                 lambda: hip_grouped_linear_backward(torch.zeros(4, 8, dtype=BF16), x, w, plan, gather=True)):
+        with pytest.raises(ValueError, match="the plan orders"):
+            call()
+
+
+def test_rows_that_fit_reach_the_device_check():
+    w = torch.zeros(2, 8, 16, dtype=BF16)
+    for rows, plan, gather in ((2, PLAN, True), (4, PLAN, False), (2, PLAN._replace(slots=None), True), (4, PLAN._replace(slots=None), True)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            hip_grouped_linear(torch.zeros(rows, 16, dtype=BF16), w, plan, gather=gather)
