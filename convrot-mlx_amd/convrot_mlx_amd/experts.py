@@ -351,8 +351,10 @@ class _GroupedLinear(torch.autograd.Function):
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, *, gather: bool = False) -> torch.Tensor:
     """hip_grouped_linear, with gradients for the rows and the weights (reverse mode; dual tensors of forward
-    mode are refused)."""
+    mode are refused).  With `gather` the rows' gradient needs the plan's slots."""
     if nat.differentiated(x, weight):
+        if gather and x.requires_grad:
+            _plan_tensor("slots", plan.slots, 2)
         return _GroupedLinear.apply(x, weight, plan, gather)
     return hip_grouped_linear(x, weight, plan, gather=gather)
 

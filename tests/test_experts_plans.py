@@ -37,3 +37,17 @@ def test_rows_that_fit_reach_the_device_check():
     for rows, plan, gather in ((2, PLAN, True), (4, PLAN, False), (2, PLAN._replace(slots=None), True), (4, PLAN._replace(slots=None), True)):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             hip_grouped_linear(torch.zeros(rows, 16, dtype=BF16), w, plan, gather=gather)
+
+
+def test_gradient_of_gathered_rows_without_slots():
+    """Refused by the forward pass: the backward pass could not sum a token's choices."""
+    w, plan = torch.zeros(2, 8, 16, dtype=BF16), PLAN._replace(slots=None)
+    x = torch.zeros(2, 16, dtype=BF16, requires_grad=True)
+    with pytest.raises(ValueError, match="needs the plan's slots"):
+        grouped_linear(x, w, plan, gather=True)
+    # the weight's gradient alone, sorted rows, and no gradient at all do without
+    for call in (lambda: grouped_linear(x.detach(), w.requires_grad_(), plan, gather=True),
+                 lambda: grouped_linear(torch.zeros(4, 16, dtype=BF16, requires_grad=True), w, plan),
+                 lambda: torch.no_grad()(grouped_linear)(x, w, plan, gather=True)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
