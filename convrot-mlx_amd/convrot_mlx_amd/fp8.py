@@ -221,7 +221,7 @@ class Fp8Buffers(nn.Module):
         kept = dict(self._buffers)
         super()._apply(fn, recurse)
         for name, t in kept.items():
-            if self._buffers[name].dtype != t.dtype:
+            if t is not None and self._buffers[name].dtype != t.dtype:
                 self._buffers[name] = t.to(self._buffers[name].device)
         return self
 
