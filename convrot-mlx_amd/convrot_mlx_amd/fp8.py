@@ -278,7 +278,8 @@ class Fp8Linear(Fp8Buffers):
         """self((1 + scale) * layer_norm(x) + shift), the norm as hip_layer_norm rounds it; residual, gate and
         inplace as in forward."""
         def normed():
-            return hip_layer_norm(x, scale=scale, shift=shift, eps=eps)
+            with nat.on(x.device):  # as the linear itself
+                return hip_layer_norm(x, scale=scale, shift=shift, eps=eps)
 
         return self(nat.without_gradient(normed, "Fp8Linear", x, shift, scale), residual=residual, gate=gate,
                     inplace=inplace)
