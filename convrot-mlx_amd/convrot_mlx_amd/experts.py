@@ -190,6 +190,8 @@ def hip_combine_rows_backward(dout: torch.Tensor, rows: torch.Tensor | None, pla
     if dout.ndim != 2 or dout.shape[0] != tokens:
         raise ValueError(f"dout {tuple(dout.shape)} must have a row for each of {tokens} tokens")
     if weights is not None:
+        if rows is None:
+            raise ValueError("the gradient of weights needs the rows they weighted")
         if rows.dtype != dout.dtype or rows.ndim != 2 or rows.shape[1] != dout.shape[1]:
             raise ValueError(f"dout {dout.dtype} {tuple(dout.shape)} must match rows {rows.dtype} {tuple(rows.shape)}")
         _combine_checks(rows, plan, weights)

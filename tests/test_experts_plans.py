@@ -5,7 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from convrot_mlx_amd import ExpertPlan, grouped_linear, hip_fp8_grouped_linear, hip_grouped_linear, hip_grouped_linear_backward
+from convrot_mlx_amd import (ExpertPlan, grouped_linear, hip_combine_rows_backward, hip_fp8_grouped_linear, hip_grouped_linear,
+                             hip_grouped_linear_backward)
 
 FP8 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
@@ -51,3 +52,8 @@ def test_gradient_of_gathered_rows_without_slots():
                  lambda: torch.no_grad()(grouped_linear)(x, w, plan, gather=True)):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
+
+
+def test_gradient_of_weights_without_rows():
+    with pytest.raises(ValueError, match="needs the rows"):
+        hip_combine_rows_backward(torch.zeros(2, 6), None, PLAN, torch.ones(2, 2))
