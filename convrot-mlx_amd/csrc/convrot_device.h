@@ -306,16 +306,20 @@ __device__ __forceinline__ i32x4_sgpr dma_rsrc(const void* base, uint32_t bytes)
 // One wave-wide 16-byte-per-lane load from a buffer straight into LDS at
 // lds_addr + 16 * lane (buffer_load_dwordx4 ... lds, address in M0).  Issued
 // through asm so the compiler does not add conservative vmcnt waits before
-// LDS reads; the kernel orders these loads with explicit waits + barriers.
+// LDS reads; the kernel orders these loads with explicit waits + barriers.  The
+// s_nop is the wait state that a load to LDS needs behind the write of M0, which
+// the compiler puts only before its own loads.
 __device__ __forceinline__ void dma16(i32x4_sgpr rsrc, uint32_t voffset, uint32_t lds_addr) {
-  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr) : "memory");
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)
+               : "memory");
 }
 
 // The same with 4 bytes per lane (buffer_load_dword ... lds): LDS at
 // lds_addr + 4 * lane.  Each dword is range-checked on its own, so a ragged
 // end reads zeros exactly from the first dword past `bytes`.
 __device__ __forceinline__ void dma4(i32x4_sgpr rsrc, uint32_t voffset, uint32_t lds_addr) {
-  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr) : "memory");
+  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)
+               : "memory");
 }
 
 // 16 bytes per lane at p + OFF through a device-scope (sc1) load, coherent

@@ -17,16 +17,6 @@ constexpr int kBlock = 128;                      // features (and of a weight, o
 constexpr uint32_t kPastEnd = 0xffffff00u;       // buffer offset past every operand: reads zero
 constexpr int64_t kMaxExtent = 0xfffff000ll;     // bytes of an operand that is addressed as one buffer
 
-// dma16 and dma4 with the wait state that a load to LDS needs behind the write of its address into M0.
-__device__ __forceinline__ void load_lds16(i32x4_sgpr rsrc, uint32_t voffset, uint32_t lds_addr) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)
-               : "memory");
-}
-__device__ __forceinline__ void load_lds4(i32x4_sgpr rsrc, uint32_t voffset, uint32_t lds_addr) {
-  asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)
-               : "memory");
-}
-
 struct Fp8Scale {
   float inverse, scale;
 };

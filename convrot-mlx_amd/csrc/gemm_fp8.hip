@@ -66,13 +66,13 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(Fp8Operands p, const 
 
   // the weights' scales, and the rows: as they are, 16-byte chunks of [row][n 128], or their codes and scales
   const i32x4_sgpr rs = dma_rsrc(p.wscales + (int64_t)(tile * kRowsN / kBlock) * p.ws_row + kb0, (uint32_t)n * 4u);
-  for (uint32_t i0 = wave * 64u; i0 < (uint32_t)n; i0 += 256u) load_lds4(rs, (i0 + lane) * 4u, base + at.ws + i0 * 4u);
+  for (uint32_t i0 = wave * 64u; i0 < (uint32_t)n; i0 += 256u) dma4(rs, (i0 + lane) * 4u, base + at.ws + i0 * 4u);
   if constexpr (FUSED) {
     const uint32_t per_row = (uint32_t)n * 8u * ES, chunks = M * per_row;
     const i32x4_sgpr rx = dma_rsrc(x, (uint32_t)(((int64_t)(p.M - 1) * x_stride + p.K) * ES));
     for (uint32_t i0 = wave * 64u; i0 < chunks; i0 += 256u) {
       const uint32_t i = i0 + (uint32_t)lane, r = M == 1 ? 0u : i / per_row, b = k0 * ES + (i - r * per_row) * 16u;
-      load_lds16(rx, i < chunks && b < (uint32_t)p.K * ES ? r * (uint32_t)x_stride * ES + b : kPastEnd,
+      dma16(rx, i < chunks && b < (uint32_t)p.K * ES ? r * (uint32_t)x_stride * ES + b : kPastEnd,
                  base + at.raw + i0 * 16u);
     }
   } else {
@@ -81,12 +81,12 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(Fp8Operands p, const 
     for (uint32_t i0 = wave * 64u; i0 < chunks; i0 += 256u) {
       const uint32_t i = i0 + (uint32_t)lane, b = i / per_block, r = (i - b * per_block) >> 3;
       const uint32_t k = k0 + b * 128u + (((i & 7u) ^ (uint32_t)chunk_swizzle((int)r)) << 4);
-      load_lds16(ra, i < chunks && k < k16 ? r * (uint32_t)p.lda + k : kPastEnd, base + at.codes + i0 * 16u);
+      dma16(ra, i < chunks && k < k16 ? r * (uint32_t)p.lda + k : kPastEnd, base + at.codes + i0 * 16u);
     }
     const i32x4_sgpr rx = dma_rsrc(p.xscales, (uint32_t)((p.M - 1) * p.xs_row + (kblocks - 1) * p.xs_block) * 4u + 4u);
     for (uint32_t i0 = wave * 64u; i0 < M * (uint32_t)n; i0 += 256u) {
       const uint32_t i = i0 + (uint32_t)lane, b = i / M, r = i - b * M;
-      load_lds4(rx, i < M * (uint32_t)n ? (r * (uint32_t)p.xs_row + (kb0 + b) * (uint32_t)p.xs_block) * 4u : kPastEnd,
+      dma4(rx, i < M * (uint32_t)n ? (r * (uint32_t)p.xs_row + (kb0 + b) * (uint32_t)p.xs_block) * 4u : kPastEnd,
                 base + at.xs + i0 * 4u);
     }
   }
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(Fp8Operands p, const 
     for (int j = 0; j < 2; ++j) {
       uint32_t off = vw[j] + kb * 128u;
       if (kb == tail_kb) off = past[j] ? kPastEnd : off;
-      load_lds16(rw, off, ring + (uint32_t)(stage * 2048 + j * 1024));
+      dma16(rw, off, ring + (uint32_t)(stage * 2048 + j * 1024));
     }
   };
 #pragma unroll

@@ -133,7 +133,7 @@ struct Fp8Engine {
     const float* base = p.wscales + (int64_t)expert * p.ws_expert + (int64_t)(n0 / kBlock) * p.ws_row;
     for (int d = wave; d < nb * pieces; d += NW) {
       const int j = d / pieces, at = d - j * pieces;
-      load_lds4(dma_rsrc(base + j * p.ws_row, (uint32_t)blocks * 4u), (uint32_t)(at * 256 + lane * 4),
+      dma4(dma_rsrc(base + j * p.ws_row, (uint32_t)blocks * 4u), (uint32_t)(at * 256 + lane * 4),
            smem_addr + (uint32_t)(WS_OFF + d * 256));
     }
   }
@@ -145,15 +145,15 @@ struct Fp8Engine {
     for (int i = 0; i < APW; ++i) {
       uint32_t off = va[i] == kPastEnd ? kPastEnd : va[i] + k;
       if (last) off = past_a[i & 1] ? kPastEnd : off;
-      load_lds16(ra, off, base + (uint32_t)(wave * APW + i) * 1024u);
+      dma16(ra, off, base + (uint32_t)(wave * APW + i) * 1024u);
     }
 #pragma unroll
     for (int i = 0; i < BPW; ++i) {
       uint32_t off = vw[i] + k;
       if (last) off = past_w[i & 1] ? kPastEnd : off;
-      load_lds16(rw, off, base + (uint32_t)BM * 128u + (uint32_t)(wave * BPW + i) * 1024u);
+      dma16(rw, off, base + (uint32_t)BM * 128u + (uint32_t)(wave * BPW + i) * 1024u);
     }
-    load_lds4(dma_rsrc(xs_base + (int64_t)kb * xs_block, xs_bytes), vx, base + (uint32_t)XS_OFF + (uint32_t)wave * 256u);
+    dma4(dma_rsrc(xs_base + (int64_t)kb * xs_block, xs_bytes), vx, base + (uint32_t)XS_OFF + (uint32_t)wave * 256u);
   }
 
   __device__ __forceinline__ i32x8 fragment(const uint8_t* row) const {

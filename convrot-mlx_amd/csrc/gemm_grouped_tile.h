@@ -210,7 +210,7 @@ struct Side {
       o = o == kPastEnd ? kPastEnd : o + kb * 128u;
       if (kb == tail) o = past[i & 1] ? kPastEnd : o;
     }
-    load_lds16(r, o, lds + (uint32_t)(wave * PW + i) * 1024u);
+    dma16(r, o, lds + (uint32_t)(wave * PW + i) * 1024u);
   }
 
   // The address of this lane's part of fragment 0 of the wave's corner at `first`, k-step 0; of

@@ -18,10 +18,18 @@ def _resource(fn: Function, i: int):
             yield "resource", f"{other.text} | {between} | {load.text}"
 
 
+def _m0(fn: Function, i: int):
+    """A load to LDS begins a wait state behind the write of its address into M0, or later."""
+    for other, _ in fn.before(i, 1):
+        if "m0" in other.writes():
+            yield "m0", f"{other.text} | {fn[i].text}"
+
+
 def check(fn: Function) -> list:
     found = []
     for i in fn.find(" lds"):
         found += _resource(fn, i)
+        found += _m0(fn, i)
     return [(kind, fn.name, text) for kind, text in found]
 
 
@@ -59,5 +67,16 @@ def test_the_check_of_resources():
     assert check(function(write, "s_branch 1 -> 3", "s_nop 7", "s_nop 3", LOAD)) == []
 
 
+def test_the_check_of_m0():
+    for write in ("s_mov_b32 m0, s3", "s_add_i32 m0, s3, s4"):
+        assert [k for k, _, _ in check(function(write, LOAD))] == ["m0"]
+        assert check(function(write, "s_nop 0", LOAD)) == []
+    assert check(function("s_mov_b32 s3, m0", LOAD)) == []
+
+
 def test_resources(found):
     assert found["resource"] == []
+
+
+def test_m0(found):
+    assert found["m0"] == []
