@@ -1710,7 +1710,9 @@ struct Fp6Engine {
 
   __device__ __forceinline__ void run(int n, f32x4 (&acc)[FN][FM]) {
     static_assert(LPW <= 2 * FN * HM, "DMA pieces fit the half");
-    const int scale = (int)0x82828282u;  // E8M0 scales of 2^3 (one byte per 32-feature group)
+    int scale = (int)0x82828282u;  // E8M0 scales of 2^3 (one byte per 32-feature group)
+    // two wait states between the vector unit's write and the first MFMA, and no writing it anew later
+    asm volatile("s_nop 1" : "+v"(scale));
     if constexpr (CW) {
       const uint32_t z0 = __builtin_amdgcn_readfirstlane(kFp6cZ0), z1 = __builtin_amdgcn_readfirstlane(kFp6cZ1);
       i32x6 a[FM], b[FN];

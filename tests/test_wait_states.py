@@ -25,11 +25,22 @@ def _m0(fn: Function, i: int):
             yield "m0", f"{other.text} | {fn[i].text}"
 
 
+def _operands(fn: Function, i: int):
+    """A matrix instruction reads what the vector unit wrote 2 wait states later or more."""
+    mfma = fn[i]
+    read = registers(" ".join(mfma.operands[1:]))
+    for other, between in fn.before(i, 2):
+        if other.op.startswith("v_") and not other.op.startswith("v_mfma") and other.writes() & read:
+            yield "operand", f"{other.text} | {between} | {mfma.text}"
+
+
 def check(fn: Function) -> list:
     found = []
     for i in fn.find(" lds"):
         found += _resource(fn, i)
         found += _m0(fn, i)
+    for i in fn.find("v_mfma"):
+        found += _operands(fn, i)
     return [(kind, fn.name, text) for kind, text in found]
 
 
@@ -40,7 +51,7 @@ def found(tmp_path_factory):
     if not OBJDUMP.exists():
         pytest.skip("no disassembler")
     out = defaultdict(list)
-    for kind, name, text in check_library(_native.LIB_PATH, tmp_path_factory.mktemp("code"), (" lds",), check):
+    for kind, name, text in check_library(_native.LIB_PATH, tmp_path_factory.mktemp("code"), (" lds", "v_mfma"), check):
         out[kind].append((name, text))
     return out
 
@@ -74,9 +85,24 @@ def test_the_check_of_m0():
     assert check(function("s_mov_b32 s3, m0", LOAD)) == []
 
 
+MFMA = "v_mfma_i32_16x16x64_i8 a[0:3], v[4:7], v[8:11], a[0:3]"
+SCALED = "v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[4:9], v[12:17], a[0:3], v20, v20 op_sel_hi:[0,0,0] cbsz:2 blgp:2"
+
+
+def test_the_check_of_operands():
+    for write, mfma in (("v_mov_b32_e32 v11, 0", MFMA), ("v_mov_b32_e32 v20, 0x82", SCALED), ("v_accvgpr_write_b32 a2, 0", MFMA)):
+        assert [k for k, _, _ in check(function(write, "s_mov_b32 s1, 0", mfma))] == ["operand"]
+        assert check(function(write, "s_nop 1", mfma)) == []
+    assert check(function("v_mov_b32_e32 v3, 0", MFMA)) == [] and check(function(MFMA, MFMA)) == []
+
+
 def test_resources(found):
     assert found["resource"] == []
 
 
 def test_m0(found):
     assert found["m0"] == []
+
+
+def test_operands(found):
+    assert found["operand"] == []
