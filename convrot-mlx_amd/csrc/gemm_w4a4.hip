@@ -490,21 +490,18 @@ __device__ __forceinline__ void mfma_drain(i32x4 (&acc)[FN][FM]) {
 // The 32 x 32 x 32 form: acc (16 AGPRs, a 32 x 32 int32 block) += b . a.  Lane
 // l supplies row l % 32 of each operand and 16 bytes of its k-group l / 32;
 // the result's register v of lane l is (n = 8 (v / 4) + 4 (l / 32) + v % 4,
-// m = l % 32) of the block.  Hazards as for mfma_agpr (the drain's 24 wait
-// states also cover this MFMA's longer result latency).
+// m = l % 32) of the block.  Hazards as for mfma_agpr; its results take 12 wait
+// states (mfma_settle32).
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ void mfma_agpr32(i32x16& c, const i32x4& b, const i32x4& a) {
   asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(c) : "v"(b), "v"(a) : "memory");
 }
 
-template <int FN, int FM>
-__device__ __forceinline__ void mfma_drain32(i32x16 (&acc)[FN][FM]) {
-  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
-#pragma unroll
-  for (int fn = 0; fn < FN; ++fn)
-#pragma unroll
-    for (int fm = 0; fm < FM; ++fm) asm volatile("" : "+a"(acc[fn][fm]));
-}
+// At the end of each turn of the k-loop: the 12 wait states that its last MFMA's results need.  Inside the loop, as
+// the compiler moves accumulators to other registers on the way out of it, in front of whatever stands behind it
+// (with the waits there it read the last ones 3 wait states early).  The next turn's first MFMA has to wait for 8 of
+// the 12 in any case: 16 cycles of a turn's 2048.
+__device__ __forceinline__ void mfma_settle32() { asm volatile("s_nop 7\n\ts_nop 3" ::: "memory"); }
 
 // Global slot (0 .. 31) of the second half-block at which DMA piece p of the
 // 32 x 32 k-loop is issued: the 12 pieces spread evenly over its 32 MFMAs.
@@ -977,8 +974,8 @@ struct DmaEngine {
       agpr32_kstep<2>(st, nst, dma_kb, bq, a, w, acc);
       agpr32_kstep<3>(st, nst, dma_kb, bq, a, w, acc);
       st = nst;
+      mfma_settle32();
     }
-    mfma_drain32(acc);
     wait_vmcnt<0>();  // the DMAs past the last block have landed before the ring is reused
   }
 

@@ -34,6 +34,23 @@ def _operands(fn: Function, i: int):
             yield "operand", f"{other.text} | {between} | {mfma.text}"
 
 
+# wait states behind a matrix instruction before anything but one of its kind, on the same sums, may touch its results
+RESULT = {"v_mfma_i32_16x16x64_i8": 8, "v_mfma_f32_16x16x32_bf16": 8, "v_mfma_f32_16x16x32_f16": 8, "v_mfma_i32_32x32x32_i8": 12,
+          "v_mfma_f32_16x16x128_f8f6f4": 12, "v_mfma_scale_f32_16x16x128_f8f6f4": 12, "v_mfma_f32_4x4x4_16b_bf16": 5}
+
+
+def _result(fn: Function, i: int):
+    """The results of a matrix instruction are read and written over after its passes."""
+    mfma = fn[i]
+    out = registers(mfma.operands[0])
+    for other, between in fn.after(i, RESULT[mfma.op]):
+        if other is mfma or not other.op.startswith(("v_", "buffer_", "global_", "ds_")):
+            continue
+        touched = registers(" ".join(other.operands[1:3] if other.op.startswith("v_mfma") else other.operands))
+        if touched & out:
+            yield "result", f"{mfma.text} | {between} | {other.text}"
+
+
 def check(fn: Function) -> list:
     found = []
     for i in fn.find(" lds"):
@@ -41,6 +58,7 @@ def check(fn: Function) -> list:
         found += _m0(fn, i)
     for i in fn.find("v_mfma"):
         found += _operands(fn, i)
+        found += _result(fn, i)
     return [(kind, fn.name, text) for kind, text in found]
 
 
@@ -96,6 +114,16 @@ def test_the_check_of_operands():
     assert check(function("v_mov_b32_e32 v3, 0", MFMA)) == [] and check(function(MFMA, MFMA)) == []
 
 
+def test_the_check_of_results():
+    for read in ("v_accvgpr_read_b32 v1, a2", "v_accvgpr_write_b32 a2, 0", "buffer_store_dword a2, v1, s[0:3], 0 offen"):
+        assert [k for k, _, _ in check(function(MFMA, "s_nop 6", read))] == ["result"]
+        assert check(function(MFMA, "s_nop 7", read)) == []
+    assert check(function(MFMA, MFMA, "v_accvgpr_read_b32 v1, a4")) == []
+    # at the end of a loop, and in its next turn
+    assert check(function("v_accvgpr_read_b32 v1, a2", "s_nop 7", MFMA, "s_cbranch_scc1 65532 -> 0", "s_nop 7"))
+    assert check(function(MFMA, "s_cbranch_scc1 65534 -> 0", "v_accvgpr_read_b32 v1, a2"))
+
+
 def test_resources(found):
     assert found["resource"] == []
 
@@ -106,3 +134,7 @@ def test_m0(found):
 
 def test_operands(found):
     assert found["operand"] == []
+
+
+def test_results(found):
+    assert found["result"] == []
