@@ -31,7 +31,9 @@ MAX_STRIDE = 1 << 21
 class ExpertPlan(NamedTuple):
     """Sorted rows by expert, int32 on the device: expert e has rows offsets[e] .. offsets[e + 1] - 1
     (offsets [E + 1], from 0), row s is choice order[s] (token order[s] // C, order [T C]), and choice
-    (t, c) is row slots[t, c].  order and slots may be None for rows that a caller sorted itself."""
+    (t, c) is row slots[t, c].  order and slots may be None for rows that a caller sorted itself.  A caller's own
+    may hold places out of range (a row of no choice, a choice without a row); else they are each other's
+    inverse, and no two choices share a row: gradients follow order and slots where they agree."""
 
     offsets: torch.Tensor
     order: torch.Tensor | None = None
@@ -183,8 +185,9 @@ def hip_combine_rows(rows: torch.Tensor, plan: ExpertPlan, weights: torch.Tensor
 
 def hip_combine_rows_backward(dout: torch.Tensor, rows: torch.Tensor | None, plan: ExpertPlan,
                               weights: torch.Tensor | None = None):
-    """Gradients of hip_combine_rows from dout [T, N]: (drows [T C, N] = weights[t, c] * dout[t], dweights [T, C] =
-    <dout[t], rows[slots[t, c]]> of the weights' type); without weights dweights is None and rows are not read."""
+    """Gradients of hip_combine_rows from dout [T, N]: (drows [T C, N] = weights[t, c] * dout[t], zeros in rows
+    that are no choice's, dweights [T, C] = <dout[t], rows[slots[t, c]]> of the weights' type); without weights
+    dweights is None and rows are not read."""
     slots, order = _plan_tensor("slots", plan.slots, 2), _plan_tensor("order", plan.order, 1)
     tokens, choices = slots.shape
     if dout.ndim != 2 or dout.shape[0] != tokens:

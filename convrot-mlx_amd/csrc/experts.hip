@@ -1,6 +1,8 @@
 // What lies around the linears of a mixture of experts: the order of the tokens'
 // choices by expert, rows gathered in that order, and the experts' rows summed back to
 // tokens with its gradient.
+#include <algorithm>
+
 #include "convrot_launch.h"
 #include "row_device.h"
 
@@ -237,17 +239,46 @@ __global__ __launch_bounds__(256) void combine_kernel(const typename Elem<DT>::T
   }
 }
 
+// Zeros in the rows of dy from row0 to row_end that no choice has: order names none for them, or one whose place is
+// another row (in a caller's own plan).  A wave looks at 64 rows at a time.
+template <int DT, bool VEC>
+__device__ __forceinline__ void clear_rows_of_none(const int* __restrict__ order, const int* __restrict__ slots,
+                                                   int64_t row0, int64_t row_end, int64_t rows, int features, int wave,
+                                                   int waves, typename Elem<DT>::T* __restrict__ dy) {
+  const int lane = threadIdx.x & 63;
+  constexpr int W = Piece<DT, VEC>::W;
+  for (int64_t s0 = row0 + (int64_t)wave * 64; s0 < row_end; s0 += (int64_t)waves * 64) {
+    const int64_t s = s0 + lane;
+    const int i = s < row_end ? order[s] : -1;
+    uint64_t none = __ballot(s < row_end && !(i >= 0 && i < rows && slots[i] == (int)s));
+    for (; none; none &= none - 1) {
+      typename Elem<DT>::T* row = dy + (s0 + __builtin_ctzll(none)) * features;
+      const Piece<DT, VEC> zero{};
+      for (int f = lane * W; f < features; f += 64 * W) zero.store(row + f);
+    }
+  }
+}
+
 // dy[s] = weights[t][c] * dout[t] and dweights[t][c] = <dout[t], y[s]>, s = slots[t][c], a token's
 // threads together: dout is read once, y once, dy written once.  A row is written by the choice that
-// `order` names for it alone, so none is written twice.
+// `order` names for it alone, so none is written twice; the last `clearing` workgroups clear those of no choice, among
+// the rows whose numbers are the launch's choices (36864 rows of 4096: 134 to 137 us with them and without; looked
+// for by the tokens' own threads, whose loads then wait for two more, 175).
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void combine_backward_kernel(
     const typename Elem<DT>::T* __restrict__ dout, int64_t dout_stride, const typename Elem<DT>::T* __restrict__ y,
     int64_t y_rows, int64_t y_stride, const int* __restrict__ order, const int* __restrict__ slots,
     const float* __restrict__ weights, int64_t token0, int64_t tokens, int choices, int features, int threads,
-    typename Elem<DT>::T* __restrict__ dy, float* __restrict__ dweights) {
+    unsigned clearing, typename Elem<DT>::T* __restrict__ dy, float* __restrict__ dweights) {
   __shared__ float part[4][4];  // [choice of the batch][wave]
   const int each = 256 / threads, at = threadIdx.x & (threads - 1), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (blockIdx.x >= gridDim.x - clearing) {
+    const unsigned mine = blockIdx.x - (gridDim.x - clearing);
+    const int64_t end = min(tokens, token0 + (int64_t)(gridDim.x - clearing) * each) * choices;
+    clear_rows_of_none<DT, VEC>(order, slots, token0 * choices, end, y_rows, features, (int)mine * 4 + wave,
+                                (int)clearing * 4, dy);
+    return;
+  }
   const int64_t t = token0 + (int64_t)blockIdx.x * each + threadIdx.x / threads;
   constexpr int W = Piece<DT, VEC>::W, BATCH = 4;
   const bool on = t < tokens;
@@ -337,10 +368,10 @@ bool in_pieces(int64_t features, std::initializer_list<const void*> bases, std::
   return good;
 }
 
-// Launches of at most as many workgroups as one takes: run(first row, workgroups).
+// Launches of at most as many workgroups as one takes, `more` beside the rows': run(first row, the rows' workgroups).
 template <class F>
-hipError_t in_launches(int64_t rows, int threads, F&& run) {
-  const int64_t each = 256 / threads, most = max_groups(256) * each;
+hipError_t in_launches(int64_t rows, int threads, F&& run, unsigned more = 0) {
+  const int64_t each = 256 / threads, most = (max_groups(256) - more) * each;
   for (int64_t r0 = 0; r0 < rows; r0 += most) {
     const int64_t some = rows - r0 < most ? rows - r0 : most;
     run(r0, dim3((unsigned)((some + each - 1) / each)));
@@ -388,16 +419,19 @@ hipError_t combine_backward_t(const void* dout, int64_t dout_stride, const void*
   typedef typename Elem<DT>::T T;
   const bool vec = in_pieces<DT>(features, {dout, y, dy}, {dout_stride, y_stride});
   const int threads = threads_of(features, vec);
+  // a workgroup for 1024 rows, up to one a CU
+  const unsigned clearing = dy ? (unsigned)std::min<int64_t>((y_rows + 1023) / 1024, 256) : 0;
   return in_launches(tokens, threads, [&](int64_t t0, dim3 grid) {
+    grid.x += clearing;
     if (vec)
       combine_backward_kernel<DT, true><<<grid, dim3(256), 0, s>>>(
           (const T*)dout, dout_stride, (const T*)y, y_rows, y_stride, order, slots, weights, t0, tokens, choices,
-          (int)features, threads, (T*)dy, dweights);
+          (int)features, threads, clearing, (T*)dy, dweights);
     else
       combine_backward_kernel<DT, false><<<grid, dim3(256), 0, s>>>(
           (const T*)dout, dout_stride, (const T*)y, y_rows, y_stride, order, slots, weights, t0, tokens, choices,
-          (int)features, threads, (T*)dy, dweights);
-  });
+          (int)features, threads, clearing, (T*)dy, dweights);
+  }, clearing);
 }
 
 }  // namespace

@@ -648,8 +648,10 @@ int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_str
  * convrot_combine_rows: out[t] = sum over c of weights[t][c] * y[slots[t][c]] (weights NULL: 1), in float32,
  * the choices in order, rounded once; a slot outside 0 .. y_rows - 1 adds nothing.
  * convrot_combine_rows_backward: dy[s] = weights[t][c] * dout[t] for s = slots[t][c] with order[s] = t * choices + c, dy
- * [y_rows, features], and dweights[t][c] = <dout[t], y[slots[t][c]]> (either may be NULL; y is read for
- * dweights alone); y_rows = tokens * choices.  Sums in a fixed order.
+ * [y_rows, features] (zeros in a row that no choice has so: every row is written), and dweights[t][c] =
+ * <dout[t], y[slots[t][c]]> (either may be NULL; y is read for dweights alone); y_rows = tokens * choices.  order and
+ * slots are each other's inverse but for places out of range; of choices that share a place dy takes the one that
+ * order names alone.  Sums in a fixed order.
  */
 int64_t convrot_expert_plan_workspace_bytes(int64_t count, int64_t experts);
 int convrot_expert_plan(const void* ids, int ids_bits, int64_t count, int64_t experts, int32_t* offsets, int32_t* order,
