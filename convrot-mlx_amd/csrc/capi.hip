@@ -1262,10 +1262,11 @@ int convrot_fp8_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t
 namespace {
 
 constexpr int64_t kMaxPlanExperts = 1024;  // one thread of the ordering workgroup each
+constexpr int64_t kMaxRowFeatures = kMaxRows - 2047;  // a row is walked with 32 bits, up to 2048 features a step
 
 int check_token_rows(const char* what, const void* y, int dtype, int64_t rows, int64_t features, int64_t stride,
                      int64_t tokens, int64_t choices) {
-  if (int rc = check_rows(what, y, dtype, rows, features, stride, kMaxRows)) return rc;
+  if (int rc = check_rows(what, y, dtype, rows, features, stride, kMaxRowFeatures)) return rc;
   if (tokens < 0 || choices < 1 || tokens * choices > kMaxRows || choices > kMaxRows)
     return fail(CONVROT_ERR_INVALID, "%s: invalid shape of %lld tokens of %lld choices", what, (long long)tokens,
                 (long long)choices);
@@ -1301,7 +1302,7 @@ int convrot_expert_plan(const void* ids, int ids_bits, int64_t count, int64_t ex
 
 int convrot_gather_rows(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const int32_t* index,
                         int64_t choices, int64_t rows, int64_t features, void* out, void* stream) {
-  if (int rc = check_rows("gathered rows", x, dtype, x_rows, features, x_stride, kMaxRows)) return rc;
+  if (int rc = check_rows("gathered rows", x, dtype, x_rows, features, x_stride, kMaxRowFeatures)) return rc;
   if (rows < 0 || rows > kMaxRows || choices < 1 || choices > kMaxRows)
     return fail(CONVROT_ERR_INVALID, "invalid shape of %lld gathered rows (%lld choices)", (long long)rows, (long long)choices);
   if (rows == 0 || features == 0) return ok();
@@ -1336,7 +1337,7 @@ int convrot_combine_rows_backward(const void* dout, int64_t dout_stride, const v
   if (y_rows != tokens * choices)
     return fail(CONVROT_ERR_INVALID, "%lld rows for %lld choices", (long long)y_rows, (long long)(tokens * choices));
   if (dweights)
-    if (int rc = check_rows("the gradient of combined rows", y, dtype, y_rows, features, y_stride, kMaxRows)) return rc;
+    if (int rc = check_rows("the gradient of combined rows", y, dtype, y_rows, features, y_stride, kMaxRowFeatures)) return rc;
   if (tokens == 0 || (!dy && !dweights)) return ok();
   if (!slots || (dy && !order)) return fail(CONVROT_ERR_INVALID, "null pointer argument");
   if (!aligned(order, 4) || !aligned(slots, 4) || !aligned(weights, 4) || !aligned(dweights, 4) ||

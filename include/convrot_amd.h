@@ -651,7 +651,7 @@ int convrot_grouped_linear_weight_grad(const void* dy, int dtype, int64_t dy_str
  * [y_rows, features] (zeros in a row that no choice has so: every row is written), and dweights[t][c] =
  * <dout[t], y[slots[t][c]]> (either may be NULL; y is read for dweights alone); y_rows = tokens * choices.  order and
  * slots are each other's inverse but for places out of range; of choices that share a place dy takes the one that
- * order names alone.  Sums in a fixed order.
+ * order names alone.  Sums in a fixed order.  Rows of all three have at most 2^31 - 2048 features.
  */
 int64_t convrot_expert_plan_workspace_bytes(int64_t count, int64_t experts);
 int convrot_expert_plan(const void* ids, int ids_bits, int64_t count, int64_t experts, int32_t* offsets, int32_t* order,

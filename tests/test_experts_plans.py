@@ -8,6 +8,8 @@ import torch
 from convrot_mlx_amd import (ExpertPlan, grouped_linear, hip_combine_rows_backward, hip_fp8_grouped_linear, hip_grouped_linear,
                              hip_grouped_linear_backward)
 
+P = 4096  # stands for any aligned device address: never read
+MOST = 2 ** 31 - 2048  # features of a row that is walked in 32 bits, up to 2048 a step
 FP8 = torch.float8_e4m3fn
 BF16 = torch.bfloat16
 
@@ -57,3 +59,15 @@ def test_gradient_of_gathered_rows_without_slots():
 def test_gradient_of_weights_without_rows():
     with pytest.raises(ValueError, match="needs the rows"):
         hip_combine_rows_backward(torch.zeros(2, 6), None, PLAN, torch.ones(2, 2))
+
+
+@pytest.mark.parametrize("features", [MOST + 1, 2 ** 31 - 1])
+def test_rows_too_long_to_walk(features):
+    from convrot_mlx_amd import _native
+
+    lib = _native.load()
+    for status in (lib.convrot_gather_rows(P, 2, 4, features, P, 2, 8, features, P, None),
+                   lib.convrot_combine_rows(P, 2, 8, features, P, P, 4, 2, features, P, None),
+                   lib.convrot_combine_rows_backward(P, features, P, features, 2, 8, P, P, P, 4, 2, features, P, P, None),
+                   lib.convrot_combine_rows_backward(P, features, None, 0, 2, 8, P, P, None, 4, 2, features, P, None, None)):
+        assert status == 2 and f"at most {MOST} features" in lib.convrot_last_error().decode()
