@@ -8,7 +8,7 @@ import torch
 
 from tests import _plain_fp8 as plain
 from tests._plain64 import U, assert_within
-from tests.test_gpu_experts import check_products, choose, fp8_weight, normal
+from tests.test_gpu_experts import check_products, choose, fp8_weight, normal, product16
 from tests.test_gpu_fp8 import weight
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +129,41 @@ def test_gathered_rows(dev, rows, choices, n, dtype):
             view.data_ptr(), _native.dtype_code(dtype), rows, view.stride(0), i.data_ptr(), choices, len(index), n, out.data_ptr(),
             _native.stream_handle(out.device)))
         assert torch.equal(out.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,k", [(1, 65536), (16, 65521), (40, 65536), (300, 65536)])
+def test_longest_rows(dev, m, k, dtype):
+    """512 blocks, whose scales lie in LDS together; few tiles share K (up to 64 additions more, of 1024 in the bound)."""
+    from convrot_mlx_amd import hip_fp8_linear
+
+    n = 70
+    q, ws = weight(k, n, k, dev)
+    bias, x = normal(n, n).to(dev), normal(m, m, k).to(dtype)
+    want, spread = wanted(x, q, ws, bias, dev)
+    assert_within(hip_fp8_linear(x.to(dev), q, ws, bias), want, 2 * spread)
+
+
+def test_most_experts(dev):
+    """65536 experts, rows of a few of them: the first, the last and some between."""
+    from convrot_mlx_amd import ExpertPlan, hip_fp8_grouped_linear, hip_grouped_linear, hip_grouped_linear_backward
+
+    experts, n, k, rows = 65536, 16, 24, 90
+    at = torch.zeros(experts + 1, dtype=torch.int32)
+    met = {0: 3, 63: 1, 64: 40, 4096: 7, 40000: 20, 65535: 19}
+    for e, count in met.items():
+        at[e + 1:] += count
+    assert at[-1] == rows
+    plan = ExpertPlan(at.to(dev))
+    w, x, dy = (normal(i, *s).to(BF16).to(dev) for i, s in enumerate(((experts, n, k), (rows, k), (rows, n))))
+    q, ws = fp8_weight(1, experts, n, k, dev)
+    values = plain.row_values(*plain.codes(x.cpu())).to(dev)
+    out, (dx, dw) = hip_grouped_linear(x, w, plan), hip_grouped_linear_backward(dy, x, w, plan)
+    codes = hip_fp8_grouped_linear(x, q, ws, plan)
+    for e in met:
+        r = slice(int(at[e]), int(at[e + 1]))
+        assert_within(out[r], *product16(x[r].double(), w[e].double(), k), f"forward {e}")
+        assert_within(dx[r], *product16(dy[r].double(), w[e].double().t().contiguous(), n), f"rows {e}")
+        assert_within(dw[e], *product16(dy[r].double().t().contiguous(), x[r].double().t().contiguous(), met[e]), f"weights {e}")
+        assert_within(codes[r], *plain.product(values[r], plain.weight_values(q[e], ws[e]), False), f"8 bits {e}")
+    assert int(dw.flatten(1).any(1).sum()) == len(met)
