@@ -7,19 +7,6 @@
 namespace convrot {
 namespace {
 
-__device__ __forceinline__ uint32_t most_of(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
-  return m;
-}
-__device__ __forceinline__ uint32_t max_of_16(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xf, 0xf, true));
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xf, 0xf, true));
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppHalfMirror, 0xf, 0xf, true));
-  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppMirror, 0xf, 0xf, true));
-}
-
 // Eight features from k on of a row of K (zeros past its end).
 template <int DT, bool VEC>
 __device__ __forceinline__ void load_features(const typename Elem<DT>::T* row, int64_t k, int64_t K, float (&v)[8]) {
@@ -55,7 +42,8 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const typename Elem<DT>::
   }
 }
 
-// A workgroup a block of 128 x 128: each thread holds 8 rows' 8 features, so the weight is read once.
+// A workgroup a block of 128 x 128: each thread holds 8 rows' 8 features, so the weight is read once: 8192 x 8192 in
+// bfloat16 40 us (5.0 TB/s), 2048 x 2048 of one expert 9.2.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void fp8_weight_kernel(const typename Elem<DT>::T* __restrict__ w, int64_t N,
                                                          int64_t K, int64_t w_stride, uint8_t* __restrict__ codes,

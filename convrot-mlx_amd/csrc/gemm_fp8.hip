@@ -28,13 +28,6 @@ constexpr int kRowsMax = 16, kRowsN = 64;
 constexpr int64_t kFusedRowBytes = 32768, kFusedBytes = 16384;
 constexpr size_t kTwoPerCu = 79 * 1024;    // dynamic LDS of two workgroups a CU
 
-__device__ __forceinline__ uint32_t max_of_16(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xf, 0xf, true));
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xf, 0xf, true));
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppHalfMirror, 0xf, 0xf, true));
-  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppMirror, 0xf, 0xf, true));
-}
-
 // LDS of the few-row kernel, in bytes from its start: the rings, the codes [block][row][128], the scales of
 // rows [block][row] and of the weights [block], and (fused) the rows as they are.
 struct RowsLds {
@@ -126,10 +119,7 @@ __global__ __launch_bounds__(256) void fp8_few_rows_kernel(Fp8Operands p, const 
       const uint32_t r = M == 1 ? 0u : i / (uint32_t)n, b = i - r * (uint32_t)n;
       float v[8];
       load8<DT>((const T*)(smem + at.raw) + (i * 128u + sub * 8u), v);
-      uint32_t most = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
-      const Fp8Scale sc = fp8_scale(max_of_16(most));
+      const Fp8Scale sc = fp8_scale(max_of_16(most_of(v)));
       const uint2 w = {fp8_codes4(v, sc.inverse), fp8_codes4(v + 4, sc.inverse)};
       const uint32_t row = b * M + r, chunk = (sub >> 1) ^ (uint32_t)chunk_swizzle((int)r);
       *(uint2*)(smem + at.codes + row * 128u + (chunk << 4) + (sub & 1u) * 8u) = w;

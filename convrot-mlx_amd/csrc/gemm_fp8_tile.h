@@ -16,7 +16,8 @@
 // one (measured with single products; sums of different sixteens are float32's own), up
 // to 15 * 2^-13 of the largest product, 1.5e-5 of a sum of normal values: a sixteenth of
 // float16's own rounding.  Float32 outputs get their products added at float32 instead,
-// on bf16 MFMAs (codes are exact in bf16), at half the rate.
+// on bf16 MFMAs (codes are exact in bf16), at half the rate: 8800 x 8192 -> 4096 from codes
+// 604 us, bfloat16 outputs 291.
 //
 // Operands: codes row-major, rows of 16-byte aligned strides that cover K rounded up to
 // 16, zeros from K on.  Each 1 KB piece of a block (8 rows x 128 bytes: whole cache
@@ -234,6 +235,7 @@ struct Fp8Engine {
   // do not.)
   __device__ __forceinline__ void run_slots(uint32_t kb0, int n, const float* ws, f32x4 (&acc)[FN][FM]) const {
     constexpr int LAG = FM - 1, SLOTS = FN * FM;
+    static_assert(LAG > 0, "an MFMA is not followed by its own FMAs");
     const uint32_t last = kb0 + (uint32_t)n - 1;
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) issue(min(kb0 + s, last), s);
@@ -274,7 +276,7 @@ struct Fp8Engine {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[on][of][j] = __builtin_fmaf(part[of][j], s[of], acc[on][of][j]);
         if constexpr (fn == 0) {
-          if constexpr (LAG > 0 && fm < LAG) s[of] = xs[of] * wsv;
+          if constexpr (fm < LAG) s[of] = xs[of] * wsv;
           if constexpr (fm == 0) s[0] = xs[0] * wsv;
         }
         part[fm] = now;

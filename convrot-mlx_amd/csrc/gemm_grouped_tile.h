@@ -13,8 +13,8 @@
 //   weights   A = dy (across)  B = x (across), c runs over the expert's rows
 //
 // Rows of x through the index: forward by the offsets of a tile's rows, in the weights' gradient by scalar loads of 16
-// numbers a wave and block, a block ahead (4608 tokens of 2 choices, 8 experts, 4096 -> 2048: 178 us, on gathered rows 163
-// and 25 for the gather, which also holds them in memory).
+// numbers a wave and block, a block ahead (4608 tokens of 2 choices, 8 experts, 4096 -> 2048, in a graph: 177 us, on
+// gathered rows 160 and 25 for the gather, which also holds them in memory; eager calls 190 to 201, and 182 and 23).
 //
 // An operand "across" is loaded as it lies, 64 rows of c, and transposed on the way from LDS to
 // the registers (ds_read_b64_tr_b16: 16 lanes read a 4 x 16 block and get its columns), so

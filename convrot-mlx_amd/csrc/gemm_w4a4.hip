@@ -2355,7 +2355,9 @@ hipError_t launch_dma(const Plan& plan, const void* act, const float* xs, const 
       }
       if constexpr (ODT != kF32) {
         // 32x32x32 MFMAs where the grid leaves CUs idle (at most 7/8 of them
-        // busy): 5-14 % faster there, 4 % slower with every CU busy, where the
+        // busy): up to 14 % faster there (1536 x 3072 -> 9216 42.0 us against
+        // 45.1, 1000 x 3072 -> 2000 32.5 and 37.5, 4608 x 12288 -> 3072 129.1 and
+        // 128.3), 4 % slower with every CU busy, where the
         // shader clock drops further under its higher MFMA rate.  The
         // gemm_mfma32 tuning override forces it off (0) or on (1).
         const int m32 = tuning(kTuneGemmMfma32);

@@ -176,6 +176,20 @@ __device__ __forceinline__ float group_sum(float v) {
 }
 __device__ __forceinline__ float wave_sum(float v) { return group_sum<64>(v); }
 
+// The bits of the largest magnitude of 8 values, and over 16 neighbouring lanes.
+__device__ __forceinline__ uint32_t most_of(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu);
+  return m;
+}
+__device__ __forceinline__ uint32_t max_of_16(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xf, 0xf, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppHalfMirror, 0xf, 0xf, true));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppMirror, 0xf, 0xf, true));
+}
+
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   auto other = [](uint32_t x, auto ctrl) {
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xf, 0xf, true);
